@@ -66,6 +66,11 @@ class WkvDesc(C.Structure):
         (n, _vp) for n in ("w0", "u", "norm", "w2")]
 
 
+class Kv4Desc(C.Structure):
+    """Mirror of ``caten_b200_kv4_desc``."""
+    _fields_ = [(n, C.c_int32) for n in ("heads", "kv_heads", "dim", "type", "page")] + [("scale", C.c_float), ("pages", _i64)]
+
+
 class LayerDesc(C.Structure):
     """Mirror of ``caten_b200_layer_desc``."""
     _fields_ = [(n, C.c_int32) for n in ("mixer", "heads", "dim", "kv_heads", "vdim", "window", "rot_dims", "qk_norm", "gated")] + [
@@ -142,6 +147,16 @@ SIGNATURES = {
     "caten_b200_rmsnorm": (C.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, C.c_float]),
     "caten_b200_rope": (C.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, C.c_float, _i64]),
     "caten_b200_sample": (C.c_int, [_vp, _vp, _i64, _i64, C.c_float, C.c_int, _vp, _vp]),
+    "caten_b200_beam_select_work": (_i64, [_i64, _i64, _i64, _i64]),
+    "caten_b200_beam_select": (C.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "caten_b200_beam_reorder": (C.c_int, [_vp, _PFP, _i64, _vp, _i64, _i64, _i64, _i64, _i64]),
+    "caten_b200_beam_reorder_pages": (C.c_int, [_vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64]),
+    "caten_b200_kv_pages": (C.c_int, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64]),
+    "caten_b200_kv4_nbytes": (_i64, [C.POINTER(Kv4Desc)]),
+    "caten_b200_kv4_store": (C.c_int, [_vp, C.POINTER(Kv4Desc), _vp, _vp, _vp, _i64, _vp, _i64]),
+    "caten_b200_kv4_load": (C.c_int, [_vp, C.POINTER(Kv4Desc), _vp, _vp, _i64, _vp, _vp, _i64]),
+    "caten_b200_kv4_attention_work": (_i64, [C.POINTER(Kv4Desc), _i64, _i64, _i64, _i64]),
+    "caten_b200_kv4_attention": (C.c_int, [_vp, C.POINTER(Kv4Desc), _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
     "caten_b200_gpt2_create": (C.c_int, [_vp, C.POINTER(GPT2Desc), _PFP]),
     "caten_b200_gpt2_destroy": (C.c_int, [_vp]),
     "caten_b200_gpt2_step": (C.c_int, [_vp, _vp, _i64, _i64, _vp]),

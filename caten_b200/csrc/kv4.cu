@@ -1,0 +1,396 @@
+// Paged 4-bit key/value cache: page tables and slots from request lengths, rows into the cache and back.  (Attention over it:
+// kv4_attention.cu.)  No counterpart in the reference, whose cache is one fp32 array a layer (external/llm/layers.lisp:25-26).
+#include "common.cuh"
+#include "kv4.cuh"
+
+namespace cb {
+
+// ---- page tables and slots -------------------------------------------------------------------------
+// One block does the whole plan: with a few hundred requests the work is some thousand integers and the launch is the time.  Two scans: totals
+// first, so that a plan that cannot be carried out changes nothing, then request by request the pages given back, the pages taken and the
+// tokens' slots.  A warp walks its 32 requests, lanes over pages and tokens, and skips those without any.
+constexpr int PG_THREADS = 1024;
+
+struct PagesArgs {
+  const int *have, *want;
+  int *table, *free, *state, *starts, *slots;
+  int requests, page, max_pages, capacity, max_tokens;
+};
+
+__device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((long long)tokens + page - 1) / page); }
+
+// exclusive prefix over the block of three numbers a thread; totals in sum[]
+__device__ __forceinline__ void block_scan3(int (&v)[3], int (&sum)[3], int (*warps)[32]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    inc[k] = v[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc[k], o);
+      if (lane >= o) inc[k] += up;
+    }
+  }
+  __syncthreads();   // the last call's totals have been read
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    if (lane == 31) warps[k][warp] = inc[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    int w = warps[k][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += up;
+    }
+    sum[k] = __shfl_sync(0xffffffffu, w, 31);
+    const int before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+    v[k] = inc[k] - v[k] + (warp ? before : 0);
+  }
+}
+
+__global__ void __launch_bounds__(PG_THREADS) kv_pages_kernel(PagesArgs a) {
+  __shared__ long long total[3];   // tokens, pages taken, pages given back
+  __shared__ int bad;
+  __shared__ int warps[3][32];
+  pdl_enter();
+  const int tid = threadIdx.x, lane = tid & 31;
+  if (tid < 3) total[tid] = 0;
+  if (tid == 3) bad = 0;
+  __syncthreads();
+  {
+    long long t[3] = {0, 0, 0};
+    bool wrong = false;
+    for (int r = tid; r < a.requests; r += PG_THREADS) {
+      const int have = a.have[r], want = a.want[r];
+      if (have < 0 || want < 0 || pages_of(have, a.page) > a.max_pages || pages_of(want, a.page) > a.max_pages) { wrong = true; continue; }
+      const int d = pages_of(want, a.page) - pages_of(have, a.page);
+      t[0] += want > have ? want - have : 0;
+      t[1] += d > 0 ? d : 0;
+      t[2] += d < 0 ? -d : 0;
+    }
+    if (wrong) bad = 1;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      for (int o = 16; o > 0; o >>= 1) t[k] += __shfl_xor_sync(0xffffffffu, t[k], o);
+      if (lane == 0 && t[k]) atomicAdd((unsigned long long *)&total[k], (unsigned long long)t[k]);
+    }
+  }
+  __syncthreads();
+  const int n_free = a.state[0];
+  const long long missing = total[1] - total[2] - n_free;
+  int why = bad;                                                                       // 1: lengths that do not fit
+  if (!why && total[0] > a.max_tokens) why = 2;                                        // more tokens than slots
+  if (!why && (n_free < 0 || n_free + total[2] > a.capacity)) why = 3;                 // a free list that was not this pool's
+  const bool go = !why && missing <= 0;
+  __syncthreads();   // state[0] has been read
+  if (tid == 0) {
+    a.state[1] = go ? (int)total[0] : 0;
+    a.state[2] = !why && missing > 0 ? (int)(missing < 0x7fffffff ? missing : 0x7fffffff) : 0;
+    a.state[3] = why;
+    if (go) a.state[0] = (int)(n_free + total[2] - total[1]);
+  }
+  if (!go) {
+    for (int r = tid; r <= a.requests; r += PG_THREADS) a.starts[r] = 0;
+    for (int i = tid; i < a.max_tokens; i += PG_THREADS) a.slots[i] = -1;
+    return;
+  }
+  const int added = (int)total[0], top = (int)(n_free + total[2]);
+  // pages given back: behind the free ones, in the order of requests and of their pages
+  if (total[2]) {
+    int carry = 0;
+    for (int base = 0; base < a.requests; base += PG_THREADS) {
+      const int r = base + tid;
+      const int from = r < a.requests ? pages_of(a.want[r], a.page) : 0, to = r < a.requests ? pages_of(a.have[r], a.page) : 0;
+      int v[3] = {to > from ? to - from : 0, 0, 0}, sum[3];
+      block_scan3(v, sum, warps);
+      for (unsigned todo = __ballot_sync(0xffffffffu, to > from); todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        const int f = __shfl_sync(0xffffffffu, from, src), n = __shfl_sync(0xffffffffu, to, src) - f, at = n_free + carry + __shfl_sync(0xffffffffu, v[0], src);
+        int *row = a.table + (long long)(r - lane + src) * a.max_pages + f;
+        for (int j = lane; j < n; j += 32) {
+          a.free[at + j] = row[j];
+          row[j] = -1;
+        }
+      }
+      carry += sum[0];
+    }
+    __syncthreads();
+  }
+  // pages taken from the end of the list, and the slots of the new tokens
+  int taken = 0, tokens = 0;
+  for (int base = 0; base < a.requests; base += PG_THREADS) {
+    const int r = base + tid;
+    const int have = r < a.requests ? a.have[r] : 0, want = r < a.requests ? a.want[r] : 0;
+    const int more = want > have ? want - have : 0, first = pages_of(have, a.page), take = more ? pages_of(want, a.page) - first : 0;
+    int v[3] = {take, more, 0}, sum[3];
+    block_scan3(v, sum, warps);
+    const int pages_before = taken + v[0], tokens_before = tokens + v[1];
+    if (r < a.requests) a.starts[r] = tokens_before;
+    for (unsigned todo = __ballot_sync(0xffffffffu, more > 0); todo; todo &= todo - 1) {
+      const int src = __ffs(todo) - 1;
+      const int f = __shfl_sync(0xffffffffu, first, src), n = __shfl_sync(0xffffffffu, take, src), p = top - 1 - __shfl_sync(0xffffffffu, pages_before, src);
+      const int start = __shfl_sync(0xffffffffu, tokens_before, src), m = __shfl_sync(0xffffffffu, more, src), h = __shfl_sync(0xffffffffu, have, src);
+      int *row = a.table + (long long)(r - lane + src) * a.max_pages;
+      for (int j = lane; j < n; j += 32) row[f + j] = a.free[p - j];
+      __syncwarp();
+      for (int i = lane; i < m; i += 32) {
+        const int at = h + i, id = row[at / a.page];
+        a.slots[start + i] = id >= 0 && id < a.capacity ? id * a.page + at % a.page : -1;
+      }
+    }
+    taken += sum[0];
+    tokens += sum[1];
+  }
+  if (tid == 0) a.starts[a.requests] = added;
+  for (int i = added + tid; i < a.max_tokens; i += PG_THREADS) a.slots[i] = -1;
+}
+
+// ---- rows into the cache ---------------------------------------------------------------------------
+// A block of 32 values is eight lanes' float4.  Codes are those of the GGUF formats: Q4_0  d = (value of largest magnitude) / -8,
+// code = min(15, trunc(x / d + 8.5)); Q4_1  d = (max - min) / 15, code = min(15, trunc((x - min) / d + 0.5)).  Which code is nearest is decided
+// exactly: in fp32, whose error here is below 4e-6, unless the quotient is within 1e-5 of a border, then in 64 bits.  d and the minimum are
+// rounded to fp16 (half a step: 2^-11) because that is what the formats hold.
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+
+__device__ __forceinline__ uint32_t kv4_code(float x, float inverse, float offset, double d, float low) {
+  const float y = fmaf(x - low, inverse, offset);
+  if (fabsf(y - rintf(y)) >= 1e-5f) return (uint32_t)min(15, max(0, (int)y));
+  const double e = ((double)x - (double)low) / d + (double)offset;
+  return (uint32_t)min(15, max(0, (int)e));
+}
+
+// this lane's four values of a block that eight consecutive lanes hold -> four codes (low bits first), scale and minimum
+template <bool Q41>
+__device__ __forceinline__ uint32_t kv4_quantise(float4 x, __half *scale, __half *minimum) {
+  const float v[4] = {x.x, x.y, x.z, x.w};
+  uint32_t codes = 0;
+  if (Q41) {
+    float hi = v[0], lo = v[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) { hi = max_nan(hi, v[i]); lo = min_nan(lo, v[i]); }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    }
+    const double d = ((double)hi - (double)lo) / 15.0;
+    *scale = __float2half_rn((float)d);
+    *minimum = __float2half_rn(lo);
+    const float inverse = 1.0f / (float)d;
+    if (__half2float(*scale) != 0.0f)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) codes |= kv4_code(v[i], inverse, 0.5f, d, lo) << (4 * i);
+  } else {
+    // the value of largest magnitude, the first of equal ones; magnitudes compared as bits, NaN above infinity
+    float m = v[0];
+    int at = (threadIdx.x & 7) * 4;
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+      if ((__float_as_uint(v[i]) & 0x7fffffffu) > (__float_as_uint(m) & 0x7fffffffu)) { m = v[i]; at = (threadIdx.x & 7) * 4 + i; }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, m, o);
+      const int oat = __shfl_xor_sync(0xffffffffu, at, o);
+      const uint32_t a = __float_as_uint(m) & 0x7fffffffu, b = __float_as_uint(om) & 0x7fffffffu;
+      if (b > a || (b == a && oat < at)) { m = om; at = oat; }
+    }
+    const float d = m / -8.0f;
+    *scale = __float2half_rn(d);
+    const float inverse = 1.0f / d;
+    if (__half2float(*scale) != 0.0f) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) codes |= kv4_code(v[i], inverse, 8.5f, (double)d, 0.0f) << (4 * i);
+    } else {
+      codes = 0x8888u;
+    }
+  }
+  return codes;
+}
+
+struct RowsArgs {
+  float *k, *v;              // store: read only
+  uint8_t *pool;
+  const int *slots;
+  int *status;
+  int64_t ld, tokens;
+  Kv4Shape s;
+  int vec;                   // rows can be read and written by 16 bytes
+};
+
+__device__ __forceinline__ bool kv4_slot(const RowsArgs &a, int64_t token, int64_t *page_id, int *within) {
+  const int slot = a.slots[token];
+  if (slot < 0) {
+    if (slot < -1) report_bad_index(a.status, 40, slot);
+    return false;
+  }
+  *page_id = slot / a.s.page;
+  *within = slot % a.s.page;
+  if (kv4_page_ok(a.s, *page_id)) return true;
+  report_bad_index(a.status, 40, slot);
+  return false;
+}
+
+template <bool Q41>
+__global__ void __launch_bounds__(256) kv4_store_kernel(RowsArgs a) {
+  pdl_enter();
+  const int quads = a.s.kv_heads * a.s.dim / 4;   // float4 of a token's keys
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = a.tokens * 2 * quads;
+  const bool there = i < all;                     // (whole groups of eight lanes: quads is a multiple of 16)
+  const int64_t token = there ? i / (2 * quads) : 0;
+  const int c = there ? (int)(i % (2 * quads)) : 0;
+  const bool of_k = c < quads;
+  const int col = (of_k ? c : c - quads) * 4;
+  int64_t page_id = 0;
+  int within = 0;
+  const bool ok = there && kv4_slot(a, token, &page_id, &within);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (ok) {
+    const float *src = (of_k ? a.k : a.v) + token * a.ld + col;
+    if (a.vec) x = __ldcs(reinterpret_cast<const float4 *>(src));
+    else x = make_float4(src[0], src[1], src[2], src[3]);
+  }
+  __half d, m;
+  const uint32_t codes = kv4_quantise<Q41>(x, &d, &m);
+  const uint32_t next = __shfl_down_sync(0xffffffffu, codes, 1);
+  if (!ok) return;
+  const int head = col / a.s.dim, dim = col % a.s.dim, tok = within % 16;
+  uint8_t *part = a.pool + kv4_tile_at(a.s, page_id, head, within) + (of_k ? 0 : kv4_part_bytes(a.s));
+  if (of_k) {
+    if (dim % 8 == 0) *reinterpret_cast<uint32_t *>(part + kv4_k_byte(tok, dim)) = codes | next << 16;
+  } else {
+    *reinterpret_cast<uint16_t *>(part + kv4_v_byte(tok, dim)) = (uint16_t)codes;
+  }
+  if (dim % 32 == 0) {
+    __half *scales = reinterpret_cast<__half *>(part + 8 * a.s.dim) + kv4_scale_index(tok, dim / 32, a.s.dim);
+    scales[0] = d;
+    if (Q41) scales[a.s.dim / 2] = m;
+  }
+}
+
+// ---- rows out of the cache -------------------------------------------------------------------------
+template <bool Q41>
+__global__ void __launch_bounds__(256) kv4_load_kernel(RowsArgs a) {
+  pdl_enter();
+  const int quads = a.s.kv_heads * a.s.dim / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.tokens * 2 * quads) return;
+  const int64_t token = i / (2 * quads);
+  const int c = (int)(i % (2 * quads));
+  const bool of_k = c < quads;
+  const int col = (of_k ? c : c - quads) * 4;
+  int64_t page_id;
+  int within;
+  if (!kv4_slot(a, token, &page_id, &within)) return;
+  const int head = col / a.s.dim, dim = col % a.s.dim, tok = within % 16;
+  const uint8_t *part = a.pool + kv4_tile_at(a.s, page_id, head, within) + (of_k ? 0 : kv4_part_bytes(a.s));
+  const uint32_t codes = *reinterpret_cast<const uint16_t *>(part + (of_k ? kv4_k_byte(tok, dim) : kv4_v_byte(tok, dim)));
+  const __half *scales = reinterpret_cast<const __half *>(part + 8 * a.s.dim) + kv4_scale_index(tok, dim / 32, a.s.dim);
+  const float d = __half2float(scales[0]), m = Q41 ? __half2float(scales[a.s.dim / 2]) : 0.0f;
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int code = (int)(codes >> (4 * e) & 15u);
+    y[e] = Q41 ? d * (float)code + m : d * (float)(code - 8);
+  }
+  float *dst = (of_k ? a.k : a.v) + token * a.ld + col;
+  if (a.vec) __stcs(reinterpret_cast<float4 *>(dst), make_float4(y[0], y[1], y[2], y[3]));
+  else { dst[0] = y[0]; dst[1] = y[1]; dst[2] = y[2]; dst[3] = y[3]; }
+}
+
+// ---- checks ----------------------------------------------------------------------------------------
+int kv4_check(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_desc *c, Kv4Shape *s) {
+  if (!c) return fail(ctx, CATEN_B200_EINVAL, "%s: the description is NULL", who);
+  if (c->type != CATEN_B200_Q4_0 && c->type != CATEN_B200_Q4_1) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: cache of type %d (Q4_0 and Q4_1 are stored)", who, c->type);
+  if (c->dim != 64 && c->dim != 128 && c->dim != 192 && c->dim != 256) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: heads of %d (64, 128, 192 or 256)", who, c->dim);
+  if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: pages of %d tokens (16, 32, 64 or 128)", who, c->page);
+  if (c->kv_heads <= 0 || c->kv_heads > 65535 || c->heads <= 0 || c->heads > 65535 || c->heads % c->kv_heads) return fail(ctx, CATEN_B200_EINVAL, "%s: %d heads over %d", who, c->heads, c->kv_heads);
+  if (c->pages <= 0 || c->pages > 0x7fffffffll / c->page) return fail(ctx, CATEN_B200_EINVAL, "%s: %lld pages of %d tokens (slots are 32-bit numbers)", who, (long long)c->pages, c->page);
+  *s = {c->kv_heads, c->dim, c->type == CATEN_B200_Q4_1, c->page, c->pages};
+  return 0;
+}
+
+static int rows_check(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_desc *c, const void *pool, const float *k, const float *v, int64_t ld,
+                      const int32_t *slots, int64_t tokens, RowsArgs *a) {
+  if (int rc = kv4_check(ctx, who, c, &a->s)) return rc;
+  if (tokens < 0 || tokens > 0x7fffffff) return fail(ctx, CATEN_B200_EINVAL, "%s: %lld tokens", who, (long long)tokens);
+  if (tokens && (!pool || !k || !v || !slots)) return fail(ctx, CATEN_B200_EINVAL, "%s: NULL argument", who);
+  if (ld < (int64_t)c->kv_heads * c->dim) return fail(ctx, CATEN_B200_EINVAL, "%s: ld=%lld, rows have %lld values", who, (long long)ld, (long long)c->kv_heads * c->dim);
+  if ((uintptr_t)pool % 16) return fail(ctx, CATEN_B200_EINVAL, "%s: the pool has to start on a multiple of 16 bytes", who);
+  if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)slots) % 4) return fail(ctx, CATEN_B200_EINVAL, "%s: misaligned pointer", who);
+  a->k = const_cast<float *>(k); a->v = const_cast<float *>(v);
+  a->pool = (uint8_t *)const_cast<void *>(pool);
+  a->slots = slots;
+  a->ld = ld; a->tokens = tokens;
+  a->vec = ld % 4 == 0 && ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
+  const int64_t blocks = (tokens * 2 * (c->kv_heads * (int64_t)c->dim / 4) + 255) / 256;
+  if (blocks > 0x7fffffff) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: %lld tokens in one call", who, (long long)tokens);
+  return 0;
+}
+
+static int rows_launch(caten_b200_ctx *ctx, RowsArgs a, bool store) {
+  a.status = ctx->d_status;
+  const unsigned blocks = (unsigned)((a.tokens * 2 * (a.s.kv_heads * (int64_t)a.s.dim / 4) + 255) / 256);
+  void (*kernel)(RowsArgs) = store ? (a.s.q41 ? kv4_store_kernel<true> : kv4_store_kernel<false>) : (a.s.q41 ? kv4_load_kernel<true> : kv4_load_kernel<false>);
+  CB_CUDA(ctx, launch_k(ctx, kernel, dim3(blocks), dim3(256), 0, a));
+  CB_LAUNCH_CHECK(ctx, store ? "kv4_store_kernel" : "kv4_load_kernel");
+  return 0;
+}
+
+}  // namespace cb
+
+using namespace cb;
+
+extern "C" {
+
+// Arguments are checked before the context is touched.
+int caten_b200_kv_pages(caten_b200_ctx *ctx, const int32_t *d_have, const int32_t *d_want, int64_t requests, int64_t page, int32_t *d_table,
+                        int64_t max_pages, int32_t *d_free, int64_t pages, int32_t *d_state, int32_t *d_starts, int32_t *d_slots, int64_t max_tokens) {
+  if (requests < 0 || requests > (1 << 24) || max_pages <= 0 || max_tokens < 0 || max_tokens > (1 << 30)) return fail(ctx, CATEN_B200_EINVAL, "kv_pages: bad shape");
+  if (page <= 0 || pages <= 0 || page > 0x7fffffff || pages > 0x7fffffffll / page || max_pages > 0x7fffffffll / page)
+    return fail(ctx, CATEN_B200_EINVAL, "kv_pages: %lld pages of %lld tokens, %lld a request (slots and positions are 32-bit numbers)", (long long)pages, (long long)page, (long long)max_pages);
+  if (!d_free || !d_state || !d_starts || (requests && (!d_have || !d_want || !d_table)) || (max_tokens && !d_slots)) return fail(ctx, CATEN_B200_EINVAL, "kv_pages: NULL argument");
+  if (!ctx) return fail(nullptr, CATEN_B200_EINVAL, "kv_pages: ctx is NULL");
+  cudaSetDevice(ctx->device);
+  ctx->work_outside = true;
+  ProfScope prof(ctx, CATEN_B200_K_PREP);
+  PagesArgs a = {d_have, d_want, d_table, d_free, d_state, d_starts, d_slots, (int)requests, (int)page, (int)max_pages, (int)pages, (int)max_tokens};
+  CB_CUDA(ctx, launch_k(ctx, kv_pages_kernel, dim3(1), dim3(PG_THREADS), 0, a));
+  CB_LAUNCH_CHECK(ctx, "kv_pages_kernel");
+  return 0;
+}
+
+int64_t caten_b200_kv4_nbytes(const caten_b200_kv4_desc *desc) {
+  Kv4Shape s;
+  if (kv4_check(nullptr, "kv4_nbytes", desc, &s)) return -1;
+  return kv4_page_bytes(s) * s.pages;
+}
+
+int caten_b200_kv4_store(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, void *d_pool, const float *d_k, const float *d_v, int64_t ld,
+                         const int32_t *d_slots, int64_t tokens) {
+  RowsArgs a = {};
+  if (int rc = rows_check(ctx, "kv4_store", desc, d_pool, d_k, d_v, ld, d_slots, tokens, &a)) return rc;
+  if (!ctx) return fail(nullptr, CATEN_B200_EINVAL, "kv4_store: ctx is NULL");
+  cudaSetDevice(ctx->device);
+  ctx->work_outside = true;
+  if (tokens == 0) return 0;
+  ProfScope prof(ctx, CATEN_B200_K_PREP);
+  return rows_launch(ctx, a, true);
+}
+
+int caten_b200_kv4_load(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, const void *d_pool, const int32_t *d_slots, int64_t tokens, float *d_k,
+                        float *d_v, int64_t ld) {
+  RowsArgs a = {};
+  if (int rc = rows_check(ctx, "kv4_load", desc, d_pool, d_k, d_v, ld, d_slots, tokens, &a)) return rc;
+  if (!ctx) return fail(nullptr, CATEN_B200_EINVAL, "kv4_load: ctx is NULL");
+  cudaSetDevice(ctx->device);
+  ctx->work_outside = true;
+  if (tokens == 0) return 0;
+  ProfScope prof(ctx, CATEN_B200_K_PREP);
+  return rows_launch(ctx, a, false);
+}
+
+}  // extern "C"

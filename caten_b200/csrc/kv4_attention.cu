@@ -1,0 +1,467 @@
+// Attention over a paged 4-bit cache: o = sum_t softmax_t(scale q . k_t) v_t over the tokens that a query sees, keys and values
+// d code + m (Q4_0: m = -8 d) in blocks of 32 dims.
+//
+// Both products run as 16 x 8 x 16 matrix products on fp16 operands, in which code - 8 is exact: four bits or-ed into 1024 (or, four bits up, 64
+// in sixteenths) and 1032 (72) taken off, two codes at a time.  (Masked where they stand, as subnormal halves, codes need no second instruction, but
+// the tensor cores align products by the operands' exponent fields, so the ten leading zeros are lost from their 24 bits: errors of 1e-5.)  The other
+// operand is split in two halves (22 bits): q, scaled to the top of fp16's range by a power of two, in rows r and r + 8 of the first product, whose sums
+// are added; p d in two of the second.  Scales and minima stay outside the products, in fp32:
+//   score(r, t) = sum over blocks of d_t,b (q_r . (codes - 8)) + n_t,b sum(q_r)          out(r, j) = sum_t (p_rt d_t,b) (code_tj - 8) + sum_t p_rt n_t,b
+// with n = 0 (Q4_0) or the minimum + 8 d (Q4_1).  From the middle of the codes, because a sum of thousands of p d code is many times what is left when
+// 8 p d is taken off it, and so is its error (100001 tokens: 3e-4).
+// A warp has 8 rows (tokens x the heads that share a key head) and takes 64 tokens at a time: running maximum and sum of the softmax per row, the
+// group's p d scaled by a power of two for each block, so that the largest is near the top of fp16 whatever the cache's scales are, and joined
+// to the running sums in fp32.
+#include "common.cuh"
+#include "kv4.cuh"
+
+namespace cb {
+
+constexpr int K4_WARPS = 8;        // of a block; they share a row tile's tokens, 64 at a time
+constexpr int K4_GROUP = 64;       // tokens
+constexpr int K4_ROWS = 8;
+
+struct Kv4AttnArgs {
+  const float *q;
+  const uint8_t *pool;
+  const int *table, *lengths, *starts;
+  float *out, *part;
+  int *status;
+  int64_t ldq, rows;
+  Kv4Shape s;
+  int heads, group, max_pages, max_new, max_length, batch;
+  int row_tiles, parts, part_tokens;
+  float scale;
+};
+
+// rows of a sequence and how far they see; what a plan's device memory says is checked against the call's arguments here
+struct Kv4Seq {
+  int64_t first;   // row of q and out
+  int count, length;
+};
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs &a, int b, bool tells) {
+  Kv4Seq q;
+  q.first = a.starts ? a.starts[b] : b;
+  const int64_t end = a.starts ? a.starts[b + 1] : b + 1;
+  const int length = a.lengths[b];
+  q.count = (int)(end - q.first);
+  q.length = length;
+  if (q.first < 0 || end < q.first || end > a.rows || end - q.first > a.max_new) {
+    if (tells) report_bad_index(a.status, 44, b);
+    q.count = 0;
+  }
+  if (length < 0 || length > a.max_length) {
+    if (tells) report_bad_index(a.status, 45, length);
+    q.length = length < 0 ? 0 : a.max_length;
+  }
+  return q;
+}
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack_half_lo(float a, float b, uint32_t hi) {
+  const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+  return pack_half(a - h.x, b - h.y);
+}
+// code - 8 of the low four bits of both halves of w; of the next four
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+  uint32_t r;
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"((w & 0x000f000fu) | 0x64006400u), "r"(0x64086408u));   // 1024 + c - 1032
+  return r;
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"((w & 0x00f000f0u) | 0x64006400u), "r"(0x2c002c00u), "r"(0xd480d480u));   // (1024 + 16 c) / 16 - 72
+  return r;
+}
+__device__ __forceinline__ float2 half_pair(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// power of two 2^(14 - floor(log2 x)), kept inside fp32's normal range; 1 for zero
+__device__ __forceinline__ float to_top(float x) {
+  const int e = (int)(__float_as_uint(x) >> 23 & 0xff);
+  if (x == 0.0f) return 1.0f;
+  return __uint_as_float((uint32_t)min(max(127 + 14 - (e - 127), 30), 240) << 23);
+}
+
+template <int NC, bool Q41>
+__global__ void __launch_bounds__(K4_WARPS * 32) kv4_attention_kernel(const Kv4AttnArgs a) {
+  constexpr int NB = 2 * NC, D = 64 * NC;
+  __shared__ float sm[K4_WARPS][K4_ROWS], sl[K4_WARPS][K4_ROWS];
+  extern __shared__ float so[];   // [warp][row][D]
+  pdl_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  int64_t u = blockIdx.x;
+  const int part = (int)(u % a.parts); u /= a.parts;
+  const int rt = (int)(u % a.row_tiles); u /= a.row_tiles;
+  const int head = (int)(u % a.s.kv_heads);
+  const int b = (int)(u / a.s.kv_heads);
+  const Kv4Seq seq = kv4_seq(a, b, threadIdx.x == 0 && part == 0 && rt == 0 && head == 0);
+  const int count = seq.count * a.group;   // rows of this key head
+  if (rt * K4_ROWS >= count) return;
+  // row g of the tile: token r / group, query head head * group + r % group
+  const int r = rt * K4_ROWS + g;
+  const int tok = r / a.group;
+  const int sees = r < count ? max(0, seq.length - seq.count + tok + 1) : 0;   // tokens before and at its position
+  const int last = min(count, rt * K4_ROWS + K4_ROWS) - 1;
+  const int most = max(0, seq.length - seq.count + last / a.group + 1);
+  const int t0 = part * a.part_tokens, t1 = min(most, t0 + a.part_tokens);
+  if (t0 >= t1 && part > 0) return;
+
+  // q as the first product's operand: a block's two steps, {dims 8t + 0, 4 | 8t + 1, 5} and {2, 6 | 3, 7}; hi in rows g, lo in rows g + 8
+  uint32_t qa[NB][2][4];
+  float qsum[NB];
+  float factor;
+  {
+    const float *q = a.q + (seq.first + tok) * a.ldq + (int64_t)(head * a.group + r % a.group) * D + 8 * t;
+    float x[NB][8], top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[k][j] = r < count ? q[32 * k + j] : 0.0f;
+        top = fmaxf(top, fabsf(x[k][j]));
+      }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float up = to_top(top);
+    factor = a.scale * 1.4426950408889634f * (1.0f / up);
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[k][j] *= up;
+        sum += x[k][j];
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      qsum[k] = sum;
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        qa[k][st][0] = pack_half(x[k][2 * st], x[k][2 * st + 4]);
+        qa[k][st][1] = pack_half_lo(x[k][2 * st], x[k][2 * st + 4], qa[k][st][0]);
+        qa[k][st][2] = pack_half(x[k][2 * st + 1], x[k][2 * st + 5]);
+        qa[k][st][3] = pack_half_lo(x[k][2 * st + 1], x[k][2 * st + 5], qa[k][st][2]);
+      }
+    }
+  }
+
+  float run_max = -INFINITY, run_sum = 0.0f;   // of row g (run_sum: this lane's tokens)
+  float off[NB];                               // Q4_1: sum of p (m + 8 d) of row g, this lane's tokens
+  float o[NB][2][4];                           // rows 2t, 2t + 1; dims 4g + {0, 1} and 4g + {2, 3} of a block
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    off[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] = 0.0f;
+  }
+
+  const int part_bytes = kv4_part_bytes(a.s), tile_bytes = 2 * part_bytes;
+  for (int base = t0 + warp * K4_GROUP; base < t1; base += K4_WARPS * K4_GROUP) {
+    float s[4][4];
+    const uint8_t *tile[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = base + 16 * i;
+      tile[i] = nullptr;
+      if (at < t1) {
+        const int id = a.table[(int64_t)b * a.max_pages + at / a.s.page];
+        if (kv4_page_ok(a.s, id)) tile[i] = a.pool + kv4_tile_at(a.s, id, head, at % a.s.page);
+        else if (lane == 0) report_bad_index(a.status, 46, id);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = -INFINITY;
+      if (!tile[i]) continue;   // (the same for all lanes)
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(tile[i] + c * 512 + lane * 16);
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int blk = 2 * c + k;
+          const uint8_t *sc = tile[i] + 8 * D + (t * NB + blk) * 8;
+          const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
+          const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
+          float d[4] = {d01.x, d01.y, d23.x, d23.y}, m[4];
+          if (Q41) {
+            const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
+            const float2 m01 = half_pair(m2.x), m23 = half_pair(m2.y);
+            m[0] = m01.x; m[1] = m01.y; m[2] = m23.x; m[3] = m23.y;
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {   // tokens 0..7, 8..15
+            const uint32_t lo = words[2 * n + k], hi = lo >> 8;
+            float p[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_16816(p, qa[blk][0], codes_lo(lo), codes_hi(lo));
+            mma_16816(p, qa[blk][1], codes_lo(hi), codes_hi(hi));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float dot = p[j] + p[2 + j];
+              const int e = 2 * n + j;
+              acc[e] = fmaf(d[e], dot, Q41 ? fmaf(fmaf(8.0f, d[e], m[e]), qsum[blk], acc[e]) : acc[e]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1);
+        if (at < sees && at < t1) s[i][e] = acc[e] * factor;
+      }
+    }
+    // running maximum
+    float top = run_max;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    const float corr = exp2_fast(run_max - ref);   // (-inf: 0)
+    run_max = top;
+    run_sum *= corr;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[i][e] = exp2_fast(s[i][e] - ref);
+        run_sum += s[i][e];
+      }
+    const float corr0 = __shfl_sync(0xffffffffu, corr, 8 * t), corr1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
+    // values
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      uint4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = tile[i] ? *reinterpret_cast<const uint4 *>(tile[i] + part_bytes + c * 512 + lane * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int blk = 2 * c + k;
+        float pd[4][4], big = 0.0f;
+        float add = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f};
+          if (tile[i]) {
+            const uint8_t *sc = tile[i] + part_bytes + 8 * D + (t * NB + blk) * 8;
+            const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
+            const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
+            d[0] = d01.x; d[1] = d01.y; d[2] = d23.x; d[3] = d23.y;
+            if (Q41) {
+              const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
+              const float2 m01 = half_pair(m2.x), m23 = half_pair(m2.y);
+              m[0] = m01.x; m[1] = m01.y; m[2] = m23.x; m[3] = m23.y;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1);
+            const bool in = at < t1;   // (what stands behind a page's last token may be anything)
+            big = fmaxf(big, in ? fabsf(d[e]) : 0.0f);
+            pd[i][e] = at < sees ? s[i][e] * d[e] : 0.0f;
+            if (Q41 && at < sees) add = fmaf(s[i][e], fmaf(8.0f, d[e], m[e]), add);
+          }
+        }
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        const float up = to_top(big), down = 1.0f / up;
+        off[blk] = fmaf(off[blk], corr, add);
+        float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t h0 = pack_half(pd[i][0] * up, pd[i][1] * up), h1 = pack_half(pd[i][2] * up, pd[i][3] * up);
+          const uint32_t l0 = pack_half_lo(pd[i][0] * up, pd[i][1] * up, h0), l1 = pack_half_lo(pd[i][2] * up, pd[i][3] * up, h1);
+          const uint32_t x = __byte_perm(w[i].x, w[i].y, k ? 0x7632 : 0x5410), y = __byte_perm(w[i].z, w[i].w, k ? 0x7632 : 0x5410);
+          const uint32_t a0[4] = {codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y)};
+          const uint32_t a1[4] = {codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8)};
+          mma_16816(acc[0], a0, h0, h1);
+          mma_16816(acc[0], a0, l0, l1);
+          mma_16816(acc[1], a1, h0, h1);
+          mma_16816(acc[1], a1, l0, l1);
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          o[blk][n][0] = fmaf(o[blk][n][0], corr0, acc[n][0] * down);
+          o[blk][n][1] = fmaf(o[blk][n][1], corr1, acc[n][1] * down);
+          o[blk][n][2] = fmaf(o[blk][n][2], corr0, acc[n][2] * down);
+          o[blk][n][3] = fmaf(o[blk][n][3], corr1, acc[n][3] * down);
+        }
+      }
+    }
+  }
+
+  // the warp's sums: over the four lanes of a row, then the blocks' constant parts to the lanes that hold the outputs
+  run_sum += __shfl_xor_sync(0xffffffffu, run_sum, 1);
+  run_sum += __shfl_xor_sync(0xffffffffu, run_sum, 2);
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    if (Q41) {
+      off[k] += __shfl_xor_sync(0xffffffffu, off[k], 1);
+      off[k] += __shfl_xor_sync(0xffffffffu, off[k], 2);
+    }
+    const float c0 = Q41 ? __shfl_sync(0xffffffffu, off[k], 8 * t) : 0.0f, c1 = Q41 ? __shfl_sync(0xffffffffu, off[k], 8 * t + 4) : 0.0f;
+    float *dst = so + (warp * K4_ROWS + 2 * t) * D + 32 * k + 4 * g;
+    *reinterpret_cast<float4 *>(dst) = make_float4(o[k][0][0] + c0, o[k][0][2] + c0, o[k][1][0] + c0, o[k][1][2] + c0);
+    *reinterpret_cast<float4 *>(dst + D) = make_float4(o[k][0][1] + c1, o[k][0][3] + c1, o[k][1][1] + c1, o[k][1][3] + c1);
+  }
+  if (t == 0) { sm[warp][g] = run_max; sl[warp][g] = run_sum; }
+  __syncthreads();
+  // the warps' sums into one
+  for (int i = threadIdx.x; i < K4_ROWS * D; i += K4_WARPS * 32) {
+    const int row = i / D, j = i % D;
+    float top = sm[0][row];
+#pragma unroll
+    for (int w = 1; w < K4_WARPS; ++w) top = fmaxf(top, sm[w][row]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, x = 0.0f;
+#pragma unroll
+    for (int w = 0; w < K4_WARPS; ++w) {
+      const float e = exp2_fast(sm[w][row] - ref);
+      sum = fmaf(sl[w][row], e, sum);
+      x = fmaf(so[(w * K4_ROWS + row) * D + j], e, x);
+    }
+    const int rr = rt * K4_ROWS + row;
+    if (rr >= count) continue;
+    if (a.parts == 1) {
+      a.out[(seq.first + rr / a.group) * (int64_t)a.heads * D + (int64_t)(head * a.group + rr % a.group) * D + j] = sum == 0.0f ? 0.0f : x / sum;
+    } else {
+      float *p = a.part + (int64_t)blockIdx.x * K4_ROWS * (D + 2) + row * (D + 2);
+      p[j] = x;
+      if (j == 0) { p[D] = top; p[D + 1] = sum; }
+    }
+  }
+}
+
+// The parts of a row tile into one.  A block has a row tile; parts behind what its rows see were not written.
+__global__ void __launch_bounds__(256) kv4_attention_join_kernel(const Kv4AttnArgs a) {
+  pdl_enter();
+  const int D = a.s.dim;
+  int64_t u = blockIdx.x;
+  const int rt = (int)(u % a.row_tiles); u /= a.row_tiles;
+  const int head = (int)(u % a.s.kv_heads);
+  const int b = (int)(u / a.s.kv_heads);
+  const Kv4Seq seq = kv4_seq(a, b, false);
+  const int count = seq.count * a.group;
+  if (rt * K4_ROWS >= count) return;
+  const int last = min(count, rt * K4_ROWS + K4_ROWS) - 1;
+  const int most = max(0, seq.length - seq.count + last / a.group + 1);
+  const int parts = max(1, (most + a.part_tokens - 1) / a.part_tokens);
+  for (int i = threadIdx.x; i < K4_ROWS * D; i += 256) {
+    const int row = i / D, j = i % D, rr = rt * K4_ROWS + row;
+    if (rr >= count) break;
+    const float *p = a.part + (int64_t)blockIdx.x * a.parts * K4_ROWS * (D + 2) + row * (D + 2);
+    const int64_t step = (int64_t)K4_ROWS * (D + 2);
+    float top = -INFINITY;
+    for (int k = 0; k < parts; ++k) top = fmaxf(top, p[k * step + D]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, x = 0.0f;
+    for (int k = 0; k < parts; ++k) {
+      const float e = exp2_fast(p[k * step + D] - ref);
+      sum = fmaf(p[k * step + D + 1], e, sum);
+      x = fmaf(p[k * step + j], e, x);
+    }
+    a.out[(seq.first + rr / a.group) * (int64_t)a.heads * D + (int64_t)(head * a.group + rr % a.group) * D + j] = sum == 0.0f ? 0.0f : x / sum;
+  }
+}
+
+// How a call is cut: row tiles of 8, and parts of the tokens where row tiles alone leave SMs idle.  By sizes that the host knows.
+struct Kv4Plan {
+  int64_t units;   // row tiles of all sequences and key heads
+  int row_tiles, parts, part_tokens;
+};
+static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_desc *c, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length, Kv4Plan *p) {
+  Kv4Shape s;
+  if (int rc = kv4_check(ctx, who, c, &s)) return rc;
+  if (batch < 0 || batch > (1 << 24) || rows < 0 || rows > 0x7fffffff || max_new <= 0 || max_length < 0 || max_length > 0x3fffffff) return fail(ctx, CATEN_B200_EINVAL, "%s: bad shape", who);
+  const int64_t group = c->heads / c->kv_heads;
+  if (max_new > (1 << 24) || max_new * group > 0x3fffffff) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: %lld new tokens of a sequence", who, (long long)max_new);
+  p->row_tiles = (int)((max_new * group + K4_ROWS - 1) / K4_ROWS);
+  if (batch && (int64_t)c->kv_heads * p->row_tiles > 0x7fffffff / batch) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
+  p->units = batch * c->kv_heads * p->row_tiles;
+  const int64_t groups = (max_length + K4_GROUP - 1) / K4_GROUP;
+  int64_t parts = p->units ? (148 * 3 + p->units - 1) / p->units : 1;
+  const int64_t most = (groups + 2 * K4_WARPS - 1) / (2 * K4_WARPS);   // a part gives each warp two groups at least
+  if (parts > most) parts = most;
+  if (parts < 1) parts = 1;
+  const int64_t each = groups ? (groups + parts - 1) / parts : 1;
+  p->part_tokens = (int)(each * K4_GROUP);
+  p->parts = (int)(groups ? (groups + each - 1) / each : 1);
+  if (p->units * p->parts > 0x7fffffff) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
+  return 0;
+}
+
+template <int NC, bool Q41>
+static int kv4_attention_launch(caten_b200_ctx *ctx, const Kv4AttnArgs &a, int64_t units) {
+  const int smem = K4_WARPS * K4_ROWS * NC * 64 * (int)sizeof(float);
+  CB_CUDA(ctx, cudaFuncSetAttribute(kv4_attention_kernel<NC, Q41>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  CB_CUDA(ctx, launch_k(ctx, kv4_attention_kernel<NC, Q41>, dim3((unsigned)(units * a.parts)), dim3(K4_WARPS * 32), smem, a));
+  CB_LAUNCH_CHECK(ctx, "kv4_attention_kernel");
+  if (a.parts == 1) return 0;
+  CB_CUDA(ctx, launch_k(ctx, kv4_attention_join_kernel, dim3((unsigned)units), dim3(256), 0, a));
+  CB_LAUNCH_CHECK(ctx, "kv4_attention_join_kernel");
+  return 0;
+}
+
+}  // namespace cb
+
+using namespace cb;
+
+extern "C" {
+
+// Arguments are checked before the context is touched.
+int64_t caten_b200_kv4_attention_work(const caten_b200_kv4_desc *desc, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length) {
+  Kv4Plan p;
+  if (kv4_plan(nullptr, "kv4_attention_work", desc, batch, rows, max_new, max_length, &p)) return -1;
+  return p.parts > 1 ? p.units * p.parts * K4_ROWS * (desc->dim + 2) * (int64_t)sizeof(float) : 16;
+}
+
+int caten_b200_kv4_attention(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, const float *d_q, int64_t ldq, const void *d_pool, const int32_t *d_table,
+                             int64_t max_pages, const int32_t *d_lengths, const int32_t *d_starts, int64_t batch, int64_t rows, int64_t max_new,
+                             int64_t max_length, float *d_out, void *d_work) {
+  Kv4Plan p;
+  if (int rc = kv4_plan(ctx, "kv4_attention", desc, batch, rows, max_new, max_length, &p)) return rc;
+  if (max_pages <= 0 || max_pages > 0x7fffffff || max_length > max_pages * desc->page)
+    return fail(ctx, CATEN_B200_EINVAL, "kv4_attention: lengths up to %lld in tables of %lld pages of %d", (long long)max_length, (long long)max_pages, desc->page);
+  if (!d_starts && (rows != batch || max_new != 1)) return fail(ctx, CATEN_B200_EINVAL, "kv4_attention: without starts every sequence has one row");
+  if (ldq < (int64_t)desc->heads * desc->dim) return fail(ctx, CATEN_B200_EINVAL, "kv4_attention: ldq=%lld, rows have %lld values", (long long)ldq, (long long)desc->heads * desc->dim);
+  if (batch && rows && (!d_q || !d_pool || !d_table || !d_lengths || !d_out || !d_work)) return fail(ctx, CATEN_B200_EINVAL, "kv4_attention: NULL argument");
+  if (((uintptr_t)d_pool | (uintptr_t)d_work) % 16) return fail(ctx, CATEN_B200_EINVAL, "kv4_attention: pool and workspace have to start on a multiple of 16 bytes");
+  if (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_table | (uintptr_t)d_lengths | (uintptr_t)d_starts) % 4) return fail(ctx, CATEN_B200_EINVAL, "kv4_attention: misaligned pointer");
+  if (!ctx) return fail(nullptr, CATEN_B200_EINVAL, "kv4_attention: ctx is NULL");
+  cudaSetDevice(ctx->device);
+  ctx->work_outside = true;
+  if (!batch || !rows) return 0;
+  ProfScope prof(ctx, max_new == 1 ? CATEN_B200_K_ATTN_DECODE : CATEN_B200_K_ATTN_PREFILL);
+  Kv4AttnArgs a = {};
+  kv4_check(ctx, "kv4_attention", desc, &a.s);
+  a.q = d_q; a.ldq = ldq; a.rows = rows;
+  a.pool = (const uint8_t *)d_pool;
+  a.table = d_table; a.lengths = d_lengths; a.starts = d_starts;
+  a.out = d_out; a.part = (float *)d_work; a.status = ctx->d_status;
+  a.heads = desc->heads; a.group = desc->heads / desc->kv_heads;
+  a.max_pages = (int)max_pages; a.max_new = (int)max_new; a.max_length = (int)max_length; a.batch = (int)batch;
+  a.row_tiles = p.row_tiles; a.parts = p.parts; a.part_tokens = p.part_tokens;
+  a.scale = desc->scale;
+  const bool q41 = a.s.q41;
+  switch (desc->dim / 64) {
+    case 1: return q41 ? kv4_attention_launch<1, true>(ctx, a, p.units) : kv4_attention_launch<1, false>(ctx, a, p.units);
+    case 2: return q41 ? kv4_attention_launch<2, true>(ctx, a, p.units) : kv4_attention_launch<2, false>(ctx, a, p.units);
+    case 3: return q41 ? kv4_attention_launch<3, true>(ctx, a, p.units) : kv4_attention_launch<3, false>(ctx, a, p.units);
+    default: return q41 ? kv4_attention_launch<4, true>(ctx, a, p.units) : kv4_attention_launch<4, false>(ctx, a, p.units);
+  }
+}
+
+}  // extern "C"

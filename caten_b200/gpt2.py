@@ -14,7 +14,7 @@ from typing import Optional
 import numpy as np
 
 from . import _lib as L
-from .model import Model, generate
+from .model import Model, beam_search, generate
 from .runtime import B200Buffer, B200Runtime, B200Weight
 from .synthetic import GPT2_SIZES, GPT2Params, Packed
 
@@ -128,11 +128,17 @@ class GPT2(Model):
 
     def kv_cache(self, layer: int):
         """(k, v) of one layer as numpy arrays [batch, heads, max_seq_len, 64]."""
+        k, v = self._kv(layer)
+        return k.numpy(), v.numpy()
+
+    def _kv(self, layer: int):
         k, v = C.c_void_p(), C.c_void_p()
         L.check(self.rt.ctx, self.rt.lib.caten_b200_gpt2_kv(self._h, layer, C.byref(k), C.byref(v)))
         shp = (self.batch, self.params.n_heads, self.max_seq_len, 64)
-        return (B200Buffer(self.rt, k.value, shp, np.float32, owned=False).numpy(),
-                B200Buffer(self.rt, v.value, shp, np.float32, owned=False).numpy())
+        return B200Buffer(self.rt, k.value, shp, np.float32, owned=False), B200Buffer(self.rt, v.value, shp, np.float32, owned=False)
+
+    def _caches(self) -> list:
+        return [c for layer in range(self.params.n_layers) for c in self._kv(layer)]
 
     @property
     def launch_count(self) -> int:
@@ -167,6 +173,7 @@ def make_gpt2(model_type, state_dict: dict, runtime: Optional[B200Runtime] = Non
     return GPT2(rt, params, state_dict, max_seq_len=max_seq_len, batch=batch, precision=precision, **kw)
 
 
+gpt2_beam_search = beam_search
 gpt2_generate = generate   # `gpt2-generate` (apps/gpt2/gpt2.lisp:97-113) without the tokenizer
 
 

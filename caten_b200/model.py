@@ -29,6 +29,10 @@ class Model:
     def _logits_ptr(self) -> int:
         raise NotImplementedError
 
+    def _caches(self) -> list:
+        """Device arrays [batch, heads, max_seq_len, head], one row a sequence: what beam search moves with its hypotheses."""
+        raise NotImplementedError(f"{type(self).__name__} keeps states that beam search cannot move")
+
     # -- one step from host ids: the call a token loop makes --
     def forward(self, x, s: Optional[int] = None, n: int = 0) -> np.ndarray:
         """x: [batch, s] token ids (any numeric dtype) at positions n ..; returns int64 [batch]: argmax of
@@ -71,6 +75,10 @@ class Model:
         ids.close()
         return out
 
+    def reorder(self, parents: B200Buffer, positions: int) -> None:
+        """Sequence i of each group of ``parents`` [groups, beams] goes on from what sequence parents[i] was, ``positions`` tokens long."""
+        self.rt.beam_reorder(self._caches(), parents, positions)
+
 
 def generate(model: Model, prompt_ids, max_length: int = 100, temperature: float = 0.0, top_k: int = 0, seed: int = 0) -> np.ndarray:
     """`gpt2-generate` (apps/gpt2/gpt2.lisp:97-113) on token ids: the first call feeds the whole
@@ -89,3 +97,44 @@ def generate(model: Model, prompt_ids, max_length: int = 100, temperature: float
         start_pos = tokens.shape[1]
         tokens = np.concatenate([tokens, out.reshape(-1, 1)], axis=1)
     return tokens
+
+
+def beam_search(model: Model, prompt_ids, beams: int, max_length: int = 100, eos: int = -1):
+    """The ``beams`` most probable continuations that a beam of that width finds, for each prompt; beyond the reference, whose loop is
+    greedy (apps/gpt2/gpt2.lisp:97-113).  prompt_ids [model.batch / beams, s]; returns (tokens [prompts, beams, s + max_length], scores [prompts,
+    beams]: sums of log probabilities), best first.  A hypothesis that has produced ``eos`` keeps its score and repeats it.  Everything stays on
+    the device; the host traces the hypotheses back at the end."""
+    if beams <= 0 or model.batch % beams:
+        raise ValueError(f"beam_search: {beams} beams over a batch of {model.batch}")
+    rt, groups = model.rt, model.batch // beams
+    prompt = np.ascontiguousarray(prompt_ids, dtype=np.int64).reshape(groups, -1)
+    n = prompt.shape[1]
+    if max_length <= 0:
+        return np.repeat(prompt[:, None], beams, 1), np.zeros((groups, beams), np.float32)
+    caches = model._caches()
+    model.forward(np.repeat(prompt, beams, 0), n, 0)
+    first = np.full((groups, beams), -np.inf, np.float32)   # the hypotheses of a prompt are still one
+    first[:, 0] = 0.0
+    shape = (groups, beams)
+    scores = [rt.transfer_from_array(first), rt.open_buffer(shape, np.float32)]
+    ended = [rt.open_buffer(shape, np.uint8), rt.open_buffer(shape, np.uint8)]
+    parents, tokens = rt.open_buffer((max_length,) + shape, np.int32), rt.open_buffer((max_length,) + shape, np.int64)
+    unused = rt.open_buffer((model.batch,), np.int64)
+    work = rt.open_buffer(rt.beam_select_work(groups, beams, model.vocab_size, beams), np.uint8)
+    for i in range(max_length):
+        at = i * model.batch
+        out = scores[(i + 1) % 2], parents.view(at, shape), tokens.view(at, shape), ended[(i + 1) % 2]
+        rt.beam_select(model._logits_buffer(), scores[i % 2], beams, ended=ended[i % 2] if eos >= 0 else None, eos=eos, out=out, work=work)
+        if i + 1 < max_length:
+            rt.beam_reorder(caches, out[1], n)
+            model.forward_device(tokens.view(at, (model.batch, 1)), 1, n, unused)
+            n += 1
+    p, t, s = parents.numpy(), tokens.numpy(), scores[max_length % 2].numpy()
+    for b in (*scores, *ended, parents, tokens, unused, work):
+        b.close()
+    found = np.empty((groups, beams, max_length), np.int64)
+    rows, beam = np.arange(groups)[:, None], np.repeat(np.arange(beams)[None], groups, 0)
+    for i in range(max_length - 1, -1, -1):
+        found[:, :, i] = t[i][rows, beam]
+        beam = p[i][rows, beam]
+    return np.concatenate([np.repeat(prompt[:, None], beams, 1), found], axis=2), s

@@ -268,3 +268,137 @@ class B200Runtime:
         out = self.open_buffer((rows,), np.int64)
         L.check(self.ctx, self.lib.caten_b200_sample(self.ctx, logits.ptr, rows, V, float(temperature), int(top_k), u.ptr, out.ptr))
         return out
+
+    # ---- beam search ----
+    def beam_select_work(self, batch: int, beams: int, V: int, keep: int) -> int:
+        """Bytes of workspace that a ``beam_select`` of these sizes needs."""
+        n = self.lib.caten_b200_beam_select_work(batch, beams, V, keep)
+        if n < 0:
+            L.check(None, L.EINVAL)
+        return n
+
+    def beam_select(self, logits: B200Buffer, scores: B200Buffer, keep: int, ended: Optional[B200Buffer] = None, eos: int = -1, out=None,
+                    work: Optional[B200Buffer] = None):
+        """The ``keep`` best continuations of each request's hypotheses (``caten_b200_beam_select``).  logits [batch * beams, V], scores
+        [batch, beams], ended [batch, beams] uint8; returns (scores, parents int32, tokens int64, ended uint8), each [batch, keep]."""
+        (B, beams), V = scores.shape, logits.shape[-1]
+        if int(np.prod(logits.shape[:-1], dtype=np.int64)) != B * beams or (ended is not None and ended.shape != scores.shape):
+            raise ValueError(f"beam_select: logits {logits.shape} and ended {ended and ended.shape} for scores {scores.shape}")
+        _kinds("beam_select", (logits, np.float32), (scores, np.float32), (ended, np.uint8))
+        need = self.beam_select_work(B, beams, V, keep)
+        out = out or tuple(self.open_buffer((B, keep), t) for t in (np.float32, np.int32, np.int64, np.uint8))
+        if any(b is not None and b.shape != (B, keep) for b in out):
+            raise ValueError(f"beam_select: outputs are [{B}, {keep}]")
+        _kinds("beam_select", *zip(out, (np.float32, np.int32, np.int64, np.uint8)))
+        own = None if work else self.open_buffer(need, np.uint8)
+        _room("beam_select", work or own, need)
+        L.check(self.ctx, self.lib.caten_b200_beam_select(self.ctx, logits.ptr, scores.ptr, ended.ptr if ended else None, B, beams, V, eos, keep,
+                                                          out[0].ptr, out[1].ptr, out[2].ptr, out[3].ptr if out[3] else None, (work or own).ptr))
+        if own:
+            own.close()   # (waits for the kernels)
+        return out
+
+    def beam_reorder(self, states: Sequence[B200Buffer], parents: B200Buffer, positions: int) -> None:
+        """Rows of caches [batch * beams, H, T, X] become those of their parents [batch, beams], in place, the first ``positions`` of T
+        (``caten_b200_beam_reorder``)."""
+        if not states:
+            return
+        groups, beams = parents.shape
+        n, H, T, X = states[0].shape
+        size = states[0].dtype.itemsize
+        if n != groups * beams or not 0 <= positions <= T or any(b.shape != states[0].shape or b.dtype != states[0].dtype for b in states):
+            raise ValueError(f"beam_reorder: states like {states[0].shape}, {positions} positions, parents {parents.shape}")
+        _kinds("beam_reorder", (parents, np.int32))
+        arr = (C.c_void_p * len(states))(*[b.ptr for b in states])
+        L.check(self.ctx, self.lib.caten_b200_beam_reorder(self.ctx, arr, len(states), parents.ptr, groups, beams, H, T * X * size, positions * X * size))
+
+    def beam_reorder_pages(self, pool: B200Buffer, table: B200Buffer, lengths: B200Buffer, parents: B200Buffer, page: int) -> None:
+        """The same for sequences in pages: ``pool`` [pages, bytes or values of a page], ``table`` [batch * beams, max_pages]
+        (``caten_b200_beam_reorder_pages``)."""
+        groups, beams = parents.shape
+        if len(pool.shape) != 2 or table.shape[0] != groups * beams or lengths.shape != (groups * beams,):
+            raise ValueError(f"beam_reorder_pages: pool {pool.shape}, table {table.shape}, lengths {lengths.shape}, parents {parents.shape}")
+        _kinds("beam_reorder_pages", (table, np.int32), (lengths, np.int32), (parents, np.int32))
+        L.check(self.ctx, self.lib.caten_b200_beam_reorder_pages(self.ctx, pool.ptr, pool.shape[0], pool.shape[1] * pool.dtype.itemsize, table.ptr, table.shape[1],
+                                                                 lengths.ptr, page, parents.ptr, groups, beams))
+
+    # ---- key/value cache of 4-bit blocks in pages ----
+    def kv4_pool(self, desc: L.Kv4Desc) -> B200Buffer:
+        """A pool for ``desc``: [pages, bytes of a page]."""
+        n = self.lib.caten_b200_kv4_nbytes(C.byref(desc))
+        if n < 0:
+            L.check(None, L.EINVAL)
+        return self.open_buffer((desc.pages, n // desc.pages), np.uint8)
+
+    def kv_pages(self, have: B200Buffer, want: B200Buffer, page: int, table: B200Buffer, free: B200Buffer, state: B200Buffer, starts: B200Buffer,
+                 slots: B200Buffer) -> None:
+        """Pages and slots for requests that go from ``have`` to ``want`` tokens (``caten_b200_kv_pages``); all int32, ``state`` [4] as there."""
+        n = have.shape[0]
+        if have.shape != (n,) or want.shape != (n,) or table.shape[0] != n or starts.shape != (n + 1,) or state.shape != (4,):
+            raise ValueError(f"kv_pages: have {have.shape}, want {want.shape}, table {table.shape}, starts {starts.shape}, state {state.shape}")
+        _kinds("kv_pages", *((b, np.int32) for b in (have, want, table, free, state, starts, slots)))
+        L.check(self.ctx, self.lib.caten_b200_kv_pages(self.ctx, have.ptr, want.ptr, n, page, table.ptr, table.shape[1], free.ptr, free.shape[0], state.ptr,
+                                                       starts.ptr, slots.ptr, slots.shape[0]))
+
+    def kv4_store(self, desc: L.Kv4Desc, pool: B200Buffer, k: B200Buffer, v: B200Buffer, slots: B200Buffer, ld: Optional[int] = None) -> None:
+        """Rows k, v [tokens, kv_heads * dim] into the slots of a cache (``caten_b200_kv4_store``).  ``ld``: floats between rows, for
+        views of a wider matrix."""
+        self._kv4_rows("kv4_store", desc, pool, k, v, slots)
+        L.check(self.ctx, self.lib.caten_b200_kv4_store(self.ctx, C.byref(desc), pool.ptr, k.ptr, v.ptr, ld or k.shape[-1], slots.ptr, slots.shape[0]))
+
+    def kv4_load(self, desc: L.Kv4Desc, pool: B200Buffer, slots: B200Buffer, k: Optional[B200Buffer] = None, v: Optional[B200Buffer] = None,
+                 ld: Optional[int] = None):
+        """Rows (k, v) that the slots of a cache hold, as fp32 (``caten_b200_kv4_load``)."""
+        shape = (slots.shape[0], desc.kv_heads * desc.dim)
+        k, v = k or self.open_buffer(shape), v or self.open_buffer(shape)
+        self._kv4_rows("kv4_load", desc, pool, k, v, slots)
+        L.check(self.ctx, self.lib.caten_b200_kv4_load(self.ctx, C.byref(desc), pool.ptr, slots.ptr, slots.shape[0], k.ptr, v.ptr, ld or k.shape[-1]))
+        return k, v
+
+    def _kv4_rows(self, who, desc, pool, k, v, slots):
+        shape = (slots.shape[0], desc.kv_heads * desc.dim)
+        if k.shape != shape or v.shape != shape:
+            raise ValueError(f"{who}: k {k.shape} and v {v.shape}, expected {shape}")
+        _kinds(who, (k, np.float32), (v, np.float32), (slots, np.int32))
+        _room(who, pool, self.lib.caten_b200_kv4_nbytes(C.byref(desc)))
+
+    def kv4_attention_work(self, desc: L.Kv4Desc, batch: int, rows: int, max_new: int, max_length: int) -> int:
+        """Bytes of workspace that a ``kv4_attention`` of these sizes needs."""
+        n = self.lib.caten_b200_kv4_attention_work(C.byref(desc), batch, rows, max_new, max_length)
+        if n < 0:
+            L.check(None, L.EINVAL)
+        return n
+
+    def kv4_attention(self, desc: L.Kv4Desc, q: B200Buffer, pool: B200Buffer, table: B200Buffer, lengths: B200Buffer, starts: Optional[B200Buffer] = None,
+                      max_new: int = 1, max_length: int = 0, out: Optional[B200Buffer] = None, work: Optional[B200Buffer] = None) -> B200Buffer:
+        """Attention of rows q [rows, >= heads * dim] over a paged 4-bit cache (``caten_b200_kv4_attention``): sequence b has ``lengths[b]`` tokens, its
+        last are the rows starts[b] .. starts[b + 1] (None: row b).  ``max_length`` 0: whatever the table holds."""
+        B, rows = lengths.shape[0], q.shape[0]
+        width = desc.heads * desc.dim
+        max_length = max_length or table.shape[1] * desc.page
+        if lengths.shape != (B,) or table.shape[0] != B or (starts is not None and starts.shape != (B + 1,)) or len(q.shape) != 2 or q.shape[1] < width:
+            raise ValueError(f"kv4_attention: q {q.shape}, lengths {lengths.shape}, table {table.shape}, starts {starts and starts.shape}")
+        need = self.kv4_attention_work(desc, B, rows, max_new, max_length)
+        out = out or self.open_buffer((rows, width))
+        if out.shape != (rows, width):
+            raise ValueError(f"kv4_attention: out {out.shape}, expected {(rows, width)}")
+        _kinds("kv4_attention", (q, np.float32), (out, np.float32), (table, np.int32), (lengths, np.int32), (starts, np.int32))
+        _room("kv4_attention", pool, self.lib.caten_b200_kv4_nbytes(C.byref(desc)))
+        own = None if work else self.open_buffer(need, np.uint8)
+        _room("kv4_attention", work or own, need)
+        L.check(self.ctx, self.lib.caten_b200_kv4_attention(self.ctx, C.byref(desc), q.ptr, q.shape[1], pool.ptr, table.ptr, table.shape[1], lengths.ptr,
+                                                            starts.ptr if starts else None, B, rows, max_new, max_length, out.ptr, (work or own).ptr))
+        if own:
+            own.close()   # (waits for the kernels)
+        return out
+
+
+def _kinds(who, *pairs):
+    for b, kind in pairs:
+        if b is not None and b.dtype != kind:
+            raise ValueError(f"{who}: a buffer of {b.dtype} where {np.dtype(kind)} is expected")
+
+
+def _room(who, buf, need):
+    if buf.nbytes < need:
+        raise ValueError(f"{who}: a buffer of {buf.nbytes} bytes where {need} are needed")

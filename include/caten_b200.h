@@ -239,6 +239,80 @@ int caten_b200_rmsnorm(caten_b200_ctx *ctx, const float *d_x, const float *d_wei
 int caten_b200_rope(caten_b200_ctx *ctx, const float *d_x, float *d_y, int64_t B, int64_t S, int64_t H,
                     int64_t head_dim, float base, int64_t pos0);
 
+/* ---- beam search -----------------------------------------------------------------------------------
+ * (No counterpart in the reference, whose generate loop is greedy, apps/gpt2/gpt2.lisp:97-113.)
+ * One step of `batch` requests with `beams` hypotheses each: d_logits [batch * beams, V], d_scores [batch, beams] the hypotheses' sums of
+ * log probabilities so far.  Candidate (beam b, token v) has the value score_b + x_v - log(sum exp(x)); a hypothesis whose d_ended byte is not 0
+ * (NULL: none) has one candidate, (b, eos) with the value score_b, and its logits are not read.  Writes the `keep` candidates of largest value,
+ * equal ones in the order of b * V + v: values rounded to fp32, the beam each goes on from, its token, and (d_out_ended not NULL) whether it has
+ * ended.  The order is decided in 64 bits.  Candidates whose value is -inf or NaN (masked tokens, hypotheses with score -inf, rows with a NaN
+ * or +inf) are never taken; place i that none is left for has score -inf, parent min(i, beams - 1) and token eos (0 without one).
+ * beams, keep <= 32; batch * beams <= 65535; eos < 0: none (d_ended NULL).  Outputs [batch, keep]; they do not overlap the inputs.
+ * d_work: beam_select_work(..) bytes, 8-byte aligned, nothing of which is kept from call to call; calls that may overlap on the GPU need one
+ * each.  beam_select_work is -1 for a call that would be refused. */
+int64_t caten_b200_beam_select_work(int64_t batch, int64_t beams, int64_t V, int64_t keep);
+int caten_b200_beam_select(caten_b200_ctx *ctx, const float *d_logits, const float *d_scores, const uint8_t *d_ended, int64_t batch, int64_t beams,
+                           int64_t V, int64_t eos, int64_t keep, float *d_out_scores, int32_t *d_out_parents, int64_t *d_out_tokens,
+                           uint8_t *d_out_ended, void *d_work);
+/* States follow: in each of `count` arrays (h_states: host array of device pointers, none overlapping) [groups * beams, planes, plane_stride bytes],
+ * row i of a group becomes what row d_parents[group, i] was, in place, the first `nbytes` of each plane (a KV cache [.., H, T, 64]: planes H,
+ * stride 256 T, nbytes 256 times the positions in use).  Any parents are allowed, the same one many times; one outside [0, beams) leaves its row as
+ * it was and is reported (CATEN_B200_EDEVICE) by the next synchronising call.  Multiples of 4 bytes (16 are faster); beams <= 32,
+ * count <= 1024. */
+int caten_b200_beam_reorder(caten_b200_ctx *ctx, void *const *h_states, int64_t count, const int32_t *d_parents, int64_t groups, int64_t beams,
+                            int64_t planes, int64_t plane_stride, int64_t nbytes);
+/* The same for a cache in pages, of any format: the pages of sequence i, d_table [groups * beams, max_pages] up to its d_lengths [groups * beams]
+ * tokens of `page` a page, become what its parent's were.  A sequence is at most as long as its parent; no page has two places in the table.
+ * A page number outside [0, pages) is skipped and reported.  d_pool 16-byte aligned, page_nbytes a multiple of 16. */
+int caten_b200_beam_reorder_pages(caten_b200_ctx *ctx, void *d_pool, int64_t pages, int64_t page_nbytes, const int32_t *d_table, int64_t max_pages,
+                                  const int32_t *d_lengths, int64_t page, const int32_t *d_parents, int64_t groups, int64_t beams);
+
+/* ---- key/value cache of 4-bit blocks, in pages ------------------------------------------------------
+ * (No counterpart in the reference, whose cache is one fp32 array per layer, external/llm/layers.lisp:25-26.)  For hosts with requests of
+ * different lengths that come and go: a pool of pages of `page` tokens, a table of page numbers for every request, and keys and values in
+ * blocks of 32 dims with the codes of the weight formats Q4_0 (18 bytes) or Q4_1 (20 bytes).  A step is kv_pages (tables and slots for
+ * the tokens to come), then for every layer kv4_store and kv4_attention.
+ *
+ * kv_pages: requests hold pages for d_have[r] tokens and are to hold them for d_want[r] (both [requests], not written).  Table d_table
+ * [requests, max_pages] of page numbers, -1 behind a request's last; free pages d_free [pages], their number in d_state[0].  Requests that
+ * shrink (to 0: that end) give their last pages back, appended to the free ones in order; requests that grow take pages from the end of the list.
+ * d_starts [requests + 1]: where each request's new tokens begin among all new tokens (request by request, by position); d_slots [max_tokens]: page
+ * * page size + place in the page of every new token, -1 behind the last.  d_state [4]: free pages, new tokens, pages that were missing, and
+ * what was wrong: 1 a length below 0 or beyond max_pages, 2 more new tokens than max_tokens, 3 more free pages than the pool has.  If either
+ * of the last two is not 0, nothing changed, all starts are 0 and all slots -1.  Asynchronous: the host reads d_state when it wants. */
+int caten_b200_kv_pages(caten_b200_ctx *ctx, const int32_t *d_have, const int32_t *d_want, int64_t requests, int64_t page, int32_t *d_table,
+                        int64_t max_pages, int32_t *d_free, int64_t pages, int32_t *d_state, int32_t *d_starts, int32_t *d_slots, int64_t max_tokens);
+typedef struct {
+  int32_t heads, kv_heads, dim;   /* query head h reads key/value head h / (heads / kv_heads); dim 64, 128, 192 or 256 */
+  int32_t type;                   /* CATEN_B200_Q4_0 or CATEN_B200_Q4_1 */
+  int32_t page;                   /* tokens a page: 16, 32, 64 or 128 */
+  float scale;                    /* of q . k */
+  int64_t pages;                  /* in the pool; pages * page < 2^31 */
+} caten_b200_kv4_desc;
+/* Bytes of a pool (page p: the bytes [p, p + 1) * nbytes / pages; csrc/kv4_layout.h has the order inside); -1 for a description that is refused. */
+int64_t caten_b200_kv4_nbytes(const caten_b200_kv4_desc *desc);
+/* Rows into the cache: d_k, d_v [tokens, kv_heads * dim] fp32, rows ld floats apart (parts of a qkv matrix); row i goes to slot d_slots[i], -1 nowhere.
+ * Slots of a call are distinct; one outside the pool is skipped and reported (CATEN_B200_EDEVICE) by the next synchronising call.  Per block of 32:
+ *   Q4_0  d = x / -8 of the value x of largest magnitude (the first of equal ones), code = min(15, trunc(x / d + 8.5)), value d (code - 8)
+ *   Q4_1  d = (max - min) / 15, code = min(15, trunc((x - min) / d + 0.5)), value d code + min
+ * with d and min rounded to fp16 in the cache, the codes decided from unrounded ones in 64 bits. */
+int caten_b200_kv4_store(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, void *d_pool, const float *d_k, const float *d_v, int64_t ld,
+                         const int32_t *d_slots, int64_t tokens);
+/* Rows out of the cache, as the fp32 values they stand for; rows of slot -1 are left as they were. */
+int caten_b200_kv4_load(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, const void *d_pool, const int32_t *d_slots, int64_t tokens, float *d_k,
+                        float *d_v, int64_t ld);
+/* Attention over the cache.  Sequence b holds d_lengths[b] tokens, its last ones (those of this step, stored already) are the rows [d_starts[b],
+ * d_starts[b + 1]) of d_q [rows, ldq] (heads * dim columns used) and of d_out [rows, heads * dim]: a row sees its own token and all before it.
+ * d_starts NULL: one row a sequence, row b (rows == batch).  A row that sees nothing (a sequence of length 0, or shorter than its rows) is 0; rows of no
+ * sequence are left as they were.  max_new: rows of a sequence at most; max_length: bound of the lengths, at most max_pages * page.  Arithmetic: codes are
+ * exact operands of tensor-core products, q and the probabilities are split in two fp16 halves (2^-22), sums and softmax fp32.
+ * Lengths, starts or page numbers outside what the call allows are cut or skipped and reported (CATEN_B200_EDEVICE) by the next synchronising call.
+ * d_work: kv4_attention_work(..) bytes, 16-byte aligned, nothing of which is kept from call to call; calls that may overlap on the GPU need one each. */
+int64_t caten_b200_kv4_attention_work(const caten_b200_kv4_desc *desc, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length);
+int caten_b200_kv4_attention(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, const float *d_q, int64_t ldq, const void *d_pool,
+                             const int32_t *d_table, int64_t max_pages, const int32_t *d_lengths, const int32_t *d_starts, int64_t batch, int64_t rows,
+                             int64_t max_new, int64_t max_length, float *d_out, void *d_work);
+
 /* ---- whole GPT-2 step ---------------------------------------------------------------------------
  * Replaces one `(forward runtime (x . tokens) (s . len) (n . start-pos))` of
  * apps/gpt2/gpt2.lisp:104 on the GraphRuntime built by make-gpt2 (gpt2.lisp:82-93): the whole

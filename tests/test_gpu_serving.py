@@ -1,0 +1,692 @@
+"""GPU tests of the serving operators (pages and slots, 4-bit rows, attention over them, beam selection, reordering) against the plain
+statements in oracle/serving_ref.py, at the sizes and masks where each can go wrong, and of a run of them together.
+
+Tolerances.  Attention: u = 2^-23 a rounding (tensor-core sums may cut instead of round: a whole step).  A score is a sum over blocks of
+d (sum q code + 8 sum q) with q in two halves (2^-22): its error is at most scale * sum |q| |d| (code + 8) * (16 + 16 + 16 + 16 + 4 + n blocks)
+roundings of that magnitude, 80 u with room for the factors' own; probabilities then err by twice that relatively (numerator and sum), and the
+second product, likewise a sum of d (code + 8)-sized terms, by (80 + tokens / 16) u of sum p |d| (code + 8) <= 23 max |d|.  Q4_1 has minima in the place
+of 8 d.  Everything else (stores, pages, choices, moves) is exact."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from caten_b200 import _lib as L
+from caten_b200 import synthetic as S
+from caten_b200._lib import B200Error
+from oracle import serving_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"q4_0": L.Q4_0, "q4_1": L.Q4_1}
+
+
+def rng_of(*seed):
+    return np.random.Generator(np.random.PCG64(abs(hash(seed)) % (1 << 32) if any(isinstance(s, str) for s in seed) else list(seed)))
+
+
+def put(rt, a, kind=None):
+    return rt.transfer_from_array(np.ascontiguousarray(a, kind))
+
+
+# ---- pages and slots ------------------------------------------------------------------------------
+def run_pages(rt, have, want, page, table, free, n_free, max_tokens):
+    n = len(have)
+    b = dict(have=put(rt, have, np.int32), want=put(rt, want, np.int32), table=put(rt, table, np.int32), free=put(rt, free, np.int32),
+             state=put(rt, [n_free, 7, 7, 7], np.int32), starts=put(rt, np.full(n + 1, 99), np.int32), slots=put(rt, np.full(max_tokens, 99), np.int32))
+    rt.kv_pages(b["have"], b["want"], page, b["table"], b["free"], b["state"], b["starts"], b["slots"])
+    return [b[k].numpy() for k in ("table", "free", "state", "starts", "slots")]
+
+
+def some_pages(rng, n, page, longest, pool=None):
+    have = rng.integers(0, longest + 1, n)
+    have[rng.random(n) < 0.3] = 0
+    want = np.where(rng.random(n) < 0.4, have + 1, rng.integers(0, longest + 2, n))
+    want[rng.random(n) < 0.2] = 0
+    columns = longest // page + 2
+    pool = pool or n * columns + 3
+    order = rng.permutation(pool)
+    table, at = np.full((n, columns), -1), 0
+    for r in range(n):
+        c = -(-have[r] // page)
+        table[r, :c] = order[at:at + c]
+        at += c
+    free = np.full(pool, -1)
+    free[:pool - at] = order[at:]
+    return have, want, columns, table, free, pool - at
+
+
+@pytest.mark.parametrize("n,page,longest", [(1, 16, 40), (2, 64, 1), (31, 16, 700), (33, 128, 300), (64, 64, 1000), (1024, 16, 90), (2500, 32, 100), (3, 16, 30000)])
+def test_pages_against_the_plain_plan(rt, n, page, longest):
+    rng = rng_of(n, page, longest)
+    have, want, columns, table, free, n_free = some_pages(rng, n, page, longest)
+    tokens = int(np.maximum(want - have, 0).sum())
+    for spare in (0, 5):
+        got = run_pages(rt, have, want, page, table, free, n_free, tokens + spare)
+        for g, w in zip(got, ref.pages(have, want, page, table, free, n_free, tokens + spare)):
+            np.testing.assert_array_equal(g, w)
+
+
+def test_pages_that_do_not_suffice_change_nothing(rt):
+    rng = rng_of(5)
+    have, want, columns, table, free, n_free = some_pages(rng, 40, 16, 200)
+    want = np.maximum(want, have) + 40
+    want = np.minimum(want, columns * 16)
+    tokens = int((want - have).sum())
+    takes = int((-(-want // 16) - -(-have // 16)).sum())
+    few = takes - 3                      # three pages are missing
+    bad = []
+    for change, why in ((lambda h, w: w.__setitem__(7, -1), 1), (lambda h, w: h.__setitem__(39, -5), 1), (lambda h, w: w.__setitem__(0, columns * 16 + 1), 1),
+                        (lambda h, w: w.__setitem__(0, 2**31 - 1), 1)):
+        h, w = have.copy(), want.copy()
+        change(h, w)
+        bad.append((h, w, n_free, tokens + 500, why, 0))
+    bad += [(have, want, few, tokens, 0, 3), (have, want, n_free, tokens - 1, 2, 0), (have, want, -1, tokens, 3, 0), (have, want, len(free) + 1, tokens, 3, 0)]
+    for h, w, free_now, room, why, missing in bad:
+        got = run_pages(rt, h, w, 16, table, free, free_now, room)
+        np.testing.assert_array_equal(got[0], table)
+        np.testing.assert_array_equal(got[1], free)
+        assert got[2].tolist() == [free_now, 0, missing, why]
+        assert (got[3] == 0).all() and (got[4] == -1).all()
+
+
+def test_pages_of_no_requests(rt):
+    got = run_pages(rt, [], [], 16, np.zeros((0, 3)), np.arange(9), 9, 4)
+    assert got[2].tolist() == [9, 0, 0, 0] and got[3].tolist() == [0] and (got[4] == -1).all()
+    got = run_pages(rt, [3], [3], 16, [[2, -1]], np.arange(9), 5, 0)
+    assert got[2].tolist() == [5, 0, 0, 0] and got[3].tolist() == [0, 0]
+
+
+# ---- rows -----------------------------------------------------------------------------------------
+def description(kind, dim, page, pages, heads, kv_heads, scale=None):
+    return L.Kv4Desc(heads=heads, kv_heads=kv_heads, dim=dim, type=TYPES[kind], page=page, pages=pages, scale=scale or dim ** -0.5)
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("dim,page,kv,tokens,extra,shift", [(64, 16, 1, 1, 0, 0), (64, 64, 25, 7, 64, 0), (128, 32, 3, 33, 1, 0), (192, 16, 2, 50, 0, 1), (256, 128, 1, 130, 4, 2)])
+def test_rows_in_and_out(rt, kind, dim, page, kv, tokens, extra, shift):
+    """Values, and the pool's bytes; rows of any stride and alignment, slots in any order, rows that go nowhere."""
+    rng = rng_of(dim, page, tokens)
+    cols, pages = kv * dim, -(-tokens // page) + 2
+    ld = 2 * cols + extra
+    x = rng.standard_normal(tokens * ld + shift, dtype=np.float32) * np.exp(rng.standard_normal(tokens * ld + shift, dtype=np.float32))
+    x = x.astype(np.float32)
+    rows = x[shift:].reshape(tokens, ld)
+    rows[0, :32] = 0.0                                     # a block of zeros
+    rows[0, 32:64] = 1e-9                                  # whose scale is none in 16 bits
+    rows[-1, cols:cols + 32] = np.tile([3.0, -3.0], 16)    # equal magnitudes
+    rows[-1, :32] = np.arange(32) / 31 * 15                # codes' own values, and halves of steps
+    rows[tokens // 2, :32] = np.arange(32) / 2 - 8
+    rows[tokens // 2, 32:64] = 7.25                        # one value only
+    slots = rng.permutation(pages * page)[:tokens]
+    if tokens > 5:
+        slots[3] = slots[tokens - 2] = -1
+    d = description(kind, dim, page, pages, kv, kv)
+    pool = rt.kv4_pool(d)
+    dx = put(rt, x)
+    rt.kv4_store(d, pool, dx.view(shift, (tokens, cols)), dx.view(shift + cols, (tokens, cols)), put(rt, slots, np.int32), ld=ld)
+    k, v = (put(rt, np.full((tokens, cols), 55.0), np.float32) for _ in range(2))
+    rt.kv4_load(d, pool, put(rt, slots, np.int32), k, v)
+    want_pool = np.zeros(pool.shape, np.uint8)
+    for got, part in ((k.numpy(), rows[:, :cols]), (v.numpy(), rows[:, cols:2 * cols])):
+        want = ref.values(part, kind == "q4_1")
+        np.testing.assert_array_equal(got[slots >= 0], want[slots >= 0])
+        assert (got[slots < 0] == 55.0).all()
+    for i, slot in enumerate(slots):
+        for h in range(kv if slot >= 0 else 0):
+            ref.put(want_pool, page, kv, dim, kind == "q4_1", slot, h, rows[i, h * dim:(h + 1) * dim], rows[i, cols + h * dim:cols + (h + 1) * dim])
+    np.testing.assert_array_equal(pool.numpy(), want_pool)   # the rest is as it was
+    # out again into rows of a wider matrix that cannot be written by 16 bytes
+    step = 2 * cols + 3
+    wide = put(rt, np.zeros(tokens * step + 1, np.float32))
+    rt.kv4_load(d, pool, put(rt, slots, np.int32), wide.view(1, (tokens, cols)), wide.view(1 + cols, (tokens, cols)), ld=step)
+    got = wide.numpy()[1:].reshape(tokens, step)
+    np.testing.assert_array_equal(got[slots >= 0][:, :2 * cols], np.concatenate([ref.values(rows[:, i:i + cols], kind == "q4_1") for i in (0, cols)], 1)[slots >= 0])
+    assert (got[:, 2 * cols:] == 0).all() and (got[slots < 0] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+def test_codes_next_to_a_border(rt, kind):
+    """Values half a step apart, moved by single roundings: the codes are those that 64 bits give."""
+    rng = rng_of(11)
+    steps = rng.integers(-8, 8, (4000, 64)) + 0.5
+    top = np.float32(2.0) ** rng.integers(-9, 9, (4000, 1)) * rng.choice([1.0, 1.3, 0.7], (4000, 1)).astype(np.float32)
+    x = (steps.astype(np.float32) * top).astype(np.float32)
+    x[:, 0::32] = -8 * top
+    x[:, 1::32] = 7 * top
+    x = np.nextafter(x, np.float32(1e30) * rng.integers(-1, 2, x.shape).astype(np.float32), dtype=np.float32)
+    x = np.where(rng.random(x.shape) < 0.3, np.nextafter(x, np.float32(-1e30)), x).astype(np.float32)
+    d = description(kind, 64, 16, 250, 1, 1)
+    pool = rt.kv4_pool(d)
+    slots = put(rt, np.arange(4000), np.int32)
+    rt.kv4_store(d, pool, put(rt, x), put(rt, -x), slots)
+    k, v = rt.kv4_load(d, pool, slots)
+    np.testing.assert_array_equal(k.numpy(), ref.values(x, kind == "q4_1"))
+    np.testing.assert_array_equal(v.numpy(), ref.values(-x, kind == "q4_1"))
+
+
+def test_rows_that_are_not_finite_or_too_large_stay_in_their_blocks(rt):
+    x = np.ones((4, 128), np.float32)
+    x[0, 5], x[1, 40], x[2, 70], x[3, 100] = np.nan, np.inf, -np.inf, 3e38
+    for kind in ("q4_0", "q4_1"):
+        d = description(kind, 128, 16, 1, 1, 1)
+        pool = rt.kv4_pool(d)
+        slots = put(rt, np.arange(4), np.int32)
+        rt.kv4_store(d, pool, put(rt, x), put(rt, x), slots)
+        for y in rt.kv4_load(d, pool, slots):
+            y = y.numpy().reshape(4, 4, 32)
+            hit = np.eye(4, dtype=bool)
+            assert not np.isfinite(y[hit]).all(1).any()     # each such block says so
+            assert (y[~hit] == 1.0).all() and not np.isnan(y[~hit]).any()
+        assert np.isnan(y[0, 0]).all()
+
+
+def test_slots_outside_the_pool_are_skipped_and_reported(rt):
+    d = description("q4_0", 64, 16, 3, 1, 1)
+    pool = rt.kv4_pool(d)
+    x = put(rt, np.ones((5, 64)), np.float32)
+    slots = put(rt, [0, 48, 47, -2, -2**31], np.int32)
+    rt.kv4_store(d, pool, x, x, slots)
+    with pytest.raises(B200Error) as e:
+        rt.sync()
+    assert e.value.code == L.EDEVICE and "bad index" in str(e.value)
+    out = [put(rt, np.zeros((5, 64)), np.float32) for _ in range(2)]
+    rt.kv4_load(d, pool, slots, *out)
+    with pytest.raises(B200Error):
+        rt.sync()
+    np.testing.assert_array_equal(out[0].numpy()[:, 0], [1, 0, 1, 0, 0])
+    rt.sync()
+
+
+# ---- attention ------------------------------------------------------------------------------------
+class Cache:
+    """A pool in which sequences' pages lie in no order, full of NaN where nothing was stored."""
+
+    def __init__(self, rt, rng, kind, dim, page, heads, kv, lengths, spare=2, k_scale=1.0, pages=None, scale=None):
+        count = [-(-n // page) for n in lengths]
+        columns = max(1, max(count, default=1)) + spare
+        pages = pages or sum(count) + 3
+        self.desc = description(kind, dim, page, pages, heads, kv, scale)
+        self.pool = rt.kv4_pool(self.desc)
+        L.check(rt.ctx, rt.lib.caten_b200_memset(rt.ctx, self.pool.ptr, 0xff, self.pool.nbytes))
+        order, at = rng.permutation(pages) if pages < 1e6 else np.arange(pages - 1, 0, -1), 0
+        self.table = np.full((len(lengths), columns), -1)
+        slots = []
+        for b, n in enumerate(lengths):
+            self.table[b, :count[b]] = order[at:at + count[b]]
+            at += count[b]
+            slots += [self.table[b, t // page] * page + t % page for t in range(n)]
+        total = len(slots)
+        k = rng.standard_normal((total, kv * dim), dtype=np.float32) * np.float32(k_scale)
+        v = rng.standard_normal((total, kv * dim), dtype=np.float32) * np.exp(rng.standard_normal((total, 1), dtype=np.float32))
+        if total:
+            rt.kv4_store(self.desc, self.pool, put(rt, k), put(rt, v), put(rt, slots, np.int32))
+        q41 = kind == "q4_1"
+        self.k, self.v = (ref.values(x, q41).reshape(total, kv, dim) for x in (k, v.astype(np.float32)))
+        self.lengths, self.first = list(lengths), np.concatenate([[0], np.cumsum(lengths)]).astype(int)
+        self.size = max([1e-3] + [np.abs(x).max() for x in (self.v,) if x.size])
+
+
+def bound(c, q, tokens):
+    """The stated tolerance: blocks' d (code + 8) is at most 3 (Q4_0) times their largest magnitude, minima included."""
+    u = 2.0 ** -23
+    if not c.k.size:
+        return 0.0
+    score = c.desc.scale * np.abs(q).reshape(-1, c.desc.dim).sum(1).max() * 3 * np.abs(c.k).max() * 80 * u
+    return (2 * score + (80 + tokens / 16) * u * 3) * c.size
+
+
+def check_attention(rt, c, q, news, extra_cols=0, rows_behind=0, starts=True, tol=None, max_length=0):
+    heads, dim = c.desc.heads, c.desc.dim
+    at = np.concatenate([[0], np.cumsum(news)]).astype(int)
+    rows = at[-1] + rows_behind
+    assert q.shape == (rows, heads, dim)
+    wide = np.zeros((rows, heads * dim + extra_cols), np.float32)
+    wide[:, :heads * dim] = q.reshape(rows, -1)
+    out = put(rt, np.full((rows, heads * dim), 77.0), np.float32)
+    rt.kv4_attention(c.desc, put(rt, wide), c.pool, put(rt, c.table, np.int32), put(rt, c.lengths, np.int32), put(rt, at, np.int32) if starts else None,
+                     max_new=max(1, max(news)), max_length=max_length, out=out)
+    got = out.numpy().reshape(rows, heads, dim)
+    for b, n in enumerate(c.lengths):
+        part = slice(c.first[b], c.first[b + 1])
+        want = ref.attention(q[at[b]:at[b + 1]], c.k[part], c.v[part], n, c.desc.scale)
+        np.testing.assert_allclose(got[at[b]:at[b + 1]], want, rtol=0, atol=tol or bound(c, q, n), err_msg=f"sequence {b} of {n}")
+    assert (got[at[-1]:] == 77.0).all()
+    return got
+
+
+LENGTHS = [1, 15, 16, 17, 0, 63, 64, 65, 130, 257]
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("dim,page,heads,kv", [(64, 64, 25, 25), (64, 16, 4, 1), (128, 32, 6, 2), (128, 128, 16, 2), (192, 16, 3, 3), (256, 64, 10, 1)])
+def test_single_tokens(rt, kind, dim, page, heads, kv):
+    rng = rng_of(dim, page, heads)
+    c = Cache(rt, rng, kind, dim, page, heads, kv, LENGTHS)
+    q = rng.standard_normal((len(LENGTHS), heads, dim), dtype=np.float32) * 2
+    check_attention(rt, c, q, [1] * len(LENGTHS), starts=False)
+    check_attention(rt, c, q, [1] * len(LENGTHS), extra_cols=5)
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("dim,page,heads,kv", [(64, 16, 4, 4), (64, 64, 5, 1), (128, 32, 8, 2), (192, 128, 2, 2), (256, 16, 3, 1)])
+def test_several_tokens_and_prompts(rt, kind, dim, page, heads, kv):
+    """Rows of their own number a sequence, over a history or none; sequences without rows, without tokens, with fewer tokens than rows;
+    rows behind the last sequence."""
+    rng = rng_of(dim, page, heads, 2)
+    lengths, news = [70, 33, 0, 100, 129, 3, 0, 40], [5, 33, 0, 0, 97, 7, 2, 1]
+    c = Cache(rt, rng, kind, dim, page, heads, kv, lengths)
+    q = rng.standard_normal((sum(news) + 3, heads, dim), dtype=np.float32)
+    check_attention(rt, c, q, news, rows_behind=3, extra_cols=64)
+
+
+@pytest.mark.parametrize("kind,dim,heads,kv,lengths,news", [("q4_0", 64, 2, 2, [5000], [1]), ("q4_1", 128, 8, 1, [4097, 1], [1, 1]), ("q4_0", 64, 2, 1, [3000, 2, 700], [9, 2, 1]),
+                                                            ("q4_1", 256, 1, 1, [2500], [1]), ("q4_0", 128, 4, 4, [1, 1, 2100], [1, 0, 3])])
+def test_long_histories_are_shared_out(rt, kind, dim, heads, kv, lengths, news):
+    rng = rng_of(dim, heads, 3)
+    c = Cache(rt, rng, kind, dim, 64, heads, kv, lengths, k_scale=0.5)
+    q = rng.standard_normal((sum(news), heads, dim), dtype=np.float32) * 2
+    check_attention(rt, c, q, news)
+    check_attention(rt, c, q, news, max_length=max(lengths))
+
+
+def test_results_are_the_same_every_time(rt):
+    rng = rng_of(21)
+    c = Cache(rt, rng, "q4_0", 64, 64, 4, 2, [3000, 65, 900])
+    q = rng.standard_normal((3, 4, 64), dtype=np.float32)
+    one = check_attention(rt, c, q, [1, 1, 1])
+    for _ in range(3):
+        np.testing.assert_array_equal(check_attention(rt, c, q, [1, 1, 1]), one)
+
+
+@pytest.mark.parametrize("k_scale,q_scale", [(1e-3, 1e3), (300.0, 1e-3), (30.0, 1.0), (1.0, 1e-30), (1.0, 0.0)])
+def test_scales_far_from_one(rt, k_scale, q_scale):
+    """Operands are brought into fp16's range by powers of two, whatever the sizes; sharp softmaxes pick single tokens."""
+    rng = rng_of(31)
+    for kind in ("q4_0", "q4_1"):
+        c = Cache(rt, rng, kind, 64, 32, 2, 1, [150], k_scale=k_scale)
+        q = rng.standard_normal((4, 2, 64), dtype=np.float32) * np.float32(q_scale)
+        check_attention(rt, c, q, [4])
+
+
+def test_values_of_very_different_sizes(rt):
+    """Tokens of large values with small probabilities beside small values with large ones."""
+    rng = rng_of(33)
+    for kind in ("q4_0", "q4_1"):
+        c = Cache(rt, rng, kind, 64, 16, 1, 1, [96])
+        k, v = c.k.reshape(96, 64).copy(), c.v.reshape(96, 64) * np.exp(3 * rng.standard_normal((96, 1))).astype(np.float32)
+        slots = [c.table[0, t // 16] * 16 + t % 16 for t in range(96)]
+        rt.kv4_store(c.desc, c.pool, put(rt, k), put(rt, v), put(rt, slots, np.int32))
+        c.k, c.v = (ref.values(x.astype(np.float32), kind == "q4_1").reshape(96, 1, 64) for x in (k, v))
+        c.size = np.abs(c.v).max()
+        check_attention(rt, c, rng.standard_normal((1, 1, 64), dtype=np.float32) * 2, [1])
+
+
+def test_nan_in_a_row_stays_in_it(rt):
+    rng = rng_of(35)
+    c = Cache(rt, rng, "q4_0", 64, 16, 2, 1, [40, 40])
+    q = rng.standard_normal((6, 2, 64), dtype=np.float32)
+    clean = check_attention(rt, c, q, [3, 3])
+    bad = q.copy()
+    bad[1, 0, 7], bad[5, 1, 0] = np.nan, np.inf
+    out = rt.kv4_attention(c.desc, put(rt, bad.reshape(6, -1)), c.pool, put(rt, c.table, np.int32), put(rt, c.lengths, np.int32), put(rt, [0, 3, 6], np.int32),
+                           max_new=3).numpy().reshape(6, 2, 64)
+    hit = np.zeros((6, 2), bool)
+    hit[1, 0] = hit[5, 1] = True
+    assert np.isnan(out[hit]).all()
+    np.testing.assert_array_equal(out[~hit], clean[~hit])
+
+
+def test_what_the_device_says_is_checked(rt):
+    """Page numbers, lengths and starts outside what the call allows: skipped or cut, reported by the next synchronising call; other sequences
+    are answered."""
+    rng = rng_of(37)
+    c = Cache(rt, rng, "q4_0", 64, 16, 2, 1, [40, 50, 20])
+    q = rng.standard_normal((3, 2, 64), dtype=np.float32)
+    clean = check_attention(rt, c, q, [1, 1, 1])
+    pages = c.desc.pages
+
+    def run(table=c.table, lengths=c.lengths, starts=(0, 1, 2, 3)):
+        out = put(rt, np.full((3, 128), 77.0), np.float32)
+        rt.kv4_attention(c.desc, put(rt, q.reshape(3, -1)), c.pool, put(rt, table, np.int32), put(rt, lengths, np.int32), put(rt, starts, np.int32), max_new=1, out=out)
+        with pytest.raises(B200Error) as e:
+            rt.sync()
+        assert e.value.code == L.EDEVICE
+        return out.numpy().reshape(3, 2, 64)
+    for wrong in (-1, pages, 2**31 - 1, -2**31):
+        t = c.table.copy()
+        t[1, 1] = wrong
+        got = run(table=t)
+        np.testing.assert_array_equal(got[[0, 2]], clean[[0, 2]])
+    for wrong in (-1, 2**31 - 1, c.table.shape[1] * 16 + 1):
+        got = run(lengths=[40, wrong, 20])
+        np.testing.assert_array_equal(got[[0, 2]], clean[[0, 2]])
+    for wrong in ([0, 1, 5, 3], [-1, 1, 2, 3], [0, 3, 2, 3], [0, 1, 1, 3]):
+        got = run(starts=wrong)
+        for b in range(3):
+            if wrong[b:b + 2] == [b, b + 1]:
+                np.testing.assert_array_equal(got[b], clean[b])
+    rt.sync()
+
+
+def test_pages_beyond_four_gigabytes(rt):
+    rng = rng_of(39)
+    pages = 5 * 2**30 // (128 * 2 * 64 * 18 // 32 * 4)
+    c = Cache(rt, rng, "q4_0", 64, 128, 4, 4, [300, 131], pages=pages)
+    c.table[0, :3] = [pages - 1, pages - 2, pages // 2]
+    c.table[1, :2] = [0, pages - 3]
+    slots = [c.table[b, t // 128] * 128 + t % 128 for b, n in enumerate(c.lengths) for t in range(n)]
+    k, v = (rng.standard_normal((431, 256), dtype=np.float32) for _ in range(2))
+    rt.kv4_store(c.desc, c.pool, put(rt, k), put(rt, v), put(rt, slots, np.int32))
+    got = rt.kv4_load(c.desc, c.pool, put(rt, slots, np.int32))
+    c.k, c.v = (ref.values(x, False).reshape(431, 4, 64) for x in (k, v))
+    np.testing.assert_array_equal(got[0].numpy(), c.k.reshape(431, 256))
+    np.testing.assert_array_equal(got[1].numpy(), c.v.reshape(431, 256))
+    check_attention(rt, c, rng.standard_normal((2, 4, 64), dtype=np.float32), [1, 1])
+    c.pool.close()
+
+
+# ---- beam selection -------------------------------------------------------------------------------
+def check_select(rt, logits, scores, keep, ended=None, eos=-1, shift=0):
+    groups, beams = scores.shape
+    V = logits.shape[-1]
+    flat = np.concatenate([np.zeros(shift, np.float32), logits.astype(np.float32).ravel()])
+    dx = put(rt, flat).view(shift, (groups * beams, V))
+    out = rt.beam_select(dx, put(rt, scores, np.float32), keep, ended=put(rt, ended, np.uint8) if ended is not None else None, eos=eos)
+    got = [b.numpy() for b in out]
+    for r in range(groups):
+        want = ref.select(logits.reshape(groups, beams, V)[r].astype(np.float32), scores[r].astype(np.float32), ended[r] if ended is not None else np.zeros(beams), eos, keep)
+        # a value is rounded once; its log of the sum is off by the exponentials' 2^-21 at most
+        fin = np.isfinite(want[0])
+        assert (got[0][r][~fin] == want[0][~fin]).all()
+        np.testing.assert_allclose(got[0][r][fin], want[0][fin], rtol=2.0 ** -23, atol=2.0 ** -21)
+        for g, w in zip(got[1:], want[1:]):
+            np.testing.assert_array_equal(g[r], w)
+    return got
+
+
+@pytest.mark.parametrize("groups,beams,V,keep", [(1, 1, 1, 1), (1, 1, 7, 3), (2, 3, 2, 8), (3, 4, 50257, 4), (2, 5, 32000, 10), (1, 32, 1003, 32), (7, 2, 8192, 31), (1, 16, 8189, 32),
+                                                 (1, 8, 130001, 16), (65, 1, 300, 2)])
+def test_selection(rt, groups, beams, V, keep):
+    rng = rng_of(groups, beams, V, keep)
+    logits = rng.standard_normal((groups, beams, V), dtype=np.float32) * 3
+    scores = -rng.random((groups, beams)).astype(np.float32) * 4
+    for shift in range(4):
+        check_select(rt, logits, scores, keep, shift=shift)
+    ended = rng.random((groups, beams)) < 0.4
+    check_select(rt, logits, scores, keep, ended=ended, eos=V // 2)
+    check_select(rt, logits, scores, keep, ended=np.ones((groups, beams), bool), eos=0)
+    first = np.where(np.arange(beams) == 0, 0.0, -np.inf) + np.zeros((groups, 1))
+    check_select(rt, logits, first, keep, ended=np.zeros((groups, beams), bool), eos=V - 1)
+
+
+def test_selection_of_equal_values_takes_the_lowest_index(rt):
+    beams, V = 3, 20000
+    flat = np.zeros((2, beams, V), np.float32)
+    check_select(rt, flat, np.zeros((2, beams)), 32)                       # everything is equal
+    check_select(rt, flat, np.array([[0, 1, 1], [-1, -1, 0]]), 20)
+    flat[:, :, 1::2] = -0.0                                                # (zeros of both signs)
+    check_select(rt, flat, np.zeros((2, beams)), 32)
+    rng = rng_of(41)
+    few = rng.integers(0, 3, (2, beams, V)).astype(np.float32)             # a few values, many times each
+    check_select(rt, few, np.zeros((2, beams)), 32)
+
+
+@pytest.mark.parametrize("order", ["up", "down"])
+def test_selection_from_sorted_logits(rt, order):
+    """The largest logits lie side by side, in one block's share."""
+    V = 30011
+    x = np.linspace(-6, 6, V, dtype=np.float32)[None, None].repeat(2, 1)
+    check_select(rt, x if order == "up" else x[:, :, ::-1].copy(), np.array([[0.0, -0.25]]), 32)
+
+
+def test_selection_with_masks(rt):
+    rng = rng_of(43)
+    V = 9001
+    x = rng.standard_normal((6, 4, V), dtype=np.float32)
+    x[0, :, 100:] = -np.inf                      # a short list of allowed ids
+    x[1, 1] = -np.inf                            # a hypothesis that cannot go on
+    x[2, :, :] = -np.inf                         # none can
+    x[2, 3, 8999] = 1.0
+    x[3] = -np.inf                               # nothing at all
+    x[4, 2, 17], x[4, 0, 5], x[4, 1] = np.nan, np.inf, np.finfo(np.float32).min   # rows without a distribution; the lowest value as a mask
+    x[5, :, ::2] = np.finfo(np.float32).min
+    scores = -rng.random((6, 4)).astype(np.float32)
+    scores[5] = [-np.inf, 0, np.nan, -1]
+    for keep in (1, 8, 32):
+        check_select(rt, x, scores, keep, ended=np.zeros((6, 4), bool), eos=3)
+        ended = np.zeros((6, 4), bool)
+        ended[2:4, 1] = True
+        check_select(rt, x, scores, keep, ended=ended, eos=3)
+
+
+def test_selection_leaves_the_logits_of_ended_hypotheses_alone_and_needs_no_flags_out(rt):
+    rng = rng_of(45)
+    x = rng.standard_normal((4, 500), dtype=np.float32)
+    x[1] = np.nan
+    out = rt.beam_select(put(rt, x), put(rt, [[-1, -2, -3, -4]], np.float32), 4, ended=put(rt, [[0, 1, 0, 0]], np.uint8), eos=7,
+                         out=(rt.open_buffer((1, 4)), rt.open_buffer((1, 4), np.int32), rt.open_buffer((1, 4), np.int64), None))
+    want = ref.select(x, np.array([-1, -2, -3, -4.0]), np.array([0, 1, 0, 0]), 7, 4)
+    np.testing.assert_array_equal(out[1].numpy()[0], want[1])
+    np.testing.assert_array_equal(out[2].numpy()[0], want[2])
+
+
+# ---- reordering -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("groups,beams,H,T,X,n,kind", [(1, 2, 1, 1, 64, 1, np.float32), (3, 4, 5, 40, 64, 17, np.float32), (2, 7, 2, 9, 3, 5, np.float32), (1, 16, 2, 33, 64, 33, np.float32),
+                                                       (2, 32, 1, 20, 16, 19, np.int32), (5, 1, 2, 4, 4, 4, np.float32), (2, 5, 3, 12, 8, 0, np.float32), (4, 9, 1, 6, 6, 6, np.float16)])
+def test_reordering(rt, groups, beams, H, T, X, n, kind):
+    rng = rng_of(groups, beams, H, T)
+    states = [(rng.standard_normal((groups * beams, H, T, X)) * 100).astype(kind) for _ in range(3)]
+    some = [rng.integers(0, beams, (groups, beams)), np.stack([rng.permutation(beams) for _ in range(groups)]), np.tile(np.roll(np.arange(beams), 1), (groups, 1)),
+            np.full((groups, beams), beams - 1), np.tile(np.arange(beams), (groups, 1))]
+    for parents in some:
+        b = [put(rt, x) for x in states]
+        rt.beam_reorder(b, put(rt, parents, np.int32), n)
+        source = (parents + np.arange(groups)[:, None] * beams).ravel()
+        for x, y in zip(states, b):
+            want = x.copy()
+            want[:, :, :n] = x[source][:, :, :n]
+            np.testing.assert_array_equal(y.numpy(), want)
+
+
+def test_reordering_many_states_in_one_call(rt):
+    """More than one launch's worth, at addresses of every alignment."""
+    rng = rng_of(51)
+    x = rng.standard_normal((301, 2 * 3 * 1 * 4 * 4 + 1), dtype=np.float32)
+    buf = put(rt, x)
+    states = [buf.view(i * x.shape[1], (6, 1, 4, 4)) for i in range(301)]
+    parents = np.array([[1, 2, 0], [2, 2, 2]])
+    rt.beam_reorder(states, put(rt, parents, np.int32), 3)
+    want = x[:, :-1].reshape(301, 6, 4, 4).copy()
+    want[:, :, :3] = x[:, :-1].reshape(301, 6, 4, 4)[:, [1, 2, 0, 5, 5, 5]][:, :, :3]
+    got = buf.numpy()
+    np.testing.assert_array_equal(got[:, :-1].reshape(301, 6, 4, 4), want)
+    np.testing.assert_array_equal(got[:, -1], x[:, -1])
+    rt.beam_reorder([], put(rt, parents, np.int32), 3)
+
+
+def test_parents_out_of_range_leave_rows_and_are_reported(rt):
+    x = np.arange(4 * 2 * 3 * 4, dtype=np.float32).reshape(4, 2, 3, 4)
+    for wrong in (-1, 4, 2**31 - 1, -2**31):
+        b = put(rt, x)
+        rt.beam_reorder([b], put(rt, [[1, wrong, 0, 2]], np.int32), 3)
+        with pytest.raises(B200Error) as e:
+            rt.sync()
+        assert e.value.code == L.EDEVICE
+        np.testing.assert_array_equal(b.numpy(), x[[1, 1, 0, 2]])
+
+
+@pytest.mark.parametrize("groups,beams,page,width,longest", [(1, 2, 16, 16, 5), (3, 4, 16, 4624, 100), (2, 8, 64, 48, 300), (1, 32, 32, 160, 64), (2, 13, 16, 32, 40)])
+def test_reordering_pages(rt, groups, beams, page, width, longest):
+    rng = rng_of(groups, beams, page)
+    columns, n = -(-longest // page) + 1, groups * beams
+    lengths = np.repeat(rng.integers(0, longest + 1, groups), beams)
+    lengths[:beams] = longest
+    pages = n * columns
+    pool = rng.integers(0, 256, (pages, width)).astype(np.uint8)
+    table = np.where(np.arange(columns) * page < lengths[:, None], rng.permutation(pages).reshape(n, columns), -1)
+    for parents in (rng.integers(0, beams, (groups, beams)), np.stack([rng.permutation(beams) for _ in range(groups)])):
+        b = put(rt, pool)
+        rt.beam_reorder_pages(b, put(rt, table, np.int32), put(rt, lengths, np.int32), put(rt, parents, np.int32), page)
+        want = pool.copy()
+        for i, p in enumerate((parents + np.arange(groups)[:, None] * beams).ravel()):
+            for j in range(-(-lengths[i] // page)):
+                want[table[i, j]] = pool[table[p, j]]
+        np.testing.assert_array_equal(b.numpy(), want)
+    # a page number that is none, in the second sequence of a pair
+    t, p = table.copy(), np.tile(np.arange(beams), (groups, 1))
+    t[1, 0], p[0, 0] = pages, 1
+    b = put(rt, pool)
+    rt.beam_reorder_pages(b, put(rt, t, np.int32), put(rt, lengths, np.int32), put(rt, p, np.int32), page)
+    with pytest.raises(B200Error):
+        rt.sync()
+    np.testing.assert_array_equal(b.numpy()[table[0, 1:][table[0, 1:] >= 0]], pool[table[1, 1:][table[1, 1:] >= 0]])
+
+
+# ---- together -------------------------------------------------------------------------------------
+def test_a_serving_loop(rt):
+    """Requests of their own lengths come, grow and end: every turn plans pages, stores its rows and attends, against caches that are kept
+    plainly on the host."""
+    rng = rng_of(61)
+    R, page, heads, kv, dim, pool_pages, columns = 5, 16, 4, 2, 64, 24, 8
+    for kind in ("q4_0", "q4_1"):
+        d = description(kind, dim, page, pool_pages, heads, kv)
+        pool = rt.kv4_pool(d)
+        table, free, state = put(rt, np.full((R, columns), -1), np.int32), put(rt, rng.permutation(pool_pages), np.int32), put(rt, [pool_pages, 0, 0, 0], np.int32)
+        starts, slots = rt.open_buffer((R + 1,), np.int32), rt.open_buffer((128,), np.int32)
+        kept = [np.zeros((0, 2, kv, dim), np.float32) for _ in range(R)]
+        lengths = np.zeros(R, int)
+        plan = [[20, 0, 5, 33, 0], [21, 16, 6, 34, 1], [22, 17, 0, 35, 2], [23, 18, 40, 20, 3], [0, 19, 41, 21, 4], [60, 20, 42, 22, 0], [61, 21, 43, 23, 9]]
+        for want in plan:
+            want = np.array(want)
+            before, after = put(rt, lengths, np.int32), put(rt, want, np.int32)
+            rt.kv_pages(before, after, page, table, free, state, starts, slots)
+            assert state.numpy()[2:].tolist() == [0, 0]
+            news = np.maximum(want - lengths, 0)
+            T = int(news.sum())
+            qkv = rng.standard_normal((128, (heads + 2 * kv) * dim), dtype=np.float32)
+            dq = put(rt, qkv)
+            rt.kv4_store(d, pool, dq.view(heads * dim, (128, kv * dim)), dq.view((heads + kv) * dim, (128, kv * dim)), slots, ld=qkv.shape[1])
+            out = rt.kv4_attention(d, dq, pool, table, after, starts, max_new=int(news.max()), max_length=int(want.max())).numpy().reshape(128, heads, dim)
+            at = 0
+            for r in range(R):
+                rows = qkv[at:at + news[r]]
+                new = np.stack([ref.values(rows[:, (heads + i * kv) * dim:(heads + (i + 1) * kv) * dim], kind == "q4_1").reshape(-1, kv, dim) for i in range(2)], 1)
+                kept[r] = np.concatenate([kept[r][:min(lengths[r], want[r])], new])
+                want_out = ref.attention(rows[:, :heads * dim].reshape(-1, heads, dim), kept[r][:, 0], kept[r][:, 1], want[r], d.scale)
+                np.testing.assert_allclose(out[at:at + news[r]], want_out, rtol=0, atol=2e-3)   # (bound() of these sizes: 4e-3)
+                at += news[r]
+            assert at == T
+            lengths = want
+        held = sum(-(-n // page) for n in lengths)
+        assert state.numpy()[0] == pool_pages - held
+        ids = np.concatenate([free.numpy()[:pool_pages - held], table.numpy()[table.numpy() >= 0]])
+        assert sorted(ids) == list(range(pool_pages))   # no page lost, none twice
+
+
+def test_captured_and_replayed_on_a_stream_of_the_caller(rt):
+    """Plan, rows, attention and selection in one graph, twice over: two graphs with workspaces of their own are replayed on two streams at once."""
+    import torch
+    from caten_b200.runtime import B200Runtime
+    rng = rng_of(63)
+    r = B200Runtime(0)
+    try:
+        sets = []
+        for which in range(2):
+            c = Cache(r, rng, "q4_0", 64, 64, 4, 2, [1500, 70])
+            slots = [c.table[b, (n - 1) // 64] * 64 + (n - 1) % 64 for b, n in enumerate(c.lengths)]
+            x = rng.standard_normal((2, 8 * 64), dtype=np.float32)
+            logits = rng.standard_normal((8, 20000), dtype=np.float32)
+            s = dict(c=c, x=put(r, x), slots=put(r, slots, np.int32), table=put(r, c.table, np.int32), lengths=put(r, c.lengths, np.int32), out=r.open_buffer((2, 256)),
+                     work=r.open_buffer(r.kv4_attention_work(c.desc, 2, 2, 1, 1500), np.uint8), logits=put(r, logits), scores=put(r, np.zeros((2, 4)), np.float32),
+                     picked=tuple(r.open_buffer((2, 4), t) for t in (np.float32, np.int32, np.int64, np.uint8)),
+                     swork=r.open_buffer(r.beam_select_work(2, 4, 20000, 4), np.uint8), host=(x, logits), stream=torch.cuda.Stream(), graph=torch.cuda.CUDAGraph())
+
+            def step(s=s, c=c):
+                r.kv4_store(c.desc, c.pool, s["x"].view(256, (2, 128)), s["x"].view(384, (2, 128)), s["slots"], ld=512)
+                r.kv4_attention(c.desc, s["x"], c.pool, s["table"], s["lengths"], max_length=1500, out=s["out"], work=s["work"])
+                r.beam_select(s["logits"], s["scores"], 4, out=s["picked"], work=s["swork"])
+            step()
+            r.sync()
+            L.check(r.ctx, r.lib.caten_b200_set_stream(r.ctx, s["stream"].cuda_stream))
+            with torch.cuda.graph(s["graph"], stream=s["stream"], capture_error_mode="thread_local"):
+                step()
+            L.check(r.ctx, r.lib.caten_b200_set_stream(r.ctx, None))
+            sets.append(s)
+        want = []
+        for s in sets:
+            for b in (s["out"], s["picked"][0]):
+                L.check(r.ctx, r.lib.caten_b200_memset(r.ctx, b.ptr, 0, b.nbytes))
+        r.sync()
+        for _ in range(5):
+            for s in sets:
+                with torch.cuda.stream(s["stream"]):
+                    s["graph"].replay()
+        torch.cuda.synchronize()
+        for s in sets:
+            c, (x, logits) = s["c"], s["host"]
+            for b, n in enumerate(c.lengths):
+                part = slice(c.first[b], c.first[b + 1])
+                k, v = c.k[part].copy(), c.v[part].copy()
+                k[-1], v[-1] = (ref.values(x[b, i:i + 128], False).reshape(2, 64) for i in (256, 384))
+                want = ref.attention(x[b, :256].reshape(1, 4, 64), k, v, n, c.desc.scale)
+                np.testing.assert_allclose(s["out"].numpy()[b].reshape(1, 4, 64), want, rtol=0, atol=bound(c, x[:, :256], n))
+                sel = ref.select(logits[4 * b:4 * b + 4], np.zeros(4), np.zeros(4), -1, 4)
+                np.testing.assert_array_equal(s["picked"][2].numpy()[b], sel[2])
+            del s["graph"]
+    finally:
+        r.close()
+
+
+def plain_beam_search(logits_of, prompt, beams, steps, eos):
+    """[(tokens, score)] by beam search on the host, and the smallest gap between the last value taken and the first left."""
+    hyps, gap = [(list(prompt), 0.0, False)], np.inf
+    for _ in range(steps):
+        cand = []
+        for i, (t, s, end) in enumerate(hyps):
+            if end:
+                cand.append((s, i, eos))
+                continue
+            x = logits_of(t).astype(np.float64)
+            lp = x - x.max() - np.log(np.exp(x - x.max()).sum())
+            cand += [(s + lp[j], i, int(j)) for j in np.argsort(-lp)[:beams + 1]]
+        cand.sort(key=lambda c: -c[0])
+        values = [c[0] for c in cand[:beams + 1]]
+        gap = min([gap] + [a - b for a, b in zip(values, values[1:])])
+        hyps = [(hyps[i][0] + [j], s, hyps[i][2] or j == eos) for s, i, j in cand[:beams]]
+    return hyps, gap
+
+
+@pytest.mark.parametrize("wtype,eos", [("f32", -1), ("q8_0", 5)])
+def test_beam_search_of_gpt2(rt, wtype, eos):
+    """`beam_search` (caches moved with their hypotheses, everything on the device) against a search on the host that reads every hypothesis anew."""
+    from caten_b200.gpt2 import GPT2, gpt2_beam_search, gpt2_generate
+    p = S.GPT2Params(n_layers=3, n_heads=2, dim=128, vocab_size=1003)
+    sd = S.synth_state_dict(p, wtype, seed=4, max_seq_len=32, trivial_affine=False, weight_std=0.12)
+    one = GPT2(rt, p, sd, max_seq_len=32, batch=1)
+
+    def logits_of(tokens):
+        one.forward([tokens], len(tokens), 0)
+        return one.logits()[0]
+    prompts = S.synth_prompts(2, 6, p.vocab_size, seed=3)
+    if eos >= 0:   # an id that the search does meet: the likeliest third token of the first prompt
+        eos = int(plain_beam_search(logits_of, prompts[0].tolist(), 1, 3, -1)[0][0][0][-1])
+    beams, steps = 4, 10
+    m = GPT2(rt, p, sd, max_seq_len=32, batch=2 * beams)
+    tokens, scores = gpt2_beam_search(m, prompts, beams, steps, eos)
+    assert tokens.shape == (2, beams, 16) and (np.diff(scores, axis=1) <= 0).all()
+    for g in range(2):
+        want, gap = plain_beam_search(logits_of, prompts[g].tolist(), beams, steps, eos)
+        assert gap > 1e-5, "the search's choices are too close to compare"
+        np.testing.assert_array_equal(tokens[g], np.array([h[0] for h in want]))
+        np.testing.assert_allclose(scores[g], [h[1] for h in want], rtol=0, atol=2e-3)
+    m.close()
+    one.close()
+    # one beam is greedy; no step returns the prompt
+    m = GPT2(rt, p, sd, max_seq_len=32, batch=2)
+    np.testing.assert_array_equal(gpt2_beam_search(m, prompts, 1, 8)[0][:, 0], gpt2_generate(m, prompts, 8))
+    t, s = gpt2_beam_search(m, prompts[:1], 2, 0)
+    np.testing.assert_array_equal(t, np.repeat(prompts[:1][:, None], 2, 1))
+    with pytest.raises(ValueError):
+        gpt2_beam_search(m, prompts, 3, 2)
+    m.close()

@@ -1,0 +1,232 @@
+"""CPU tests of the serving operators' boundary: what the entry points refuse (arguments are checked before the context is touched, so no
+GPU is needed), where the cache's values lie, and the plain statements that the GPU tests compare with."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+from oracle import serving_ref as ref
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from caten_b200 import _lib, build
+    build.build()
+    return _lib.load()
+
+
+def desc(**kw):
+    from caten_b200 import _lib as L
+    d = dict(heads=8, kv_heads=4, dim=64, type=L.Q4_0, page=32, scale=0.125, pages=10)
+    d.update(kw)
+    return L.Kv4Desc(**d)
+
+
+def refused(lib, rc, *words):
+    from caten_b200 import _lib as L
+    said = lib.caten_b200_last_error(None).decode()
+    assert rc in (L.EINVAL, L.EUNSUPPORTED, -1) and all(w in said for w in words), (rc, said)
+
+
+A = 1 << 20   # an aligned address that is never followed
+
+
+def test_descriptions_that_are_refused(lib):
+    for kw, word in ((dict(dim=80), "heads of 80"), (dict(dim=32), "heads of 32"), (dict(page=24), "pages of 24"), (dict(page=0), "pages of 0"), (dict(type=8), "type 8"),
+                     (dict(heads=6), "6 heads"), (dict(kv_heads=0), "heads"), (dict(pages=0), "0 pages"), (dict(pages=1 << 27), "32-bit")):
+        d = desc(**kw)
+        refused(lib, lib.caten_b200_kv4_nbytes(C.byref(d)), word)
+        refused(lib, lib.caten_b200_kv4_store(None, C.byref(d), A, A, A, 256, A, 1), word)
+        refused(lib, lib.caten_b200_kv4_load(None, C.byref(d), A, A, 1, A, A, 256), word)
+        refused(lib, lib.caten_b200_kv4_attention(None, C.byref(d), A, 512, A, A, 4, A, None, 1, 1, 1, 64, A, A), word)
+    refused(lib, lib.caten_b200_kv4_nbytes(None), "NULL")
+
+
+def test_pool_sizes(lib):
+    assert lib.caten_b200_kv4_nbytes(C.byref(desc())) == 10 * 32 * 4 * 2 * 64 * 18 // 32
+    assert lib.caten_b200_kv4_nbytes(C.byref(desc(type=3, dim=192))) == 10 * 32 * 4 * 2 * 192 * 20 // 32
+
+
+def test_rows_that_are_refused(lib):
+    d = desc()
+    for bad in ((None, A, A, 256, A, 1), (A, None, A, 256, A, 1), (A, A, None, 256, A, 1), (A, A, A, 256, None, 1)):
+        refused(lib, lib.caten_b200_kv4_store(None, C.byref(d), *bad), "NULL")
+    refused(lib, lib.caten_b200_kv4_store(None, C.byref(d), A, A, A, 255, A, 1), "ld=255")
+    refused(lib, lib.caten_b200_kv4_store(None, C.byref(d), A + 8, A, A, 256, A, 1), "16 bytes")
+    refused(lib, lib.caten_b200_kv4_store(None, C.byref(d), A, A + 2, A, 256, A, 1), "misaligned")
+    refused(lib, lib.caten_b200_kv4_store(None, C.byref(d), A, A, A, 256, A, -1), "-1 tokens")
+    refused(lib, lib.caten_b200_kv4_load(None, C.byref(d), A, A, 1 << 31, A, A, 256), "tokens")
+    refused(lib, lib.caten_b200_kv4_store(None, C.byref(d), A, A, A, 256, A, 1), "ctx is NULL")   # all else is in order
+
+
+def test_attention_calls_that_are_refused(lib):
+    d = desc()
+    call = lambda **k: lib.caten_b200_kv4_attention(None, C.byref(d), *[dict(q=A, ldq=512, pool=A, table=A, max_pages=4, lengths=A, starts=A, batch=2, rows=5,   # noqa: E731
+                                                                             max_new=3, max_length=128, out=A, work=A, **{})[n] if n not in k else k[n]
+                                                                        for n in ("q", "ldq", "pool", "table", "max_pages", "lengths", "starts", "batch", "rows", "max_new",
+                                                                                  "max_length", "out", "work")])
+    refused(lib, call(), "ctx is NULL")
+    for n in ("q", "pool", "table", "lengths", "out", "work"):
+        refused(lib, call(**{n: None}), "NULL argument")
+    refused(lib, call(ldq=511), "ldq=511")
+    refused(lib, call(max_length=129), "lengths up to 129")
+    refused(lib, call(max_pages=0), "tables of 0")
+    refused(lib, call(starts=None), "without starts")
+    refused(lib, call(starts=None, rows=2), "without starts")
+    refused(lib, call(max_new=0), "bad shape")
+    refused(lib, call(rows=-1), "bad shape")
+    refused(lib, call(pool=A + 4), "16 bytes")
+    refused(lib, call(work=A + 4), "16 bytes")
+    refused(lib, call(out=A + 2), "misaligned")
+    assert lib.caten_b200_kv4_attention_work(C.byref(d), 2, 5, 3, 128) >= 16
+    refused(lib, lib.caten_b200_kv4_attention_work(C.byref(d), 2, 5, 0, 128), "bad shape")
+
+
+def test_page_plans_that_are_refused(lib):
+    call = lambda *k: lib.caten_b200_kv_pages(None, *k)   # noqa: E731
+    good = [A, A, 3, 16, A, 4, A, 100, A, A, A, 50]
+    refused(lib, call(*good), "ctx is NULL")
+    for i in (0, 1, 4, 6, 8, 9, 10):
+        bad = list(good)
+        bad[i] = None
+        refused(lib, call(*bad), "NULL argument")
+    for i, v in ((2, -1), (3, 0), (5, 0), (7, 0), (7, 1 << 28), (11, -1), (11, 1 << 31), (5, 1 << 28)):
+        bad = list(good)
+        bad[i] = v
+        refused(lib, call(*bad), "kv_pages")
+        assert "ctx" not in lib.caten_b200_last_error(None).decode()
+
+
+def test_beam_calls_that_are_refused(lib):
+    work = lib.caten_b200_beam_select_work
+    assert work(2, 4, 50257, 8) > 0 and work(0, 4, 50257, 8) >= 0
+    for bad in ((2, 33, 100, 4), (2, 4, 100, 33), (2, 4, 0, 4), (2, 0, 100, 4), (-1, 4, 100, 4), (2, 4, 100, 0), (65536, 1, 100, 1), (1 << 60, 32, 100, 1), (2, 4, 1 << 30, 4)):
+        refused(lib, work(*bad), "beam_select")
+    call = lambda **k: lib.caten_b200_beam_select(None, *[k.get(n, v) for n, v in dict(x=A, s=A, e=A, batch=2, beams=4, V=100, eos=5, keep=4, os=A, op=A, ot=A, oe=A, w=A).items()])   # noqa: E731
+    refused(lib, call(), "ctx is NULL")
+    refused(lib, call(e=None, oe=None, eos=-1), "ctx is NULL")
+    for n in ("x", "s", "os", "op", "ot", "w"):
+        refused(lib, call(**{n: None}), "NULL argument")
+    refused(lib, call(eos=100), "eos=100")
+    refused(lib, call(eos=-1), "need an eos")
+    refused(lib, call(ot=A + 4), "misaligned")
+    refused(lib, call(x=A + 2), "misaligned")
+    states = lambda *p: (C.c_void_p * len(p))(*p)   # noqa: E731
+    move = lambda st, n, *k: lib.caten_b200_beam_reorder(None, st, n, *k)   # noqa: E731
+    refused(lib, move(states(A), 1, A, 2, 4, 3, 1024, 256), "ctx is NULL")
+    refused(lib, move(states(A), 1, A, 2, 33, 3, 1024, 256), "33 beams")
+    refused(lib, move(states(A), 1, A, 2, 4, 3, 1024, 1028), "bad shape")
+    refused(lib, move(states(A), 1, A, 2, 4, 3, 1024, 258), "multiples of 4")
+    refused(lib, move(states(None), 1, A, 2, 4, 3, 1024, 256), "state 0")
+    refused(lib, move(states(A, A + 2), 2, A, 2, 4, 3, 1024, 256), "state 1")
+    refused(lib, move(states(A), 1, None, 2, 4, 3, 1024, 256), "NULL")
+    refused(lib, move(states(A), 1, A, 65536, 4, 3, 1024, 256), "bad shape")
+    refused(lib, move(states(A, A + 8 * 3 * 1024 - 16), 2, A, 2, 4, 3, 1024, 256), "overlap")
+    refused(lib, move(states(A, 5 * A, A), 3, A, 2, 4, 3, 1024, 256), "overlap")
+    paged = lambda **k: lib.caten_b200_beam_reorder_pages(None, *[k.get(n, v) for n, v in dict(pool=A, pages=9, nb=1024, table=A, mp=4, lens=A, page=16, par=A, groups=2, beams=4).items()])   # noqa: E731
+    refused(lib, paged(), "ctx is NULL")
+    for n in ("pool", "table", "lens", "par"):
+        refused(lib, paged(**{n: None}), "NULL argument")
+    refused(lib, paged(nb=1000), "multiple of 16")
+    refused(lib, paged(beams=40), "40 beams")
+    refused(lib, paged(mp=65536), "bad shape")
+    refused(lib, paged(pool=A + 8), "16 bytes")
+
+
+def test_layout_is_the_stated_one(tmp_path):
+    """The index arithmetic that the kernels use (csrc/kv4_layout.h, as plain C++): every value has a place of its own, the stated one, inside its
+    page; page numbers outside the pool are told apart."""
+    src = tmp_path / "layout.cpp"
+    src.write_text('#include <cstdio>\n#include <initializer_list>\n#include "kv4_layout.h"\nusing namespace cb;\nint main() {\n'
+                   '  for (int q41 = 0; q41 < 2; ++q41) for (int dim = 64; dim <= 256; dim += 64) {\n'
+                   '    Kv4Shape s = {3, dim, q41, 32, 7};\n'
+                   '    printf("s %d %d %d %lld %lld\\n", q41, dim, kv4_part_bytes(s), (long long)kv4_page_bytes(s), (long long)kv4_tile_at(s, 5, 2, 17));\n'
+                   '    for (int t = 0; t < 16; ++t) for (int j = 0; j < dim; ++j) printf("c %d %d\\n", kv4_k_byte(t, j), kv4_v_byte(t, j));\n'
+                   '    for (int t = 0; t < 16; ++t) for (int b = 0; b < dim / 32; ++b) printf("h %d\\n", kv4_scale_index(t, b, dim));\n'
+                   '  }\n  Kv4Shape s = {3, 64, 0, 32, 7};\n'
+                   '  for (long long p : {-1ll, 0ll, 6ll, 7ll, 1ll << 31, -(1ll << 31)}) printf("p %d\\n", (int)kv4_page_ok(s, p));\n'
+                   '  Kv4Shape far = {8, 128, 1, 128, 1 << 20};\n  printf("f %lld\\n", (long long)kv4_tile_at(far, (1 << 20) - 1, 7, 127));\n}\n')
+    exe = tmp_path / "layout"
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "caten_b200", "csrc"), str(src), "-o", str(exe)], check=True)
+    lines = [x.split() for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()]
+    at = 0
+    for q41 in (0, 1):
+        for dim in (64, 128, 192, 256):
+            part = dim * (10 if q41 else 9)
+            assert lines[at] == ["s", str(q41), str(dim), str(part), str(3 * 2 * 2 * part), str(5 * 12 * part + (2 * 2 + 1) * 2 * part)]
+            codes = np.array([[int(a), int(b)] for _, a, b in lines[at + 1:at + 1 + 16 * dim]]).reshape(16, dim, 2)
+            halves = np.array([int(a) for _, a in lines[at + 1 + 16 * dim:at + 1 + 16 * dim + dim // 2]])
+            assert (np.bincount(codes[..., 0].ravel(), minlength=8 * dim) == 2).all() and (np.bincount(codes[..., 1].ravel(), minlength=8 * dim) == 2).all()
+            assert (codes[:, 0::2] == codes[:, 1::2]).all()   # an odd code beside its even one
+            assert sorted(halves) == list(range(dim // 2))
+            # one token by the plain statement: its codes and scales lie where the arithmetic says
+            pool = np.zeros((7, 3 * 2 * 2 * part), np.uint8)
+            k = np.linspace(-1, 1, dim, dtype=np.float32)
+            ref.put(pool, 32, 3, dim, bool(q41), 5 * 32 + 16 + 11, 2, k, k[::-1].copy())
+            base = (2 * 2 + 1) * 2 * part
+            for which, x in ((0, k), (1, k[::-1].copy())):
+                code, d, _ = ref.blocks(x.reshape(-1, 32), bool(q41))
+                for j in range(dim):
+                    assert pool[5, base + which * part + codes[11, j, which]] >> j % 2 * 4 & 15 == code[j // 32, j % 32]
+                for b in range(dim // 32):
+                    place = base + which * part + 8 * dim + 2 * halves[11 * (dim // 32) + b]
+                    assert pool[5, place:place + 2].tobytes() == d[b].tobytes()
+            at += 1 + 16 * dim + dim // 2
+    assert [x[1] for x in lines[at:at + 6]] == ["0", "1", "1", "0", "0", "0"]
+    assert int(lines[at + 6][1]) == ((1 << 20) - 1) * 8 * 8 * 2560 + (7 * 8 + 7) * 2560   # beyond 32 bits
+
+
+def test_plain_blocks_are_those_of_the_file_format():
+    """At values that are not next to a border: the codes of the GGUF package's quantisers, which work in fp32."""
+    from gguf import quants
+    rng = np.random.Generator(np.random.PCG64(3))
+    x = rng.standard_normal((200, 32), dtype=np.float32)
+    for q4_1, kind in ((False, quants.Q4_0), (True, quants.Q4_1)):
+        np.testing.assert_array_equal(ref.values(x, q4_1), kind.dequantize_blocks(kind.quantize_blocks(x.copy())))
+
+
+def test_runtime_refuses_buffers_that_do_not_fit(lib):
+    """The Python methods' own checks, on buffers without memory."""
+    from caten_b200 import _lib as L
+    from caten_b200.runtime import B200Buffer, B200Runtime
+    rt = B200Runtime.__new__(B200Runtime)
+    rt.lib, rt.ctx = lib, None
+    buf = lambda kind, *shape: B200Buffer(rt, A, shape, kind, owned=False)   # noqa: E731
+    f, i, u = np.float32, np.int32, np.uint8
+    out = lambda n, kind=i: (buf(f, 2, n), buf(kind, 2, n), buf(np.int64, 2, n), buf(u, 2, n))   # noqa: E731
+    work = buf(u, 1 << 20)
+    for bad in (dict(logits=buf(f, 7, 50)), dict(scores=buf(np.float64, 2, 4)), dict(ended=buf(u, 2, 3)), dict(out=out(5)), dict(out=out(4, f)), dict(work=buf(u, 8))):
+        a = dict(logits=buf(f, 8, 50), scores=buf(f, 2, 4), keep=4, ended=buf(u, 2, 4), eos=3, out=out(4), work=work)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            rt.beam_select(**a)
+    d = desc()
+    pool = buf(u, 10, lib.caten_b200_kv4_nbytes(C.byref(d)) // 10)
+    with pytest.raises(ValueError):
+        rt.kv4_store(d, pool, buf(f, 5, 256), buf(f, 5, 255), buf(i, 5))
+    with pytest.raises(ValueError):
+        rt.kv4_store(d, buf(u, 100), buf(f, 5, 256), buf(f, 5, 256), buf(i, 5))
+    for bad in (dict(q=buf(f, 2, 511)), dict(lengths=buf(np.int64, 2)), dict(table=buf(i, 3, 4)), dict(starts=buf(i, 2)), dict(out=buf(f, 2, 511)), dict(pool=buf(u, 10, 10))):
+        a = dict(desc=d, q=buf(f, 2, 512), pool=pool, table=buf(i, 2, 4), lengths=buf(i, 2), out=buf(f, 2, 512), work=work)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            rt.kv4_attention(**a)
+    with pytest.raises(ValueError):
+        rt.beam_reorder([buf(f, 8, 3, 10, 64)], buf(i, 2, 4), 11)
+    with pytest.raises(ValueError):
+        rt.beam_reorder([buf(f, 8, 3, 10, 64), buf(f, 8, 3, 11, 64)], buf(i, 2, 4), 5)
+    with pytest.raises(ValueError):
+        rt.kv_pages(buf(i, 3), buf(i, 4), 16, buf(i, 3, 4), buf(i, 9), buf(i, 4), buf(i, 4), buf(i, 8))
+    with pytest.raises(L.B200Error):
+        rt.kv4_attention_work(desc(dim=48), 1, 1, 1, 10)
+
+
+def test_command_refuses_beams_it_cannot_have():
+    from caten_b200.generate import main
+    for bad in (["--beams", "33"], ["--beams", "-1"], ["--beams", "4", "--temperature", "1"]):
+        with pytest.raises(SystemExit):
+            main(["--model", "none", "--ids", "1"] + bad)
