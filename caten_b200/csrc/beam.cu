@@ -4,7 +4,8 @@
 // Selection.  Candidate (beam b, token v) has the value score_b + x_bv - lse_b, lse_b = max + log(sum exp(x - max)); the first `keep` by value,
 // equal ones by b * V + v.  Within a beam that order is the order of the logits, so a pass over the logits needs no lse: each block reads a chunk
 // of a row once into registers and leaves its maximum, its sum of exponentials and its `keep` largest logits; a second kernel joins the
-// chunks' sums in 64 bits, turns the few logits left into values and merges them.
+// chunks' sums in 64 bits, turns the few logits left into values and picks among them.  Both pick by a bound first: the smallest of `keep` or more
+// disjoint groups' largest has `keep` at or above it, and with a few dozen candidates left each counts those before it, which is its place.
 #include <algorithm>
 
 #include "common.cuh"
@@ -12,8 +13,9 @@
 
 namespace cb {
 
-constexpr int BS_THREADS = 256, BS_VECS = 8, BS_CHUNK = BS_THREADS * BS_VECS * 4;   // a thread holds 32 logits
-constexpr int BS_KEEP = 32;   // a warp's lanes
+constexpr int BS_THREADS = 256;
+constexpr int BS_KEEP = 32;     // a warp's lanes
+constexpr int BS_FEW = 64;      // threads of a block that may have candidates (of at most 32 logits each) without a closer look
 
 typedef unsigned long long u64;
 
@@ -42,190 +44,197 @@ __device__ __forceinline__ u64 warp_sort(u64 key) {
     }
   return key;
 }
-// the 32 largest of two descending lists, descending
-__device__ __forceinline__ u64 warp_merge(u64 a, u64 b) {
-  const int lane = threadIdx.x & 31;
-  const u64 r = __shfl_sync(0xffffffffu, b, 31 - lane);
-  u64 key = a > r ? a : r;
+
+// The `keep`-th largest of the block's keys (one a thread, 0: none; all others different), 1 if there are fewer.  A key's rank is the number of
+// larger ones, found in each warp's descending list by bisection.  Called by the whole block; `lists` and `answer` are its scratch.
+__device__ u64 block_kth_key(u64 key, int keep, u64 (*lists)[32], u64 *answer) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  key = warp_sort(key);
+  lists[warp][lane] = key;
+  if (threadIdx.x == 0) *answer = 1;
+  __syncthreads();
+  if (lane < keep && key) {
+    int rank = 0;
+#pragma unroll 1
+    for (int w = 0; w < BS_THREADS / 32; ++w) {
+      int lo = 0;
 #pragma unroll
-  for (int j = 16; j > 0; j >>= 1) {
-    const u64 other = __shfl_xor_sync(0xffffffffu, key, j);
-    key = ((lane & j) == 0) == (other > key) ? other : key;
+      for (int step = 16; step > 0; step >>= 1)
+        if (lists[w][lo + step - 1] > key) lo += step;
+      rank += lo + (lists[w][lo] > key ? 1 : 0);
+    }
+    if (rank == keep - 1) *answer = key;
   }
-  return key;
+  __syncthreads();
+  return *answer;
 }
 
 // What a block leaves of its chunk: `keep` keys (descending, 0 behind the last), then maximum and sum.
 __host__ __device__ __forceinline__ int64_t beam_part_words(int keep) { return keep + 1; }
 
+template <int VECS>
 __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__restrict__ x, const uint8_t *__restrict__ ended, int64_t V, int keep, u64 *__restrict__ parts) {
-  __shared__ float red[BS_THREADS / 32];
-  __shared__ u64 lists[BS_THREADS / 32][32];
-  __shared__ u64 found[BS_KEEP * BS_VECS * 4];
-  __shared__ u64 threshold;
-  __shared__ int count;
+  constexpr int CHUNK = BS_THREADS * VECS * 4;
+  __shared__ float group_top[32], sums[BS_THREADS / 32];
+  __shared__ u64 lists[BS_THREADS / 32][32], answer;
+  __shared__ u64 found[BS_FEW * VECS * 4];
+  __shared__ int count, threads;
   pdl_enter();
   const int64_t row = blockIdx.y;
   if (ended && ended[row]) return;   // its one candidate needs no logits
   const float *p = x + row * V;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // chunks start on 16-byte boundaries of memory, wherever the row does
-  const int64_t e0 = (int64_t)blockIdx.x * BS_CHUNK - (int64_t)(((uintptr_t)p >> 2) & 3);
-  float v[BS_VECS][4];
+  const int64_t e0 = (int64_t)blockIdx.x * CHUNK - (int64_t)(((uintptr_t)p >> 2) & 3);
+  float v[VECS][4];
+  if (e0 >= 0 && e0 + CHUNK <= V) {
 #pragma unroll
-  for (int i = 0; i < BS_VECS; ++i) {
-    const int64_t e = e0 + (i * BS_THREADS + tid) * 4;
-    if (e >= 0 && e + 4 <= V) {
-      const float4 q = __ldcs(reinterpret_cast<const float4 *>(p + e));
+    for (int i = 0; i < VECS; ++i) {
+      const float4 q = __ldcs(reinterpret_cast<const float4 *>(p + e0) + i * BS_THREADS + tid);
       v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
-    } else {
+    }
+  } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = e + j >= 0 && e + j < V ? p[e + j] : -INFINITY;
+    for (int i = 0; i < VECS; ++i) {
+      const int64_t e = e0 + (i * BS_THREADS + tid) * 4;
+      if (e >= 0 && e + 4 <= V) {
+        const float4 q = __ldcs(reinterpret_cast<const float4 *>(p + e));
+        v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = e + j >= 0 && e + j < V ? p[e + j] : -INFINITY;
+      }
     }
   }
-  // the thread's largest, the block's
+  if (tid == 0) { count = 0; threads = 0; }
+  // the largest of each thread, of groups of threads (8, 16 or 32 of them in the block: the least power of two from `keep`, 8 at least), of the block
   float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < BS_VECS; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = fmaxf(top, v[i][j]);
-  u64 best = 0;
-#pragma unroll
-  for (int i = BS_VECS - 1; i >= 0; --i)
-#pragma unroll
-    for (int j = 3; j >= 0; --j)
-      if (v[i][j] == top) best = beam_key(v[i][j], (int)(e0 + (i * BS_THREADS + tid) * 4 + j));   // (the lowest index of equal ones)
-  float m = top;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) red[warp] = m;
-  lists[warp][lane] = warp_sort(best);
-  if (tid == 0) { threshold = 1; count = 0; }
+  for (int i = 0; i < VECS; ++i) top = fmaxf(top, fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3])));
+  const int per_warp = keep <= 8 ? 1 : keep <= 16 ? 2 : 4, width = 32 / per_warp, groups = per_warp * (BS_THREADS / 32);
+  float gt = top;
+  for (int o = 1; o < width; o <<= 1) gt = fmaxf(gt, __shfl_xor_sync(0xffffffffu, gt, o));
+  if (lane % width == 0) group_top[warp * per_warp + lane / width] = gt;
   __syncthreads();
-  m = red[0];
+  float m = lane < groups ? group_top[lane] : -INFINITY, least = lane < groups ? m : INFINITY;
 #pragma unroll
-  for (int w = 1; w < BS_THREADS / 32; ++w) m = fmaxf(m, red[w]);
-  // the keep-th largest of the threads' largest: nothing below it is among the chunk's `keep` largest.  A key's rank is the number of
-  // larger ones, found in each warp's descending list by bisection.
-  if (lane < keep) {
-    const u64 mine = lists[warp][lane];
-    int rank = 0;
-#pragma unroll
-    for (int w = 0; w < BS_THREADS / 32; ++w) {
-      int lo = 0;
-#pragma unroll
-      for (int step = 16; step > 0; step >>= 1)
-        if (lists[w][lo + step - 1] > mine) lo += step;
-      rank += lo + (lists[w][lo] > mine ? 1 : 0);
-    }
-    if (mine && rank == keep - 1) threshold = mine;
+  for (int o = 16; o > 0; o >>= 1) {
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
   }
+  const bool may = top >= least && top > -INFINITY;
+  const unsigned who = __ballot_sync(0xffffffffu, may);
+  if (lane == 0 && who) atomicAdd(&threads, __popc(who));
   // sum of exponentials; a maximum of -inf (nothing left) makes it 0, a NaN or +inf makes it NaN
-  // (x - max) log2 e with the constant in two parts: rounded to one, it would shift every sum by 1e-8 of the distance
   const float base = m == -INFINITY ? 0.0f : m;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < BS_VECS; ++i)
+  for (int i = 0; i < VECS; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float d = v[i][j] - base;
       float e;
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(d, 1.44269502162933349609375f, d * 1.925963033500e-8f)));
-      s[j] += m < INFINITY ? e : NAN;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((v[i][j] - base) * 1.4426950408889634f));
+      s[j] += e;
     }
-  float sum = (s[0] + s[1]) + (s[2] + s[3]);
-  sum = warp_sum(sum);
-  __syncthreads();   // threshold, and red has been read
-  if (lane == 0) red[warp] = sum;
-  const u64 least = threshold;
-  if (best >= least) {
-    const float floor_value = beam_key_value(least);
+  float sum = warp_sum((s[0] + s[1]) + (s[2] + s[3]));
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  // Many threads at the bound: equal logits (a mask's value), or masks that empty whole groups.  Then by keys, which are all different.
+  u64 bound = 1;
+  bool look = may;
+  if (threads > BS_FEW) {
+    u64 best = 0;
 #pragma unroll
-    for (int i = 0; i < BS_VECS; ++i)
+    for (int i = VECS - 1; i >= 0; --i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (least == 1 || v[i][j] >= floor_value) {
+      for (int j = 3; j >= 0; --j)
+        if (v[i][j] == top) best = beam_key(v[i][j], (int)(e0 + (i * BS_THREADS + tid) * 4 + j));   // (the lowest index of equal ones)
+    bound = block_kth_key(best, keep, lists, &answer);
+    look = best >= bound;   // (`keep` threads, or fewer than that in all)
+  }
+  if (look) {
+    const float floor_value = bound == 1 ? least : beam_key_value(bound);
+#pragma unroll
+    for (int i = 0; i < VECS; ++i)
+      if (fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3])) >= floor_value)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
           const u64 key = beam_key(v[i][j], (int)(e0 + (i * BS_THREADS + tid) * 4 + j));
-          if (key >= least) found[atomicAdd(&count, 1)] = key;   // (at most `keep` threads, or fewer, get here: at most 32 keys each)
+          if (v[i][j] >= floor_value && key >= bound) found[atomicAdd(&count, 1)] = key;
         }
   }
   __syncthreads();
-  if (warp) return;
   const int n = count;
-  u64 list = warp_sort(lane < n ? found[lane] : 0ull);
-  for (int i = 32; i < n; i += 32) list = warp_merge(list, warp_sort(i + lane < n ? found[i + lane] : 0ull));
   u64 *part = parts + (row * gridDim.x + blockIdx.x) * beam_part_words(keep);
-  if (lane < keep) part[lane] = list;
-  sum = red[0];
+  for (int i = tid; i < n; i += BS_THREADS) {
+    const u64 key = found[i];
+    int place = 0;
+    for (int j = 0; j < n && place < keep; ++j) place += found[j] > key;
+    if (place < keep) part[place] = key;
+  }
+  for (int i = n + tid; i < keep; i += BS_THREADS) part[i] = 0;
+  if (tid == 0) {
+    sum = sums[0];
 #pragma unroll
-  for (int w = 1; w < BS_THREADS / 32; ++w) sum += red[w];
-  if (lane == 0) part[keep] = (u64)__float_as_uint(base) << 32 | __float_as_uint(sum);
+    for (int w = 1; w < BS_THREADS / 32; ++w) sum += sums[w];
+    part[keep] = (u64)__float_as_uint(base) << 32 | __float_as_uint(m < INFINITY ? sum : NAN);
+  }
 }
 
 // ---- the chunks' lists into one --------------------------------------------------------------------
-struct Cand {
-  u64 value;      // order-preserving image of the 64-bit value; 0: none
-  uint32_t index; // beam * V + token, complemented
-  __device__ __forceinline__ bool operator>(const Cand &o) const { return value > o.value || (value == o.value && index > o.index); }
-};
+// order-preserving image of a 64-bit value; 0: none
 __device__ __forceinline__ u64 order_of(double x) {
   const u64 b = (u64)__double_as_longlong(x + 0.0);
   return !(x > -INFINITY) ? 0ull : (b >> 63) ? ~b : (b | 0x8000000000000000ull);
 }
 __device__ __forceinline__ double value_of(u64 k) { return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k)); }
-__device__ __forceinline__ Cand cand_shfl_xor(const Cand &c, int j) { return {__shfl_xor_sync(0xffffffffu, c.value, j), __shfl_xor_sync(0xffffffffu, c.index, j)}; }
-__device__ __forceinline__ Cand cand_merge(const Cand &a, const Cand &b) {
-  const int lane = threadIdx.x & 31;
-  const Cand r = {__shfl_sync(0xffffffffu, b.value, 31 - lane), __shfl_sync(0xffffffffu, b.index, 31 - lane)};
-  Cand c = a > r ? a : r;
-#pragma unroll
-  for (int j = 16; j > 0; j >>= 1) {
-    const Cand o = cand_shfl_xor(c, j);
-    c = ((lane & j) == 0) == (o > c) ? o : c;
-  }
-  return c;
-}
 
 constexpr int BJ_THREADS = 256;
 constexpr int BJ_BEAMS = 32;
+constexpr int BJ_LISTS = 4096;   // of a request: beams x chunks
+constexpr int BJ_FOUND = BS_KEEP * BS_KEEP;
+
+// A candidate: the order-preserving image of its value, and b * V + token; larger: earlier in the result.
+struct Cand {
+  u64 value;
+  uint32_t id;
+  __device__ __forceinline__ bool operator>(const Cand &o) const { return value > o.value || (value == o.value && id < o.id); }
+};
 
 __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__restrict__ parts, int chunks, const float *__restrict__ scores, const uint8_t *__restrict__ ended,
                                                                int beams, int64_t V, int64_t eos, int keep, float *__restrict__ out_scores, int *__restrict__ out_parents,
                                                                int64_t *__restrict__ out_tokens, uint8_t *__restrict__ out_ended) {
   __shared__ double base[BJ_BEAMS], tops[BJ_BEAMS];   // a candidate's value: base + (x - top)
   __shared__ uint8_t over[BJ_BEAMS];
-  __shared__ Cand lists[BJ_THREADS / 32][32];
+  __shared__ Cand found[BJ_FOUND], bound;
+  __shared__ int queue[BS_KEEP];
+  __shared__ int count, queued;
   pdl_enter();
   const int64_t batch = blockIdx.x;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t words = beam_part_words(keep);
+  const int lists = beams * chunks;
+  const u64 *mine = parts + batch * lists * words;
+  if (tid == 0) { bound = {1, 0xffffffffu}; count = 0; queued = 0; }   // (that bound: every candidate)
   for (int b = warp; b < beams; b += BJ_THREADS / 32) {
     const int64_t row = batch * beams + b;
     const float score = scores[row];
     const bool end = ended && ended[row];
     double log_sum = 0.0, top = 0.0;
     if (!end) {
-      const u64 *part = parts + row * chunks * words + keep;
+      const u64 *part = mine + (int64_t)b * chunks * words + keep;
       float m = -INFINITY;
-      bool none = true;
+      for (int c = lane; c < chunks; c += 32)
+        if ((uint32_t)part[c * words] != 0u) m = fmaxf(m, __uint_as_float((uint32_t)(part[c * words] >> 32)));   // (sum 0: nothing in that chunk)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       double s = 0.0;
       for (int c = lane; c < chunks; c += 32) {
         const u64 w = part[c * words];
-        const float pm = __uint_as_float((uint32_t)(w >> 32)), ps = __uint_as_float((uint32_t)w);
-        if (ps == 0.0f) continue;   // nothing in that chunk
-        if (none || pm > m) { s = none ? (double)ps : s * exp((double)m - (double)pm) + (double)ps; m = pm; }
-        else s += (double)ps * exp((double)pm - (double)m);
-        none = false;
+        if ((uint32_t)w != 0u) s += (double)__uint_as_float((uint32_t)w) * exp((double)__uint_as_float((uint32_t)(w >> 32)) - (double)m);
       }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o);
-        const double os = __shfl_xor_sync(0xffffffffu, s, o);
-        const float both = fmaxf(m, om);
-        const double a = m == -INFINITY ? 0.0 : s * exp((double)m - (double)both), c = om == -INFINITY ? 0.0 : os * exp((double)om - (double)both);
-        s = a + c;
-        m = both;
-      }
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       log_sum = log(s);   // (nothing left in the row: -inf, but then there is no key either)
       top = (double)m;
     }
@@ -236,56 +245,96 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
     }
   }
   __syncthreads();
-  Cand best = {0ull, 0u};
-  const int total = beams * chunks;
-  for (int i = warp; i < total; i += BJ_THREADS / 32) {
-    const int b = i / chunks, c = i % chunks;
-    const int64_t row = batch * beams + b;
-    Cand mine = {0ull, 0u};
-    if (over[b]) {
-      if (c == 0 && lane == 0 && eos >= 0 && eos < V) {
-        mine.value = order_of(base[b]);
-        mine.index = ~(uint32_t)(b * V + eos);
-      }
-    } else {
-      const u64 key = lane < keep ? parts[(row * chunks + c) * words + lane] : 0ull;
-      if (key) {
-        mine.value = order_of(base[b] + ((double)beam_key_value(key) - tops[b]));
-        mine.index = ~(uint32_t)(b * V + beam_key_index(key));
-      }
+  // entry j of list i
+  auto entry = [&](int i, int j) -> Cand {
+    const int b = i / chunks;
+    if (over[b])   // its one candidate stands first in its first list
+      return {i == b * chunks && j == 0 && eos >= 0 ? order_of(base[b]) : 0ull, (uint32_t)(b * V + eos)};
+    const u64 key = mine[(int64_t)i * words + j];
+    return {key ? order_of(base[b] + ((double)beam_key_value(key) - tops[b])) : 0ull, (uint32_t)(b * V + beam_key_index(key))};
+  };
+  // the `keep`-th of n candidates (all different but for those without a value), if there are as many
+  auto bound_of = [&](int n) {
+    for (int i = tid; i < n; i += BJ_THREADS) {
+      const Cand c = found[i];
+      int place = 0;
+      for (int j = 0; j < n && place < keep; ++j) place += found[j] > c;
+      if (c.value && place == keep - 1) bound = c;
     }
-    if (!mine.value) mine.index = 0;
-    // (a list whose first is behind this warp's last so far adds nothing)
-    const u64 head = __shfl_sync(0xffffffffu, mine.value, 0), tail = __shfl_sync(0xffffffffu, best.value, keep - 1);
-    if (head && head >= tail) best = cand_merge(best, mine);
+  };
+  // The keep-th of the lists' first entries: `keep` candidates are not behind it, and at most `keep` lists have any that are not.  Where a thread
+  // has several lists, the threads' best give a first bound, and the few first entries that it leaves the second.
+  Cand best = {0ull, 0xffffffffu};
+  for (int i = tid; i < lists; i += BJ_THREADS) {
+    const Cand c = entry(i, 0);
+    if (c > best) best = c;
   }
-  lists[warp][lane] = best;
+  found[tid] = best;
   __syncthreads();
-  if (warp) return;
-#pragma unroll 1
-  for (int w = 1; w < BJ_THREADS / 32; ++w) {
-    const Cand other = lists[w][lane];
-    if (__shfl_sync(0xffffffffu, other.value, 0)) best = cand_merge(best, other);
+  bound_of(min(lists, BJ_THREADS));
+  __syncthreads();
+  if (lists > BJ_THREADS) {
+    const Cand first = bound;
+    __syncthreads();
+    for (int i = tid; i < lists; i += BJ_THREADS) {
+      const Cand c = entry(i, 0);
+      if (c.value && !(first > c)) found[atomicAdd(&count, 1)] = c;   // (of at most `keep` threads, 16 lists each)
+    }
+    __syncthreads();
+    const int n = count;
+    bound_of(n);
+    __syncthreads();
+    if (tid == 0) count = 0;
   }
-  if (lane < keep) {
-    const int64_t at = batch * keep + lane;
-    const bool there = best.value != 0;
-    const uint32_t index = ~best.index;
-    const int parent = there ? (int)(index / (uint64_t)V) : min(lane, beams - 1);
-    const int64_t token = there ? (int64_t)(index % (uint64_t)V) : eos >= 0 ? eos : 0;
-    out_scores[at] = there ? (float)value_of(best.value) : -INFINITY;
+  const Cand least = bound;
+  __syncthreads();
+  for (int i = tid; i < lists; i += BJ_THREADS) {
+    const Cand c = entry(i, 0);
+    if (c.value && !(least > c)) queue[atomicAdd(&queued, 1)] = i;
+  }
+  __syncthreads();
+  for (int q = warp; q < queued; q += BJ_THREADS / 32) {
+    Cand c = {0ull, 0u};
+    if (lane < keep) c = entry(queue[q], lane);
+    if (c.value && !(least > c)) found[atomicAdd(&count, 1)] = c;
+  }
+  __syncthreads();
+  const int n = count;
+  for (int i = tid; i < max(n, keep); i += BJ_THREADS) {
+    const bool there = i < n;
+    int place = i;
+    Cand c = {0ull, 0u};
+    if (there) {
+      c = found[i];
+      place = 0;
+      for (int j = 0; j < n && place < keep; ++j) place += found[j] > c;
+    }
+    if (place >= keep) continue;
+    const int64_t at = batch * keep + place;
+    const int parent = there ? (int)(c.id / (uint32_t)V) : min(place, beams - 1);
+    const int64_t token = there ? (int64_t)(c.id % (uint32_t)V) : eos >= 0 ? eos : 0;
+    out_scores[at] = there ? (float)value_of(c.value) : -INFINITY;
     out_parents[at] = parent;
     out_tokens[at] = token;
     if (out_ended) out_ended[at] = over[parent] || (eos >= 0 && token == eos);
   }
 }
 
-static int64_t beam_chunks(int64_t V) { return (V + 3 + BS_CHUNK - 1) / BS_CHUNK; }
+// Chunks of 8192 logits, or of 2048 where the larger ones would not give every SM a block.
+constexpr int64_t BS_VOCAB = (1 << 20) - 8192;
+static_assert(BJ_BEAMS * ((BS_VOCAB + 3 + 8191) / 8192) <= BJ_LISTS && BS_KEEP * (BJ_LISTS / BJ_THREADS) <= BJ_FOUND, "lists of a request");
+static int beam_vecs(int64_t batch, int64_t beams, int64_t V) {
+  return batch * beams * ((V + 3 + 8191) / 8192) >= 148 || beams * ((V + 3 + 2047) / 2048) > BJ_LISTS ? 8 : 2;
+}
+static int64_t beam_chunks(int64_t batch, int64_t beams, int64_t V) {
+  const int64_t chunk = beam_vecs(batch, beams, V) * BS_THREADS * 4;
+  return (V + 3 + chunk - 1) / chunk;
+}
 
 static int beam_check(caten_b200_ctx *ctx, const char *who, int64_t batch, int64_t beams, int64_t V, int64_t keep) {
   if (batch < 0 || beams <= 0 || V <= 0 || keep <= 0) return fail(ctx, CATEN_B200_EINVAL, "%s: bad shape", who);
   if (beams > BJ_BEAMS || keep > BS_KEEP) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: %lld beams, %lld kept (at most %d)", who, (long long)beams, (long long)keep, BS_KEEP);
-  if (V > 0x7fffffffll / BJ_BEAMS) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: V=%lld", who, (long long)V);
+  if (V > BS_VOCAB) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: V=%lld", who, (long long)V);
   if (batch > 65535 || batch * beams > 65535) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: %lld rows", who, (long long)(batch * beams));
   return 0;
 }
@@ -399,7 +448,7 @@ extern "C" {
 // Arguments are checked before the context is touched.
 int64_t caten_b200_beam_select_work(int64_t batch, int64_t beams, int64_t V, int64_t keep) {
   if (beam_check(nullptr, "beam_select_work", batch, beams, V, keep)) return -1;
-  return (batch * beams * beam_chunks(V) * beam_part_words((int)keep) + 1) * (int64_t)sizeof(u64);
+  return (batch * beams * beam_chunks(batch, beams, V) * beam_part_words((int)keep) + 1) * (int64_t)sizeof(u64);
 }
 
 int caten_b200_beam_select(caten_b200_ctx *ctx, const float *d_logits, const float *d_scores, const uint8_t *d_ended, int64_t batch, int64_t beams, int64_t V,
@@ -415,8 +464,9 @@ int caten_b200_beam_select(caten_b200_ctx *ctx, const float *d_logits, const flo
   ctx->work_outside = true;
   if (batch == 0) return 0;
   ProfScope prof(ctx, CATEN_B200_K_ARGMAX);
-  const int64_t chunks = beam_chunks(V);
-  CB_CUDA(ctx, launch_k(ctx, beam_chunk_kernel, dim3((unsigned)chunks, (unsigned)(batch * beams)), dim3(BS_THREADS), 0, d_logits, d_ended, V, (int)keep, (u64 *)d_work));
+  const int64_t chunks = beam_chunks(batch, beams, V);
+  const dim3 grid((unsigned)chunks, (unsigned)(batch * beams));
+  CB_CUDA(ctx, launch_k(ctx, beam_vecs(batch, beams, V) == 8 ? beam_chunk_kernel<8> : beam_chunk_kernel<2>, grid, dim3(BS_THREADS), 0, d_logits, d_ended, V, (int)keep, (u64 *)d_work));
   CB_LAUNCH_CHECK(ctx, "beam_chunk_kernel");
   CB_CUDA(ctx, launch_k(ctx, beam_join_kernel, dim3((unsigned)batch), dim3(BJ_THREADS), 0, (const u64 *)d_work, (int)chunks, d_scores, d_ended, (int)beams, V, eos, (int)keep,
                         d_out_scores, d_out_parents, d_out_tokens, d_out_ended));

@@ -6,10 +6,12 @@
 namespace cb {
 
 // ---- page tables and slots -------------------------------------------------------------------------
-// One block does the whole plan: with a few hundred requests the work is some thousand integers and the launch is the time.  Two scans: totals
-// first, so that a plan that cannot be carried out changes nothing, then request by request the pages given back, the pages taken and the
-// tokens' slots.  A warp walks its 32 requests, lanes over pages and tokens, and skips those without any.
-constexpr int PG_THREADS = 1024;
+// Some thousand integers, so the launch and the chain of dependent loads are the time.  One block: lengths are read once, one scan gives every
+// request's pages given back, pages taken and tokens before it, and decides whether the plan can be carried out (if not, nothing changes).  Then
+// threads take single pages, and tokens, of all requests together and find the request by bisection in shared memory: a warp that walked its
+// requests one after another had their chains of loads in a row (1000 requests: 83 us).  A token's page is read from where its request took it, not
+// from the table, so slots wait for nothing that this kernel writes.  Many slots go to a grid of their own.
+constexpr int PG_MOST = 4096;     // slots that the one block writes itself
 
 struct PagesArgs {
   const int *have, *want;
@@ -17,53 +19,35 @@ struct PagesArgs {
   int requests, page, max_pages, capacity, max_tokens;
 };
 
-__device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((long long)tokens + page - 1) / page); }
+__device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((unsigned)tokens + (unsigned)page - 1u) / (unsigned)page); }   // tokens >= 0
 
-// exclusive prefix over the block of three numbers a thread; totals in sum[]
-__device__ __forceinline__ void block_scan3(int (&v)[3], int (&sum)[3], int (*warps)[32]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int inc[3];
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    inc[k] = v[k];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, inc[k], o);
-      if (lane >= o) inc[k] += up;
-    }
+// last index i of [0, n) with at[i] <= x (at ascending, at[0] = 0)
+__device__ __forceinline__ int last_not_above(const int *at, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (at[mid] <= x) lo = mid;
+    else hi = mid;
   }
-  __syncthreads();   // the last call's totals have been read
-#pragma unroll
-  for (int k = 0; k < 3; ++k)
-    if (lane == 31) warps[k][warp] = inc[k];
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    int w = warps[k][lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += up;
-    }
-    sum[k] = __shfl_sync(0xffffffffu, w, 31);
-    const int before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
-    v[k] = inc[k] - v[k] + (warp ? before : 0);
-  }
+  return lo;
 }
 
-__global__ void __launch_bounds__(PG_THREADS) kv_pages_kernel(PagesArgs a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_pages_kernel(PagesArgs a, int own_slots) {
+  __shared__ int warps[3][32];
   __shared__ long long total[3];   // tokens, pages taken, pages given back
   __shared__ int bad;
-  __shared__ int warps[3][32];
+  __shared__ int at_give[THREADS], at_take[THREADS], at_token[THREADS], first_page[THREADS], had[THREADS];
   pdl_enter();
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < 3) total[tid] = 0;
   if (tid == 3) bad = 0;
+  const int n_free = a.state[0];
   __syncthreads();
   {
     long long t[3] = {0, 0, 0};
     bool wrong = false;
-    for (int r = tid; r < a.requests; r += PG_THREADS) {
+    for (int r = tid; r < a.requests; r += THREADS) {
       const int have = a.have[r], want = a.want[r];
       if (have < 0 || want < 0 || pages_of(have, a.page) > a.max_pages || pages_of(want, a.page) > a.max_pages) { wrong = true; continue; }
       const int d = pages_of(want, a.page) - pages_of(have, a.page);
@@ -79,13 +63,11 @@ __global__ void __launch_bounds__(PG_THREADS) kv_pages_kernel(PagesArgs a) {
     }
   }
   __syncthreads();
-  const int n_free = a.state[0];
   const long long missing = total[1] - total[2] - n_free;
   int why = bad;                                                                       // 1: lengths that do not fit
   if (!why && total[0] > a.max_tokens) why = 2;                                        // more tokens than slots
   if (!why && (n_free < 0 || n_free + total[2] > a.capacity)) why = 3;                 // a free list that was not this pool's
   const bool go = !why && missing <= 0;
-  __syncthreads();   // state[0] has been read
   if (tid == 0) {
     a.state[1] = go ? (int)total[0] : 0;
     a.state[2] = !why && missing > 0 ? (int)(missing < 0x7fffffff ? missing : 0x7fffffff) : 0;
@@ -93,59 +75,105 @@ __global__ void __launch_bounds__(PG_THREADS) kv_pages_kernel(PagesArgs a) {
     if (go) a.state[0] = (int)(n_free + total[2] - total[1]);
   }
   if (!go) {
-    for (int r = tid; r <= a.requests; r += PG_THREADS) a.starts[r] = 0;
-    for (int i = tid; i < a.max_tokens; i += PG_THREADS) a.slots[i] = -1;
+    for (int r = tid; r <= a.requests; r += THREADS) a.starts[r] = 0;
+    for (int i = tid; own_slots && i < a.max_tokens; i += THREADS) a.slots[i] = -1;
     return;
   }
-  const int added = (int)total[0], top = (int)(n_free + total[2]);
-  // pages given back: behind the free ones, in the order of requests and of their pages
-  if (total[2]) {
-    int carry = 0;
-    for (int base = 0; base < a.requests; base += PG_THREADS) {
-      const int r = base + tid;
-      const int from = r < a.requests ? pages_of(a.want[r], a.page) : 0, to = r < a.requests ? pages_of(a.have[r], a.page) : 0;
-      int v[3] = {to > from ? to - from : 0, 0, 0}, sum[3];
-      block_scan3(v, sum, warps);
-      for (unsigned todo = __ballot_sync(0xffffffffu, to > from); todo; todo &= todo - 1) {
-        const int src = __ffs(todo) - 1;
-        const int f = __shfl_sync(0xffffffffu, from, src), n = __shfl_sync(0xffffffffu, to, src) - f, at = n_free + carry + __shfl_sync(0xffffffffu, v[0], src);
-        int *row = a.table + (long long)(r - lane + src) * a.max_pages + f;
-        for (int j = lane; j < n; j += 32) {
-          a.free[at + j] = row[j];
-          row[j] = -1;
+  const int top = (int)(n_free + total[2]);
+  // THREADS requests at a time.  Two rounds, because a page that one request gives back may be the one that another takes: the first appends the
+  // pages given back to the free ones, in the order of requests and of their pages; the second takes from the end.
+  for (int round = total[2] ? 0 : 1; round < 2; ++round) {
+    int carry[3] = {0, 0, 0};
+    for (int base = 0; base < a.requests; base += THREADS) {
+      const int r = base + tid, n = min(THREADS, a.requests - base);
+      const int have = r < a.requests ? a.have[r] : 0, want = r < a.requests ? a.want[r] : 0;
+      const int held = pages_of(have, a.page), wanted = pages_of(want, a.page);
+      int v[3] = {max(0, held - wanted), max(0, wanted - held), max(0, want - have)}, sum[3];
+      int inc[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        inc[k] = v[k];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, inc[k], o);
+          if (lane >= o) inc[k] += up;
         }
       }
-      carry += sum[0];
+      __syncthreads();   // the arrays of the requests before have been read
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (lane == 31) warps[k][warp] = inc[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        int w = lane < THREADS / 32 ? warps[k][lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, w, o);
+          if (lane >= o) w += up;
+        }
+        sum[k] = __shfl_sync(0xffffffffu, w, 31);
+        const int before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+        v[k] = inc[k] - v[k] + (warp ? before : 0);
+      }
+      at_give[tid] = v[0];
+      at_take[tid] = v[1];
+      at_token[tid] = v[2];
+      first_page[tid] = round ? held : wanted;   // the first that is taken (given back)
+      had[tid] = have;
+      __syncthreads();
+      if (round == 0) {
+        for (int i = tid; i < sum[0]; i += THREADS) {
+          const int q = last_not_above(at_give, n, i);
+          int *cell = a.table + (long long)(base + q) * a.max_pages + first_page[q] + i - at_give[q];
+          a.free[n_free + carry[0] + i] = *cell;
+          *cell = -1;
+        }
+      } else {
+        if (r < a.requests) a.starts[r] = carry[2] + v[2];
+        for (int i = tid; i < sum[1]; i += THREADS) {
+          const int q = last_not_above(at_take, n, i);
+          a.table[(long long)(base + q) * a.max_pages + first_page[q] + i - at_take[q]] = a.free[top - 1 - carry[1] - i];
+        }
+        for (int i = tid; own_slots && i < sum[2]; i += THREADS) {
+          const int q = last_not_above(at_token, n, i);
+          const int pos = had[q] + i - at_token[q], nth = (unsigned)pos / (unsigned)a.page;
+          const int id = nth < first_page[q] ? a.table[(long long)(base + q) * a.max_pages + nth] : a.free[top - 1 - carry[1] - at_take[q] - (nth - first_page[q])];
+          a.slots[carry[2] + i] = id >= 0 && id < a.capacity ? id * a.page + pos - nth * a.page : -1;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) carry[k] += sum[k];
     }
     __syncthreads();
   }
-  // pages taken from the end of the list, and the slots of the new tokens
-  int taken = 0, tokens = 0;
-  for (int base = 0; base < a.requests; base += PG_THREADS) {
-    const int r = base + tid;
-    const int have = r < a.requests ? a.have[r] : 0, want = r < a.requests ? a.want[r] : 0;
-    const int more = want > have ? want - have : 0, first = pages_of(have, a.page), take = more ? pages_of(want, a.page) - first : 0;
-    int v[3] = {take, more, 0}, sum[3];
-    block_scan3(v, sum, warps);
-    const int pages_before = taken + v[0], tokens_before = tokens + v[1];
-    if (r < a.requests) a.starts[r] = tokens_before;
-    for (unsigned todo = __ballot_sync(0xffffffffu, more > 0); todo; todo &= todo - 1) {
-      const int src = __ffs(todo) - 1;
-      const int f = __shfl_sync(0xffffffffu, first, src), n = __shfl_sync(0xffffffffu, take, src), p = top - 1 - __shfl_sync(0xffffffffu, pages_before, src);
-      const int start = __shfl_sync(0xffffffffu, tokens_before, src), m = __shfl_sync(0xffffffffu, more, src), h = __shfl_sync(0xffffffffu, have, src);
-      int *row = a.table + (long long)(r - lane + src) * a.max_pages;
-      for (int j = lane; j < n; j += 32) row[f + j] = a.free[p - j];
-      __syncwarp();
-      for (int i = lane; i < m; i += 32) {
-        const int at = h + i, id = row[at / a.page];
-        a.slots[start + i] = id >= 0 && id < a.capacity ? id * a.page + at % a.page : -1;
-      }
+  if (tid == 0) a.starts[a.requests] = (int)total[0];
+  for (int i = (int)total[0] + tid; own_slots && i < a.max_tokens; i += THREADS) a.slots[i] = -1;
+}
+
+// The slots of a finished plan, four tokens a thread.
+__global__ void __launch_bounds__(256) kv_slots_kernel(PagesArgs a) {
+  pdl_enter();
+  const int i0 = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i0 >= a.max_tokens) return;
+  const int added = a.state[1];
+  int r = i0 < added ? last_not_above(a.starts, a.requests, i0) : a.requests;
+  int slot[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    slot[e] = -1;
+    if (i0 + e < added) {
+      while (r + 1 < a.requests && a.starts[r + 1] <= i0 + e) ++r;   // (requests without new tokens are passed over)
+      const int pos = a.have[r] + i0 + e - a.starts[r], nth = (unsigned)pos / (unsigned)a.page;
+      const int id = a.table[(long long)r * a.max_pages + nth];
+      if (id >= 0 && id < a.capacity) slot[e] = id * a.page + pos - nth * a.page;
     }
-    taken += sum[0];
-    tokens += sum[1];
   }
-  if (tid == 0) a.starts[a.requests] = added;
-  for (int i = added + tid; i < a.max_tokens; i += PG_THREADS) a.slots[i] = -1;
+  if (i0 + 4 <= a.max_tokens && (uintptr_t)a.slots % 16 == 0) *reinterpret_cast<int4 *>(a.slots + i0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+  else
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i0 + e < a.max_tokens) a.slots[i0 + e] = slot[e];
 }
 
 // ---- rows into the cache ---------------------------------------------------------------------------
@@ -358,8 +386,13 @@ int caten_b200_kv_pages(caten_b200_ctx *ctx, const int32_t *d_have, const int32_
   ctx->work_outside = true;
   ProfScope prof(ctx, CATEN_B200_K_PREP);
   PagesArgs a = {d_have, d_want, d_table, d_free, d_state, d_starts, d_slots, (int)requests, (int)page, (int)max_pages, (int)pages, (int)max_tokens};
-  CB_CUDA(ctx, launch_k(ctx, kv_pages_kernel, dim3(1), dim3(PG_THREADS), 0, a));
+  const int own_slots = max_tokens <= PG_MOST;
+  if (requests <= 128 && own_slots) CB_CUDA(ctx, launch_k(ctx, kv_pages_kernel<128>, dim3(1), dim3(128), 0, a, own_slots));
+  else CB_CUDA(ctx, launch_k(ctx, kv_pages_kernel<1024>, dim3(1), dim3(1024), 0, a, own_slots));
   CB_LAUNCH_CHECK(ctx, "kv_pages_kernel");
+  if (own_slots) return 0;
+  CB_CUDA(ctx, launch_k(ctx, kv_slots_kernel, dim3((unsigned)((max_tokens + 1023) / 1024)), dim3(256), 0, a));
+  CB_LAUNCH_CHECK(ctx, "kv_slots_kernel");
   return 0;
 }
 

@@ -31,6 +31,8 @@ struct Kv4AttnArgs {
   Kv4Shape s;
   int heads, group, max_pages, max_new, max_length, batch;
   int row_tiles, parts, part_tokens;
+  int tile_rows;   // 8, or 1: the kernel for single rows
+  int warps;       // of that kernel, that share a unit
   float scale;
 };
 
@@ -83,15 +85,15 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
 }
 __device__ __forceinline__ float2 half_pair(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// power of two 2^(14 - floor(log2 x)), kept inside fp32's normal range; 1 for zero
-__device__ __forceinline__ float to_top(float x) {
+// power of two 2^(k - floor(log2 x)), kept inside fp32's normal range; 1 for zero
+__device__ __forceinline__ float to_top(float x, int k = 14) {
   const int e = (int)(__float_as_uint(x) >> 23 & 0xff);
   if (x == 0.0f) return 1.0f;
-  return __uint_as_float((uint32_t)min(max(127 + 14 - (e - 127), 30), 240) << 23);
+  return __uint_as_float((uint32_t)min(max(127 + k - (e - 127), 30), 240) << 23);
 }
 
 template <int NC, bool Q41>
-__global__ void __launch_bounds__(K4_WARPS * 32) kv4_attention_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(K4_WARPS * 32, NC <= 2 ? 2 : 1) kv4_attention_kernel(const Kv4AttnArgs a) {
   constexpr int NB = 2 * NC, D = 64 * NC;
   __shared__ float sm[K4_WARPS][K4_ROWS], sl[K4_WARPS][K4_ROWS];
   extern __shared__ float so[];   // [warp][row][D]
@@ -345,25 +347,361 @@ __global__ void __launch_bounds__(K4_WARPS * 32) kv4_attention_kernel(const Kv4A
   }
 }
 
+// ---- one row a sequence and key head ---------------------------------------------------------------
+// Whole numbers: codes - 8, sixteen times, are signed bytes (a mask and an exclusive or, where fp16 needs an addition besides), the other operand is
+// a fixed-point number of 31 bits in four signed bytes, each a column of its own: column 4 (block % 2) + j of the first product is digit j of q in that
+// block, zero for the other block, so that one accumulator gathers two blocks for 16 tokens and each lane scales the sums of one; in the second product
+// (32 tokens) it is digit j of p d.  Sums are exact; they start at the integer that is 1.5 * 2^23 as a float, and so need no conversion.  A score
+// ends up in one lane (64 tokens: two registers a lane), so softmax and p d are not computed eight times over as by rows that are not there.
+// What it is bound by: instructions, then HBM.  (256 x 25 heads x 768 tokens: 139 us with fp16 operands, 261 instructions for 16 tokens of 64 dims.)
+constexpr int K1_WARPS = 4;      // of a block; 1, 2 or 4 of them share a sequence and key head's tokens
+constexpr int K1_MAGIC = 0x4b400000;
+constexpr float K1_MAGIC_F = 12582912.0f;
+
+__device__ __forceinline__ void mma_16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 (code - 8) of the low (high) four bits of each byte
+__device__ __forceinline__ uint32_t bytes_lo(uint32_t w) { return (w << 4 & 0xf0f0f0f0u) ^ 0x80808080u; }
+__device__ __forceinline__ uint32_t bytes_hi(uint32_t w) { return (w & 0xf0f0f0f0u) ^ 0x80808080u; }
+__device__ __forceinline__ float sum_of(int c) { return __int_as_float(c) - K1_MAGIC_F; }
+// byte `digit` (as a selector of two words' such bytes) of four numbers below 2^30 in signed base 256
+__device__ __forceinline__ uint32_t digits_of(float x0, float x1, float x2, float x3, uint32_t pick) {
+  const uint32_t u0 = (uint32_t)__float2int_rn(x0) + 0x80808080u, u1 = (uint32_t)__float2int_rn(x1) + 0x80808080u;
+  const uint32_t u2 = (uint32_t)__float2int_rn(x2) + 0x80808080u, u3 = (uint32_t)__float2int_rn(x3) + 0x80808080u;
+  return __byte_perm(__byte_perm(u0, u1, pick), __byte_perm(u2, u3, pick), 0x5410) ^ 0x80808080u;
+}
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <int NC, bool Q41, bool WIDE>   // WIDE: pages hold 64 tokens or more
+__global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const Kv4AttnArgs a) {
+  constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART;
+  __shared__ float sm[K1_WARPS], sl[K1_WARPS];
+  __shared__ __align__(16) float so[K1_WARPS][D];
+  pdl_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int share = a.warps, first_warp = warp / share * share;
+  int64_t u = (int64_t)blockIdx.x * (K1_WARPS / share) + warp / share;
+  const int64_t unit = u;
+  const int part = (int)(u % a.parts); u /= a.parts;
+  const int head = (int)(u % a.s.kv_heads);
+  const int64_t b = u / a.s.kv_heads;
+  Kv4Seq seq = {0, 0, 0};
+  if (b < a.batch) seq = kv4_seq(a, (int)b, lane == 0 && warp == first_warp && part == 0 && head == 0);
+  const int t0 = part * a.part_tokens, t1 = seq.count ? min(seq.length, t0 + a.part_tokens) : 0;
+  const bool live = seq.count && (t0 < t1 || part == 0);
+
+  float run_max = -INFINITY, run_sum = 0.0f;   // the row's; of this lane's tokens
+  float off[NC];                               // Q4_1: sum of p (m + 8 d), block g / 4 of a pair, this lane's tokens
+  float o[NC][2][4];                           // columns 2t, 2t + 1 (digits of block t / 2) of dims 4 g + {0 | 1} and 4 g + {2 | 3}
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    off[c] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[c][i >> 2][i & 3] = 0.0f;
+  }
+  const uint32_t pick = (uint32_t)(g & 3) | (uint32_t)(4 + (g & 3)) << 4;
+  const float w0 = t & 1 ? 65536.0f : 1.0f, w1 = 256.0f * w0;
+
+  if (live && t0 + (warp - first_warp) * K4_GROUP < t1) {
+    // q's digits: this lane's column; dims 8 t + {0, 2, 4, 6} and {1, 3, 5, 7} of a block
+    uint32_t qb[NC][2][2];   // [pair][block of it][dims]
+    float qsum[NC], factor;
+    {
+      const float *q = a.q + seq.first * a.ldq + (int64_t)head * D + 8 * t + 32 * (g >> 2);
+      float x[NC][8], top = 0.0f;
+      bool finite = true;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[c][j] = q[64 * c + j];
+          top = fmaxf(top, fabsf(x[c][j]));
+          finite &= fabsf(x[c][j]) < INFINITY;
+        }
+      top = warp_max(top);
+      const float up = to_top(top, 29);
+      factor = __all_sync(0xffffffffu, finite) ? a.scale * 1.4426950408889634f * (0.0625f / up) : NAN;   // (conversions would lose a NaN)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[c][j] *= up;
+          sum += x[c][j];
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum = __shfl_sync(0xffffffffu, sum, 16 * (t >> 1)) * 16.0f;
+        qsum[c] = t & 1 ? 0.0f : sum;   // (two lanes have a block)
+        const uint32_t d0 = digits_of(x[c][0], x[c][2], x[c][4], x[c][6], pick), d1 = digits_of(x[c][1], x[c][3], x[c][5], x[c][7], pick);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          qb[c][k][0] = (g >> 2) == k ? d0 : 0u;
+          qb[c][k][1] = (g >> 2) == k ? d1 : 0u;
+        }
+      }
+    }
+    const int *table = a.table + b * a.max_pages;
+    const int64_t page_bytes = kv4_page_bytes(a.s);
+    const int tile_shift = a.s.page == 16 ? 0 : a.s.page == 32 ? 1 : a.s.page == 64 ? 2 : 3;   // tiles of a page, log2
+    const uint8_t *of_head = a.pool + (int64_t)(head << tile_shift) * TILE + lane * 16;
+    const int k_scale = 8 * D + ((g >> 1) * NB + (t >> 1)) * 8 - lane * 16, v_scale = PART + 8 * D + (t * NB + (g >> 2)) * 8 - lane * 16;
+
+    for (int base = t0 + (warp - first_warp) * K4_GROUP; base < t1; base += share * K4_GROUP) {
+      // where the four tiles are; one that cannot be followed reads the pool's first and counts for nothing
+      const uint8_t *tile[4];
+      unsigned there = 0;
+      if (WIDE) {
+        const int n = base >> 4, id = table[n >> tile_shift];
+        if (kv4_page_ok(a.s, id)) there = (1u << min(4, (t1 - base + 15) >> 4)) - 1u;
+        else if (lane == 0) report_bad_index(a.status, 46, id);
+        tile[0] = there ? of_head + id * page_bytes + (n & ((1 << tile_shift) - 1)) * TILE : a.pool + lane * 16;
+#pragma unroll
+        for (int i = 1; i < 4; ++i) tile[i] = tile[0] + i * TILE;   // (all in the page, whatever of them is in use)
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = (base >> 4) + i;
+          int id = -1;
+          if (base + 16 * i < t1) {
+            id = table[n >> tile_shift];
+            if (kv4_page_ok(a.s, id)) there |= 1u << i;
+            else if (lane == 0) report_bad_index(a.status, 46, id);
+          }
+          tile[i] = there >> i & 1 ? of_head + id * page_bytes + (n & ((1 << tile_shift) - 1)) * TILE : a.pool + lane * 16;
+        }
+      }
+      uint4 kw[4][NC], vw[4][NC];
+      uint2 kd[4][NC], vd[4][NC], km[4][NC], vm[4][NC];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          kw[i][c] = __ldcs(reinterpret_cast<const uint4 *>(tile[i] + c * 512));
+          kd[i][c] = *reinterpret_cast<const uint2 *>(tile[i] + k_scale + c * 16);
+          if (Q41) km[i][c] = *reinterpret_cast<const uint2 *>(tile[i] + k_scale + D + c * 16);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          vw[i][c] = __ldcs(reinterpret_cast<const uint4 *>(tile[i] + PART + c * 512));
+          vd[i][c] = *reinterpret_cast<const uint2 *>(tile[i] + v_scale + c * 16);
+          if (Q41) vm[i][c] = *reinterpret_cast<const uint2 *>(tile[i] + v_scale + D + c * 16);
+        }
+      // scores: tokens g and g + 8 of each tile, this lane's digits and blocks
+      float x[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i][0] = x[i][1] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          int acc[4] = {K1_MAGIC, K1_MAGIC, K1_MAGIC, K1_MAGIC};
+          const uint4 w = kw[i][c];   // tokens g (x, y) and g + 8 (z, w); even and odd block
+          const uint32_t a0[4] = {bytes_lo(w.x), bytes_lo(w.z), bytes_hi(w.x), bytes_hi(w.z)};
+          const uint32_t a1[4] = {bytes_lo(w.y), bytes_lo(w.w), bytes_hi(w.y), bytes_hi(w.w)};
+          mma_16832(acc, a0, qb[c][0][0], qb[c][0][1]);
+          mma_16832(acc, a1, qb[c][1][0], qb[c][1][1]);
+          const float2 d = half_pair(__byte_perm(kd[i][c].x, kd[i][c].y, g & 1 ? 0x7632 : 0x5410));
+          x[i][0] = fmaf(d.x, fmaf(sum_of(acc[0]), w0, sum_of(acc[1]) * w1), x[i][0]);
+          x[i][1] = fmaf(d.y, fmaf(sum_of(acc[2]), w0, sum_of(acc[3]) * w1), x[i][1]);
+          if (Q41) {
+            const float2 m = half_pair(__byte_perm(km[i][c].x, km[i][c].y, g & 1 ? 0x7632 : 0x5410));
+            x[i][0] = fmaf(fmaf(8.0f, d.x, m.x), qsum[c], x[i][0]);
+            x[i][1] = fmaf(fmaf(8.0f, d.y, m.y), qsum[c], x[i][1]);
+          }
+        }
+      }
+      // summed over the four lanes, which keep a tile each
+      float sc[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool up2 = t & 2, up1 = t & 1;
+        const float y0 = (up2 ? x[2][e] : x[0][e]) + __shfl_xor_sync(0xffffffffu, up2 ? x[0][e] : x[2][e], 2);
+        const float y1 = (up2 ? x[3][e] : x[1][e]) + __shfl_xor_sync(0xffffffffu, up2 ? x[1][e] : x[3][e], 2);
+        const float z = (up1 ? y1 : y0) + __shfl_xor_sync(0xffffffffu, up1 ? y0 : y1, 1);
+        sc[e] = z * factor;
+      }
+      if (base + K4_GROUP > t1 || there != 15u) {
+        // what stands behind the last token may be anything: it has no score, and its values' scales are none
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (base + 16 * t + g + 8 * e >= t1 || !(there >> t & 1)) sc[e] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = base + 16 * i + 2 * t;
+          const bool ok = there >> i & 1;
+          const uint32_t keep0 = (ok && at < t1 ? 0xffffu : 0u) | (ok && at + 1 < t1 ? 0xffff0000u : 0u);
+          const uint32_t keep1 = (ok && at + 8 < t1 ? 0xffffu : 0u) | (ok && at + 9 < t1 ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            vd[i][c].x &= keep0;
+            vd[i][c].y &= keep1;
+            if (Q41) { vm[i][c].x &= keep0; vm[i][c].y &= keep1; }
+          }
+        }
+      }
+      const float top = fmaxf(run_max, warp_max(fmaxf(sc[0], sc[1])));
+      const float ref = top == -INFINITY ? 0.0f : top;
+      const float corr = exp2_fast(run_max - ref);
+      run_max = top;
+      sc[0] = exp2_fast(sc[0] - ref);
+      sc[1] = exp2_fast(sc[1] - ref);
+      run_sum = fmaf(run_sum, corr, sc[0] + sc[1]);
+      float p[4][4];   // tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each tile
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i][0] = __shfl_sync(0xffffffffu, sc[0], 8 * t + i);
+        p[i][1] = __shfl_sync(0xffffffffu, sc[0], 8 * t + 4 + i);
+        p[i][2] = __shfl_sync(0xffffffffu, sc[1], 8 * t + i);
+        p[i][3] = __shfl_sync(0xffffffffu, sc[1], 8 * t + 4 + i);
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        __half2 big = __float2half2_rn(0.0f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          big = __hmax2_nan(big, __habs2(*reinterpret_cast<const __half2 *>(&vd[i][c].x)));
+          big = __hmax2_nan(big, __habs2(*reinterpret_cast<const __half2 *>(&vd[i][c].y)));
+        }
+        const uint32_t bw = *reinterpret_cast<const uint32_t *>(&big);   // (as whole numbers: a NaN is above infinity)
+        uint32_t most = max(bw & 0xffffu, bw >> 16);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const float up = to_top(__half2float(__ushort_as_half((unsigned short)most)), 29);
+        float add = 0.0f;
+        uint32_t digits[4];   // of the four tiles
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 d01 = half_pair(vd[i][c].x), d23 = half_pair(vd[i][c].y);
+          if (Q41) {
+            const float2 m01 = half_pair(vm[i][c].x), m23 = half_pair(vm[i][c].y);
+            add = fmaf(p[i][0], fmaf(8.0f, d01.x, m01.x), add);
+            add = fmaf(p[i][1], fmaf(8.0f, d01.y, m01.y), add);
+            add = fmaf(p[i][2], fmaf(8.0f, d23.x, m23.x), add);
+            add = fmaf(p[i][3], fmaf(8.0f, d23.y, m23.y), add);
+          }
+          digits[i] = digits_of(p[i][0] * (d01.x * up), p[i][1] * (d01.y * up), p[i][2] * (d23.x * up), p[i][3] * (d23.y * up), pick);
+        }
+        if (Q41) off[c] = fmaf(off[c], corr, add);
+        int acc[2][4] = {{K1_MAGIC, K1_MAGIC, K1_MAGIC, K1_MAGIC}, {K1_MAGIC, K1_MAGIC, K1_MAGIC, K1_MAGIC}};
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {   // 32 tokens
+          uint32_t bytes[2][4];            // of the lane's four tokens: dims 4 g + {0, 1} and {2, 3} of the even block, of the odd one
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 w = vw[i + h][c];
+            const uint32_t e0 = __byte_perm(w.x, w.y, 0x5140), e1 = __byte_perm(w.z, w.w, 0x5140);
+            const uint32_t o0 = __byte_perm(w.x, w.y, 0x7362), o1 = __byte_perm(w.z, w.w, 0x7362);
+            bytes[h][0] = __byte_perm(e0, e1, 0x5410);
+            bytes[h][1] = __byte_perm(e0, e1, 0x7632);
+            bytes[h][2] = __byte_perm(o0, o1, 0x5410);
+            bytes[h][3] = __byte_perm(o0, o1, 0x7632);
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t b0 = (g >> 2) == k ? digits[i] : 0u, b1 = (g >> 2) == k ? digits[i + 1] : 0u;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const uint32_t av[4] = {bytes_lo(bytes[0][2 * k + n]), bytes_hi(bytes[0][2 * k + n]), bytes_lo(bytes[1][2 * k + n]), bytes_hi(bytes[1][2 * k + n])};
+              mma_16832(acc[n], av, b0, b1);
+            }
+          }
+        }
+        // (a scale that is not finite makes its block's values NaN, as it does in the formula)
+        const float down = __shfl_sync(0xffffffffu, most < 0x7c00u ? 0.0625f / up : NAN, 16 * (t >> 1));
+        const float f0 = down * w0, f1 = down * w1;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[c][n][e] = fmaf(o[c][n][e], corr, sum_of(acc[n][e]) * (e & 1 ? f1 : f0));
+      }
+    }
+  }
+
+  // digits and lanes together: both lanes of a block get its four dims, one writes the first two, the other the last
+  run_sum = warp_sum(run_sum);
+  float2 r[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    float y[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        y[n][e] = o[c][n][2 * e] + o[c][n][2 * e + 1];
+        y[n][e] += __shfl_xor_sync(0xffffffffu, y[n][e], 1);
+      }
+    r[c] = t & 1 ? make_float2(y[1][0], y[1][1]) : make_float2(y[0][0], y[0][1]);
+    if (Q41) {
+      off[c] += __shfl_xor_sync(0xffffffffu, off[c], 1);
+      off[c] += __shfl_xor_sync(0xffffffffu, off[c], 2);
+      const float add = __shfl_sync(0xffffffffu, off[c], 16 * (t >> 1));
+      r[c].x += add;
+      r[c].y += add;
+    }
+  }
+  const int at = 32 * (t >> 1) + 4 * g + 2 * (t & 1);   // of a pair of blocks
+  float top = run_max, sum = run_sum;
+  if (share > 1) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) *reinterpret_cast<float2 *>(&so[warp][64 * c + at]) = r[c];
+    if (lane == 0) { sm[warp] = run_max; sl[warp] = run_sum; }
+    __syncthreads();
+    if (warp != first_warp) return;
+    for (int w = warp + 1; w < warp + share; ++w) top = fmaxf(top, sm[w]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) r[c] = make_float2(0.0f, 0.0f);
+    for (int w = warp; w < warp + share; ++w) {
+      const float e = exp2_fast(sm[w] - ref);
+      sum = fmaf(sl[w], e, sum);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const float2 y = *reinterpret_cast<const float2 *>(&so[w][64 * c + at]);
+        r[c].x = fmaf(y.x, e, r[c].x);
+        r[c].y = fmaf(y.y, e, r[c].y);
+      }
+    }
+  }
+  if (!live) return;
+  float *dst = a.parts == 1 ? a.out + seq.first * a.heads * D + (int64_t)head * D : a.part + unit * (D + 2);
+  const float scale = a.parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    dst[64 * c + at] = r[c].x * scale;
+    dst[64 * c + at + 1] = r[c].y * scale;
+  }
+  if (a.parts > 1 && lane == 0) { dst[D] = top; dst[D + 1] = sum; }
+}
+
 // The parts of a row tile into one.  A block has a row tile; parts behind what its rows see were not written.
 __global__ void __launch_bounds__(256) kv4_attention_join_kernel(const Kv4AttnArgs a) {
   pdl_enter();
-  const int D = a.s.dim;
+  const int D = a.s.dim, tile_rows = a.tile_rows;
   int64_t u = blockIdx.x;
   const int rt = (int)(u % a.row_tiles); u /= a.row_tiles;
   const int head = (int)(u % a.s.kv_heads);
   const int b = (int)(u / a.s.kv_heads);
   const Kv4Seq seq = kv4_seq(a, b, false);
   const int count = seq.count * a.group;
-  if (rt * K4_ROWS >= count) return;
-  const int last = min(count, rt * K4_ROWS + K4_ROWS) - 1;
+  if (rt * tile_rows >= count) return;
+  const int last = min(count, rt * tile_rows + tile_rows) - 1;
   const int most = max(0, seq.length - seq.count + last / a.group + 1);
   const int parts = max(1, (most + a.part_tokens - 1) / a.part_tokens);
-  for (int i = threadIdx.x; i < K4_ROWS * D; i += 256) {
-    const int row = i / D, j = i % D, rr = rt * K4_ROWS + row;
+  for (int i = threadIdx.x; i < tile_rows * D; i += 256) {
+    const int row = i / D, j = i % D, rr = rt * tile_rows + row;
     if (rr >= count) break;
-    const float *p = a.part + (int64_t)blockIdx.x * a.parts * K4_ROWS * (D + 2) + row * (D + 2);
-    const int64_t step = (int64_t)K4_ROWS * (D + 2);
+    const float *p = a.part + (int64_t)blockIdx.x * a.parts * tile_rows * (D + 2) + row * (D + 2);
+    const int64_t step = (int64_t)tile_rows * (D + 2);
     float top = -INFINITY;
     for (int k = 0; k < parts; ++k) top = fmaxf(top, p[k * step + D]);
     const float ref = top == -INFINITY ? 0.0f : top;
@@ -377,10 +715,10 @@ __global__ void __launch_bounds__(256) kv4_attention_join_kernel(const Kv4AttnAr
   }
 }
 
-// How a call is cut: row tiles of 8, and parts of the tokens where row tiles alone leave SMs idle.  By sizes that the host knows.
+// How a call is cut: row tiles, and parts of the tokens where row tiles alone leave SMs idle.  By sizes that the host knows.
 struct Kv4Plan {
   int64_t units;   // row tiles of all sequences and key heads
-  int row_tiles, parts, part_tokens;
+  int tile_rows, row_tiles, parts, part_tokens, warps;
 };
 static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_desc *c, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length, Kv4Plan *p) {
   Kv4Shape s;
@@ -388,12 +726,16 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
   if (batch < 0 || batch > (1 << 24) || rows < 0 || rows > 0x7fffffff || max_new <= 0 || max_length < 0 || max_length > 0x3fffffff) return fail(ctx, CATEN_B200_EINVAL, "%s: bad shape", who);
   const int64_t group = c->heads / c->kv_heads;
   if (max_new > (1 << 24) || max_new * group > 0x3fffffff) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: %lld new tokens of a sequence", who, (long long)max_new);
-  p->row_tiles = (int)((max_new * group + K4_ROWS - 1) / K4_ROWS);
+  p->tile_rows = max_new * group == 1 ? 1 : K4_ROWS;
+  p->row_tiles = (int)((max_new * group + p->tile_rows - 1) / p->tile_rows);
   if (batch && (int64_t)c->kv_heads * p->row_tiles > 0x7fffffff / batch) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
   p->units = batch * c->kv_heads * p->row_tiles;
   const int64_t groups = (max_length + K4_GROUP - 1) / K4_GROUP;
-  int64_t parts = p->units ? (148 * 3 + p->units - 1) / p->units : 1;
-  const int64_t most = (groups + 2 * K4_WARPS - 1) / (2 * K4_WARPS);   // a part gives each warp two groups at least
+  // single rows: a warp each where that is enough to fill the SMs (20 warps an SM), otherwise four
+  p->warps = p->tile_rows > 1 ? K4_WARPS : p->units >= 148 * 16 ? 1 : K1_WARPS;
+  const int64_t fill = p->tile_rows > 1 ? 148 * 3 : 148 * 20 / p->warps;
+  int64_t parts = p->units ? (fill + p->units - 1) / p->units : 1;
+  const int64_t most = (groups + 2 * p->warps - 1) / (2 * p->warps);   // a part gives each warp two groups at least
   if (parts > most) parts = most;
   if (parts < 1) parts = 1;
   const int64_t each = groups ? (groups + parts - 1) / parts : 1;
@@ -405,10 +747,17 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
 
 template <int NC, bool Q41>
 static int kv4_attention_launch(caten_b200_ctx *ctx, const Kv4AttnArgs &a, int64_t units) {
-  const int smem = K4_WARPS * K4_ROWS * NC * 64 * (int)sizeof(float);
-  CB_CUDA(ctx, cudaFuncSetAttribute(kv4_attention_kernel<NC, Q41>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  CB_CUDA(ctx, launch_k(ctx, kv4_attention_kernel<NC, Q41>, dim3((unsigned)(units * a.parts)), dim3(K4_WARPS * 32), smem, a));
-  CB_LAUNCH_CHECK(ctx, "kv4_attention_kernel");
+  if (a.tile_rows == 1) {
+    const int64_t per_block = K1_WARPS / a.warps;
+    CB_CUDA(ctx, launch_k(ctx, a.s.page >= K4_GROUP ? kv4_attention_row_kernel<NC, Q41, true> : kv4_attention_row_kernel<NC, Q41, false>,
+                          dim3((unsigned)((units * a.parts + per_block - 1) / per_block)), dim3(K1_WARPS * 32), 0, a));
+    CB_LAUNCH_CHECK(ctx, "kv4_attention_row_kernel");
+  } else {
+    const int smem = K4_WARPS * K4_ROWS * NC * 64 * (int)sizeof(float);
+    CB_CUDA(ctx, cudaFuncSetAttribute(kv4_attention_kernel<NC, Q41>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    CB_CUDA(ctx, launch_k(ctx, kv4_attention_kernel<NC, Q41>, dim3((unsigned)(units * a.parts)), dim3(K4_WARPS * 32), smem, a));
+    CB_LAUNCH_CHECK(ctx, "kv4_attention_kernel");
+  }
   if (a.parts == 1) return 0;
   CB_CUDA(ctx, launch_k(ctx, kv4_attention_join_kernel, dim3((unsigned)units), dim3(256), 0, a));
   CB_LAUNCH_CHECK(ctx, "kv4_attention_join_kernel");
@@ -425,7 +774,7 @@ extern "C" {
 int64_t caten_b200_kv4_attention_work(const caten_b200_kv4_desc *desc, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length) {
   Kv4Plan p;
   if (kv4_plan(nullptr, "kv4_attention_work", desc, batch, rows, max_new, max_length, &p)) return -1;
-  return p.parts > 1 ? p.units * p.parts * K4_ROWS * (desc->dim + 2) * (int64_t)sizeof(float) : 16;
+  return p.parts > 1 ? p.units * p.parts * p.tile_rows * (desc->dim + 2) * (int64_t)sizeof(float) : 16;
 }
 
 int caten_b200_kv4_attention(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, const float *d_q, int64_t ldq, const void *d_pool, const int32_t *d_table,
@@ -453,7 +802,7 @@ int caten_b200_kv4_attention(caten_b200_ctx *ctx, const caten_b200_kv4_desc *des
   a.out = d_out; a.part = (float *)d_work; a.status = ctx->d_status;
   a.heads = desc->heads; a.group = desc->heads / desc->kv_heads;
   a.max_pages = (int)max_pages; a.max_new = (int)max_new; a.max_length = (int)max_length; a.batch = (int)batch;
-  a.row_tiles = p.row_tiles; a.parts = p.parts; a.part_tokens = p.part_tokens;
+  a.tile_rows = p.tile_rows; a.warps = p.warps; a.row_tiles = p.row_tiles; a.parts = p.parts; a.part_tokens = p.part_tokens;
   a.scale = desc->scale;
   const bool q41 = a.s.q41;
   switch (desc->dim / 64) {

@@ -12,12 +12,16 @@ through CFFI is ``lisp/b200.lisp`` at the top of this repository.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Optional, Sequence
 
 import numpy as np
 
 from . import _lib as L
 from .synthetic import Packed
+
+
+F32, I32, I64, U8 = (np.dtype(t) for t in (np.float32, np.int32, np.int64, np.uint8))
 
 
 class B200Buffer:
@@ -28,7 +32,7 @@ class B200Buffer:
 
     @property
     def nbytes(self) -> int:
-        return int(np.prod(self.shape, dtype=np.int64)) * self.dtype.itemsize
+        return math.prod(self.shape) * self.dtype.itemsize
 
     def numpy(self) -> np.ndarray:
         return self.runtime.transfer_into_array(self)
@@ -282,14 +286,17 @@ class B200Runtime:
         """The ``keep`` best continuations of each request's hypotheses (``caten_b200_beam_select``).  logits [batch * beams, V], scores
         [batch, beams], ended [batch, beams] uint8; returns (scores, parents int32, tokens int64, ended uint8), each [batch, keep]."""
         (B, beams), V = scores.shape, logits.shape[-1]
-        if int(np.prod(logits.shape[:-1], dtype=np.int64)) != B * beams or (ended is not None and ended.shape != scores.shape):
+        if math.prod(logits.shape[:-1]) != B * beams or (ended is not None and ended.shape != scores.shape):
             raise ValueError(f"beam_select: logits {logits.shape} and ended {ended and ended.shape} for scores {scores.shape}")
-        _kinds("beam_select", (logits, np.float32), (scores, np.float32), (ended, np.uint8))
         need = self.beam_select_work(B, beams, V, keep)
-        out = out or tuple(self.open_buffer((B, keep), t) for t in (np.float32, np.int32, np.int64, np.uint8))
-        if any(b is not None and b.shape != (B, keep) for b in out):
-            raise ValueError(f"beam_select: outputs are [{B}, {keep}]")
-        _kinds("beam_select", *zip(out, (np.float32, np.int32, np.int64, np.uint8)))
+        out = out or tuple(self.open_buffer((B, keep), t) for t in (F32, I32, I64, U8))
+        for b in out:
+            if b is not None and b.shape != (B, keep):
+                raise ValueError(f"beam_select: outputs are [{B}, {keep}]")
+        _kinds("beam_select", F32, logits, scores, out[0])
+        _kinds("beam_select", I32, out[1])
+        _kinds("beam_select", I64, out[2])
+        _kinds("beam_select", U8, ended, out[3])
         own = None if work else self.open_buffer(need, np.uint8)
         _room("beam_select", work or own, need)
         L.check(self.ctx, self.lib.caten_b200_beam_select(self.ctx, logits.ptr, scores.ptr, ended.ptr if ended else None, B, beams, V, eos, keep,
@@ -308,7 +315,7 @@ class B200Runtime:
         size = states[0].dtype.itemsize
         if n != groups * beams or not 0 <= positions <= T or any(b.shape != states[0].shape or b.dtype != states[0].dtype for b in states):
             raise ValueError(f"beam_reorder: states like {states[0].shape}, {positions} positions, parents {parents.shape}")
-        _kinds("beam_reorder", (parents, np.int32))
+        _kinds("beam_reorder", I32, parents)
         arr = (C.c_void_p * len(states))(*[b.ptr for b in states])
         L.check(self.ctx, self.lib.caten_b200_beam_reorder(self.ctx, arr, len(states), parents.ptr, groups, beams, H, T * X * size, positions * X * size))
 
@@ -318,7 +325,7 @@ class B200Runtime:
         groups, beams = parents.shape
         if len(pool.shape) != 2 or table.shape[0] != groups * beams or lengths.shape != (groups * beams,):
             raise ValueError(f"beam_reorder_pages: pool {pool.shape}, table {table.shape}, lengths {lengths.shape}, parents {parents.shape}")
-        _kinds("beam_reorder_pages", (table, np.int32), (lengths, np.int32), (parents, np.int32))
+        _kinds("beam_reorder_pages", I32, table, lengths, parents)
         L.check(self.ctx, self.lib.caten_b200_beam_reorder_pages(self.ctx, pool.ptr, pool.shape[0], pool.shape[1] * pool.dtype.itemsize, table.ptr, table.shape[1],
                                                                  lengths.ptr, page, parents.ptr, groups, beams))
 
@@ -336,7 +343,7 @@ class B200Runtime:
         n = have.shape[0]
         if have.shape != (n,) or want.shape != (n,) or table.shape[0] != n or starts.shape != (n + 1,) or state.shape != (4,):
             raise ValueError(f"kv_pages: have {have.shape}, want {want.shape}, table {table.shape}, starts {starts.shape}, state {state.shape}")
-        _kinds("kv_pages", *((b, np.int32) for b in (have, want, table, free, state, starts, slots)))
+        _kinds("kv_pages", I32, have, want, table, free, state, starts, slots)
         L.check(self.ctx, self.lib.caten_b200_kv_pages(self.ctx, have.ptr, want.ptr, n, page, table.ptr, table.shape[1], free.ptr, free.shape[0], state.ptr,
                                                        starts.ptr, slots.ptr, slots.shape[0]))
 
@@ -359,7 +366,8 @@ class B200Runtime:
         shape = (slots.shape[0], desc.kv_heads * desc.dim)
         if k.shape != shape or v.shape != shape:
             raise ValueError(f"{who}: k {k.shape} and v {v.shape}, expected {shape}")
-        _kinds(who, (k, np.float32), (v, np.float32), (slots, np.int32))
+        _kinds(who, F32, k, v)
+        _kinds(who, I32, slots)
         _room(who, pool, self.lib.caten_b200_kv4_nbytes(C.byref(desc)))
 
     def kv4_attention_work(self, desc: L.Kv4Desc, batch: int, rows: int, max_new: int, max_length: int) -> int:
@@ -382,7 +390,8 @@ class B200Runtime:
         out = out or self.open_buffer((rows, width))
         if out.shape != (rows, width):
             raise ValueError(f"kv4_attention: out {out.shape}, expected {(rows, width)}")
-        _kinds("kv4_attention", (q, np.float32), (out, np.float32), (table, np.int32), (lengths, np.int32), (starts, np.int32))
+        _kinds("kv4_attention", F32, q, out)
+        _kinds("kv4_attention", I32, table, lengths, starts)
         _room("kv4_attention", pool, self.lib.caten_b200_kv4_nbytes(C.byref(desc)))
         own = None if work else self.open_buffer(need, np.uint8)
         _room("kv4_attention", work or own, need)
@@ -393,10 +402,10 @@ class B200Runtime:
         return out
 
 
-def _kinds(who, *pairs):
-    for b, kind in pairs:
-        if b is not None and b.dtype != kind:
-            raise ValueError(f"{who}: a buffer of {b.dtype} where {np.dtype(kind)} is expected")
+def _kinds(who, kind, *bufs):
+    for b in bufs:
+        if b is not None and b.dtype is not kind and b.dtype != kind:
+            raise ValueError(f"{who}: a buffer of {b.dtype} where {kind} is expected")
 
 
 def _room(who, buf, need):

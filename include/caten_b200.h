@@ -247,7 +247,7 @@ int caten_b200_rope(caten_b200_ctx *ctx, const float *d_x, float *d_y, int64_t B
  * equal ones in the order of b * V + v: values rounded to fp32, the beam each goes on from, its token, and (d_out_ended not NULL) whether it has
  * ended.  The order is decided in 64 bits.  Candidates whose value is -inf or NaN (masked tokens, hypotheses with score -inf, rows with a NaN
  * or +inf) are never taken; place i that none is left for has score -inf, parent min(i, beams - 1) and token eos (0 without one).
- * beams, keep <= 32; batch * beams <= 65535; eos < 0: none (d_ended NULL).  Outputs [batch, keep]; they do not overlap the inputs.
+ * beams, keep <= 32; V <= 1040384; batch * beams <= 65535; eos < 0: none (d_ended NULL).  Outputs [batch, keep]; they do not overlap the inputs.
  * d_work: beam_select_work(..) bytes, 8-byte aligned, nothing of which is kept from call to call; calls that may overlap on the GPU need one
  * each.  beam_select_work is -1 for a call that would be refused. */
 int64_t caten_b200_beam_select_work(int64_t batch, int64_t beams, int64_t V, int64_t keep);

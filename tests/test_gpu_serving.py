@@ -259,7 +259,8 @@ LENGTHS = [1, 15, 16, 17, 0, 63, 64, 65, 130, 257]
 
 
 @pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
-@pytest.mark.parametrize("dim,page,heads,kv", [(64, 64, 25, 25), (64, 16, 4, 1), (128, 32, 6, 2), (128, 128, 16, 2), (192, 16, 3, 3), (256, 64, 10, 1)])
+@pytest.mark.parametrize("dim,page,heads,kv", [(64, 64, 25, 25), (64, 16, 4, 1), (128, 32, 6, 2), (128, 128, 16, 2), (192, 16, 3, 3), (256, 64, 10, 1),
+                                                (64, 32, 1, 1), (128, 32, 3, 3), (256, 16, 2, 2), (256, 128, 1, 1)])
 def test_single_tokens(rt, kind, dim, page, heads, kv):
     rng = rng_of(dim, page, heads)
     c = Cache(rt, rng, kind, dim, page, heads, kv, LENGTHS)
@@ -406,7 +407,7 @@ def check_select(rt, logits, scores, keep, ended=None, eos=-1, shift=0):
 
 
 @pytest.mark.parametrize("groups,beams,V,keep", [(1, 1, 1, 1), (1, 1, 7, 3), (2, 3, 2, 8), (3, 4, 50257, 4), (2, 5, 32000, 10), (1, 32, 1003, 32), (7, 2, 8192, 31), (1, 16, 8189, 32),
-                                                 (1, 8, 130001, 16), (65, 1, 300, 2)])
+                                                 (1, 8, 130001, 16), (65, 1, 300, 2), (1, 32, 40000, 32), (1, 3, 1040384, 9), (20, 8, 20000, 16)])
 def test_selection(rt, groups, beams, V, keep):
     rng = rng_of(groups, beams, V, keep)
     logits = rng.standard_normal((groups, beams, V), dtype=np.float32) * 3
@@ -430,6 +431,9 @@ def test_selection_of_equal_values_takes_the_lowest_index(rt):
     rng = rng_of(41)
     few = rng.integers(0, 3, (2, beams, V)).astype(np.float32)             # a few values, many times each
     check_select(rt, few, np.zeros((2, beams)), 32)
+    for groups, beams, V in ((60, 2, 9000), (1, 32, 20000)):                # larger chunks; more lists than threads
+        check_select(rt, rng.integers(0, 2, (groups, beams, V)).astype(np.float32), np.zeros((groups, beams)), 32)
+        check_select(rt, np.zeros((groups, beams, V)), np.zeros((groups, beams)), 32)
 
 
 @pytest.mark.parametrize("order", ["up", "down"])
