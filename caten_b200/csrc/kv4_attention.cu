@@ -14,10 +14,11 @@
 // to the running sums in fp32.
 #include "common.cuh"
 #include "kv4.cuh"
+#include "tcgen05.cuh"
 
 namespace cb {
 
-constexpr int K4_WARPS = 8;        // of a block; they share a row tile's tokens, 64 at a time
+constexpr int K4_WARPS = 4;        // of a block
 constexpr int K4_GROUP = 64;       // tokens
 constexpr int K4_ROWS = 8;
 
@@ -32,7 +33,7 @@ struct Kv4AttnArgs {
   int heads, group, max_pages, max_new, max_length, batch;
   int row_tiles, parts, part_tokens;
   int tile_rows;   // 8, or 1: the kernel for single rows
-  int warps;       // of that kernel, that share a unit
+  int warps;       // single rows: warps that share a unit; otherwise row tiles of a block
   float scale;
 };
 
@@ -92,29 +93,70 @@ __device__ __forceinline__ float to_top(float x, int k = 14) {
   return __uint_as_float((uint32_t)min(max(127 + k - (e - 127), 30), 240) << 23);
 }
 
+// A block's four warps are `row_warps` row tiles times 4 / row_warps shares of the tokens.  The warps of a share work on one ring of two stages of 64
+// tokens, which bulk copies fill while the other is read (each stage is read by all its warps before it is filled again).
 template <int NC, bool Q41>
-__global__ void __launch_bounds__(K4_WARPS * 32, NC <= 2 ? 2 : 1) kv4_attention_kernel(const Kv4AttnArgs a) {
-  constexpr int NB = 2 * NC, D = 64 * NC;
+__global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) kv4_attention_kernel(const Kv4AttnArgs a) {
+  constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, STAGE = 4 * TILE;
   __shared__ float sm[K4_WARPS][K4_ROWS], sl[K4_WARPS][K4_ROWS];
-  extern __shared__ float so[];   // [warp][row][D]
+  __shared__ uint64_t bars[K4_WARPS][2];
+  __shared__ int gave_up[K4_WARPS];
+  __shared__ unsigned present[K4_WARPS][2];          // of a share: tiles of each stage
+  extern __shared__ __align__(128) uint8_t ring[];   // two stages a share; behind the last group, the warps' sums
   pdl_enter();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int lane = threadIdx.x & 31, warp = warp_index(), g = lane >> 2, t = lane & 3;
+  const int row_warps = a.warps, shares = K4_WARPS / row_warps, share = warp / row_warps, sub = warp % row_warps;
   int64_t u = blockIdx.x;
   const int part = (int)(u % a.parts); u /= a.parts;
-  const int rt = (int)(u % a.row_tiles); u /= a.row_tiles;
+  const int row_groups = (a.row_tiles + row_warps - 1) / row_warps;
+  const int rg = (int)(u % row_groups); u /= row_groups;
   const int head = (int)(u % a.s.kv_heads);
   const int b = (int)(u / a.s.kv_heads);
-  const Kv4Seq seq = kv4_seq(a, b, threadIdx.x == 0 && part == 0 && rt == 0 && head == 0);
+  const Kv4Seq seq = kv4_seq(a, b, threadIdx.x == 0 && part == 0 && rg == 0 && head == 0);
   const int count = seq.count * a.group;   // rows of this key head
-  if (rt * K4_ROWS >= count) return;
-  // row g of the tile: token r / group, query head head * group + r % group
-  const int r = rt * K4_ROWS + g;
-  const int tok = r / a.group;
-  const int sees = r < count ? max(0, seq.length - seq.count + tok + 1) : 0;   // tokens before and at its position
-  const int last = min(count, rt * K4_ROWS + K4_ROWS) - 1;
-  const int most = max(0, seq.length - seq.count + last / a.group + 1);
-  const int t0 = part * a.part_tokens, t1 = min(most, t0 + a.part_tokens);
+  if (rg * row_warps * K4_ROWS >= count) return;
+  // row r: token r / group, query head head * group + r % group
+  const int rt = rg * row_warps + sub, r = rt * K4_ROWS + g, tok = r / a.group;
+  auto sees_of = [&](int row) { return row < count ? max(0, seq.length - seq.count + row / a.group + 1) : 0; };   // tokens before and at its position
+  const int sees = sees_of(r), least = sees_of(rt * K4_ROWS), most = sees_of(min(count, rt * K4_ROWS + K4_ROWS) - 1);   // (least: 0 for a tile without rows)
+  const int reach = sees_of(min(count, (rg + 1) * row_warps * K4_ROWS) - 1);   // of the block
+  const int t0 = part * a.part_tokens, t1 = min(reach, t0 + a.part_tokens);
   if (t0 >= t1 && part > 0) return;
+  const bool mine = rt * K4_ROWS < count;
+
+  const uint32_t bar = smem_u32(&bars[share][0]);
+  uint8_t *const stages = ring + share * 2 * STAGE;
+  const int *table = a.table + (int64_t)b * a.max_pages;
+  const int64_t page_bytes = kv4_page_bytes(a.s);
+  const int tile_shift = a.s.page == 16 ? 0 : a.s.page == 32 ? 1 : a.s.page == 64 ? 2 : 3;   // tiles of a page, log2
+  const int first = t0 + share * K4_GROUP, step = shares * K4_GROUP;
+  // by the share's first warp, lanes over tiles: what can be followed is copied, the rest counts for nothing
+  auto page_at = [&](int base) { return lane < 4 && base + 16 * lane < t1 ? table[((base >> 4) + lane) >> tile_shift] : -1; };
+  auto issue = [&](int base, int id, int stage) {
+    const bool wanted = lane < 4 && base + 16 * lane < t1, good = wanted && kv4_page_ok(a.s, id);
+    if (wanted && !good) report_bad_index(a.status, 46, id);
+    const unsigned there = __ballot_sync(0xffffffffu, good);
+    if (lane == 0) {
+      present[share][stage] = there;
+      mbar_expect_tx(bar + 8 * stage, __popc(there) * TILE);   // (its arrival publishes `present`)
+    }
+    __syncwarp();
+    if (good) bulk_load(smem_u32(stages) + stage * STAGE + lane * TILE,
+                        a.pool + id * page_bytes + ((int64_t)(head << tile_shift) + (((base >> 4) + lane) & ((1 << tile_shift) - 1))) * TILE, TILE, bar + 8 * stage);
+  };
+  int id_next = -1;
+  if (sub == 0) {
+    if (lane == 0) {
+      mbar_init(bar, 1);
+      mbar_init(bar + 8, 1);
+      gave_up[share] = 0;
+      fence_proxy_async();
+    }
+    __syncwarp();
+    if (first < t1) issue(first, page_at(first), 0);
+    if (first + step < t1) issue(first + step, page_at(first + step), 1);
+    id_next = page_at(first + 2 * step);
+  }
 
   // q as the first product's operand: a block's two steps, {dims 8t + 0, 4 | 8t + 1, 5} and {2, 6 | 3, 7}; hi in rows g, lo in rows g + 8
   uint32_t qa[NB][2][4];
@@ -142,9 +184,11 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC <= 2 ? 2 : 1) kv4_attention_
         x[k][j] *= up;
         sum += x[k][j];
       }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      qsum[k] = sum;
+      if (Q41) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        qsum[k] = sum;
+      }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         qa[k][st][0] = pack_half(x[k][2 * st], x[k][2 * st + 4]);
@@ -164,186 +208,234 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC <= 2 ? 2 : 1) kv4_attention_
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] = 0.0f;
   }
-
-  const int part_bytes = kv4_part_bytes(a.s), tile_bytes = 2 * part_bytes;
-  for (int base = t0 + warp * K4_GROUP; base < t1; base += K4_WARPS * K4_GROUP) {
-    float s[4][4];
-    const uint8_t *tile[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = base + 16 * i;
-      tile[i] = nullptr;
-      if (at < t1) {
-        const int id = a.table[(int64_t)b * a.max_pages + at / a.s.page];
-        if (kv4_page_ok(a.s, id)) tile[i] = a.pool + kv4_tile_at(a.s, id, head, at % a.s.page);
-        else if (lane == 0) report_bad_index(a.status, 46, id);
-      }
+  __syncthreads();   // the barriers are there
+  int stage = 0;
+  uint32_t phase = 0;
+  bool all_ok = true;
+  for (int base = first; base < t1; base += step) {
+    // (a wait that runs out does not leave the loop: the share's warps meet below as often as each other, and further waits give up at once)
+    const bool ok = mbar_wait(bar + 8 * stage, phase, &gave_up[share]);
+    if (!ok && lane == 0) {
+      gave_up[share] = 1;
+      atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
+      a.status[1] = 48;
     }
+    all_ok &= ok;
+    if (ok && mine && base < most) {
+      const uint8_t *tiles = stages + stage * STAGE;
+      const unsigned there = present[share][stage];
+      const bool clean = base + K4_GROUP <= least && there == 15u;   // every row sees every token
+      float s[4][4];
+      __half2 big = __float2half2_rn(0.0f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t *tile = tiles + i * TILE;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = -INFINITY;
-      if (!tile[i]) continue;   // (the same for all lanes)
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < NC; ++c) {
+          const uint4 w = *reinterpret_cast<const uint4 *>(tile + c * 512 + lane * 16);
+          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(tile[i] + c * 512 + lane * 16);
-        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int blk = 2 * c + k;
-          const uint8_t *sc = tile[i] + 8 * D + (t * NB + blk) * 8;
-          const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
-          const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
-          float d[4] = {d01.x, d01.y, d23.x, d23.y}, m[4];
-          if (Q41) {
-            const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
-            const float2 m01 = half_pair(m2.x), m23 = half_pair(m2.y);
-            m[0] = m01.x; m[1] = m01.y; m[2] = m23.x; m[3] = m23.y;
-          }
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {   // tokens 0..7, 8..15
-            const uint32_t lo = words[2 * n + k], hi = lo >> 8;
-            float p[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_16816(p, qa[blk][0], codes_lo(lo), codes_hi(lo));
-            mma_16816(p, qa[blk][1], codes_lo(hi), codes_hi(hi));
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float dot = p[j] + p[2 + j];
-              const int e = 2 * n + j;
-              acc[e] = fmaf(d[e], dot, Q41 ? fmaf(fmaf(8.0f, d[e], m[e]), qsum[blk], acc[e]) : acc[e]);
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int at = base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1);
-        if (at < sees && at < t1) s[i][e] = acc[e] * factor;
-      }
-    }
-    // running maximum
-    float top = run_max;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    const float corr = exp2_fast(run_max - ref);   // (-inf: 0)
-    run_max = top;
-    run_sum *= corr;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[i][e] = exp2_fast(s[i][e] - ref);
-        run_sum += s[i][e];
-      }
-    const float corr0 = __shfl_sync(0xffffffffu, corr, 8 * t), corr1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
-    // values
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      uint4 w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = tile[i] ? *reinterpret_cast<const uint4 *>(tile[i] + part_bytes + c * 512 + lane * 16) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int blk = 2 * c + k;
-        float pd[4][4], big = 0.0f;
-        float add = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f};
-          if (tile[i]) {
-            const uint8_t *sc = tile[i] + part_bytes + 8 * D + (t * NB + blk) * 8;
+          for (int k = 0; k < 2; ++k) {
+            const int blk = 2 * c + k;
+            const uint8_t *sc = tile + 8 * D + (t * NB + blk) * 8;
             const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
             const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
-            d[0] = d01.x; d[1] = d01.y; d[2] = d23.x; d[3] = d23.y;
+            const float d[4] = {d01.x, d01.y, d23.x, d23.y};
+            float m[4] = {0.f, 0.f, 0.f, 0.f};
             if (Q41) {
               const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
               const float2 m01 = half_pair(m2.x), m23 = half_pair(m2.y);
               m[0] = m01.x; m[1] = m01.y; m[2] = m23.x; m[3] = m23.y;
             }
-          }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+            for (int n = 0; n < 2; ++n) {   // tokens 0..7, 8..15
+              const uint32_t lo = words[2 * n + k], hi = lo >> 8;
+              float p[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_16816(p, qa[blk][0], codes_lo(lo), codes_hi(lo));
+              mma_16816(p, qa[blk][1], codes_lo(hi), codes_hi(hi));
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int e = 2 * n + j;
+                if (Q41) acc[e] = fmaf(fmaf(8.0f, d[e], m[e]), qsum[blk], acc[e]);
+                acc[e] = fmaf(d[e], p[j] + p[2 + j], acc[e]);
+              }
+            }
+            // the values' largest scale
+            const uint2 v2 = *reinterpret_cast<const uint2 *>(sc + PART);
+            uint32_t vx = v2.x & 0x7fff7fffu, vy = v2.y & 0x7fff7fffu;
+            if (!clean) {   // what stands behind the last token may be anything
+              const int at = base + 16 * i + 2 * t;
+              const bool in = there >> i & 1;
+              vx &= (in && at < t1 ? 0xffffu : 0u) | (in && at + 1 < t1 ? 0xffff0000u : 0u);
+              vy &= (in && at + 8 < t1 ? 0xffffu : 0u) | (in && at + 9 < t1 ? 0xffff0000u : 0u);
+            }
+            big = __hmax2(big, __hmax2(*reinterpret_cast<const __half2 *>(&vx), *reinterpret_cast<const __half2 *>(&vy)));
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[i][e] = acc[e] * factor;
+          if (!clean) {
             const int at = base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1);
-            const bool in = at < t1;   // (what stands behind a page's last token may be anything)
-            big = fmaxf(big, in ? fabsf(d[e]) : 0.0f);
-            pd[i][e] = at < sees ? s[i][e] * d[e] : 0.0f;
-            if (Q41 && at < sees) add = fmaf(s[i][e], fmaf(8.0f, d[e], m[e]), add);
+            if (at >= sees || at >= t1 || !(there >> i & 1)) s[i][e] = -INFINITY;
           }
         }
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        const float up = to_top(big), down = 1.0f / up;
-        off[blk] = fmaf(off[blk], corr, add);
-        float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      }
+      // running maximum; p is taken times a power of two that brings the largest p d near the top of fp16
+      float top = run_max;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t h0 = pack_half(pd[i][0] * up, pd[i][1] * up), h1 = pack_half(pd[i][2] * up, pd[i][3] * up);
-          const uint32_t l0 = pack_half_lo(pd[i][0] * up, pd[i][1] * up, h0), l1 = pack_half_lo(pd[i][2] * up, pd[i][3] * up, h1);
-          const uint32_t x = __byte_perm(w[i].x, w[i].y, k ? 0x7632 : 0x5410), y = __byte_perm(w[i].z, w[i].w, k ? 0x7632 : 0x5410);
-          const uint32_t a0[4] = {codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y)};
-          const uint32_t a1[4] = {codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8)};
-          mma_16816(acc[0], a0, h0, h1);
-          mma_16816(acc[0], a0, l0, l1);
-          mma_16816(acc[1], a1, h0, h1);
-          mma_16816(acc[1], a1, l0, l1);
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      float largest = fmaxf(__low2float(big), __high2float(big));
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+      const float up = to_top(largest), down = 1.0f / up;
+      const float ref = top == -INFINITY ? 0.0f : top;
+      const float corr = exp2_fast(run_max - ref);   // (-inf: 0)
+      run_max = top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[i][e] = exp2_fast(s[i][e] - ref);
+          sum += s[i][e];
+          s[i][e] *= up;
         }
+      run_sum = fmaf(run_sum, corr, sum);
+      const float corr0 = __shfl_sync(0xffffffffu, corr, 8 * t), corr1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
+      // values
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          o[blk][n][0] = fmaf(o[blk][n][0], corr0, acc[n][0] * down);
-          o[blk][n][1] = fmaf(o[blk][n][1], corr1, acc[n][1] * down);
-          o[blk][n][2] = fmaf(o[blk][n][2], corr0, acc[n][2] * down);
-          o[blk][n][3] = fmaf(o[blk][n][3], corr1, acc[n][3] * down);
+      for (int c = 0; c < NC; ++c) {
+        uint4 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4 *>(tiles + i * TILE + PART + c * 512 + lane * 16);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int blk = 2 * c + k;
+          float add = 0.0f;
+          float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint8_t *sc = tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8;
+            const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
+            const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
+            float pd[4] = {s[i][0] * d01.x, s[i][1] * d01.y, s[i][2] * d23.x, s[i][3] * d23.y};
+            float pm[4] = {0.f, 0.f, 0.f, 0.f};
+            if (Q41) {
+              const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
+              const float2 m01 = half_pair(m2.x), m23 = half_pair(m2.y);
+              pm[0] = s[i][0] * m01.x; pm[1] = s[i][1] * m01.y; pm[2] = s[i][2] * m23.x; pm[3] = s[i][3] * m23.y;
+            }
+            if (!clean)   // (0 times what a scale behind the last token, or of a token that the row does not see, may be)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1) >= min(sees, t1) || !(there >> i & 1)) pd[e] = pm[e] = 0.0f;
+            if (Q41)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) add = fmaf(8.0f, pd[e], add + pm[e]);
+            const uint32_t h0 = pack_half(pd[0], pd[1]), h1 = pack_half(pd[2], pd[3]);
+            const uint32_t l0 = pack_half_lo(pd[0], pd[1], h0), l1 = pack_half_lo(pd[2], pd[3], h1);
+            const uint32_t x = __byte_perm(w[i].x, w[i].y, k ? 0x7632 : 0x5410), y = __byte_perm(w[i].z, w[i].w, k ? 0x7632 : 0x5410);
+            const uint32_t a0[4] = {codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y)};
+            const uint32_t a1[4] = {codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8)};
+            mma_16816(acc[0], a0, h0, h1);
+            mma_16816(acc[0], a0, l0, l1);
+            mma_16816(acc[1], a1, h0, h1);
+            mma_16816(acc[1], a1, l0, l1);
+          }
+          if (Q41) off[blk] = fmaf(off[blk], corr, add * down);
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[blk][n][e] = fmaf(o[blk][n][e], e & 1 ? corr1 : corr0, acc[n][e] * down);
         }
       }
     }
+    // the stage has been read by all the share's warps
+    if (row_warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + share), "r"(32 * row_warps) : "memory");
+    else __syncwarp();
+    if (sub == 0 && base + 2 * step < t1) {
+      issue(base + 2 * step, id_next, stage);
+      id_next = page_at(base + 3 * step);
+    }
+    phase ^= stage;
+    stage ^= 1;
   }
+  if (!all_ok && sub == 0)
+    for (int i = 0; i < 2; ++i) mbar_wait_thread(bar + 8 * (stage ^ i), phase ^ (stage & i), &gave_up[share]);   // copies land before the block ends
 
   // the warp's sums: over the four lanes of a row, then the blocks' constant parts to the lanes that hold the outputs
   run_sum += __shfl_xor_sync(0xffffffffu, run_sum, 1);
   run_sum += __shfl_xor_sync(0xffffffffu, run_sum, 2);
+  if (Q41)
 #pragma unroll
-  for (int k = 0; k < NB; ++k) {
-    if (Q41) {
+    for (int k = 0; k < NB; ++k) {
       off[k] += __shfl_xor_sync(0xffffffffu, off[k], 1);
       off[k] += __shfl_xor_sync(0xffffffffu, off[k], 2);
+      const float c0 = __shfl_sync(0xffffffffu, off[k], 8 * t), c1 = __shfl_sync(0xffffffffu, off[k], 8 * t + 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] += i & 1 ? c1 : c0;
     }
-    const float c0 = Q41 ? __shfl_sync(0xffffffffu, off[k], 8 * t) : 0.0f, c1 = Q41 ? __shfl_sync(0xffffffffu, off[k], 8 * t + 4) : 0.0f;
-    float *dst = so + (warp * K4_ROWS + 2 * t) * D + 32 * k + 4 * g;
-    *reinterpret_cast<float4 *>(dst) = make_float4(o[k][0][0] + c0, o[k][0][2] + c0, o[k][1][0] + c0, o[k][1][2] + c0);
-    *reinterpret_cast<float4 *>(dst + D) = make_float4(o[k][0][1] + c1, o[k][0][3] + c1, o[k][1][1] + c1, o[k][1][3] + c1);
+  float *so = reinterpret_cast<float *>(ring) + warp * K4_ROWS * D;   // [row][D]
+  if (shares > 1) {
+    __syncthreads();   // no stage is read or filled any more
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      float *dst = so + 2 * t * D + 32 * k + 4 * g;
+      *reinterpret_cast<float4 *>(dst) = make_float4(o[k][0][0], o[k][0][2], o[k][1][0], o[k][1][2]);
+      *reinterpret_cast<float4 *>(dst + D) = make_float4(o[k][0][1], o[k][0][3], o[k][1][1], o[k][1][3]);
+    }
+    if (t == 0) { sm[warp][g] = run_max; sl[warp][g] = run_sum; }
+    __syncthreads();
+    if (share > 0) return;
+  } else if (t == 0) {
+    sm[warp][g] = run_max;
+    sl[warp][g] = run_sum;
   }
-  if (t == 0) { sm[warp][g] = run_max; sl[warp][g] = run_sum; }
-  __syncthreads();
-  // the warps' sums into one
-  for (int i = threadIdx.x; i < K4_ROWS * D; i += K4_WARPS * 32) {
-    const int row = i / D, j = i % D;
-    float top = sm[0][row];
+  __syncwarp();
+  if (!mine) return;
+  const int64_t tile_of = ((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt;
 #pragma unroll
-    for (int w = 1; w < K4_WARPS; ++w) top = fmaxf(top, sm[w][row]);
+  for (int j = 0; j < 2; ++j) {   // rows 2t and 2t + 1
+    const int row = 2 * t + j, rr = rt * K4_ROWS + row;
+    float top = sm[warp][row];
+    for (int w = 1; w < shares; ++w) top = fmaxf(top, sm[warp + w * row_warps][row]);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, x = 0.0f;
+    float sum = 0.0f;
+    float4 x[NB];
+    if (shares == 1) {
+      sum = sl[warp][row];
 #pragma unroll
-    for (int w = 0; w < K4_WARPS; ++w) {
-      const float e = exp2_fast(sm[w][row] - ref);
-      sum = fmaf(sl[w][row], e, sum);
-      x = fmaf(so[(w * K4_ROWS + row) * D + j], e, x);
-    }
-    const int rr = rt * K4_ROWS + row;
-    if (rr >= count) continue;
-    if (a.parts == 1) {
-      a.out[(seq.first + rr / a.group) * (int64_t)a.heads * D + (int64_t)(head * a.group + rr % a.group) * D + j] = sum == 0.0f ? 0.0f : x / sum;
+      for (int k = 0; k < NB; ++k) x[k] = make_float4(o[k][0][j], o[k][0][2 + j], o[k][1][j], o[k][1][2 + j]);
     } else {
-      float *p = a.part + (int64_t)blockIdx.x * K4_ROWS * (D + 2) + row * (D + 2);
-      p[j] = x;
-      if (j == 0) { p[D] = top; p[D + 1] = sum; }
+#pragma unroll
+      for (int k = 0; k < NB; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < shares; ++w) {
+        const float e = exp2_fast(sm[warp + w * row_warps][row] - ref);
+        sum = fmaf(sl[warp + w * row_warps][row], e, sum);
+        const float *src = so + (w * row_warps * K4_ROWS + row) * D + 4 * g;
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+          const float4 y = *reinterpret_cast<const float4 *>(src + 32 * k);
+          x[k].x = fmaf(y.x, e, x[k].x); x[k].y = fmaf(y.y, e, x[k].y); x[k].z = fmaf(y.z, e, x[k].z); x[k].w = fmaf(y.w, e, x[k].w);
+        }
+      }
     }
+    if (rr >= count) continue;
+    float *dst = a.parts == 1 ? a.out + (seq.first + rr / a.group) * (int64_t)a.heads * D + (int64_t)(head * a.group + rr % a.group) * D
+                              : a.part + ((tile_of * a.parts + part) * K4_ROWS + row) * (D + 2);
+    const float scale = a.parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      float *p = dst + 32 * k + 4 * g;
+      p[0] = x[k].x * scale; p[1] = x[k].y * scale; p[2] = x[k].z * scale; p[3] = x[k].w * scale;
+    }
+    if (a.parts > 1 && g == 0) { dst[D] = top; dst[D + 1] = sum; }
   }
 }
 
@@ -358,6 +450,12 @@ constexpr int K1_WARPS = 4;      // of a block; 1, 2 or 4 of them share a sequen
 constexpr int K1_MAGIC = 0x4b400000;
 constexpr float K1_MAGIC_F = 12582912.0f;
 
+// the same from a first sum of K1_MAGIC, which stays in registers of its own
+__device__ __forceinline__ void mma_16832_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int first) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(first));
+}
 __device__ __forceinline__ void mma_16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
@@ -366,7 +464,8 @@ __device__ __forceinline__ void mma_16832(int (&c)[4], const uint32_t (&a)[4], u
 // 16 (code - 8) of the low (high) four bits of each byte
 __device__ __forceinline__ uint32_t bytes_lo(uint32_t w) { return (w << 4 & 0xf0f0f0f0u) ^ 0x80808080u; }
 __device__ __forceinline__ uint32_t bytes_hi(uint32_t w) { return (w & 0xf0f0f0f0u) ^ 0x80808080u; }
-__device__ __forceinline__ float sum_of(int c) { return __int_as_float(c) - K1_MAGIC_F; }
+// sum times a power of two w, neg = -K1_MAGIC_F * w: exact
+__device__ __forceinline__ float sum_times(int c, float w, float neg) { return fmaf(__int_as_float(c), w, neg); }
 // byte `digit` (as a selector of two words' such bytes) of four numbers below 2^30 in signed base 256
 __device__ __forceinline__ uint32_t digits_of(float x0, float x1, float x2, float x3, uint32_t pick) {
   const uint32_t u0 = (uint32_t)__float2int_rn(x0) + 0x80808080u, u1 = (uint32_t)__float2int_rn(x1) + 0x80808080u;
@@ -382,8 +481,11 @@ __device__ __forceinline__ float warp_max(float x) {
 template <int NC, bool Q41, bool WIDE>   // WIDE: pages hold 64 tokens or more
 __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const Kv4AttnArgs a) {
   constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART;
+  constexpr int STAGE = 4 * TILE;
   __shared__ float sm[K1_WARPS], sl[K1_WARPS];
-  __shared__ __align__(16) float so[K1_WARPS][D];
+  __shared__ uint64_t bars[K1_WARPS][2];
+  __shared__ int gave_up[K1_WARPS];
+  extern __shared__ __align__(128) uint8_t ring[];   // two stages a warp; behind the last group, the warps' sums
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int share = a.warps, first_warp = warp / share * share;
@@ -407,9 +509,56 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
     for (int i = 0; i < 8; ++i) o[c][i >> 2][i & 3] = 0.0f;
   }
   const uint32_t pick = (uint32_t)(g & 3) | (uint32_t)(4 + (g & 3)) << 4;
-  const float w0 = t & 1 ? 65536.0f : 1.0f, w1 = 256.0f * w0;
+  const float w0 = t & 1 ? 65536.0f : 1.0f, w1 = 256.0f * w0, neg0 = -K1_MAGIC_F * w0;
 
-  if (live && t0 + (warp - first_warp) * K4_GROUP < t1) {
+  const int first = t0 + (warp - first_warp) * K4_GROUP, step = share * K4_GROUP;
+  uint8_t *const mine = ring + warp * 2 * STAGE;
+  if (live && first < t1) {
+    // A stage is 64 tokens.  Lanes 0 to 3 have a tile each; of pages that hold them all, lane 0 copies what there is at once.  A tile that
+    // cannot be followed is left out and counts for nothing.
+    const uint32_t bar = smem_u32(&bars[warp][0]), dst = smem_u32(mine);
+    if (lane == 0) {
+      mbar_init(bar, 1);
+      mbar_init(bar + 8, 1);
+      gave_up[warp] = 0;
+      fence_proxy_async();
+    }
+    __syncwarp();
+    const int *table = a.table + b * a.max_pages;
+    const int64_t page_bytes = kv4_page_bytes(a.s);
+    const int tile_shift = a.s.page == 16 ? 0 : a.s.page == 32 ? 1 : a.s.page == 64 ? 2 : 3;   // tiles of a page, log2
+    const uint8_t *of_head = a.pool + (int64_t)(head << tile_shift) * TILE;
+    auto page_at = [&](int base) {
+      if (WIDE) return base < t1 ? table[base >> (4 + tile_shift)] : -1;
+      return lane < 4 && base + 16 * lane < t1 ? table[((base >> 4) + lane) >> tile_shift] : -1;
+    };
+    auto issue = [&](int base, int id, int stage) -> unsigned {
+      if (WIDE) {   // (one page; the id is every lane's)
+        const bool good = kv4_page_ok(a.s, id);
+        const int tiles = good ? min(4, (t1 - base + 15) >> 4) : 0;
+        if (lane == 0) {
+          mbar_expect_tx(bar + 8 * stage, tiles * TILE);
+          if (good) bulk_load(dst + stage * STAGE, of_head + id * page_bytes + ((base >> 4) & ((1 << tile_shift) - 1)) * TILE, tiles * TILE, bar + 8 * stage);
+          else report_bad_index(a.status, 46, id);
+        }
+        return (1u << tiles) - 1u;
+      }
+      const bool wanted = lane < 4 && base + 16 * lane < t1, good = wanted && kv4_page_ok(a.s, id);
+      if (wanted && !good) report_bad_index(a.status, 46, id);
+      const unsigned there = __ballot_sync(0xffffffffu, good);
+      if (!there) {
+        if (lane == 0) mbar_arrive(bar + 8 * stage);
+        return 0;
+      }
+      if (lane == 0) mbar_expect_tx(bar + 8 * stage, __popc(there) * TILE);
+      __syncwarp();
+      if (good) bulk_load(dst + stage * STAGE + lane * TILE, of_head + id * page_bytes + (((base >> 4) + lane) & ((1 << tile_shift) - 1)) * TILE, TILE, bar + 8 * stage);
+      return there;
+    };
+    unsigned there_now = issue(first, page_at(first), 0), there_next = 0;
+    if (first + step < t1) there_next = issue(first + step, page_at(first + step), 1);
+    int id_next = page_at(first + 2 * step);
+
     // q's digits: this lane's column; dims 8 t + {0, 2, 4, 6} and {1, 3, 5, 7} of a block
     uint32_t qb[NC][2][2];   // [pair][block of it][dims]
     float qsum[NC], factor;
@@ -448,53 +597,22 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
         }
       }
     }
-    const int *table = a.table + b * a.max_pages;
-    const int64_t page_bytes = kv4_page_bytes(a.s);
-    const int tile_shift = a.s.page == 16 ? 0 : a.s.page == 32 ? 1 : a.s.page == 64 ? 2 : 3;   // tiles of a page, log2
-    const uint8_t *of_head = a.pool + (int64_t)(head << tile_shift) * TILE + lane * 16;
-    const int k_scale = 8 * D + ((g >> 1) * NB + (t >> 1)) * 8 - lane * 16, v_scale = PART + 8 * D + (t * NB + (g >> 2)) * 8 - lane * 16;
-
-    for (int base = t0 + (warp - first_warp) * K4_GROUP; base < t1; base += share * K4_GROUP) {
-      // where the four tiles are; one that cannot be followed reads the pool's first and counts for nothing
-      const uint8_t *tile[4];
-      unsigned there = 0;
-      if (WIDE) {
-        const int n = base >> 4, id = table[n >> tile_shift];
-        if (kv4_page_ok(a.s, id)) there = (1u << min(4, (t1 - base + 15) >> 4)) - 1u;
-        else if (lane == 0) report_bad_index(a.status, 46, id);
-        tile[0] = there ? of_head + id * page_bytes + (n & ((1 << tile_shift) - 1)) * TILE : a.pool + lane * 16;
-#pragma unroll
-        for (int i = 1; i < 4; ++i) tile[i] = tile[0] + i * TILE;   // (all in the page, whatever of them is in use)
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = (base >> 4) + i;
-          int id = -1;
-          if (base + 16 * i < t1) {
-            id = table[n >> tile_shift];
-            if (kv4_page_ok(a.s, id)) there |= 1u << i;
-            else if (lane == 0) report_bad_index(a.status, 46, id);
-          }
-          tile[i] = there >> i & 1 ? of_head + id * page_bytes + (n & ((1 << tile_shift) - 1)) * TILE : a.pool + lane * 16;
-        }
-      }
-      uint4 kw[4][NC], vw[4][NC];
-      uint2 kd[4][NC], vd[4][NC], km[4][NC], vm[4][NC];
+    const int k_scale = 8 * D + ((g >> 1) * NB + (t >> 1)) * 8, v_scale = PART + 8 * D + (t * NB + (g >> 2)) * 8;
+    bool ok = true;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int base = first; base < t1; base += step) {
+      ok = mbar_wait(bar + 8 * stage, phase, &gave_up[warp]);
+      if (!ok) break;
+      const uint8_t *tiles = mine + stage * STAGE;
+      const unsigned there = there_now;
+      uint2 vd[4][NC], vm[4][NC];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          kw[i][c] = __ldcs(reinterpret_cast<const uint4 *>(tile[i] + c * 512));
-          kd[i][c] = *reinterpret_cast<const uint2 *>(tile[i] + k_scale + c * 16);
-          if (Q41) km[i][c] = *reinterpret_cast<const uint2 *>(tile[i] + k_scale + D + c * 16);
-        }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          vw[i][c] = __ldcs(reinterpret_cast<const uint4 *>(tile[i] + PART + c * 512));
-          vd[i][c] = *reinterpret_cast<const uint2 *>(tile[i] + v_scale + c * 16);
-          if (Q41) vm[i][c] = *reinterpret_cast<const uint2 *>(tile[i] + v_scale + D + c * 16);
+          vd[i][c] = *reinterpret_cast<const uint2 *>(tiles + i * TILE + v_scale + c * 16);
+          if (Q41) vm[i][c] = *reinterpret_cast<const uint2 *>(tiles + i * TILE + v_scale + D + c * 16);
         }
       // scores: tokens g and g + 8 of each tile, this lane's digits and blocks
       float x[4][2];
@@ -503,17 +621,19 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
         x[i][0] = x[i][1] = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          int acc[4] = {K1_MAGIC, K1_MAGIC, K1_MAGIC, K1_MAGIC};
-          const uint4 w = kw[i][c];   // tokens g (x, y) and g + 8 (z, w); even and odd block
+          int acc[4];
+          const uint4 w = *reinterpret_cast<const uint4 *>(tiles + i * TILE + c * 512 + lane * 16);   // tokens g (x, y) and g + 8 (z, w); even and odd block
           const uint32_t a0[4] = {bytes_lo(w.x), bytes_lo(w.z), bytes_hi(w.x), bytes_hi(w.z)};
           const uint32_t a1[4] = {bytes_lo(w.y), bytes_lo(w.w), bytes_hi(w.y), bytes_hi(w.w)};
-          mma_16832(acc, a0, qb[c][0][0], qb[c][0][1]);
+          mma_16832_first(acc, a0, qb[c][0][0], qb[c][0][1], K1_MAGIC);
           mma_16832(acc, a1, qb[c][1][0], qb[c][1][1]);
-          const float2 d = half_pair(__byte_perm(kd[i][c].x, kd[i][c].y, g & 1 ? 0x7632 : 0x5410));
-          x[i][0] = fmaf(d.x, fmaf(sum_of(acc[0]), w0, sum_of(acc[1]) * w1), x[i][0]);
-          x[i][1] = fmaf(d.y, fmaf(sum_of(acc[2]), w0, sum_of(acc[3]) * w1), x[i][1]);
+          const uint2 kd = *reinterpret_cast<const uint2 *>(tiles + i * TILE + k_scale + c * 16);
+          const float2 d = half_pair(__byte_perm(kd.x, kd.y, g & 1 ? 0x7632 : 0x5410));
+          x[i][0] = fmaf(d.x, fmaf(__int_as_float(acc[1]) - K1_MAGIC_F, w1, sum_times(acc[0], w0, neg0)), x[i][0]);
+          x[i][1] = fmaf(d.y, fmaf(__int_as_float(acc[3]) - K1_MAGIC_F, w1, sum_times(acc[2], w0, neg0)), x[i][1]);
           if (Q41) {
-            const float2 m = half_pair(__byte_perm(km[i][c].x, km[i][c].y, g & 1 ? 0x7632 : 0x5410));
+            const uint2 km = *reinterpret_cast<const uint2 *>(tiles + i * TILE + k_scale + D + c * 16);
+            const float2 m = half_pair(__byte_perm(km.x, km.y, g & 1 ? 0x7632 : 0x5410));
             x[i][0] = fmaf(fmaf(8.0f, d.x, m.x), qsum[c], x[i][0]);
             x[i][1] = fmaf(fmaf(8.0f, d.y, m.y), qsum[c], x[i][1]);
           }
@@ -591,13 +711,13 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
           digits[i] = digits_of(p[i][0] * (d01.x * up), p[i][1] * (d01.y * up), p[i][2] * (d23.x * up), p[i][3] * (d23.y * up), pick);
         }
         if (Q41) off[c] = fmaf(off[c], corr, add);
-        int acc[2][4] = {{K1_MAGIC, K1_MAGIC, K1_MAGIC, K1_MAGIC}, {K1_MAGIC, K1_MAGIC, K1_MAGIC, K1_MAGIC}};
+        int acc[2][4];
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {   // 32 tokens
           uint32_t bytes[2][4];            // of the lane's four tokens: dims 4 g + {0, 1} and {2, 3} of the even block, of the odd one
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint4 w = vw[i + h][c];
+            const uint4 w = *reinterpret_cast<const uint4 *>(tiles + (i + h) * TILE + PART + c * 512 + lane * 16);
             const uint32_t e0 = __byte_perm(w.x, w.y, 0x5140), e1 = __byte_perm(w.z, w.w, 0x5140);
             const uint32_t o0 = __byte_perm(w.x, w.y, 0x7362), o1 = __byte_perm(w.z, w.w, 0x7362);
             bytes[h][0] = __byte_perm(e0, e1, 0x5410);
@@ -611,18 +731,35 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
               const uint32_t av[4] = {bytes_lo(bytes[0][2 * k + n]), bytes_hi(bytes[0][2 * k + n]), bytes_lo(bytes[1][2 * k + n]), bytes_hi(bytes[1][2 * k + n])};
-              mma_16832(acc[n], av, b0, b1);
+              if (i == 0 && k == 0) mma_16832_first(acc[n], av, b0, b1, K1_MAGIC);
+              else mma_16832(acc[n], av, b0, b1);
             }
           }
         }
         // (a scale that is not finite makes its block's values NaN, as it does in the formula)
         const float down = __shfl_sync(0xffffffffu, most < 0x7c00u ? 0.0625f / up : NAN, 16 * (t >> 1));
-        const float f0 = down * w0, f1 = down * w1;
+        const float f0 = down * w0, f1 = down * w1, n0 = -K1_MAGIC_F * f0, n1 = -K1_MAGIC_F * f1;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[c][n][e] = fmaf(o[c][n][e], corr, sum_of(acc[n][e]) * (e & 1 ? f1 : f0));
+          for (int e = 0; e < 4; ++e) o[c][n][e] = fmaf(o[c][n][e], corr, sum_times(acc[n][e], e & 1 ? f1 : f0, e & 1 ? n1 : n0));
       }
+      __syncwarp();   // the stage has been read
+      there_now = there_next;
+      if (base + 2 * step < t1) {
+        there_next = issue(base + 2 * step, id_next, stage);
+        id_next = page_at(base + 3 * step);
+      }
+      phase ^= stage;
+      stage ^= 1;
+    }
+    if (!ok) {
+      if (lane == 0) {
+        gave_up[warp] = 1;
+        atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
+        a.status[1] = 47;
+      }
+      for (int i = 0; i < 2; ++i) mbar_wait_thread(bar + 8 * (stage ^ i), phase ^ (stage & i), &gave_up[warp]);   // copies land before the block ends
     }
   }
 
@@ -651,8 +788,10 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
   const int at = 32 * (t >> 1) + 4 * g + 2 * (t & 1);   // of a pair of blocks
   float top = run_max, sum = run_sum;
   if (share > 1) {
+    float *so = reinterpret_cast<float *>(ring);   // [warp][D], each inside the warp's own stages
+    constexpr int STRIDE = 2 * STAGE / (int)sizeof(float);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) *reinterpret_cast<float2 *>(&so[warp][64 * c + at]) = r[c];
+    for (int c = 0; c < NC; ++c) *reinterpret_cast<float2 *>(&so[warp * STRIDE + 64 * c + at]) = r[c];
     if (lane == 0) { sm[warp] = run_max; sl[warp] = run_sum; }
     __syncthreads();
     if (warp != first_warp) return;
@@ -666,7 +805,7 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
       sum = fmaf(sl[w], e, sum);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const float2 y = *reinterpret_cast<const float2 *>(&so[w][64 * c + at]);
+        const float2 y = *reinterpret_cast<const float2 *>(&so[w * STRIDE + 64 * c + at]);
         r[c].x = fmaf(y.x, e, r[c].x);
         r[c].y = fmaf(y.y, e, r[c].y);
       }
@@ -731,11 +870,17 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
   if (batch && (int64_t)c->kv_heads * p->row_tiles > 0x7fffffff / batch) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
   p->units = batch * c->kv_heads * p->row_tiles;
   const int64_t groups = (max_length + K4_GROUP - 1) / K4_GROUP;
-  // single rows: a warp each where that is enough to fill the SMs (20 warps an SM), otherwise four
-  p->warps = p->tile_rows > 1 ? K4_WARPS : p->units >= 148 * 16 ? 1 : K1_WARPS;
-  const int64_t fill = p->tile_rows > 1 ? 148 * 3 : 148 * 20 / p->warps;
-  int64_t parts = p->units ? (fill + p->units - 1) / p->units : 1;
-  const int64_t most = (groups + 2 * p->warps - 1) / (2 * p->warps);   // a part gives each warp two groups at least
+  int64_t fill, blocks, shares;   // units of work that fill the SMs; units without parts; warps over whom a unit's tokens are dealt
+  if (p->tile_rows == 1) {
+    // a warp each where that is enough (20 warps an SM), otherwise four
+    p->warps = p->units >= 148 * 16 ? 1 : K1_WARPS;
+    fill = 148 * 20 / p->warps; blocks = p->units; shares = p->warps;
+  } else {
+    p->warps = p->row_tiles >= 4 ? 4 : p->row_tiles >= 2 ? 2 : 1;
+    fill = 148 * 6; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = K4_WARPS / p->warps;
+  }
+  int64_t parts = blocks ? (fill + blocks - 1) / blocks : 1;
+  const int64_t most = (groups + 2 * shares - 1) / (2 * shares);   // a part gives each warp two groups at least
   if (parts > most) parts = most;
   if (parts < 1) parts = 1;
   const int64_t each = groups ? (groups + parts - 1) / parts : 1;
@@ -749,13 +894,16 @@ template <int NC, bool Q41>
 static int kv4_attention_launch(caten_b200_ctx *ctx, const Kv4AttnArgs &a, int64_t units) {
   if (a.tile_rows == 1) {
     const int64_t per_block = K1_WARPS / a.warps;
-    CB_CUDA(ctx, launch_k(ctx, a.s.page >= K4_GROUP ? kv4_attention_row_kernel<NC, Q41, true> : kv4_attention_row_kernel<NC, Q41, false>,
-                          dim3((unsigned)((units * a.parts + per_block - 1) / per_block)), dim3(K1_WARPS * 32), 0, a));
+    const int smem = K1_WARPS * 2 * 4 * kv4_tile_bytes(a.s);
+    void (*kernel)(const Kv4AttnArgs) = a.s.page >= K4_GROUP ? kv4_attention_row_kernel<NC, Q41, true> : kv4_attention_row_kernel<NC, Q41, false>;
+    if (smem > 48 << 10) CB_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    CB_CUDA(ctx, launch_k(ctx, kernel, dim3((unsigned)((units * a.parts + per_block - 1) / per_block)), dim3(K1_WARPS * 32), smem, a));
     CB_LAUNCH_CHECK(ctx, "kv4_attention_row_kernel");
   } else {
-    const int smem = K4_WARPS * K4_ROWS * NC * 64 * (int)sizeof(float);
-    CB_CUDA(ctx, cudaFuncSetAttribute(kv4_attention_kernel<NC, Q41>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    CB_CUDA(ctx, launch_k(ctx, kv4_attention_kernel<NC, Q41>, dim3((unsigned)(units * a.parts)), dim3(K4_WARPS * 32), smem, a));
+    const int smem = K4_WARPS / a.warps * 2 * 4 * kv4_tile_bytes(a.s);   // (no less than the sums of all warps where they are joined)
+    const int64_t blocks = units / a.row_tiles * ((a.row_tiles + a.warps - 1) / a.warps) * a.parts;
+    if (smem > 48 << 10) CB_CUDA(ctx, cudaFuncSetAttribute(kv4_attention_kernel<NC, Q41>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    CB_CUDA(ctx, launch_k(ctx, kv4_attention_kernel<NC, Q41>, dim3((unsigned)blocks), dim3(K4_WARPS * 32), smem, a));
     CB_LAUNCH_CHECK(ctx, "kv4_attention_kernel");
   }
   if (a.parts == 1) return 0;
