@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(256) kv_slots_kernel(PagesArgs a) {
 // A block of 32 values is eight lanes' float4.  Codes are those of the GGUF formats: Q4_0  d = (value of largest magnitude) / -8,
 // code = min(15, trunc(x / d + 8.5)); Q4_1  d = (max - min) / 15, code = min(15, trunc((x - min) / d + 0.5)).  Which code is nearest is decided
 // exactly: in fp32, whose error here is below 4e-6, unless the quotient is within 1e-5 of a border, then in 64 bits.  d and the minimum are
-// rounded to fp16 (half a step: 2^-11) because that is what the formats hold.
+// rounded to fp16 (half a step: 2^-11) because that is what the formats hold.  Where one of them is not finite there (a value that is not, or
+// one beyond fp16's reach), the scale is NaN: a block is what it stands for, or NaN in all of its values.
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
@@ -189,6 +190,11 @@ __device__ __forceinline__ uint32_t kv4_code(float x, float inverse, float offse
   if (fabsf(y - rintf(y)) >= 1e-5f) return (uint32_t)min(15, max(0, (int)y));
   const double e = ((double)x - (double)low) / d + (double)offset;
   return (uint32_t)min(15, max(0, (int)e));
+}
+
+__device__ __forceinline__ __half scale_or_nan(float d, float minimum) {
+  const __half h = __float2half_rn(d);
+  return fabsf(__half2float(h)) < INFINITY && fabsf(minimum) < INFINITY ? h : __ushort_as_half((unsigned short)0x7fff);
 }
 
 // this lane's four values of a block that eight consecutive lanes hold -> four codes (low bits first), scale and minimum
@@ -206,8 +212,8 @@ __device__ __forceinline__ uint32_t kv4_quantise(float4 x, __half *scale, __half
       lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     }
     const double d = ((double)hi - (double)lo) / 15.0;
-    *scale = __float2half_rn((float)d);
     *minimum = __float2half_rn(lo);
+    *scale = scale_or_nan((float)d, __half2float(*minimum));
     const float inverse = 1.0f / (float)d;
     if (__half2float(*scale) != 0.0f)
 #pragma unroll
@@ -227,7 +233,7 @@ __device__ __forceinline__ uint32_t kv4_quantise(float4 x, __half *scale, __half
       if (b > a || (b == a && oat < at)) { m = om; at = oat; }
     }
     const float d = m / -8.0f;
-    *scale = __float2half_rn(d);
+    *scale = scale_or_nan(d, 0.0f);
     const float inverse = 1.0f / d;
     if (__half2float(*scale) != 0.0f) {
 #pragma unroll

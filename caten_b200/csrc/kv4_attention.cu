@@ -85,6 +85,12 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
   return r;
 }
 __device__ __forceinline__ float2 half_pair(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+// halves that are infinite or NaN made 0
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+  return w & (((w & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) | ((w & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u));
+}
+// keeps a rare branch a branch: as selects, its instructions would be everybody's
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // power of two 2^(k - floor(log2 x)), kept inside fp32's normal range; 1 for zero
 __device__ __forceinline__ float to_top(float x, int k = 14) {
@@ -96,7 +102,7 @@ __device__ __forceinline__ float to_top(float x, int k = 14) {
 // A block's four warps are `row_warps` row tiles times 4 / row_warps shares of the tokens.  The warps of a share work on one ring of two stages of 64
 // tokens, which bulk copies fill while the other is read (each stage is read by all its warps before it is filled again).
 template <int NC, bool Q41>
-__global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) kv4_attention_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 2 : 1) kv4_attention_kernel(const Kv4AttnArgs a) {
   constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, STAGE = 4 * TILE;
   __shared__ float sm[K4_WARPS][K4_ROWS], sl[K4_WARPS][K4_ROWS];
   __shared__ uint64_t bars[K4_WARPS][2];
@@ -160,7 +166,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
 
   // q as the first product's operand: a block's two steps, {dims 8t + 0, 4 | 8t + 1, 5} and {2, 6 | 3, 7}; hi in rows g, lo in rows g + 8
   uint32_t qa[NB][2][4];
-  float qsum[NB];
+  float qsum8[NB];   // 8 sum(q) of a block
   float factor;
   {
     const float *q = a.q + (seq.first + tok) * a.ldq + (int64_t)(head * a.group + r % a.group) * D + 8 * t;
@@ -187,7 +193,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
       if (Q41) {
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        qsum[k] = sum;
+        qsum8[k] = 8.0f * sum;
       }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
@@ -200,11 +206,10 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
   }
 
   float run_max = -INFINITY, run_sum = 0.0f;   // of row g (run_sum: this lane's tokens)
-  float off[NB];                               // Q4_1: sum of p (m + 8 d) of row g, this lane's tokens
+  float off[4] = {0.f, 0.f, 0.f, 0.f};         // Q4_1: sums of p m_b (rows b of a product of their own) and p d_b (rows NB + b) for rows 2t, 2t + 1
   float o[NB][2][4];                           // rows 2t, 2t + 1; dims 4g + {0, 1} and 4g + {2, 3} of a block
 #pragma unroll
   for (int k = 0; k < NB; ++k) {
-    off[k] = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] = 0.0f;
   }
@@ -242,7 +247,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
             const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
             const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
             const float d[4] = {d01.x, d01.y, d23.x, d23.y};
-            float m[4] = {0.f, 0.f, 0.f, 0.f};
+            float m[4];
             if (Q41) {
               const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
               const float2 m01 = half_pair(m2.x), m23 = half_pair(m2.y);
@@ -251,13 +256,13 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
 #pragma unroll
             for (int n = 0; n < 2; ++n) {   // tokens 0..7, 8..15
               const uint32_t lo = words[2 * n + k], hi = lo >> 8;
-              float p[4] = {0.f, 0.f, 0.f, 0.f};
+              float p[4] = {Q41 ? qsum8[blk] : 0.0f, Q41 ? qsum8[blk] : 0.0f, 0.f, 0.f};   // (d code + m = d (code - 8 + 8) + m)
               mma_16816(p, qa[blk][0], codes_lo(lo), codes_hi(lo));
               mma_16816(p, qa[blk][1], codes_lo(hi), codes_hi(hi));
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
                 const int e = 2 * n + j;
-                if (Q41) acc[e] = fmaf(fmaf(8.0f, d[e], m[e]), qsum[blk], acc[e]);
+                if (Q41) acc[e] = fmaf(m[e], 0.125f * qsum8[blk], acc[e]);
                 acc[e] = fmaf(d[e], p[j] + p[2 + j], acc[e]);
               }
             }
@@ -265,6 +270,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
             const uint2 v2 = *reinterpret_cast<const uint2 *>(sc + PART);
             uint32_t vx = v2.x & 0x7fff7fffu, vy = v2.y & 0x7fff7fffu;
             if (!clean) {   // what stands behind the last token may be anything
+              keep_branch();
               const int at = base + 16 * i + 2 * t;
               const bool in = there >> i & 1;
               vx &= (in && at < t1 ? 0xffffu : 0u) | (in && at + 1 < t1 ? 0xffff0000u : 0u);
@@ -276,7 +282,11 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[i][e] = acc[e] * factor;
-          if (!clean) {
+        }
+        if (!clean) {
+          keep_branch();
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
             const int at = base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1);
             if (at >= sees || at >= t1 || !(there >> i & 1)) s[i][e] = -INFINITY;
           }
@@ -308,6 +318,40 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
         }
       run_sum = fmaf(run_sum, corr, sum);
       const float corr0 = __shfl_sync(0xffffffffu, corr, 8 * t), corr1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
+      if (Q41) {
+        // sum of p (m + 8 d), which the middle of the codes leaves: minima and scales lie in the cache as the product's first operand has them
+        const float lift = down * 0x1p14f;   // p at the top of fp16's range
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x[4] = {s[i][0] * lift, s[i][1] * lift, s[i][2] * lift, s[i][3] * lift};
+          const uint32_t h0 = pack_half(x[0], x[1]), h1 = pack_half(x[2], x[3]);
+          const uint32_t l0 = pack_half_lo(x[0], x[1], h0), l1 = pack_half_lo(x[2], x[3], h1);
+          uint32_t av[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (8 * h < 2 * NB) {
+              const int row = 8 * h + g;
+              if (row < 2 * NB) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (row < NB ? D : 0) + (t * NB + (row < NB ? row : row - NB)) * 8);
+                av[h] = w.x;
+                av[2 + h] = w.y;
+              }
+              if (!clean) {   // nothing of what is behind the last token, nor of what some rows may not see and is not finite (a block's minimum is finite or
+                              // its scale is NaN, and that is in p d)
+                keep_branch();
+                const int at = base + 16 * i + 2 * t;
+                const bool in = there >> i & 1;
+                av[h] = finite_halves(av[h]) & ((in && at < t1 ? 0xffffu : 0u) | (in && at + 1 < t1 ? 0xffff0000u : 0u));
+                av[2 + h] = finite_halves(av[2 + h]) & ((in && at + 8 < t1 ? 0xffffu : 0u) | (in && at + 9 < t1 ? 0xffff0000u : 0u));
+              }
+            }
+          mma_16816(acc, av, h0, h1);
+          mma_16816(acc, av, l0, l1);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) off[e] = fmaf(off[e], e & 1 ? corr1 : corr0, acc[e] * 0x1p-14f);
+      }
       // values
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -317,27 +361,18 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int blk = 2 * c + k;
-          float add = 0.0f;
           float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint8_t *sc = tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8;
-            const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
+            const uint2 d2 = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8);
             const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
             float pd[4] = {s[i][0] * d01.x, s[i][1] * d01.y, s[i][2] * d23.x, s[i][3] * d23.y};
-            float pm[4] = {0.f, 0.f, 0.f, 0.f};
-            if (Q41) {
-              const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
-              const float2 m01 = half_pair(m2.x), m23 = half_pair(m2.y);
-              pm[0] = s[i][0] * m01.x; pm[1] = s[i][1] * m01.y; pm[2] = s[i][2] * m23.x; pm[3] = s[i][3] * m23.y;
-            }
-            if (!clean)   // (0 times what a scale behind the last token, or of a token that the row does not see, may be)
+            if (!clean) {   // (0 times what a scale behind the last token, or of a token that the row does not see, may be)
+              keep_branch();
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1) >= min(sees, t1) || !(there >> i & 1)) pd[e] = pm[e] = 0.0f;
-            if (Q41)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) add = fmaf(8.0f, pd[e], add + pm[e]);
+                if (base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1) >= min(sees, t1) || !(there >> i & 1)) pd[e] = 0.0f;
+            }
             const uint32_t h0 = pack_half(pd[0], pd[1]), h1 = pack_half(pd[2], pd[3]);
             const uint32_t l0 = pack_half_lo(pd[0], pd[1], h0), l1 = pack_half_lo(pd[2], pd[3], h1);
             const uint32_t x = __byte_perm(w[i].x, w[i].y, k ? 0x7632 : 0x5410), y = __byte_perm(w[i].z, w[i].w, k ? 0x7632 : 0x5410);
@@ -348,7 +383,6 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
             mma_16816(acc[1], a1, h0, h1);
             mma_16816(acc[1], a1, l0, l1);
           }
-          if (Q41) off[blk] = fmaf(off[blk], corr, add * down);
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -374,13 +408,13 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 1) 
   run_sum += __shfl_xor_sync(0xffffffffu, run_sum, 2);
   if (Q41)
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      off[k] += __shfl_xor_sync(0xffffffffu, off[k], 1);
-      off[k] += __shfl_xor_sync(0xffffffffu, off[k], 2);
-      const float c0 = __shfl_sync(0xffffffffu, off[k], 8 * t), c1 = __shfl_sync(0xffffffffu, off[k], 8 * t + 4);
+    for (int k = 0; k < NB; ++k)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] += i & 1 ? c1 : c0;
-    }
+      for (int j = 0; j < 2; ++j) {
+        const float pm = __shfl_sync(0xffffffffu, off[k / 8 * 2 + j], k % 8 * 4 + t), pd = __shfl_sync(0xffffffffu, off[(NB + k) / 8 * 2 + j], (NB + k) % 8 * 4 + t);
+        const float add = fmaf(8.0f, pd, pm);
+        o[k][0][j] += add; o[k][0][2 + j] += add; o[k][1][j] += add; o[k][1][2 + j] += add;
+      }
   float *so = reinterpret_cast<float *>(ring) + warp * K4_ROWS * D;   // [row][D]
   if (shares > 1) {
     __syncthreads();   // no stage is read or filled any more

@@ -295,7 +295,8 @@ int64_t caten_b200_kv4_nbytes(const caten_b200_kv4_desc *desc);
  * Slots of a call are distinct; one outside the pool is skipped and reported (CATEN_B200_EDEVICE) by the next synchronising call.  Per block of 32:
  *   Q4_0  d = x / -8 of the value x of largest magnitude (the first of equal ones), code = min(15, trunc(x / d + 8.5)), value d (code - 8)
  *   Q4_1  d = (max - min) / 15, code = min(15, trunc((x - min) / d + 0.5)), value d code + min
- * with d and min rounded to fp16 in the cache, the codes decided from unrounded ones in 64 bits. */
+ * with d and min rounded to fp16 in the cache, the codes decided from unrounded ones in 64 bits.  A block of which d or min is not finite in
+ * fp16 (values that are not finite, or beyond 524032 in Q4_0, 65504 in Q4_1) stands for NaN in all its values. */
 int caten_b200_kv4_store(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, void *d_pool, const float *d_k, const float *d_v, int64_t ld,
                          const int32_t *d_slots, int64_t tokens);
 /* Rows out of the cache, as the fp32 values they stand for; rows of slot -1 are left as they were. */

@@ -176,9 +176,8 @@ def test_rows_that_are_not_finite_or_too_large_stay_in_their_blocks(rt):
         for y in rt.kv4_load(d, pool, slots):
             y = y.numpy().reshape(4, 4, 32)
             hit = np.eye(4, dtype=bool)
-            assert not np.isfinite(y[hit]).all(1).any()     # each such block says so
+            assert np.isnan(y[hit]).all()                   # each such block is NaN
             assert (y[~hit] == 1.0).all() and not np.isnan(y[~hit]).any()
-        assert np.isnan(y[0, 0]).all()
 
 
 def test_slots_outside_the_pool_are_skipped_and_reported(rt):
@@ -336,6 +335,32 @@ def test_nan_in_a_row_stays_in_it(rt):
     hit[1, 0] = hit[5, 1] = True
     assert np.isnan(out[hit]).all()
     np.testing.assert_array_equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("heads,kv", [(1, 1), (2, 1), (16, 1)])
+def test_what_later_tokens_hold_does_not_matter_to_earlier_ones(rt, kind, heads, kv):
+    """A token whose keys or values are not finite, seen by the rows from its own on: those say so, the rows before it are as they were."""
+    rng = rng_of(36, heads)
+    c = Cache(rt, rng, kind, 64, 16, heads, kv, [90])
+    q = rng.standard_normal((30, heads, 64), dtype=np.float32)
+    clean = check_attention(rt, c, q, [30])
+    for token in (60, 75, 89):
+        for which in range(2):
+            for value in (np.nan, np.inf):
+                rows = [np.zeros((1, kv * 64), np.float32) for _ in range(2)]
+                rows[which][0, 40] = value
+                slot = put(rt, [c.table[0, token // 16] * 16 + token % 16], np.int32)
+                kept = rt.kv4_load(c.desc, c.pool, slot)
+                rt.kv4_store(c.desc, c.pool, put(rt, rows[0]), put(rt, rows[1]), slot)
+                out = rt.kv4_attention(c.desc, put(rt, q.reshape(30, -1)), c.pool, put(rt, c.table, np.int32), put(rt, c.lengths, np.int32), put(rt, [0, 30], np.int32),
+                                       max_new=30).numpy().reshape(30, heads, 64)
+                seen = token - 60   # row i is token 60 + i
+                np.testing.assert_array_equal(out[:seen], clean[:seen])
+                assert not np.isfinite(out[seen:, :, 32:]).any()
+                rt.kv4_store(c.desc, c.pool, *kept, slot)
+                if kind == "q4_0":   # (its own values are stored as they are)
+                    np.testing.assert_array_equal(rt.kv4_load(c.desc, c.pool, slot)[0].numpy(), kept[0].numpy())
 
 
 def test_what_the_device_says_is_checked(rt):
