@@ -4,8 +4,8 @@
 // Selection.  Candidate (beam b, token v) has the value score_b + x_bv - lse_b, lse_b = max + log(sum exp(x - max)); the first `keep` by value,
 // equal ones by b * V + v.  Within a beam that order is the order of the logits, so a pass over the logits needs no lse: each block reads a chunk
 // of a row once into registers and leaves its maximum, its sum of exponentials and its `keep` largest logits; a second kernel joins the
-// chunks' sums in 64 bits, turns the few logits left into values and picks among them.  Both pick by a bound first: the smallest of `keep` or more
-// disjoint groups' largest has `keep` at or above it, and with a few dozen candidates left each counts those before it, which is its place.
+// chunks' sums in 64 bits, turns the few logits left into values and picks among them.  Both pick by a bound first: `keep` values
+// are not behind the `keep`-th of disjoint groups' largest, and with a few dozen candidates left each counts those before it, which is its place.
 #include <algorithm>
 
 #include "common.cuh"
@@ -43,6 +43,18 @@ __device__ __forceinline__ u64 warp_sort(u64 key) {
       key = larger == (other > key) ? other : key;
     }
   return key;
+}
+
+__device__ __forceinline__ float warp_sort_floats(float x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, x, j);
+      x = ((lane & j) == 0) == ((lane & k) == 0) ? fmaxf(x, other) : fminf(x, other);
+    }
+  return x;
 }
 
 // The `keep`-th largest of the block's keys (one a thread, 0: none; all others different), 1 if there are fewer.  A key's rank is the number of
@@ -107,21 +119,17 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
     }
   }
   if (tid == 0) { count = 0; threads = 0; }
-  // the largest of each thread, of groups of threads (8, 16 or 32 of them in the block: the least power of two from `keep`, 8 at least), of the block
+  // the largest of each thread, of each eight threads, and of those 32 in order the first and the `keep`-th
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < VECS; ++i) top = fmaxf(top, fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3])));
-  const int per_warp = keep <= 8 ? 1 : keep <= 16 ? 2 : 4, width = 32 / per_warp, groups = per_warp * (BS_THREADS / 32);
   float gt = top;
-  for (int o = 1; o < width; o <<= 1) gt = fmaxf(gt, __shfl_xor_sync(0xffffffffu, gt, o));
-  if (lane % width == 0) group_top[warp * per_warp + lane / width] = gt;
-  __syncthreads();
-  float m = lane < groups ? group_top[lane] : -INFINITY, least = lane < groups ? m : INFINITY;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
-  }
+  for (int o = 1; o < 8; o <<= 1) gt = fmaxf(gt, __shfl_xor_sync(0xffffffffu, gt, o));
+  if (lane % 8 == 0) group_top[tid / 8] = gt;
+  __syncthreads();
+  const float sorted = warp_sort_floats(group_top[lane]);
+  const float m = __shfl_sync(0xffffffffu, sorted, 0), least = __shfl_sync(0xffffffffu, sorted, keep - 1);
   const bool may = top >= least && top > -INFINITY;
   const unsigned who = __ballot_sync(0xffffffffu, may);
   if (lane == 0 && who) atomicAdd(&threads, __popc(who));
@@ -158,10 +166,11 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
     for (int i = 0; i < VECS; ++i)
       if (fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3])) >= floor_value)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const u64 key = beam_key(v[i][j], (int)(e0 + (i * BS_THREADS + tid) * 4 + j));
-          if (v[i][j] >= floor_value && key >= bound) found[atomicAdd(&count, 1)] = key;
-        }
+        for (int j = 0; j < 4; ++j)
+          if (v[i][j] >= floor_value) {
+            const u64 key = beam_key(v[i][j], (int)(e0 + (i * BS_THREADS + tid) * 4 + j));
+            if (key >= bound) found[atomicAdd(&count, 1)] = key;
+          }
   }
   __syncthreads();
   const int n = count;
@@ -169,7 +178,8 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
   for (int i = tid; i < n; i += BS_THREADS) {
     const u64 key = found[i];
     int place = 0;
-    for (int j = 0; j < n && place < keep; ++j) place += found[j] > key;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) place += found[j] > key;
     if (place < keep) part[place] = key;
   }
   for (int i = n + tid; i < keep; i += BS_THREADS) part[i] = 0;
@@ -195,7 +205,7 @@ constexpr int BJ_LISTS = 4096;   // of a request: beams x chunks
 constexpr int BJ_FOUND = BS_KEEP * BS_KEEP;
 
 // A candidate: the order-preserving image of its value, and b * V + token; larger: earlier in the result.
-struct Cand {
+struct __align__(16) Cand {
   u64 value;
   uint32_t id;
   __device__ __forceinline__ bool operator>(const Cand &o) const { return value > o.value || (value == o.value && id < o.id); }
@@ -216,6 +226,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
   const int lists = beams * chunks;
   const u64 *mine = parts + batch * lists * words;
   if (tid == 0) { bound = {1, 0xffffffffu}; count = 0; queued = 0; }   // (that bound: every candidate)
+  const u64 head = tid < lists ? mine[(int64_t)tid * words] : 0ull;     // (of an ended hypothesis: whatever is there, unused)
   for (int b = warp; b < beams; b += BJ_THREADS / 32) {
     const int64_t row = batch * beams + b;
     const float score = scores[row];
@@ -223,14 +234,15 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
     double log_sum = 0.0, top = 0.0;
     if (!end) {
       const u64 *part = mine + (int64_t)b * chunks * words + keep;
-      float m = -INFINITY;
-      for (int c = lane; c < chunks; c += 32)
-        if ((uint32_t)part[c * words] != 0u) m = fmaxf(m, __uint_as_float((uint32_t)(part[c * words] >> 32)));   // (sum 0: nothing in that chunk)
+      const u64 first = lane < chunks ? part[lane * words] : 0ull;
+      float m = (uint32_t)first != 0u ? __uint_as_float((uint32_t)(first >> 32)) : -INFINITY;   // (sum 0: nothing in that chunk)
+      for (int c = lane + 32; c < chunks; c += 32)
+        if ((uint32_t)part[c * words] != 0u) m = fmaxf(m, __uint_as_float((uint32_t)(part[c * words] >> 32)));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       double s = 0.0;
       for (int c = lane; c < chunks; c += 32) {
-        const u64 w = part[c * words];
+        const u64 w = c == lane ? first : part[c * words];
         if ((uint32_t)w != 0u) s += (double)__uint_as_float((uint32_t)w) * exp((double)__uint_as_float((uint32_t)(w >> 32)) - (double)m);
       }
 #pragma unroll
@@ -245,33 +257,30 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
     }
   }
   __syncthreads();
-  // entry j of list i
-  auto entry = [&](int i, int j) -> Cand {
+  auto cand_of = [&](int i, int j, u64 key) -> Cand {   // entry j of list i
     const int b = i / chunks;
     if (over[b])   // its one candidate stands first in its first list
       return {i == b * chunks && j == 0 && eos >= 0 ? order_of(base[b]) : 0ull, (uint32_t)(b * V + eos)};
-    const u64 key = mine[(int64_t)i * words + j];
     return {key ? order_of(base[b] + ((double)beam_key_value(key) - tops[b])) : 0ull, (uint32_t)(b * V + beam_key_index(key))};
   };
-  // the `keep`-th of n candidates (all different but for those without a value), if there are as many
-  auto bound_of = [&](int n) {
-    for (int i = tid; i < n; i += BJ_THREADS) {
-      const Cand c = found[i];
-      int place = 0;
-      for (int j = 0; j < n && place < keep; ++j) place += found[j] > c;
-      if (c.value && place == keep - 1) bound = c;
-    }
+  auto entry = [&](int i, int j) { return cand_of(i, j, mine[(int64_t)i * words + j]); };
+  // how many of the n found are before c
+  auto place_of = [&](const Cand &c, int n) {
+    int place = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) place += found[j] > c;
+    return place;
   };
   // The keep-th of the lists' first entries: `keep` candidates are not behind it, and at most `keep` lists have any that are not.  Where a thread
   // has several lists, the threads' best give a first bound, and the few first entries that it leaves the second.
-  Cand best = {0ull, 0xffffffffu};
-  for (int i = tid; i < lists; i += BJ_THREADS) {
+  Cand best = tid < lists ? cand_of(tid, 0, head) : Cand{0ull, 0xffffffffu};
+  for (int i = tid + BJ_THREADS; i < lists; i += BJ_THREADS) {
     const Cand c = entry(i, 0);
     if (c > best) best = c;
   }
   found[tid] = best;
   __syncthreads();
-  bound_of(min(lists, BJ_THREADS));
+  if (best.value && place_of(best, min(lists, BJ_THREADS)) == keep - 1) bound = best;
   __syncthreads();
   if (lists > BJ_THREADS) {
     const Cand first = bound;
@@ -282,20 +291,24 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
     }
     __syncthreads();
     const int n = count;
-    bound_of(n);
+    for (int i = tid; i < n; i += BJ_THREADS)
+      if (place_of(found[i], n) == keep - 1) bound = found[i];
     __syncthreads();
     if (tid == 0) count = 0;
   }
   const Cand least = bound;
   __syncthreads();
-  for (int i = tid; i < lists; i += BJ_THREADS) {
-    const Cand c = entry(i, 0);
-    if (c.value && !(least > c)) queue[atomicAdd(&queued, 1)] = i;
+  if (lists <= BJ_THREADS) {
+    if (best.value && !(least > best)) queue[atomicAdd(&queued, 1)] = tid;
+  } else {
+    for (int i = tid; i < lists; i += BJ_THREADS) {
+      const Cand c = entry(i, 0);
+      if (c.value && !(least > c)) queue[atomicAdd(&queued, 1)] = i;
+    }
   }
   __syncthreads();
-  for (int q = warp; q < queued; q += BJ_THREADS / 32) {
-    Cand c = {0ull, 0u};
-    if (lane < keep) c = entry(queue[q], lane);
+  for (int i = tid; i < queued * keep; i += BJ_THREADS) {
+    const Cand c = entry(queue[i / keep], i % keep);
     if (c.value && !(least > c)) found[atomicAdd(&count, 1)] = c;
   }
   __syncthreads();
@@ -306,8 +319,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
     Cand c = {0ull, 0u};
     if (there) {
       c = found[i];
-      place = 0;
-      for (int j = 0; j < n && place < keep; ++j) place += found[j] > c;
+      place = place_of(c, n);
     }
     if (place >= keep) continue;
     const int64_t at = batch * keep + place;

@@ -19,7 +19,8 @@
 namespace cb {
 
 constexpr int K4_WARPS = 4;        // of a block
-constexpr int K4_GROUP = 64;       // tokens
+constexpr int K4_GROUP = 64;       // tokens at a time with single rows
+__host__ __device__ constexpr int K4_TILES(int chunks) { return chunks == 1 ? 4 : 2; }   // 16 tokens at a time with several
 constexpr int K4_ROWS = 8;
 
 struct Kv4AttnArgs {
@@ -100,10 +101,10 @@ __device__ __forceinline__ float to_top(float x, int k = 14) {
 }
 
 // A block's four warps are `row_warps` row tiles times 4 / row_warps shares of the tokens.  The warps of a share work on one ring of two stages of 64
-// tokens, which bulk copies fill while the other is read (each stage is read by all its warps before it is filled again).
+// or 32 tokens, which bulk copies fill while the other is read (each stage is read by all its warps before it is filled again).
 template <int NC, bool Q41>
-__global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 2 : 1) kv4_attention_kernel(const Kv4AttnArgs a) {
-  constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, STAGE = 4 * TILE;
+__global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) kv4_attention_kernel(const Kv4AttnArgs a) {
+  constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, TILES = K4_TILES(NC), GROUP = 16 * TILES, STAGE = TILES * TILE;
   __shared__ float sm[K4_WARPS][K4_ROWS], sl[K4_WARPS][K4_ROWS];
   __shared__ uint64_t bars[K4_WARPS][2];
   __shared__ int gave_up[K4_WARPS];
@@ -135,11 +136,11 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 2 : 1) 
   const int *table = a.table + (int64_t)b * a.max_pages;
   const int64_t page_bytes = kv4_page_bytes(a.s);
   const int tile_shift = a.s.page == 16 ? 0 : a.s.page == 32 ? 1 : a.s.page == 64 ? 2 : 3;   // tiles of a page, log2
-  const int first = t0 + share * K4_GROUP, step = shares * K4_GROUP;
+  const int first = t0 + share * GROUP, step = shares * GROUP;
   // by the share's first warp, lanes over tiles: what can be followed is copied, the rest counts for nothing
-  auto page_at = [&](int base) { return lane < 4 && base + 16 * lane < t1 ? table[((base >> 4) + lane) >> tile_shift] : -1; };
+  auto page_at = [&](int base) { return lane < TILES && base + 16 * lane < t1 ? table[((base >> 4) + lane) >> tile_shift] : -1; };
   auto issue = [&](int base, int id, int stage) {
-    const bool wanted = lane < 4 && base + 16 * lane < t1, good = wanted && kv4_page_ok(a.s, id);
+    const bool wanted = lane < TILES && base + 16 * lane < t1, good = wanted && kv4_page_ok(a.s, id);
     if (wanted && !good) report_bad_index(a.status, 46, id);
     const unsigned there = __ballot_sync(0xffffffffu, good);
     if (lane == 0) {
@@ -229,11 +230,11 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 2 : 1) 
     if (ok && mine && base < most) {
       const uint8_t *tiles = stages + stage * STAGE;
       const unsigned there = present[share][stage];
-      const bool clean = base + K4_GROUP <= least && there == 15u;   // every row sees every token
-      float s[4][4];
+      const bool clean = base + GROUP <= least && there == (1u << TILES) - 1u;   // every row sees every token
+      float s[TILES][4];
       __half2 big = __float2half2_rn(0.0f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < TILES; ++i) {
         const uint8_t *tile = tiles + i * TILE;
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -295,7 +296,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 2 : 1) 
       // running maximum; p is taken times a power of two that brings the largest p d near the top of fp16
       float top = run_max;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < TILES; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 2 : 1) 
       run_max = top;
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < TILES; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[i][e] = exp2_fast(s[i][e] - ref);
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 2 : 1) 
         const float lift = down * 0x1p14f;   // p at the top of fp16's range
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < TILES; ++i) {
           const float x[4] = {s[i][0] * lift, s[i][1] * lift, s[i][2] * lift, s[i][3] * lift};
           const uint32_t h0 = pack_half(x[0], x[1]), h1 = pack_half(x[2], x[3]);
           const uint32_t l0 = pack_half_lo(x[0], x[1], h0), l1 = pack_half_lo(x[2], x[3], h1);
@@ -355,15 +356,15 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 2 : 1) 
       // values
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        uint4 w[4];
+        uint4 w[TILES];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4 *>(tiles + i * TILE + PART + c * 512 + lane * 16);
+        for (int i = 0; i < TILES; ++i) w[i] = *reinterpret_cast<const uint4 *>(tiles + i * TILE + PART + c * 512 + lane * 16);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int blk = 2 * c + k;
           float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < TILES; ++i) {
             const uint2 d2 = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8);
             const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
             float pd[4] = {s[i][0] * d01.x, s[i][1] * d01.y, s[i][2] * d23.x, s[i][3] * d23.y};
@@ -856,35 +857,64 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
   if (a.parts > 1 && lane == 0) { dst[D] = top; dst[D + 1] = sum; }
 }
 
-// The parts of a row tile into one.  A block has a row tile; parts behind what its rows see were not written.
-__global__ void __launch_bounds__(256) kv4_attention_join_kernel(const Kv4AttnArgs a) {
+// The parts of a row into one, a block a row: the parts' weights first, by threads over parts, then threads over dims.  Parts behind what the row's
+// tile sees were not written.
+constexpr int KJ_THREADS = 128;
+constexpr int KJ_PARTS = 1024;   // at most, of a call
+
+__global__ void __launch_bounds__(KJ_THREADS) kv4_attention_join_kernel(const Kv4AttnArgs a) {
+  __shared__ float weight[KJ_PARTS], red[2][KJ_THREADS / 32];
   pdl_enter();
-  const int D = a.s.dim, tile_rows = a.tile_rows;
-  int64_t u = blockIdx.x;
+  const int D = a.s.dim, tile_rows = a.tile_rows, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t tile = blockIdx.x / tile_rows;
+  int64_t u = tile;
   const int rt = (int)(u % a.row_tiles); u /= a.row_tiles;
   const int head = (int)(u % a.s.kv_heads);
   const int b = (int)(u / a.s.kv_heads);
   const Kv4Seq seq = kv4_seq(a, b, false);
-  const int count = seq.count * a.group;
-  if (rt * tile_rows >= count) return;
+  const int count = seq.count * a.group, row = (int)(blockIdx.x % tile_rows), rr = rt * tile_rows + row;
+  if (rr >= count) return;
   const int last = min(count, rt * tile_rows + tile_rows) - 1;
   const int most = max(0, seq.length - seq.count + last / a.group + 1);
   const int parts = max(1, (most + a.part_tokens - 1) / a.part_tokens);
-  for (int i = threadIdx.x; i < tile_rows * D; i += 256) {
-    const int row = i / D, j = i % D, rr = rt * tile_rows + row;
-    if (rr >= count) break;
-    const float *p = a.part + (int64_t)blockIdx.x * a.parts * tile_rows * (D + 2) + row * (D + 2);
-    const int64_t step = (int64_t)tile_rows * (D + 2);
-    float top = -INFINITY;
-    for (int k = 0; k < parts; ++k) top = fmaxf(top, p[k * step + D]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, x = 0.0f;
-    for (int k = 0; k < parts; ++k) {
-      const float e = exp2_fast(p[k * step + D] - ref);
-      sum = fmaf(p[k * step + D + 1], e, sum);
-      x = fmaf(p[k * step + j], e, x);
+  const int64_t step = (int64_t)tile_rows * (D + 2);
+  const float *p = a.part + tile * a.parts * step + row * (D + 2);
+  float top = -INFINITY;
+  for (int k = tid; k < parts; k += KJ_THREADS) {
+    weight[k] = p[k * step + D];
+    top = fmaxf(top, weight[k]);
+  }
+  top = warp_max(top);
+  if (lane == 0) red[0][warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < KJ_THREADS / 32; ++w) top = fmaxf(top, red[0][w]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+  for (int k = tid; k < parts; k += KJ_THREADS) {
+    const float e = exp2_fast(weight[k] - ref);
+    weight[k] = e;
+    sum = fmaf(p[k * step + D + 1], e, sum);
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) red[1][warp] = sum;
+  __syncthreads();
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < KJ_THREADS / 32; ++w) sum += red[1][w];
+  float *out = a.out + (seq.first + rr / a.group) * (int64_t)a.heads * D + (int64_t)(head * a.group + rr % a.group) * D;
+  for (int j = tid; j < D; j += KJ_THREADS) {
+    float x = 0.0f;
+    int k = 0;
+    for (; k + 8 <= parts; k += 8) {   // eight loads under way
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = p[(k + i) * step + j];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x = fmaf(y[i], weight[k + i], x);
     }
-    a.out[(seq.first + rr / a.group) * (int64_t)a.heads * D + (int64_t)(head * a.group + rr % a.group) * D + j] = sum == 0.0f ? 0.0f : x / sum;
+    for (; k < parts; ++k) x = fmaf(p[k * step + j], weight[k], x);
+    out[j] = sum == 0.0f ? 0.0f : x / sum;
   }
 }
 
@@ -911,16 +941,17 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
     fill = 148 * 20 / p->warps; blocks = p->units; shares = p->warps;
   } else {
     p->warps = p->row_tiles >= 4 ? 4 : p->row_tiles >= 2 ? 2 : 1;
-    fill = 148 * 6; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = K4_WARPS / p->warps;
+    fill = 148 * 12; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = K4_WARPS / p->warps;
   }
   int64_t parts = blocks ? (fill + blocks - 1) / blocks : 1;
   const int64_t most = (groups + 2 * shares - 1) / (2 * shares);   // a part gives each warp two groups at least
   if (parts > most) parts = most;
+  if (parts > KJ_PARTS) parts = KJ_PARTS;
   if (parts < 1) parts = 1;
   const int64_t each = groups ? (groups + parts - 1) / parts : 1;
   p->part_tokens = (int)(each * K4_GROUP);
   p->parts = (int)(groups ? (groups + each - 1) / each : 1);
-  if (p->units * p->parts > 0x7fffffff) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
+  if (p->units * p->parts > 0x7fffffff / K4_ROWS) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
   return 0;
 }
 
@@ -934,14 +965,14 @@ static int kv4_attention_launch(caten_b200_ctx *ctx, const Kv4AttnArgs &a, int64
     CB_CUDA(ctx, launch_k(ctx, kernel, dim3((unsigned)((units * a.parts + per_block - 1) / per_block)), dim3(K1_WARPS * 32), smem, a));
     CB_LAUNCH_CHECK(ctx, "kv4_attention_row_kernel");
   } else {
-    const int smem = K4_WARPS / a.warps * 2 * 4 * kv4_tile_bytes(a.s);   // (no less than the sums of all warps where they are joined)
+    const int smem = K4_WARPS / a.warps * 2 * K4_TILES(NC) * kv4_tile_bytes(a.s);   // (no less than the sums of all warps where they are joined)
     const int64_t blocks = units / a.row_tiles * ((a.row_tiles + a.warps - 1) / a.warps) * a.parts;
     if (smem > 48 << 10) CB_CUDA(ctx, cudaFuncSetAttribute(kv4_attention_kernel<NC, Q41>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     CB_CUDA(ctx, launch_k(ctx, kv4_attention_kernel<NC, Q41>, dim3((unsigned)blocks), dim3(K4_WARPS * 32), smem, a));
     CB_LAUNCH_CHECK(ctx, "kv4_attention_kernel");
   }
   if (a.parts == 1) return 0;
-  CB_CUDA(ctx, launch_k(ctx, kv4_attention_join_kernel, dim3((unsigned)units), dim3(256), 0, a));
+  CB_CUDA(ctx, launch_k(ctx, kv4_attention_join_kernel, dim3((unsigned)(units * a.tile_rows)), dim3(KJ_THREADS), 0, a));
   CB_LAUNCH_CHECK(ctx, "kv4_attention_join_kernel");
   return 0;
 }
