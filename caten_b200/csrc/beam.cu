@@ -199,7 +199,9 @@ __device__ __forceinline__ u64 order_of(double x) {
 }
 __device__ __forceinline__ double value_of(u64 k) { return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k)); }
 
-constexpr int BJ_THREADS = 256;
+constexpr int BJ_THREADS = 1024;
+constexpr int BJ_HEADS = 256;    // threads that look at the lists' first entries
+constexpr int BJ_LANES = 16;     // threads that find one candidate's place
 constexpr int BJ_BEAMS = 32;
 constexpr int BJ_LISTS = 4096;   // of a request: beams x chunks
 constexpr int BJ_FOUND = BS_KEEP * BS_KEEP;
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
   const int lists = beams * chunks;
   const u64 *mine = parts + batch * lists * words;
   if (tid == 0) { bound = {1, 0xffffffffu}; count = 0; queued = 0; }   // (that bound: every candidate)
-  const u64 head = tid < lists ? mine[(int64_t)tid * words] : 0ull;     // (of an ended hypothesis: whatever is there, unused)
+  const u64 head = tid < min(lists, BJ_HEADS) ? mine[(int64_t)tid * words] : 0ull;     // (of an ended hypothesis: whatever is there, unused)
   for (int b = warp; b < beams; b += BJ_THREADS / 32) {
     const int64_t row = batch * beams + b;
     const float score = scores[row];
@@ -264,25 +266,35 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
     return {key ? order_of(base[b] + ((double)beam_key_value(key) - tops[b])) : 0ull, (uint32_t)(b * V + beam_key_index(key))};
   };
   auto entry = [&](int i, int j) { return cand_of(i, j, mine[(int64_t)i * words + j]); };
-  // how many of the n found are before c
-  auto place_of = [&](const Cand &c, int n) {
-    int place = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) place += found[j] > c;
-    return place;
+  // for each i of the n found: then(candidate, how many are before it), by one of the threads that count them
+  auto for_places = [&](int n, auto then) {
+    for (int i0 = 0; i0 < n; i0 += BJ_THREADS / BJ_LANES) {
+      const int i = i0 + tid / BJ_LANES;
+      const Cand c = found[min(i, n - 1)];
+      int place = 0;
+#pragma unroll 4
+      for (int j = tid % BJ_LANES; j < n; j += BJ_LANES) place += found[j] > c;
+#pragma unroll
+      for (int o = 1; o < BJ_LANES; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+      if (i < n && tid % BJ_LANES == 0) then(c, place);
+    }
   };
   // The keep-th of the lists' first entries: `keep` candidates are not behind it, and at most `keep` lists have any that are not.  Where a thread
   // has several lists, the threads' best give a first bound, and the few first entries that it leaves the second.
-  Cand best = tid < lists ? cand_of(tid, 0, head) : Cand{0ull, 0xffffffffu};
-  for (int i = tid + BJ_THREADS; i < lists; i += BJ_THREADS) {
-    const Cand c = entry(i, 0);
-    if (c > best) best = c;
+  Cand best = tid < min(lists, BJ_HEADS) ? cand_of(tid, 0, head) : Cand{0ull, 0xffffffffu};
+  if (tid < BJ_HEADS) {
+    for (int i = tid + BJ_HEADS; i < lists; i += BJ_HEADS) {
+      const Cand c = entry(i, 0);
+      if (c > best) best = c;
+    }
+    found[tid] = best;
   }
-  found[tid] = best;
   __syncthreads();
-  if (best.value && place_of(best, min(lists, BJ_THREADS)) == keep - 1) bound = best;
+  for_places(min(lists, BJ_HEADS), [&](const Cand &c, int place) {
+    if (c.value && place == keep - 1) bound = c;
+  });
   __syncthreads();
-  if (lists > BJ_THREADS) {
+  if (lists > BJ_HEADS) {
     const Cand first = bound;
     __syncthreads();
     for (int i = tid; i < lists; i += BJ_THREADS) {
@@ -291,14 +303,15 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
     }
     __syncthreads();
     const int n = count;
-    for (int i = tid; i < n; i += BJ_THREADS)
-      if (place_of(found[i], n) == keep - 1) bound = found[i];
+    for_places(n, [&](const Cand &c, int place) {
+      if (place == keep - 1) bound = c;
+    });
     __syncthreads();
     if (tid == 0) count = 0;
   }
   const Cand least = bound;
   __syncthreads();
-  if (lists <= BJ_THREADS) {
+  if (lists <= BJ_HEADS) {
     if (best.value && !(least > best)) queue[atomicAdd(&queued, 1)] = tid;
   } else {
     for (int i = tid; i < lists; i += BJ_THREADS) {
@@ -312,16 +325,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
     if (c.value && !(least > c)) found[atomicAdd(&count, 1)] = c;
   }
   __syncthreads();
-  const int n = count;
-  for (int i = tid; i < max(n, keep); i += BJ_THREADS) {
-    const bool there = i < n;
-    int place = i;
-    Cand c = {0ull, 0u};
-    if (there) {
-      c = found[i];
-      place = place_of(c, n);
-    }
-    if (place >= keep) continue;
+  auto write = [&](int place, bool there, const Cand &c) {
     const int64_t at = batch * keep + place;
     const int parent = there ? (int)(c.id / (uint32_t)V) : min(place, beams - 1);
     const int64_t token = there ? (int64_t)(c.id % (uint32_t)V) : eos >= 0 ? eos : 0;
@@ -329,12 +333,17 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
     out_parents[at] = parent;
     out_tokens[at] = token;
     if (out_ended) out_ended[at] = over[parent] || (eos >= 0 && token == eos);
-  }
+  };
+  const int n = count;
+  for_places(n, [&](const Cand &c, int place) {
+    if (place < keep) write(place, true, c);
+  });
+  if (tid >= n && tid < keep) write(tid, false, Cand{0ull, 0u});
 }
 
 // Chunks of 8192 logits, or of 2048 where the larger ones would not give every SM a block.
 constexpr int64_t BS_VOCAB = (1 << 20) - 8192;
-static_assert(BJ_BEAMS * ((BS_VOCAB + 3 + 8191) / 8192) <= BJ_LISTS && BS_KEEP * (BJ_LISTS / BJ_THREADS) <= BJ_FOUND, "lists of a request");
+static_assert(BJ_BEAMS * ((BS_VOCAB + 3 + 8191) / 8192) <= BJ_LISTS && BS_KEEP * (BJ_LISTS / BJ_HEADS) <= BJ_FOUND, "lists of a request");
 static int beam_vecs(int64_t batch, int64_t beams, int64_t V) {
   return batch * beams * ((V + 3 + 8191) / 8192) >= 148 || beams * ((V + 3 + 2047) / 2048) > BJ_LISTS ? 8 : 2;
 }
