@@ -178,70 +178,85 @@ __global__ void __launch_bounds__(256) kv_slots_kernel(PagesArgs a) {
 
 // ---- rows into the cache ---------------------------------------------------------------------------
 // A block of 32 values is eight lanes' float4.  Codes are those of the GGUF formats: Q4_0  d = (value of largest magnitude) / -8,
-// code = min(15, trunc(x / d + 8.5)); Q4_1  d = (max - min) / 15, code = min(15, trunc((x - min) / d + 0.5)).  Which code is nearest is decided
-// exactly: in fp32, whose error here is below 4e-6, unless the quotient is within 1e-5 of a border, then in 64 bits.  d and the minimum are
-// rounded to fp16 (half a step: 2^-11) because that is what the formats hold.  Where one of them is not finite there (a value that is not, or
-// one beyond fp16's reach), the scale is NaN: a block is what it stands for, or NaN in all of its values.
+// code = min(15, trunc(x / d + 8.5)); Q4_1  d = (max - min) / 15, code = min(15, trunc((x - min) / d + 0.5)).  Which code is nearest, and which half d
+// rounds to (half a step: 2^-11; the formats hold halves), is decided exactly: in fp32, whose error in a code is below 6e-6 here, and in 64 bits for the
+// few blocks in which a quotient is within 1e-5 of a border or d's last bits next to one of fp16's.  Where d or the minimum is not finite in fp16
+// (a value that is not, or one beyond fp16's reach), the scale is NaN: a block is what it stands for, or NaN in all of its values.
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
-__device__ __forceinline__ uint32_t kv4_code(float x, float inverse, float offset, double d, float low) {
-  const float y = fmaf(x - low, inverse, offset);
-  if (fabsf(y - rintf(y)) >= 1e-5f) return (uint32_t)min(15, max(0, (int)y));
-  const double e = ((double)x - (double)low) / d + (double)offset;
-  return (uint32_t)min(15, max(0, (int)e));
-}
-
-__device__ __forceinline__ __half scale_or_nan(float d, float minimum) {
-  const __half h = __float2half_rn(d);
-  return fabsf(__half2float(h)) < INFINITY && fabsf(minimum) < INFINITY ? h : __ushort_as_half((unsigned short)0x7fff);
+__device__ __noinline__ uint32_t kv4_codes_exactly(float4 x, double d, double low, double offset, bool none, uint32_t without) {
+  const float v[4] = {x.x, x.y, x.z, x.w};
+  uint32_t codes = 0;
+  for (int i = 0; i < 4; ++i) codes |= (uint32_t)min(15, max(0, (int)(((double)v[i] - low) / d + offset))) << (4 * i);
+  return none ? without : codes;
 }
 
 // this lane's four values of a block that eight consecutive lanes hold -> four codes (low bits first), scale and minimum
 template <bool Q41>
 __device__ __forceinline__ uint32_t kv4_quantise(float4 x, __half *scale, __half *minimum) {
+  constexpr float MAGIC = 12582912.0f;   // 1.5 * 2^23: added, it leaves the nearest whole number in the low bits
   const float v[4] = {x.x, x.y, x.z, x.w};
-  uint32_t codes = 0;
-  if (Q41) {
-    float hi = v[0], lo = v[0];
+  float hi = max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])), lo = min_nan(min_nan(v[0], v[1]), min_nan(v[2], v[3]));
 #pragma unroll
-    for (int i = 1; i < 4; ++i) { hi = max_nan(hi, v[i]); lo = min_nan(lo, v[i]); }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    }
-    const double d = ((double)hi - (double)lo) / 15.0;
-    *minimum = __float2half_rn(lo);
-    *scale = scale_or_nan((float)d, __half2float(*minimum));
-    const float inverse = 1.0f / (float)d;
-    if (__half2float(*scale) != 0.0f)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) codes |= kv4_code(v[i], inverse, 0.5f, d, lo) << (4 * i);
-  } else {
-    // the value of largest magnitude, the first of equal ones; magnitudes compared as bits, NaN above infinity
-    float m = v[0];
-    int at = (threadIdx.x & 7) * 4;
-#pragma unroll
-    for (int i = 1; i < 4; ++i)
-      if ((__float_as_uint(v[i]) & 0x7fffffffu) > (__float_as_uint(m) & 0x7fffffffu)) { m = v[i]; at = (threadIdx.x & 7) * 4 + i; }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      const float om = __shfl_xor_sync(0xffffffffu, m, o);
-      const int oat = __shfl_xor_sync(0xffffffffu, at, o);
-      const uint32_t a = __float_as_uint(m) & 0x7fffffffu, b = __float_as_uint(om) & 0x7fffffffu;
-      if (b > a || (b == a && oat < at)) { m = om; at = oat; }
-    }
-    const float d = m / -8.0f;
-    *scale = scale_or_nan(d, 0.0f);
-    const float inverse = 1.0f / d;
-    if (__half2float(*scale) != 0.0f) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) codes |= kv4_code(v[i], inverse, 8.5f, (double)d, 0.0f) << (4 * i);
-    } else {
-      codes = 0x8888u;
-    }
+  for (int o = 1; o < 8; o <<= 1) {
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
   }
+  float d, base;
+  bool exactly = false;
+  if (Q41) {
+    base = lo;
+    // (hi - lo) / 15 with the difference's own rounding error (Knuth's two-sum) and the quotient's remainder taken back in
+    const float r = hi - lo, back = r - hi, err = (hi - (r - back)) - (lo + back);
+    const float q = r * (1.0f / 15.0f);
+    d = fmaf(fmaf(-15.0f, q, r) + err, 1.0f / 15.0f, q);
+  } else {
+    base = 0.0f;
+    const bool both = hi == -lo;   // equal magnitudes: the first one's sign (rare, and by the whole warp)
+    float m = hi > -lo ? hi : lo;
+    if (__any_sync(0xffffffffu, both && hi > 0.0f)) {
+      int at = 32;
+#pragma unroll
+      for (int i = 3; i >= 0; --i)
+        if (fabsf(v[i]) == hi) at = (threadIdx.x & 7) * 4 + i;
+      int first = at;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+      float mine = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (first == (int)(threadIdx.x & 7) * 4 + i) mine = v[i];
+      const float sign = __shfl_sync(0xffffffffu, mine, (threadIdx.x & 24) + (first & 31) / 4);
+      if (both) m = sign;
+    }
+    if (!(hi >= lo)) m = hi + lo;   // (NaN)
+    d = m / -8.0f;
+  }
+  const uint32_t bits = __float_as_uint(d) & 0x7fffffffu;
+  // next to a border between halves, or where halves are subnormal
+  if (Q41) exactly = bits < 0x38800000u || (uint32_t)((int)(bits & 0x1fffu) - 0x1000 + 2) <= 4u;
+  float inverse;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(d));
+  uint32_t codes = 0;
+#pragma unroll
+  for (int i = 3; i >= 0; --i) {
+    const float y = fminf(Q41 ? (v[i] - base) * inverse : fmaf(v[i], inverse, 8.0f), 15.25f), t = y + MAGIC;   // (up to 15.5 is 15, and so is all above)
+    exactly |= !(fabsf(y - (t - MAGIC)) < 0.49999f);
+    codes = codes * 16u + __float_as_uint(t);
+  }
+  codes -= __float_as_uint(MAGIC) * 0x1111u;
+  if (exactly) {
+    const double exact = Q41 ? ((double)hi - (double)lo) / 15.0 : (double)d;
+    d = (float)exact;
+    const bool none = __half2float(__float2half_rn(d)) == 0.0f;
+    codes = kv4_codes_exactly(x, exact, (double)base, Q41 ? 0.5 : 8.5, none, Q41 ? 0u : 0x8888u);
+  }
+  *scale = __float2half_rn(d);
+  if (Q41) *minimum = __float2half_rn(lo);
+  const bool finite = fabsf(__half2float(*scale)) < INFINITY && (!Q41 || fabsf(__half2float(*minimum)) < INFINITY);
+  if (!finite) *scale = __ushort_as_half((unsigned short)0x7fff);
+  if (__half2float(*scale) == 0.0f) codes = Q41 ? 0u : 0x8888u;
   return codes;
 }
 
@@ -252,87 +267,118 @@ struct RowsArgs {
   int *status;
   int64_t ld, tokens;
   Kv4Shape s;
+  int page_shift;
   int vec;                   // rows can be read and written by 16 bytes
 };
 
-__device__ __forceinline__ bool kv4_slot(const RowsArgs &a, int64_t token, int64_t *page_id, int *within) {
-  const int slot = a.slots[token];
-  if (slot < 0) {
-    if (slot < -1) report_bad_index(a.status, 40, slot);
-    return false;
+// A block has one head of sixteen rows of a call: rows that lie side by side in the cache have their codes in the same sectors, which come and go once.
+// What a row costs beside its values (slot, page, address) is worked out once, by a thread a row.  (A thread for any four values, 64-bit
+// divisions and all: 8191 rows of 4 x 128, stored and loaded, 47 us.)
+constexpr int KR_THREADS = 256, KR_ROWS = 16;
+
+struct RowsShared {
+  long long tile[KR_ROWS];   // byte of the tile in the pool; -1: nowhere
+  int token[KR_ROWS];        // in the tile
+};
+__device__ __forceinline__ void rows_begin(const RowsArgs &a, RowsShared &sh, int64_t first, int head, bool tells) {
+  if (threadIdx.x < KR_ROWS) {
+    const int64_t row = first + threadIdx.x;
+    long long tile = -1;
+    int token = 0;
+    if (row < a.tokens) {
+      const int slot = a.slots[row];
+      const int page_id = slot >> a.page_shift, within = slot & ((1 << a.page_shift) - 1);
+      if (slot >= 0 && kv4_page_ok(a.s, page_id)) {
+        tile = kv4_tile_at(a.s, page_id, head, within);
+        token = within & 15;
+      } else if (slot != -1 && tells) {
+        report_bad_index(a.status, 40, slot);
+      }
+    }
+    sh.tile[threadIdx.x] = tile;
+    sh.token[threadIdx.x] = token;
   }
-  *page_id = slot / a.s.page;
-  *within = slot % a.s.page;
-  if (kv4_page_ok(a.s, *page_id)) return true;
-  report_bad_index(a.status, 40, slot);
-  return false;
+  __syncthreads();
 }
 
-template <bool Q41>
-__global__ void __launch_bounds__(256) kv4_store_kernel(RowsArgs a) {
+template <int NC, bool Q41>
+__global__ void __launch_bounds__(KR_THREADS) kv4_store_kernel(RowsArgs a) {
+  constexpr int D = 64 * NC, QUADS = D / 4, PART = (Q41 ? 10 : 9) * D;
+  __shared__ RowsShared sh;
   pdl_enter();
-  const int quads = a.s.kv_heads * a.s.dim / 4;   // float4 of a token's keys
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = a.tokens * 2 * quads;
-  const bool there = i < all;                     // (whole groups of eight lanes: quads is a multiple of 16)
-  const int64_t token = there ? i / (2 * quads) : 0;
-  const int c = there ? (int)(i % (2 * quads)) : 0;
-  const bool of_k = c < quads;
-  const int col = (of_k ? c : c - quads) * 4;
-  int64_t page_id = 0;
-  int within = 0;
-  const bool ok = there && kv4_slot(a, token, &page_id, &within);
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (ok) {
-    const float *src = (of_k ? a.k : a.v) + token * a.ld + col;
-    if (a.vec) x = __ldcs(reinterpret_cast<const float4 *>(src));
-    else x = make_float4(src[0], src[1], src[2], src[3]);
+  const int64_t first = (int64_t)blockIdx.x * KR_ROWS;
+  const int head = blockIdx.y;
+  rows_begin(a, sh, first, head, head == 0);
+  constexpr int N = KR_ROWS * 2 * QUADS / KR_THREADS;
+  float4 x[N];   // all of a thread's loads are under way before the first is used
+#pragma unroll
+  for (int it = 0; it < N; ++it) {   // (groups of eight lanes have a block each)
+    const int i = it * KR_THREADS + threadIdx.x, row = i / (2 * QUADS), c = i % (2 * QUADS), dim = c % QUADS * 4;
+    x[it] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (sh.tile[row] >= 0) {
+      const float *src = (c < QUADS ? a.k : a.v) + (first + row) * a.ld + head * D + dim;
+      if (a.vec) x[it] = __ldcs(reinterpret_cast<const float4 *>(src));
+      else x[it] = make_float4(src[0], src[1], src[2], src[3]);
+    }
   }
-  __half d, m;
-  const uint32_t codes = kv4_quantise<Q41>(x, &d, &m);
-  const uint32_t next = __shfl_down_sync(0xffffffffu, codes, 1);
-  if (!ok) return;
-  const int head = col / a.s.dim, dim = col % a.s.dim, tok = within % 16;
-  uint8_t *part = a.pool + kv4_tile_at(a.s, page_id, head, within) + (of_k ? 0 : kv4_part_bytes(a.s));
-  if (of_k) {
-    if (dim % 8 == 0) *reinterpret_cast<uint32_t *>(part + kv4_k_byte(tok, dim)) = codes | next << 16;
-  } else {
-    *reinterpret_cast<uint16_t *>(part + kv4_v_byte(tok, dim)) = (uint16_t)codes;
-  }
-  if (dim % 32 == 0) {
-    __half *scales = reinterpret_cast<__half *>(part + 8 * a.s.dim) + kv4_scale_index(tok, dim / 32, a.s.dim);
-    scales[0] = d;
-    if (Q41) scales[a.s.dim / 2] = m;
+#pragma unroll
+  for (int it = 0; it < N; ++it) {
+    const int i = it * KR_THREADS + threadIdx.x, row = i / (2 * QUADS), c = i % (2 * QUADS), dim = c % QUADS * 4, tok = sh.token[row];
+    const bool of_k = c < QUADS, ok = sh.tile[row] >= 0;
+    __half d, m;
+    const uint32_t codes = kv4_quantise<Q41>(x[it], &d, &m);
+    const uint32_t next = __shfl_down_sync(0xffffffffu, codes, 1);
+    if (!ok) continue;
+    uint8_t *part = a.pool + sh.tile[row] + (of_k ? 0 : PART);
+    if (of_k) {
+      if (dim % 8 == 0) *reinterpret_cast<uint32_t *>(part + kv4_k_byte(tok, dim)) = codes | next << 16;
+    } else {
+      *reinterpret_cast<uint16_t *>(part + kv4_v_byte(tok, dim)) = (uint16_t)codes;
+    }
+    if (dim % 32 == 0) {
+      __half *scales = reinterpret_cast<__half *>(part + 8 * D) + kv4_scale_index(tok, dim / 32, D);
+      scales[0] = d;
+      if (Q41) scales[D / 2] = m;
+    }
   }
 }
 
 // ---- rows out of the cache -------------------------------------------------------------------------
-template <bool Q41>
-__global__ void __launch_bounds__(256) kv4_load_kernel(RowsArgs a) {
+template <int NC, bool Q41>
+__global__ void __launch_bounds__(KR_THREADS) kv4_load_kernel(RowsArgs a) {
+  constexpr int D = 64 * NC, QUADS = D / 4, PART = (Q41 ? 10 : 9) * D;
+  __shared__ RowsShared sh;
   pdl_enter();
-  const int quads = a.s.kv_heads * a.s.dim / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.tokens * 2 * quads) return;
-  const int64_t token = i / (2 * quads);
-  const int c = (int)(i % (2 * quads));
-  const bool of_k = c < quads;
-  const int col = (of_k ? c : c - quads) * 4;
-  int64_t page_id;
-  int within;
-  if (!kv4_slot(a, token, &page_id, &within)) return;
-  const int head = col / a.s.dim, dim = col % a.s.dim, tok = within % 16;
-  const uint8_t *part = a.pool + kv4_tile_at(a.s, page_id, head, within) + (of_k ? 0 : kv4_part_bytes(a.s));
-  const uint32_t codes = *reinterpret_cast<const uint16_t *>(part + (of_k ? kv4_k_byte(tok, dim) : kv4_v_byte(tok, dim)));
-  const __half *scales = reinterpret_cast<const __half *>(part + 8 * a.s.dim) + kv4_scale_index(tok, dim / 32, a.s.dim);
-  const float d = __half2float(scales[0]), m = Q41 ? __half2float(scales[a.s.dim / 2]) : 0.0f;
-  float y[4];
+  const int64_t first = (int64_t)blockIdx.x * KR_ROWS;
+  const int head = blockIdx.y;
+  rows_begin(a, sh, first, head, head == 0);
+  constexpr int N = KR_ROWS * 2 * QUADS / KR_THREADS;
+  uint32_t codes[N];
+  __half2 scale[N];   // d, and Q4_1's minimum
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int code = (int)(codes >> (4 * e) & 15u);
-    y[e] = Q41 ? d * (float)code + m : d * (float)(code - 8);
+  for (int it = 0; it < N; ++it) {
+    const int i = it * KR_THREADS + threadIdx.x, row = i / (2 * QUADS), c = i % (2 * QUADS), dim = c % QUADS * 4, tok = sh.token[row];
+    if (sh.tile[row] < 0) continue;
+    const uint8_t *part = a.pool + sh.tile[row] + (c < QUADS ? 0 : PART);
+    codes[it] = *reinterpret_cast<const uint16_t *>(part + (c < QUADS ? kv4_k_byte(tok, dim) : kv4_v_byte(tok, dim)));
+    const __half *scales = reinterpret_cast<const __half *>(part + 8 * D) + kv4_scale_index(tok, dim / 32, D);
+    scale[it] = __halves2half2(scales[0], Q41 ? scales[D / 2] : __ushort_as_half(0));
   }
-  float *dst = (of_k ? a.k : a.v) + token * a.ld + col;
-  if (a.vec) __stcs(reinterpret_cast<float4 *>(dst), make_float4(y[0], y[1], y[2], y[3]));
-  else { dst[0] = y[0]; dst[1] = y[1]; dst[2] = y[2]; dst[3] = y[3]; }
+#pragma unroll
+  for (int it = 0; it < N; ++it) {
+    const int i = it * KR_THREADS + threadIdx.x, row = i / (2 * QUADS), c = i % (2 * QUADS), dim = c % QUADS * 4;
+    if (sh.tile[row] < 0) continue;
+    const float d = __low2float(scale[it]), m = __high2float(scale[it]);
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float code = __uint_as_float(0x4b000000u | (codes[it] >> (4 * e) & 15u)) - (Q41 ? 8388608.0f : 8388616.0f);   // exact
+      y[e] = Q41 ? d * code + m : d * code;
+    }
+    float *dst = (c < QUADS ? a.k : a.v) + (first + row) * a.ld + head * D + dim;
+    if (a.vec) __stcs(reinterpret_cast<float4 *>(dst), make_float4(y[0], y[1], y[2], y[3]));
+    else { dst[0] = y[0]; dst[1] = y[1]; dst[2] = y[2]; dst[3] = y[3]; }
+  }
 }
 
 // ---- checks ----------------------------------------------------------------------------------------
@@ -360,16 +406,24 @@ static int rows_check(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4
   a->slots = slots;
   a->ld = ld; a->tokens = tokens;
   a->vec = ld % 4 == 0 && ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
-  const int64_t blocks = (tokens * 2 * (c->kv_heads * (int64_t)c->dim / 4) + 255) / 256;
-  if (blocks > 0x7fffffff) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: %lld tokens in one call", who, (long long)tokens);
+  a->page_shift = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
   return 0;
 }
 
+template <int NC>
+static cudaError_t rows_launch_d(caten_b200_ctx *ctx, const RowsArgs &a, bool store) {
+  const dim3 grid((unsigned)((a.tokens + KR_ROWS - 1) / KR_ROWS), (unsigned)a.s.kv_heads);
+  void (*kernel)(RowsArgs) = store ? (a.s.q41 ? kv4_store_kernel<NC, true> : kv4_store_kernel<NC, false>) : (a.s.q41 ? kv4_load_kernel<NC, true> : kv4_load_kernel<NC, false>);
+  return launch_k(ctx, kernel, grid, dim3(KR_THREADS), 0, a);
+}
 static int rows_launch(caten_b200_ctx *ctx, RowsArgs a, bool store) {
   a.status = ctx->d_status;
-  const unsigned blocks = (unsigned)((a.tokens * 2 * (a.s.kv_heads * (int64_t)a.s.dim / 4) + 255) / 256);
-  void (*kernel)(RowsArgs) = store ? (a.s.q41 ? kv4_store_kernel<true> : kv4_store_kernel<false>) : (a.s.q41 ? kv4_load_kernel<true> : kv4_load_kernel<false>);
-  CB_CUDA(ctx, launch_k(ctx, kernel, dim3(blocks), dim3(256), 0, a));
+  switch (a.s.dim / 64) {
+    case 1: CB_CUDA(ctx, rows_launch_d<1>(ctx, a, store)); break;
+    case 2: CB_CUDA(ctx, rows_launch_d<2>(ctx, a, store)); break;
+    case 3: CB_CUDA(ctx, rows_launch_d<3>(ctx, a, store)); break;
+    default: CB_CUDA(ctx, rows_launch_d<4>(ctx, a, store));
+  }
   CB_LAUNCH_CHECK(ctx, store ? "kv4_store_kernel" : "kv4_load_kernel");
   return 0;
 }
