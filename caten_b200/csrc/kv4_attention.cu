@@ -62,7 +62,7 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs &a, int b, bool tell
 }
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -102,21 +102,25 @@ __device__ __forceinline__ float to_top(float x, int k = 14) {
 
 // A block's four warps are `row_warps` row tiles times 4 / row_warps shares of the tokens.  The warps of a share work on one ring of two stages of 64
 // or 32 tokens, which bulk copies fill while the other is read (each stage is read by all its warps before it is filled again).
-template <int NC, bool Q41>
+// With four row tiles (SHARED) the warps first turn a stage's codes into operands and its scales into floats, a quarter each, in shared memory: of the
+// instructions of 16 tokens and a block of 32 dims, a hundred, that is nearly half, and each warp would do it for itself (5 prompts of 167 to 333
+// tokens, 16 heads over 4 of 128: 130 us).
+template <int NC, bool Q41, bool SHARED>
 __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) kv4_attention_kernel(const Kv4AttnArgs a) {
   constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, TILES = K4_TILES(NC), GROUP = 16 * TILES, STAGE = TILES * TILE;
   __shared__ float sm[K4_WARPS][K4_ROWS], sl[K4_WARPS][K4_ROWS];
   __shared__ uint64_t bars[K4_WARPS][2];
   __shared__ int gave_up[K4_WARPS];
   __shared__ unsigned present[K4_WARPS][2];          // of a share: tiles of each stage
-  extern __shared__ __align__(128) uint8_t ring[];   // two stages a share; behind the last group, the warps' sums
+  __shared__ unsigned largest_scale[2];              // SHARED: of a stage's values
+  extern __shared__ __align__(128) uint8_t ring[];   // two stages a share (SHARED: then the operands); behind the last group, the warps' sums
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = warp_index(), g = lane >> 2, t = lane & 3;
   const int row_warps = a.warps, shares = K4_WARPS / row_warps, share = warp / row_warps, sub = warp % row_warps;
   int64_t u = blockIdx.x;
   const int part = (int)(u % a.parts); u /= a.parts;
   const int row_groups = (a.row_tiles + row_warps - 1) / row_warps;
-  const int rg = (int)(u % row_groups); u /= row_groups;
+  const int rg = row_groups - 1 - (int)(u % row_groups); u /= row_groups;   // (later rows see more: they start first)
   const int head = (int)(u % a.s.kv_heads);
   const int b = (int)(u / a.s.kv_heads);
   const Kv4Seq seq = kv4_seq(a, b, threadIdx.x == 0 && part == 0 && rg == 0 && head == 0);
@@ -214,6 +218,11 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] = 0.0f;
   }
+  // SHARED: operands of a stage [tile][chunk][K: block, token half | V: block, dims][lane], then scales of K, of V and minima of K as floats
+  uint4 *const ops = reinterpret_cast<uint4 *>(ring + 2 * STAGE);
+  float *const floats = reinterpret_cast<float *>(ops + TILES * NC * 8 * 32);
+  constexpr int PER_TILE = 16 * NB;   // floats of a kind
+  if (SHARED && threadIdx.x < 2) largest_scale[threadIdx.x] = 0;
   __syncthreads();   // the barriers are there
   int stage = 0;
   uint32_t phase = 0;
@@ -227,6 +236,47 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
       a.status[1] = 48;
     }
     all_ok &= ok;
+    if (SHARED) {
+      const uint8_t *tiles = stages + stage * STAGE;
+      const unsigned there = present[share][stage];
+#pragma unroll
+      for (int unit0 = 0; unit0 < TILES * NC * 2; unit0 += K4_WARPS) {
+        const int unit = unit0 + sub, i = unit / (2 * NC), c = unit % NC;
+        const bool of_k = unit / NC % 2 == 0;
+        const uint4 w = *reinterpret_cast<const uint4 *>(tiles + i * TILE + (of_k ? 0 : PART) + c * 512 + lane * 16);
+        uint4 *dst = ops + ((i * NC + c) * 8 + (of_k ? 0 : 4)) * 32 + lane;
+        // K: tokens 0..7 and 8..15 of the even and the odd block; V: the halves of the even and of the odd block (tokens 2t, 2t + 1 | 2t + 8, 2t + 9)
+        const uint32_t x[4] = {of_k ? w.x : __byte_perm(w.x, w.y, 0x5410), of_k ? w.z : __byte_perm(w.z, w.w, 0x5410), of_k ? w.y : __byte_perm(w.x, w.y, 0x7632),
+                               of_k ? w.w : __byte_perm(w.z, w.w, 0x7632)};
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const uint32_t p = x[2 * n], q = x[2 * n + 1];
+          const uint32_t pl = codes_lo(p), ph = codes_hi(p), pL = codes_lo(p >> 8), pH = codes_hi(p >> 8);
+          const uint32_t ql = codes_lo(q), qh = codes_hi(q), qL = codes_lo(q >> 8), qH = codes_hi(q >> 8);
+          dst[2 * n * 32] = of_k ? make_uint4(pl, ph, pL, pH) : make_uint4(pl, ph, ql, qh);
+          dst[(2 * n + 1) * 32] = of_k ? make_uint4(ql, qh, qL, qH) : make_uint4(pL, pH, qL, qH);
+        }
+      }
+      unsigned largest = 0;
+      constexpr int KINDS = Q41 ? 3 : 2;
+      for (int j = sub * 32 + lane; j < TILES * KINDS * PER_TILE / 2; j += 32 * K4_WARPS) {
+        const int i = j / (KINDS * PER_TILE / 2), rest = j % (KINDS * PER_TILE / 2), kind = rest / (PER_TILE / 2), pair = rest % (PER_TILE / 2);
+        uint32_t h = *reinterpret_cast<const uint32_t *>(tiles + i * TILE + (kind == 1 ? PART : 0) + (kind == 2 ? 9 : 8) * D + pair * 4);
+        if (kind == 1) {   // what stands behind the last token may be anything
+          const int at = base + 16 * i + pair / 2 / NB * 2 + 8 * (pair & 1);
+          h &= (there >> i & 1 && at < t1 ? 0xffffu : 0u) | (there >> i & 1 && at + 1 < t1 ? 0xffff0000u : 0u);
+        }
+        const float2 f = half_pair(h);
+        *reinterpret_cast<float2 *>(floats + (i * KINDS + kind) * PER_TILE + pair * 2) = f;
+        if (kind == 1) {
+          const unsigned u0 = __float_as_uint(fabsf(f.x)), u1 = __float_as_uint(fabsf(f.y));
+          largest = max(largest, max(u0 < 0x7f800000u ? u0 : 0u, u1 < 0x7f800000u ? u1 : 0u));
+        }
+      }
+      largest = __reduce_max_sync(0xffffffffu, largest);
+      if (lane == 0 && largest) atomicMax(&largest_scale[stage], largest);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    }
     if (ok && mine && base < most) {
       const uint8_t *tiles = stages + stage * STAGE;
       const unsigned there = present[share][stage];
@@ -239,27 +289,43 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          const uint4 w = *reinterpret_cast<const uint4 *>(tile + c * 512 + lane * 16);
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (!SHARED) w = *reinterpret_cast<const uint4 *>(tile + c * 512 + lane * 16);
           const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const int blk = 2 * c + k;
             const uint8_t *sc = tile + 8 * D + (t * NB + blk) * 8;
-            const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
-            const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
-            const float d[4] = {d01.x, d01.y, d23.x, d23.y};
-            float m[4];
-            if (Q41) {
+            float d[4], m[4];
+            if (SHARED) {
+              const float4 f = *reinterpret_cast<const float4 *>(floats + i * (Q41 ? 3 : 2) * PER_TILE + (t * NB + blk) * 4);
+              d[0] = f.x; d[1] = f.y; d[2] = f.z; d[3] = f.w;
+              if (Q41) {
+                const float4 fm = *reinterpret_cast<const float4 *>(floats + (i * 3 + 2) * PER_TILE + (t * NB + blk) * 4);
+                m[0] = fm.x; m[1] = fm.y; m[2] = fm.z; m[3] = fm.w;
+              }
+            } else {
+              const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
+              const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
+              d[0] = d01.x; d[1] = d01.y; d[2] = d23.x; d[3] = d23.y;
+            }
+            if (Q41 && !SHARED) {
               const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
               const float2 m01 = half_pair(m2.x), m23 = half_pair(m2.y);
               m[0] = m01.x; m[1] = m01.y; m[2] = m23.x; m[3] = m23.y;
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n) {   // tokens 0..7, 8..15
-              const uint32_t lo = words[2 * n + k], hi = lo >> 8;
+              uint4 op;
+              if (SHARED) {
+                op = ops[((i * NC + c) * 8 + 2 * k + n) * 32 + lane];
+              } else {
+                const uint32_t lo = words[2 * n + k], hi = lo >> 8;
+                op = make_uint4(codes_lo(lo), codes_hi(lo), codes_lo(hi), codes_hi(hi));
+              }
               float p[4] = {Q41 ? qsum8[blk] : 0.0f, Q41 ? qsum8[blk] : 0.0f, 0.f, 0.f};   // (d code + m = d (code - 8 + 8) + m)
-              mma_16816(p, qa[blk][0], codes_lo(lo), codes_hi(lo));
-              mma_16816(p, qa[blk][1], codes_lo(hi), codes_hi(hi));
+              mma_16816(p, qa[blk][0], op.x, op.y);
+              mma_16816(p, qa[blk][1], op.z, op.w);
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
                 const int e = 2 * n + j;
@@ -267,6 +333,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
                 acc[e] = fmaf(d[e], p[j] + p[2 + j], acc[e]);
               }
             }
+            if (SHARED) continue;
             // the values' largest scale
             const uint2 v2 = *reinterpret_cast<const uint2 *>(sc + PART);
             uint32_t vx = v2.x & 0x7fff7fffu, vy = v2.y & 0x7fff7fffu;
@@ -301,9 +368,14 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
         for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      float largest = fmaxf(__low2float(big), __high2float(big));
-      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+      float largest;
+      if (SHARED) {
+        largest = __uint_as_float(largest_scale[stage]);
+      } else {
+        largest = fmaxf(__low2float(big), __high2float(big));
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+      }
       const float up = to_top(largest), down = 1.0f / up;
       const float ref = top == -INFINITY ? 0.0f : top;
       const float corr = exp2_fast(run_max - ref);   // (-inf: 0)
@@ -358,16 +430,23 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
       for (int c = 0; c < NC; ++c) {
         uint4 w[TILES];
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) w[i] = *reinterpret_cast<const uint4 *>(tiles + i * TILE + PART + c * 512 + lane * 16);
+        for (int i = 0; i < TILES; ++i)
+          if (!SHARED) w[i] = *reinterpret_cast<const uint4 *>(tiles + i * TILE + PART + c * 512 + lane * 16);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int blk = 2 * c + k;
           float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
           for (int i = 0; i < TILES; ++i) {
-            const uint2 d2 = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8);
-            const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
-            float pd[4] = {s[i][0] * d01.x, s[i][1] * d01.y, s[i][2] * d23.x, s[i][3] * d23.y};
+            float4 d;
+            if (SHARED) {
+              d = *reinterpret_cast<const float4 *>(floats + (i * (Q41 ? 3 : 2) + 1) * PER_TILE + (t * NB + blk) * 4);
+            } else {
+              const uint2 d2 = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8);
+              const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
+              d = make_float4(d01.x, d01.y, d23.x, d23.y);
+            }
+            float pd[4] = {s[i][0] * d.x, s[i][1] * d.y, s[i][2] * d.z, s[i][3] * d.w};
             if (!clean) {   // (0 times what a scale behind the last token, or of a token that the row does not see, may be)
               keep_branch();
 #pragma unroll
@@ -376,9 +455,16 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
             }
             const uint32_t h0 = pack_half(pd[0], pd[1]), h1 = pack_half(pd[2], pd[3]);
             const uint32_t l0 = pack_half_lo(pd[0], pd[1], h0), l1 = pack_half_lo(pd[2], pd[3], h1);
-            const uint32_t x = __byte_perm(w[i].x, w[i].y, k ? 0x7632 : 0x5410), y = __byte_perm(w[i].z, w[i].w, k ? 0x7632 : 0x5410);
-            const uint32_t a0[4] = {codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y)};
-            const uint32_t a1[4] = {codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8)};
+            uint4 va, vb;
+            if (SHARED) {
+              va = ops[((i * NC + c) * 8 + 4 + 2 * k) * 32 + lane];
+              vb = ops[((i * NC + c) * 8 + 5 + 2 * k) * 32 + lane];
+            } else {
+              const uint32_t x = __byte_perm(w[i].x, w[i].y, k ? 0x7632 : 0x5410), y = __byte_perm(w[i].z, w[i].w, k ? 0x7632 : 0x5410);
+              va = make_uint4(codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y));
+              vb = make_uint4(codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8));
+            }
+            const uint32_t a0[4] = {va.x, va.y, va.z, va.w}, a1[4] = {vb.x, vb.y, vb.z, vb.w};
             mma_16816(acc[0], a0, h0, h1);
             mma_16816(acc[0], a0, l0, l1);
             mma_16816(acc[1], a1, h0, h1);
@@ -394,6 +480,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
     // the stage has been read by all the share's warps
     if (row_warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + share), "r"(32 * row_warps) : "memory");
     else __syncwarp();
+    if (SHARED && threadIdx.x == 0) largest_scale[stage] = 0;   // (two barriers before it is used again)
     if (sub == 0 && base + 2 * step < t1) {
       issue(base + 2 * step, id_next, stage);
       id_next = page_at(base + 3 * step);
@@ -487,12 +574,12 @@ constexpr float K1_MAGIC_F = 12582912.0f;
 
 // the same from a first sum of K1_MAGIC, which stays in registers of its own
 __device__ __forceinline__ void mma_16832_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int first) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(first));
 }
 __device__ __forceinline__ void mma_16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -943,7 +1030,8 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
     p->warps = p->row_tiles >= 4 ? 4 : p->row_tiles >= 2 ? 2 : 1;
     fill = 148 * 12; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = K4_WARPS / p->warps;
   }
-  int64_t parts = blocks ? (fill + blocks - 1) / blocks : 1;
+  // (blocks of several rows that fill the SMs as they are would only add the join: 5 prompts of up to 333 tokens 116 -> 136 us)
+  int64_t parts = !blocks || (p->tile_rows > 1 && blocks >= 148 * 4) ? 1 : (fill + blocks - 1) / blocks;
   const int64_t most = (groups + 2 * shares - 1) / (2 * shares);   // a part gives each warp two groups at least
   if (parts > most) parts = most;
   if (parts > KJ_PARTS) parts = KJ_PARTS;
@@ -965,10 +1053,13 @@ static int kv4_attention_launch(caten_b200_ctx *ctx, const Kv4AttnArgs &a, int64
     CB_CUDA(ctx, launch_k(ctx, kernel, dim3((unsigned)((units * a.parts + per_block - 1) / per_block)), dim3(K1_WARPS * 32), smem, a));
     CB_LAUNCH_CHECK(ctx, "kv4_attention_row_kernel");
   } else {
-    const int smem = K4_WARPS / a.warps * 2 * K4_TILES(NC) * kv4_tile_bytes(a.s);   // (no less than the sums of all warps where they are joined)
+    const bool shared = a.warps == K4_WARPS;
+    // (no less than the sums of all warps where they are joined)
+    const int smem = K4_WARPS / a.warps * 2 * K4_TILES(NC) * kv4_tile_bytes(a.s) + (shared ? K4_TILES(NC) * NC * (8 * 512 + (Q41 ? 3 : 2) * 32 * 4) : 0);
+    void (*kernel)(const Kv4AttnArgs) = shared ? kv4_attention_kernel<NC, Q41, true> : kv4_attention_kernel<NC, Q41, false>;
     const int64_t blocks = units / a.row_tiles * ((a.row_tiles + a.warps - 1) / a.warps) * a.parts;
-    if (smem > 48 << 10) CB_CUDA(ctx, cudaFuncSetAttribute(kv4_attention_kernel<NC, Q41>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    CB_CUDA(ctx, launch_k(ctx, kv4_attention_kernel<NC, Q41>, dim3((unsigned)blocks), dim3(K4_WARPS * 32), smem, a));
+    if (smem > 48 << 10) CB_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    CB_CUDA(ctx, launch_k(ctx, kernel, dim3((unsigned)blocks), dim3(K4_WARPS * 32), smem, a));
     CB_LAUNCH_CHECK(ctx, "kv4_attention_kernel");
   }
   if (a.parts == 1) return 0;
