@@ -18,7 +18,7 @@
 
 namespace cb {
 
-constexpr int K4_WARPS = 4;        // of a block
+__host__ __device__ constexpr int k4_warps(bool shared) { return shared ? 8 : 4; }   // of a block
 constexpr int K4_GROUP = 64;       // tokens at a time with single rows
 __host__ __device__ constexpr int K4_TILES(int chunks) { return chunks == 1 ? 4 : 2; }   // 16 tokens at a time with several
 constexpr int K4_ROWS = 8;
@@ -100,23 +100,25 @@ __device__ __forceinline__ float to_top(float x, int k = 14) {
   return __uint_as_float((uint32_t)min(max(127 + k - (e - 127), 30), 240) << 23);
 }
 
-// A block's four warps are `row_warps` row tiles times 4 / row_warps shares of the tokens.  The warps of a share work on one ring of two stages of 64
+// A block's warps (four, eight where they make operands) are `row_warps` row tiles times shares of the tokens.  The warps of a share work on one ring of two stages of 64
 // or 32 tokens, which bulk copies fill while the other is read (each stage is read by all its warps before it is filled again).
 // With four row tiles (SHARED) the warps first turn a stage's codes into operands and its scales into floats, a quarter each, in shared memory: of the
 // instructions of 16 tokens and a block of 32 dims, a hundred, that is nearly half, and each warp would do it for itself (5 prompts of 167 to 333
 // tokens, 16 heads over 4 of 128: 130 us).
 template <int NC, bool Q41, bool SHARED>
-__global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) kv4_attention_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 : 1) : NC == 1 ? 4 : NC == 2 ? 3 : 2) kv4_attention_kernel(const Kv4AttnArgs a) {
   constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, TILES = K4_TILES(NC), GROUP = 16 * TILES, STAGE = TILES * TILE;
-  __shared__ float sm[K4_WARPS][K4_ROWS], sl[K4_WARPS][K4_ROWS];
-  __shared__ uint64_t bars[K4_WARPS][2];
-  __shared__ int gave_up[K4_WARPS];
-  __shared__ unsigned present[K4_WARPS][2];          // of a share: tiles of each stage
-  __shared__ unsigned largest_scale[2];              // SHARED: of a stage's values
-  extern __shared__ __align__(128) uint8_t ring[];   // two stages a share (SHARED: then the operands); behind the last group, the warps' sums
+  constexpr int WARPS = k4_warps(SHARED), PER_TILE = 16 * NB;   // (floats of a kind of a tile)
+  constexpr int OPS = TILES * NC * 8 * 512, FLOATS = TILES * (Q41 ? 3 : 2) * PER_TILE * 4, SHARE = 2 * STAGE + (SHARED ? OPS + FLOATS : 0);   // bytes
+  __shared__ float sm[WARPS][K4_ROWS], sl[WARPS][K4_ROWS];
+  __shared__ uint64_t bars[WARPS][2];
+  __shared__ int gave_up[WARPS];
+  __shared__ unsigned present[WARPS][2];          // of a share: tiles of each stage
+  __shared__ unsigned largest_scale[WARPS][2];       // SHARED: of a stage's values
+  extern __shared__ __align__(128) uint8_t ring[];   // two stages a share (SHARED: then its operands); behind the last group, the warps' sums
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = warp_index(), g = lane >> 2, t = lane & 3;
-  const int row_warps = a.warps, shares = K4_WARPS / row_warps, share = warp / row_warps, sub = warp % row_warps;
+  const int row_warps = a.warps, shares = WARPS / row_warps, share = warp / row_warps, sub = warp % row_warps;
   int64_t u = blockIdx.x;
   const int part = (int)(u % a.parts); u /= a.parts;
   const int row_groups = (a.row_tiles + row_warps - 1) / row_warps;
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
   const bool mine = rt * K4_ROWS < count;
 
   const uint32_t bar = smem_u32(&bars[share][0]);
-  uint8_t *const stages = ring + share * 2 * STAGE;
+  uint8_t *const stages = ring + share * SHARE;
   const int *table = a.table + (int64_t)b * a.max_pages;
   const int64_t page_bytes = kv4_page_bytes(a.s);
   const int tile_shift = a.s.page == 16 ? 0 : a.s.page == 32 ? 1 : a.s.page == 64 ? 2 : 3;   // tiles of a page, log2
@@ -211,6 +213,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
   }
 
   float run_max = -INFINITY, run_sum = 0.0f;   // of row g (run_sum: this lane's tokens)
+  float run_down = 1.0f;                       // what outputs (and Q4_1's sums) are to be multiplied with
   float off[4] = {0.f, 0.f, 0.f, 0.f};         // Q4_1: sums of p m_b (rows b of a product of their own) and p d_b (rows NB + b) for rows 2t, 2t + 1
   float o[NB][2][4];                           // rows 2t, 2t + 1; dims 4g + {0, 1} and 4g + {2, 3} of a block
 #pragma unroll
@@ -219,10 +222,9 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
     for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] = 0.0f;
   }
   // SHARED: operands of a stage [tile][chunk][K: block, token half | V: block, dims][lane], then scales of K, of V and minima of K as floats
-  uint4 *const ops = reinterpret_cast<uint4 *>(ring + 2 * STAGE);
-  float *const floats = reinterpret_cast<float *>(ops + TILES * NC * 8 * 32);
-  constexpr int PER_TILE = 16 * NB;   // floats of a kind
-  if (SHARED && threadIdx.x < 2) largest_scale[threadIdx.x] = 0;
+  uint4 *const ops = reinterpret_cast<uint4 *>(stages + 2 * STAGE);
+  float *const floats = reinterpret_cast<float *>(stages + 2 * STAGE + OPS);
+  if (SHARED && sub == 0 && lane < 2) largest_scale[share][lane] = 0;
   __syncthreads();   // the barriers are there
   int stage = 0;
   uint32_t phase = 0;
@@ -240,26 +242,27 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
       const uint8_t *tiles = stages + stage * STAGE;
       const unsigned there = present[share][stage];
 #pragma unroll
-      for (int unit0 = 0; unit0 < TILES * NC * 2; unit0 += K4_WARPS) {
+      for (int unit0 = 0; unit0 < TILES * NC * 2; unit0 += 4) {
         const int unit = unit0 + sub, i = unit / (2 * NC), c = unit % NC;
         const bool of_k = unit / NC % 2 == 0;
         const uint4 w = *reinterpret_cast<const uint4 *>(tiles + i * TILE + (of_k ? 0 : PART) + c * 512 + lane * 16);
         uint4 *dst = ops + ((i * NC + c) * 8 + (of_k ? 0 : 4)) * 32 + lane;
-        // K: tokens 0..7 and 8..15 of the even and the odd block; V: the halves of the even and of the odd block (tokens 2t, 2t + 1 | 2t + 8, 2t + 9)
-        const uint32_t x[4] = {of_k ? w.x : __byte_perm(w.x, w.y, 0x5410), of_k ? w.z : __byte_perm(w.z, w.w, 0x5410), of_k ? w.y : __byte_perm(w.x, w.y, 0x7632),
-                               of_k ? w.w : __byte_perm(w.z, w.w, 0x7632)};
+        if (of_k) {   // tokens 0..7 and 8..15 of the even and of the odd block
+          const uint32_t x[4] = {w.x, w.z, w.y, w.w};
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint32_t p = x[2 * n], q = x[2 * n + 1];
-          const uint32_t pl = codes_lo(p), ph = codes_hi(p), pL = codes_lo(p >> 8), pH = codes_hi(p >> 8);
-          const uint32_t ql = codes_lo(q), qh = codes_hi(q), qL = codes_lo(q >> 8), qH = codes_hi(q >> 8);
-          dst[2 * n * 32] = of_k ? make_uint4(pl, ph, pL, pH) : make_uint4(pl, ph, ql, qh);
-          dst[(2 * n + 1) * 32] = of_k ? make_uint4(ql, qh, qL, qH) : make_uint4(pL, pH, qL, qH);
+          for (int n = 0; n < 4; ++n) dst[n * 32] = make_uint4(codes_lo(x[n]), codes_hi(x[n]), codes_lo(x[n] >> 8), codes_hi(x[n] >> 8));
+        } else {      // of the even and of the odd block, tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t x = __byte_perm(w.x, w.y, n ? 0x7632 : 0x5410), y = __byte_perm(w.z, w.w, n ? 0x7632 : 0x5410);
+            dst[2 * n * 32] = make_uint4(codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y));
+            dst[(2 * n + 1) * 32] = make_uint4(codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8));
+          }
         }
       }
       unsigned largest = 0;
       constexpr int KINDS = Q41 ? 3 : 2;
-      for (int j = sub * 32 + lane; j < TILES * KINDS * PER_TILE / 2; j += 32 * K4_WARPS) {
+      for (int j = sub * 32 + lane; j < TILES * KINDS * PER_TILE / 2; j += 128) {
         const int i = j / (KINDS * PER_TILE / 2), rest = j % (KINDS * PER_TILE / 2), kind = rest / (PER_TILE / 2), pair = rest % (PER_TILE / 2);
         uint32_t h = *reinterpret_cast<const uint32_t *>(tiles + i * TILE + (kind == 1 ? PART : 0) + (kind == 2 ? 9 : 8) * D + pair * 4);
         if (kind == 1) {   // what stands behind the last token may be anything
@@ -274,8 +277,8 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
         }
       }
       largest = __reduce_max_sync(0xffffffffu, largest);
-      if (lane == 0 && largest) atomicMax(&largest_scale[stage], largest);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (lane == 0 && largest) atomicMax(&largest_scale[share][stage], largest);
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + share) : "memory");
     }
     if (ok && mine && base < most) {
       const uint8_t *tiles = stages + stage * STAGE;
@@ -370,16 +373,17 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       float largest;
       if (SHARED) {
-        largest = __uint_as_float(largest_scale[stage]);
+        largest = __uint_as_float(largest_scale[share][stage]);
       } else {
         largest = fmaxf(__low2float(big), __high2float(big));
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
       }
-      const float up = to_top(largest), down = 1.0f / up;
+      const float up = to_top(largest);
       const float ref = top == -INFINITY ? 0.0f : top;
-      const float corr = exp2_fast(run_max - ref);   // (-inf: 0)
+      const float corr = exp2_fast(run_max - ref), lifted = corr * (up * run_down);   // (-inf: 0); the outputs so far are times the last group's power of two
       run_max = top;
+      run_down = 1.0f / up;
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < TILES; ++i)
@@ -390,10 +394,10 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
           s[i][e] *= up;
         }
       run_sum = fmaf(run_sum, corr, sum);
-      const float corr0 = __shfl_sync(0xffffffffu, corr, 8 * t), corr1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
+      const float lifted0 = __shfl_sync(0xffffffffu, lifted, 8 * t), lifted1 = __shfl_sync(0xffffffffu, lifted, 8 * t + 4);
       if (Q41) {
         // sum of p (m + 8 d), which the middle of the codes leaves: minima and scales lie in the cache as the product's first operand has them
-        const float lift = down * 0x1p14f;   // p at the top of fp16's range
+        const float lift = run_down * 0x1p14f, unlift = up * 0x1p-14f;   // p at the top of fp16's range
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
@@ -423,7 +427,7 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
           mma_16816(acc, av, l0, l1);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) off[e] = fmaf(off[e], e & 1 ? corr1 : corr0, acc[e] * 0x1p-14f);
+        for (int e = 0; e < 4; ++e) off[e] = fmaf(off[e], e & 1 ? lifted1 : lifted0, acc[e] * unlift);
       }
       // values
 #pragma unroll
@@ -473,14 +477,14 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[blk][n][e] = fmaf(o[blk][n][e], e & 1 ? corr1 : corr0, acc[n][e] * down);
+            for (int e = 0; e < 4; ++e) o[blk][n][e] = fmaf(o[blk][n][e], e & 1 ? lifted1 : lifted0, acc[n][e]);
         }
       }
     }
     // the stage has been read by all the share's warps
     if (row_warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + share), "r"(32 * row_warps) : "memory");
     else __syncwarp();
-    if (SHARED && threadIdx.x == 0) largest_scale[stage] = 0;   // (two barriers before it is used again)
+    if (SHARED && sub == 0 && lane == 0) largest_scale[share][stage] = 0;   // (two barriers before it is used again)
     if (sub == 0 && base + 2 * step < t1) {
       issue(base + 2 * step, id_next, stage);
       id_next = page_at(base + 3 * step);
@@ -500,9 +504,13 @@ __global__ void __launch_bounds__(K4_WARPS * 32, NC == 1 ? 4 : NC == 2 ? 3 : 2) 
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float pm = __shfl_sync(0xffffffffu, off[k / 8 * 2 + j], k % 8 * 4 + t), pd = __shfl_sync(0xffffffffu, off[(NB + k) / 8 * 2 + j], (NB + k) % 8 * 4 + t);
-        const float add = fmaf(8.0f, pd, pm);
+        const float add = fmaf(8.0f, pd, pm);   // (still times 1 / run_down, as o is)
         o[k][0][j] += add; o[k][0][2 + j] += add; o[k][1][j] += add; o[k][1][2 + j] += add;
       }
+#pragma unroll
+  for (int k = 0; k < NB; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] *= run_down;
   float *so = reinterpret_cast<float *>(ring) + warp * K4_ROWS * D;   // [row][D]
   if (shares > 1) {
     __syncthreads();   // no stage is read or filled any more
@@ -1028,7 +1036,7 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
     fill = 148 * 20 / p->warps; blocks = p->units; shares = p->warps;
   } else {
     p->warps = p->row_tiles >= 4 ? 4 : p->row_tiles >= 2 ? 2 : 1;
-    fill = 148 * 12; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = K4_WARPS / p->warps;
+    fill = 148 * 12; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = k4_warps(p->warps == 4) / p->warps;
   }
   // (blocks of several rows that fill the SMs as they are would only add the join: 5 prompts of up to 333 tokens 116 -> 136 us)
   int64_t parts = !blocks || (p->tile_rows > 1 && blocks >= 148 * 4) ? 1 : (fill + blocks - 1) / blocks;
@@ -1053,13 +1061,13 @@ static int kv4_attention_launch(caten_b200_ctx *ctx, const Kv4AttnArgs &a, int64
     CB_CUDA(ctx, launch_k(ctx, kernel, dim3((unsigned)((units * a.parts + per_block - 1) / per_block)), dim3(K1_WARPS * 32), smem, a));
     CB_LAUNCH_CHECK(ctx, "kv4_attention_row_kernel");
   } else {
-    const bool shared = a.warps == K4_WARPS;
+    const bool shared = a.warps == 4;
     // (no less than the sums of all warps where they are joined)
-    const int smem = K4_WARPS / a.warps * 2 * K4_TILES(NC) * kv4_tile_bytes(a.s) + (shared ? K4_TILES(NC) * NC * (8 * 512 + (Q41 ? 3 : 2) * 32 * 4) : 0);
+    const int smem = k4_warps(shared) / a.warps * K4_TILES(NC) * (2 * kv4_tile_bytes(a.s) + (shared ? NC * (8 * 512 + (Q41 ? 3 : 2) * 32 * 4) : 0));
     void (*kernel)(const Kv4AttnArgs) = shared ? kv4_attention_kernel<NC, Q41, true> : kv4_attention_kernel<NC, Q41, false>;
     const int64_t blocks = units / a.row_tiles * ((a.row_tiles + a.warps - 1) / a.warps) * a.parts;
     if (smem > 48 << 10) CB_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    CB_CUDA(ctx, launch_k(ctx, kernel, dim3((unsigned)blocks), dim3(K4_WARPS * 32), smem, a));
+    CB_CUDA(ctx, launch_k(ctx, kernel, dim3((unsigned)blocks), dim3(k4_warps(shared) * 32), smem, a));
     CB_LAUNCH_CHECK(ctx, "kv4_attention_kernel");
   }
   if (a.parts == 1) return 0;
