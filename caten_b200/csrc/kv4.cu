@@ -80,6 +80,17 @@ __global__ void __launch_bounds__(THREADS) kv_pages_kernel(PagesArgs a, int own_
     return;
   }
   const int top = (int)(n_free + total[2]);
+  // work(i, the request that item i is of), items 0 .. count of n requests of which at[] are the first ones': a warp has items side by side, so that it
+  // looks for a request once and walks on from there
+  auto for_items = [&](const int *at, int n, int count, auto work) {
+    const int each = (count + THREADS - 1) / THREADS * 32, end = min(count, (warp + 1) * each);
+    int i = warp * each + lane;
+    if (i >= end) return;
+    for (int q = last_not_above(at, n, i); i < end; i += 32) {
+      while (q + 1 < n && at[q + 1] <= i) ++q;
+      work(i, q);
+    }
+  };
   // THREADS requests at a time.  Two rounds, because a page that one request gives back may be the one that another takes: the first appends the
   // pages given back to the free ones, in the order of requests and of their pages; the second takes from the end.
   for (int round = total[2] ? 0 : 1; round < 2; ++round) {
@@ -123,24 +134,22 @@ __global__ void __launch_bounds__(THREADS) kv_pages_kernel(PagesArgs a, int own_
       had[tid] = have;
       __syncthreads();
       if (round == 0) {
-        for (int i = tid; i < sum[0]; i += THREADS) {
-          const int q = last_not_above(at_give, n, i);
+        for_items(at_give, n, sum[0], [&](int i, int q) {
           int *cell = a.table + (long long)(base + q) * a.max_pages + first_page[q] + i - at_give[q];
           a.free[n_free + carry[0] + i] = *cell;
           *cell = -1;
-        }
+        });
       } else {
         if (r < a.requests) a.starts[r] = carry[2] + v[2];
-        for (int i = tid; i < sum[1]; i += THREADS) {
-          const int q = last_not_above(at_take, n, i);
+        for_items(at_take, n, sum[1], [&](int i, int q) {
           a.table[(long long)(base + q) * a.max_pages + first_page[q] + i - at_take[q]] = a.free[top - 1 - carry[1] - i];
-        }
-        for (int i = tid; own_slots && i < sum[2]; i += THREADS) {
-          const int q = last_not_above(at_token, n, i);
-          const int pos = had[q] + i - at_token[q], nth = (unsigned)pos / (unsigned)a.page;
-          const int id = nth < first_page[q] ? a.table[(long long)(base + q) * a.max_pages + nth] : a.free[top - 1 - carry[1] - at_take[q] - (nth - first_page[q])];
-          a.slots[carry[2] + i] = id >= 0 && id < a.capacity ? id * a.page + pos - nth * a.page : -1;
-        }
+        });
+        if (own_slots)
+          for_items(at_token, n, sum[2], [&](int i, int q) {
+            const int pos = had[q] + i - at_token[q], nth = (unsigned)pos / (unsigned)a.page;
+            const int id = nth < first_page[q] ? a.table[(long long)(base + q) * a.max_pages + nth] : a.free[top - 1 - carry[1] - at_take[q] - (nth - first_page[q])];
+            a.slots[carry[2] + i] = id >= 0 && id < a.capacity ? id * a.page + pos - nth * a.page : -1;
+          });
       }
 #pragma unroll
       for (int k = 0; k < 3; ++k) carry[k] += sum[k];
