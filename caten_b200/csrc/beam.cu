@@ -521,7 +521,7 @@ int caten_b200_beam_reorder(caten_b200_ctx *ctx, void *const *h_states, int64_t 
   if (!ctx) return fail(nullptr, CATEN_B200_EINVAL, "beam_reorder: ctx is NULL");
   cudaSetDevice(ctx->device);
   ctx->work_outside = true;
-  if (!groups || !nbytes || beams == 1) return 0;
+  if (!groups || !nbytes) return 0;
   ProfScope prof(ctx, CATEN_B200_K_PREP);
   for (int64_t first = 0; first < count; first += RO_STATES) {
     ReorderArgs a;
@@ -547,7 +547,7 @@ int caten_b200_beam_reorder_pages(caten_b200_ctx *ctx, void *d_pool, int64_t pag
   if (!ctx) return fail(nullptr, CATEN_B200_EINVAL, "beam_reorder_pages: ctx is NULL");
   cudaSetDevice(ctx->device);
   ctx->work_outside = true;
-  if (!groups || beams == 1) return 0;
+  if (!groups) return 0;
   ProfScope prof(ctx, CATEN_B200_K_PREP);
   const PagesReorderArgs a = {(uint8_t *)d_pool, d_table, d_lengths, d_parents, ctx->d_status, page_nbytes / 16, pages, (int)max_pages, (int)page, (int)beams};
   const dim3 grid((unsigned)((a.page_words + 255) / 256), (unsigned)max_pages, (unsigned)groups);

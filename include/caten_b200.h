@@ -581,7 +581,7 @@ enum {
   CATEN_B200_K_ATTN_DECODE = 4, CATEN_B200_K_ATTN_PREFILL = 5, CATEN_B200_K_ARGMAX = 6,
   CATEN_B200_K_DECODE_STEP = 7,   /* the whole single-token step of 1..4 sequences over Q4_0 / Q8_0 layers (with this class the step's kernels are not timed by themselves) */
   CATEN_B200_K_WKV = 8,           /* recurrence of a time-mixing or retention layer */
-  CATEN_B200_K_PREP = 9,          /* rotation, q/k norm and cache append; token-shift mixes; expert routing */
+  CATEN_B200_K_PREP = 9,          /* rotation, q/k norm and cache append; token-shift mixes; expert routing; page plans, rows of 4-bit caches, reordering */
   CATEN_B200_K_EXPERTS = 10,      /* linears of a mixture of experts */
   CATEN_B200_K_COUNT = 11
 };

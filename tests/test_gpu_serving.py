@@ -543,6 +543,11 @@ def test_parents_out_of_range_leave_rows_and_are_reported(rt):
             rt.sync()
         assert e.value.code == L.EDEVICE
         np.testing.assert_array_equal(b.numpy(), x[[1, 1, 0, 2]])
+    b = put(rt, x)
+    rt.beam_reorder([b], put(rt, [[0], [1], [0], [0]], np.int32), 3)   # one beam has one parent
+    with pytest.raises(B200Error):
+        rt.sync()
+    np.testing.assert_array_equal(b.numpy(), x)
 
 
 @pytest.mark.parametrize("groups,beams,page,width,longest", [(1, 2, 16, 16, 5), (3, 4, 16, 4624, 100), (2, 8, 64, 48, 300), (1, 32, 32, 160, 64), (2, 13, 16, 32, 40)])
