@@ -529,9 +529,11 @@ int caten_b200_beam_reorder(caten_b200_ctx *ctx, void *const *h_states, int64_t 
     for (int64_t i = 0; i < n; ++i) a.state[i] = h_states[first + i];
     a.parents = d_parents; a.status = ctx->d_status;
     a.planes = planes; a.stride = plane_stride / width; a.words = words; a.beams = (int)beams;
-    const dim3 grid((unsigned)((planes * words + 255) / 256), (unsigned)groups, (unsigned)n);
+    // (a group of one only has its parents checked)
+    const dim3 grid(beams == 1 ? 1u : (unsigned)((planes * words + 255) / 256), (unsigned)groups, beams == 1 ? 1u : (unsigned)n);
     CB_CUDA(ctx, width == 16 ? reorder_launch<uint4>(ctx, grid, a) : reorder_launch<uint32_t>(ctx, grid, a));
     CB_LAUNCH_CHECK(ctx, "beam_reorder_kernel");
+    if (beams == 1) break;
   }
   return 0;
 }
@@ -550,7 +552,7 @@ int caten_b200_beam_reorder_pages(caten_b200_ctx *ctx, void *d_pool, int64_t pag
   if (!groups) return 0;
   ProfScope prof(ctx, CATEN_B200_K_PREP);
   const PagesReorderArgs a = {(uint8_t *)d_pool, d_table, d_lengths, d_parents, ctx->d_status, page_nbytes / 16, pages, (int)max_pages, (int)page, (int)beams};
-  const dim3 grid((unsigned)((a.page_words + 255) / 256), (unsigned)max_pages, (unsigned)groups);
+  const dim3 grid(beams == 1 ? 1u : (unsigned)((a.page_words + 255) / 256), beams == 1 ? 1u : (unsigned)max_pages, (unsigned)groups);
   void (*kernel)(PagesReorderArgs) = beams <= 4 ? beam_reorder_pages_kernel<4> : beams <= 8 ? beam_reorder_pages_kernel<8> : beams <= 16 ? beam_reorder_pages_kernel<16> : beam_reorder_pages_kernel<32>;
   CB_CUDA(ctx, launch_k(ctx, kernel, grid, dim3(256), 0, a));
   CB_LAUNCH_CHECK(ctx, "beam_reorder_pages_kernel");

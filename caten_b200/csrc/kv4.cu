@@ -37,18 +37,20 @@ __global__ void __launch_bounds__(THREADS) kv_pages_kernel(PagesArgs a, int own_
   __shared__ int warps[3][32];
   __shared__ long long total[3];   // tokens, pages taken, pages given back
   __shared__ int bad;
-  __shared__ int at_give[THREADS], at_take[THREADS], at_token[THREADS], first_page[THREADS], had[THREADS];
+  __shared__ int at_give[THREADS], at_take[THREADS], at_token[THREADS], held_pages[THREADS], wanted_pages[THREADS], had[THREADS];
   pdl_enter();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < 3) total[tid] = 0;
   if (tid == 3) bad = 0;
   const int n_free = a.state[0];
   __syncthreads();
+  int have = 0, want = 0;   // of the last request looked at: with one request a thread, or fewer, read once
   {
     long long t[3] = {0, 0, 0};
     bool wrong = false;
     for (int r = tid; r < a.requests; r += THREADS) {
-      const int have = a.have[r], want = a.want[r];
+      have = a.have[r];
+      want = a.want[r];
       if (have < 0 || want < 0 || pages_of(have, a.page) > a.max_pages || pages_of(want, a.page) > a.max_pages) { wrong = true; continue; }
       const int d = pages_of(want, a.page) - pages_of(have, a.page);
       t[0] += want > have ? want - have : 0;
@@ -82,13 +84,22 @@ __global__ void __launch_bounds__(THREADS) kv_pages_kernel(PagesArgs a, int own_
   const int top = (int)(n_free + total[2]);
   // work(i, the request that item i is of), items 0 .. count of n requests of which at[] are the first ones': a warp has items side by side, so that it
   // looks for a request once and walks on from there
-  auto for_items = [&](const int *at, int n, int count, auto work) {
+  auto for_items = [&](const int *at, int n, int count, auto get, auto put) {
     const int each = (count + THREADS - 1) / THREADS * 32, end = min(count, (warp + 1) * each);
     int i = warp * each + lane;
     if (i >= end) return;
-    for (int q = last_not_above(at, n, i); i < end; i += 32) {
-      while (q + 1 < n && at[q + 1] <= i) ++q;
-      work(i, q);
+    for (int q = last_not_above(at, n, i); i < end; i += 4 * 32) {   // four loads under way
+      int of[4], x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + 32 * e < end) {
+          while (q + 1 < n && at[q + 1] <= i + 32 * e) ++q;
+          of[e] = q;
+          x[e] = get(i + 32 * e, q);
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + 32 * e < end) put(i + 32 * e, of[e], x[e]);
     }
   };
   // THREADS requests at a time.  Two rounds, because a page that one request gives back may be the one that another takes: the first appends the
@@ -97,7 +108,10 @@ __global__ void __launch_bounds__(THREADS) kv_pages_kernel(PagesArgs a, int own_
     int carry[3] = {0, 0, 0};
     for (int base = 0; base < a.requests; base += THREADS) {
       const int r = base + tid, n = min(THREADS, a.requests - base);
-      const int have = r < a.requests ? a.have[r] : 0, want = r < a.requests ? a.want[r] : 0;
+      if (a.requests > THREADS) {
+        have = r < a.requests ? a.have[r] : 0;
+        want = r < a.requests ? a.want[r] : 0;
+      }
       const int held = pages_of(have, a.page), wanted = pages_of(want, a.page);
       int v[3] = {max(0, held - wanted), max(0, wanted - held), max(0, want - have)}, sum[3];
       int inc[3];
@@ -130,26 +144,29 @@ __global__ void __launch_bounds__(THREADS) kv_pages_kernel(PagesArgs a, int own_
       at_give[tid] = v[0];
       at_take[tid] = v[1];
       at_token[tid] = v[2];
-      first_page[tid] = round ? held : wanted;   // the first that is taken (given back)
+      held_pages[tid] = held;
+      wanted_pages[tid] = wanted;
       had[tid] = have;
       __syncthreads();
       if (round == 0) {
-        for_items(at_give, n, sum[0], [&](int i, int q) {
-          int *cell = a.table + (long long)(base + q) * a.max_pages + first_page[q] + i - at_give[q];
-          a.free[n_free + carry[0] + i] = *cell;
-          *cell = -1;
-        });
+        auto cell = [&](int i, int q) { return a.table + (long long)(base + q) * a.max_pages + wanted_pages[q] + i - at_give[q]; };
+        for_items(at_give, n, sum[0], [&](int i, int q) { return *cell(i, q); },
+                  [&](int i, int q, int id) {
+                    a.free[n_free + carry[0] + i] = id;
+                    *cell(i, q) = -1;
+                  });
       } else {
         if (r < a.requests) a.starts[r] = carry[2] + v[2];
-        for_items(at_take, n, sum[1], [&](int i, int q) {
-          a.table[(long long)(base + q) * a.max_pages + first_page[q] + i - at_take[q]] = a.free[top - 1 - carry[1] - i];
-        });
+        for_items(at_take, n, sum[1], [&](int i, int) { return a.free[top - 1 - carry[1] - i]; },
+                  [&](int i, int q, int id) { a.table[(long long)(base + q) * a.max_pages + held_pages[q] + i - at_take[q]] = id; });
         if (own_slots)
-          for_items(at_token, n, sum[2], [&](int i, int q) {
-            const int pos = had[q] + i - at_token[q], nth = (unsigned)pos / (unsigned)a.page;
-            const int id = nth < first_page[q] ? a.table[(long long)(base + q) * a.max_pages + nth] : a.free[top - 1 - carry[1] - at_take[q] - (nth - first_page[q])];
-            a.slots[carry[2] + i] = id >= 0 && id < a.capacity ? id * a.page + pos - nth * a.page : -1;
-          });
+          for_items(at_token, n, sum[2],
+                    [&](int i, int q) {
+                      const int pos = had[q] + i - at_token[q], nth = (unsigned)pos / (unsigned)a.page;
+                      const int id = nth < held_pages[q] ? a.table[(long long)(base + q) * a.max_pages + nth] : a.free[top - 1 - carry[1] - at_take[q] - (nth - held_pages[q])];
+                      return id >= 0 && id < a.capacity ? id * a.page + pos - nth * a.page : -1;
+                    },
+                    [&](int i, int, int slot) { a.slots[carry[2] + i] = slot; });
       }
 #pragma unroll
       for (int k = 0; k < 3; ++k) carry[k] += sum[k];

@@ -1040,7 +1040,10 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
   }
   // (blocks of several rows that fill the SMs as they are would only add the join: 5 prompts of up to 333 tokens 116 -> 136 us)
   int64_t parts = !blocks || (p->tile_rows > 1 && blocks >= 148 * 4) ? 1 : (fill + blocks - 1) / blocks;
-  const int64_t most = (groups + 2 * shares - 1) / (2 * shares);   // a part gives each warp two groups at least
+  // A part gives each warp two groups at least.  Single rows of up to four groups a warp are left whole: two groups less take no longer than the join
+  // and its launch (25 heads x 700 tokens 7.2 us in parts, 5.3 whole; 1000 7.2 and 6.2; 1500 7.4 and 7.9).
+  const bool whole = p->tile_rows == 1 && groups <= 4 * shares;
+  const int64_t most = whole ? 1 : (groups + 2 * shares - 1) / (2 * shares);
   if (parts > most) parts = most;
   if (parts > KJ_PARTS) parts = KJ_PARTS;
   if (parts < 1) parts = 1;
