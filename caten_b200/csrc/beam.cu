@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
   __shared__ float group_top[32], sums[BS_THREADS / 32];
   __shared__ u64 lists[BS_THREADS / 32][32], answer;
   __shared__ u64 found[BS_FEW * VECS * 4];
-  __shared__ int count, threads;
+  __shared__ float kth_top;
+  __shared__ int count;
   pdl_enter();
   const int64_t row = blockIdx.y;
   if (ended && ended[row]) return;   // its one candidate needs no logits
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // chunks start on 16-byte boundaries of memory, wherever the row does
   const int64_t e0 = (int64_t)blockIdx.x * CHUNK - (int64_t)(((uintptr_t)p >> 2) & 3);
+  const int index0 = (int)e0 + tid * 4;
   float v[VECS][4];
   if (e0 >= 0 && e0 + CHUNK <= V) {
 #pragma unroll
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
       }
     }
   }
-  if (tid == 0) { count = 0; threads = 0; }
+  if (tid == 0) count = 0;
   // the largest of each thread, of each eight threads, and of those 32 in order the first and the `keep`-th
   float top = -INFINITY;
 #pragma unroll
@@ -128,11 +130,15 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
   for (int o = 1; o < 8; o <<= 1) gt = fmaxf(gt, __shfl_xor_sync(0xffffffffu, gt, o));
   if (lane % 8 == 0) group_top[tid / 8] = gt;
   __syncthreads();
-  const float sorted = warp_sort_floats(group_top[lane]);
-  const float m = __shfl_sync(0xffffffffu, sorted, 0), least = __shfl_sync(0xffffffffu, sorted, keep - 1);
-  const bool may = top >= least && top > -INFINITY;
-  const unsigned who = __ballot_sync(0xffffffffu, may);
-  if (lane == 0 && who) atomicAdd(&threads, __popc(who));
+  float m = group_top[lane];
+  if (warp == 0) {   // (the others go on; the bound is needed behind the next barrier)
+    const float sorted = warp_sort_floats(m);
+    if (lane == keep - 1) kth_top = sorted;
+    m = __shfl_sync(0xffffffffu, sorted, 0);
+  } else {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  }
   // sum of exponentials; a maximum of -inf (nothing left) makes it 0, a NaN or +inf makes it NaN
   const float base = m == -INFINITY ? 0.0f : m;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -147,6 +153,9 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
   float sum = warp_sum((s[0] + s[1]) + (s[2] + s[3]));
   if (lane == 0) sums[warp] = sum;
   __syncthreads();
+  const float least = kth_top;
+  const bool may = top >= least && top > -INFINITY;
+  const int threads = __syncthreads_count(may);
   // Many threads at the bound: equal logits (a mask's value), or masks that empty whole groups.  Then by keys, which are all different.
   u64 bound = 1;
   bool look = may;
@@ -156,7 +165,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
     for (int i = VECS - 1; i >= 0; --i)
 #pragma unroll
       for (int j = 3; j >= 0; --j)
-        if (v[i][j] == top) best = beam_key(v[i][j], (int)(e0 + (i * BS_THREADS + tid) * 4 + j));   // (the lowest index of equal ones)
+        if (v[i][j] == top) best = beam_key(v[i][j], index0 + i * BS_THREADS * 4 + j);   // (the lowest index of equal ones)
     bound = block_kth_key(best, keep, lists, &answer);
     look = best >= bound;   // (`keep` threads, or fewer than that in all)
   }
@@ -168,7 +177,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (v[i][j] >= floor_value) {
-            const u64 key = beam_key(v[i][j], (int)(e0 + (i * BS_THREADS + tid) * 4 + j));
+            const u64 key = beam_key(v[i][j], index0 + i * BS_THREADS * 4 + j);
             if (key >= bound) found[atomicAdd(&count, 1)] = key;
           }
   }
