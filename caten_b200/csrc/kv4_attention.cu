@@ -33,8 +33,8 @@ struct Kv4AttnArgs {
   Kv4Shape s;
   int heads, group, max_pages, max_new, max_length, batch;
   int row_tiles, parts, part_tokens;
-  int tile_rows;   // 8, or 1: the kernel for single rows
-  int warps;       // single rows: warps that share a unit; otherwise row tiles of a block
+  int tile_rows;   // 1, 4 or 8: which kernel
+  int warps;       // 1 and 4 rows: warps that share a unit; 8: row tiles of a block
   float scale;
 };
 
@@ -86,6 +86,12 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
   return r;
 }
 __device__ __forceinline__ float2 half_pair(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // halves that are infinite or NaN made 0
 __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   return w & (((w & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) | ((w & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u));
@@ -569,6 +575,335 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
   }
 }
 
+// ---- two to four rows -------------------------------------------------------------------------------
+// Key heads shared by two to four query heads, or as many tokens of one: with codes as the first operand (16 tokens) and the rows in the eight
+// columns, halves side by side (column 2 r + h), nothing is empty: half the products of the kernel above, a score in one lane (row t, tokens g and
+// g + 8), half the softmax; in the second product columns 2 r + h again, whose two sums a lane has both.  Each warp has a ring of its own.
+// Bound by instructions (unpacking, two roundings of p d).  4 heads to a key head of 128, Q4_0: 256 sequences of 768 tokens 84 us (the kernel above
+// 111), 64 of 768 25 (45), 3 of 100001 132 (167: 346 MB, 2.6 TB/s); Q4_1 the last in 152 (186); 32 heads over 16 key heads of 256, 8 sequences of
+// 2900 63 (76).
+constexpr int K2_WARPS = 4;   // of a block; 1 or 4 of them share a unit
+constexpr int K2_ROWS = 4;
+
+template <int NC, bool Q41>
+__global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_few_kernel(const Kv4AttnArgs a) {
+  constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, TILES = K4_TILES(NC), GROUP = 16 * TILES, STAGE = TILES * TILE;
+  __shared__ float sm[K2_WARPS][K2_ROWS], sl[K2_WARPS][K2_ROWS];
+  __shared__ uint64_t bars[K2_WARPS][2];
+  __shared__ int gave_up[K2_WARPS];
+  extern __shared__ __align__(128) uint8_t ring[];   // two stages a warp; behind the last group, the warps' sums
+  pdl_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int share = a.warps, first_warp = warp / share * share;
+  int64_t u = (int64_t)blockIdx.x * (K2_WARPS / share) + warp / share;
+  const int part = (int)(u % a.parts); u /= a.parts;
+  const int64_t tile_of = u;
+  const int rt = (int)(u % a.row_tiles); u /= a.row_tiles;
+  const int head = (int)(u % a.s.kv_heads);
+  const int64_t b = u / a.s.kv_heads;
+  Kv4Seq seq = {0, 0, 0};
+  if (b < a.batch) seq = kv4_seq(a, (int)b, lane == 0 && warp == first_warp && part == 0 && rt == 0 && head == 0);
+  const int count = seq.count * a.group, r0 = rt * K2_ROWS;
+  auto sees_of = [&](int row) { return row < count ? max(0, seq.length - seq.count + row / a.group + 1) : 0; };   // tokens before and at its position
+  const int sees = sees_of(r0 + t), sees_col = sees_of(r0 + (g >> 1)), least = sees_of(r0), most = sees_of(min(count, r0 + K2_ROWS) - 1);
+  const int t0 = part * a.part_tokens, t1 = r0 < count ? min(most, t0 + a.part_tokens) : 0;
+  const bool live = r0 < count && (t0 < t1 || part == 0);
+
+  float run_max = -INFINITY, run_sum = 0.0f, run_down = 1.0f;   // of row t (run_sum: this lane's tokens); what outputs are to be multiplied with
+  float off[4] = {0.f, 0.f, 0.f, 0.f};                          // Q4_1: sums of p m_b (rows b of a product of their own) and p d_b (rows NB + b)
+  float o[NB][2][4];                                            // columns 2t, 2t + 1; dims 4g + {0 | 1} and 4g + {2 | 3} of a block
+#pragma unroll
+  for (int k = 0; k < NB; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] = 0.0f;
+
+  const int first = t0 + (warp - first_warp) * GROUP, step = share * GROUP;
+  uint8_t *const mine = ring + warp * 2 * STAGE;
+  if (live && first < t1) {
+    const uint32_t bar = smem_u32(&bars[warp][0]), dst = smem_u32(mine);
+    if (lane == 0) {
+      mbar_init(bar, 1);
+      mbar_init(bar + 8, 1);
+      gave_up[warp] = 0;
+      fence_proxy_async();
+    }
+    __syncwarp();
+    const int *table = a.table + b * a.max_pages;
+    const int64_t page_bytes = kv4_page_bytes(a.s);
+    const int tile_shift = a.s.page == 16 ? 0 : a.s.page == 32 ? 1 : a.s.page == 64 ? 2 : 3;   // tiles of a page, log2
+    auto page_at = [&](int base) { return lane < TILES && base + 16 * lane < t1 ? table[((base >> 4) + lane) >> tile_shift] : -1; };
+    auto issue = [&](int base, int id, int stage) -> unsigned {   // lanes over tiles: what can be followed is copied, the rest counts for nothing
+      const bool wanted = lane < TILES && base + 16 * lane < t1, good = wanted && kv4_page_ok(a.s, id);
+      if (wanted && !good) report_bad_index(a.status, 46, id);
+      const unsigned there = __ballot_sync(0xffffffffu, good);
+      if (lane == 0) mbar_expect_tx(bar + 8 * stage, __popc(there) * TILE);
+      __syncwarp();
+      if (good) bulk_load(dst + stage * STAGE + lane * TILE,
+                          a.pool + id * page_bytes + ((int64_t)(head << tile_shift) + (((base >> 4) + lane) & ((1 << tile_shift) - 1))) * TILE, TILE, bar + 8 * stage);
+      return there;
+    };
+    unsigned there_now = issue(first, page_at(first), 0), there_next = 0;
+    if (first + step < t1) there_next = issue(first + step, page_at(first + step), 1);
+    int id_next = page_at(first + 2 * step);
+
+    // q: this lane's column (row g / 2, half g % 2); dims {0, 4 | 1, 5} and {2, 6 | 3, 7} of the lane's eight in each block
+    uint32_t qb[NB][4];
+    float qsum8[NB];   // Q4_1: 8 sum(q) of a block, row t
+    float factor;
+    {
+      const int r = r0 + (g >> 1);
+      const float *q = a.q + (seq.first + r / a.group) * a.ldq + (int64_t)(head * a.group + r % a.group) * D + 8 * t;
+      float top = 0.0f;
+      if (r < count)
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(q[32 * k + j]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float up = to_top(top);
+      factor = __shfl_sync(0xffffffffu, a.scale * 1.4426950408889634f * (1.0f / up), 8 * t);
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        float y[8], sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float z = r < count ? q[32 * k + j] * up : 0.0f, hi = __half2float(__float2half_rn(z));
+          sum += z;
+          y[j] = g & 1 ? z - hi : hi;
+        }
+        if (Q41) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          qsum8[k] = 8.0f * __shfl_sync(0xffffffffu, sum, 8 * t);
+        }
+        qb[k][0] = pack_half(y[0], y[4]);
+        qb[k][1] = pack_half(y[1], y[5]);
+        qb[k][2] = pack_half(y[2], y[6]);
+        qb[k][3] = pack_half(y[3], y[7]);
+      }
+    }
+    bool ok = true;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int base = first; base < t1; base += step) {
+      ok = mbar_wait(bar + 8 * stage, phase, &gave_up[warp]);
+      if (!ok) break;
+      const uint8_t *tiles = mine + stage * STAGE;
+      const unsigned there = there_now;
+      const bool clean = base + GROUP <= least && there == (1u << TILES) - 1u;   // every row sees every token
+      float s[TILES][2];
+      __half2 big = __float2half2_rn(0.0f);   // the values' largest scale, lanes over blocks
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) {
+        const uint8_t *tile = tiles + i * TILE;
+        float x0 = 0.0f, x1 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const uint4 w = *reinterpret_cast<const uint4 *>(tile + c * 512 + lane * 16);   // tokens g (x, y) and g + 8 (z, w); even and odd block
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int blk = 2 * c + k;
+            const uint32_t x = k ? w.y : w.x, y = k ? w.w : w.z;
+            const uint32_t a0[4] = {codes_lo(x), codes_lo(y), codes_hi(x), codes_hi(y)};
+            const uint32_t a1[4] = {codes_lo(x >> 8), codes_lo(y >> 8), codes_hi(x >> 8), codes_hi(y >> 8)};
+            float p[4] = {Q41 ? qsum8[blk] : 0.0f, 0.f, Q41 ? qsum8[blk] : 0.0f, 0.f};   // (d code + m = d (code - 8 + 8) + m)
+            mma_16816(p, a0, qb[blk][0], qb[blk][1]);
+            mma_16816(p, a1, qb[blk][2], qb[blk][3]);
+            const uint8_t *sc = tile + 8 * D + ((g >> 1) * NB + blk) * 8;
+            const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
+            const float2 d = half_pair(__byte_perm(d2.x, d2.y, g & 1 ? 0x7632 : 0x5410));
+            if (Q41) {
+              const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
+              const float2 m = half_pair(__byte_perm(m2.x, m2.y, g & 1 ? 0x7632 : 0x5410));
+              x0 = fmaf(m.x, 0.125f * qsum8[blk], x0);
+              x1 = fmaf(m.y, 0.125f * qsum8[blk], x1);
+            }
+            x0 = fmaf(d.x, p[0] + p[1], x0);
+            x1 = fmaf(d.y, p[2] + p[3], x1);
+          }
+        }
+        s[i][0] = x0 * factor;
+        s[i][1] = x1 * factor;
+        const uint2 v2 = *reinterpret_cast<const uint2 *>(tile + PART + 8 * D + (t * NB + g % NB) * 8);
+        uint32_t vx = v2.x & 0x7fff7fffu, vy = v2.y & 0x7fff7fffu;
+        if (!clean) {   // what stands behind the last token may be anything
+          keep_branch();
+          const bool in = there >> i & 1;
+          const int at = base + 16 * i + 2 * t;
+          vx &= (in && at < t1 ? 0xffffu : 0u) | (in && at + 1 < t1 ? 0xffff0000u : 0u);
+          vy &= (in && at + 8 < t1 ? 0xffffu : 0u) | (in && at + 9 < t1 ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (base + 16 * i + g + 8 * e >= min(sees, t1) || !in) s[i][e] = -INFINITY;
+        }
+        big = __hmax2(big, __hmax2(*reinterpret_cast<const __half2 *>(&vx), *reinterpret_cast<const __half2 *>(&vy)));
+      }
+      float top = run_max;
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) top = fmaxf(top, fmaxf(s[i][0], s[i][1]));
+#pragma unroll
+      for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+      const float up = to_top(warp_max(fmaxf(__low2float(big), __high2float(big))));
+      const float ref = top == -INFINITY ? 0.0f : top;
+      const float corr = exp2_fast(run_max - ref), lifted = corr * (up * run_down);   // (-inf: 0); outputs so far are times the last group's power of two
+      run_max = top;
+      run_down = 1.0f / up;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[i][e] = exp2_fast(s[i][e] - ref);
+          sum += s[i][e];
+          s[i][e] *= up;
+        }
+      run_sum = fmaf(run_sum, corr, sum);
+      // p of the column's row and tokens 2t, 2t + 1, 2t + 8, 2t + 9
+      float p[TILES][4];
+#pragma unroll
+      for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[i][e] = __shfl_sync(0xffffffffu, s[i][e >> 1], 8 * t + 4 * (e & 1) + (g >> 1));
+      // the upper eleven bits of a number in an even column, what they leave in an odd one
+      auto half_of = [&](float x) {
+        float y = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
+        if (g & 1) y = x - y;
+        return y;
+      };
+      if (Q41) {   // minima and scales themselves as the first operand, as above
+        const float lift = run_down * 0x1p14f, unlift = up * 0x1p-14f;   // p at the top of fp16's range
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+          uint32_t av[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (8 * h < 2 * NB) {
+              const int row = 8 * h + g;
+              if (row < 2 * NB) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (row < NB ? D : 0) + (t * NB + (row < NB ? row : row - NB)) * 8);
+                av[h] = w.x;
+                av[2 + h] = w.y;
+              }
+              if (!clean) {
+                keep_branch();
+                const int at = base + 16 * i + 2 * t;
+                const bool in = there >> i & 1;
+                av[h] = finite_halves(av[h]) & ((in && at < t1 ? 0xffffu : 0u) | (in && at + 1 < t1 ? 0xffff0000u : 0u));
+                av[2 + h] = finite_halves(av[2 + h]) & ((in && at + 8 < t1 ? 0xffffu : 0u) | (in && at + 9 < t1 ? 0xffff0000u : 0u));
+              }
+            }
+          mma_16816(acc, av, pack_half(half_of(p[i][0] * lift), half_of(p[i][1] * lift)), pack_half(half_of(p[i][2] * lift), half_of(p[i][3] * lift)));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) off[e] = fmaf(off[e], lifted, acc[e] * unlift);
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        uint4 w[TILES];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) w[i] = *reinterpret_cast<const uint4 *>(tiles + i * TILE + PART + c * 512 + lane * 16);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int blk = 2 * c + k;
+          float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int i = 0; i < TILES; ++i) {
+            const uint2 d2 = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8);
+            const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
+            float pd[4] = {p[i][0] * d01.x, p[i][1] * d01.y, p[i][2] * d23.x, p[i][3] * d23.y};
+            if (!clean) {   // (0 times what a scale behind the last token, or of a token that the row does not see, may be)
+              keep_branch();
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1) >= min(sees_col, t1) || !(there >> i & 1)) pd[e] = 0.0f;
+            }
+            const uint32_t b0 = pack_half(half_of(pd[0]), half_of(pd[1])), b1 = pack_half(half_of(pd[2]), half_of(pd[3]));
+            const uint32_t x = __byte_perm(w[i].x, w[i].y, k ? 0x7632 : 0x5410), y = __byte_perm(w[i].z, w[i].w, k ? 0x7632 : 0x5410);
+            const uint32_t a0[4] = {codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y)};
+            const uint32_t a1[4] = {codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8)};
+            mma_16816(acc[0], a0, b0, b1);
+            mma_16816(acc[1], a1, b0, b1);
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[blk][n][e] = fmaf(o[blk][n][e], lifted, acc[n][e]);
+        }
+      }
+      __syncwarp();   // the stage has been read
+      there_now = there_next;
+      if (base + 2 * step < t1) {
+        there_next = issue(base + 2 * step, id_next, stage);
+        id_next = page_at(base + 3 * step);
+      }
+      phase ^= stage;
+      stage ^= 1;
+    }
+    if (!ok) {
+      if (lane == 0) {
+        gave_up[warp] = 1;
+        atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
+        a.status[1] = 49;
+      }
+      for (int i = 0; i < 2; ++i) mbar_wait_thread(bar + 8 * (stage ^ i), phase ^ (stage & i), &gave_up[warp]);   // copies land before the block ends
+    }
+  }
+
+  // row t: its sum over the lanes of its tokens; its outputs, halves together: four dims of a block a lane
+#pragma unroll
+  for (int k = 4; k < 32; k <<= 1) run_sum += __shfl_xor_sync(0xffffffffu, run_sum, k);
+  const float off_lo = off[0] + off[1], off_hi = off[2] + off[3];
+  float4 x[NB];
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    float add = 0.0f;
+    if (Q41) {
+      const float pm = __shfl_sync(0xffffffffu, k < 8 ? off_lo : off_hi, k % 8 * 4 + t), pd = __shfl_sync(0xffffffffu, NB + k < 8 ? off_lo : off_hi, (NB + k) % 8 * 4 + t);
+      add = fmaf(8.0f, pd, pm);
+    }
+    x[k] = make_float4((o[k][0][0] + o[k][0][1] + add) * run_down, (o[k][0][2] + o[k][0][3] + add) * run_down, (o[k][1][0] + o[k][1][1] + add) * run_down,
+                       (o[k][1][2] + o[k][1][3] + add) * run_down);
+  }
+  float top = run_max, sum = run_sum;
+  if (share > 1) {
+    float *so = reinterpret_cast<float *>(ring);   // [warp][row][D], each inside the warp's own stages
+    constexpr int STRIDE = 2 * STAGE / (int)sizeof(float);
+    static_assert(STRIDE >= K2_ROWS * D, "the warps' sums fit their rings");
+#pragma unroll
+    for (int k = 0; k < NB; ++k) *reinterpret_cast<float4 *>(so + warp * STRIDE + t * D + 32 * k + 4 * g) = x[k];
+    if (g == 0) { sm[warp][t] = run_max; sl[warp][t] = run_sum; }
+    __syncthreads();
+    if (warp != first_warp) return;
+    for (int w = warp + 1; w < warp + share; ++w) top = fmaxf(top, sm[w][t]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = warp; w < warp + share; ++w) {
+      const float e = exp2_fast(sm[w][t] - ref);
+      sum = fmaf(sl[w][t], e, sum);
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const float4 y = *reinterpret_cast<const float4 *>(so + w * STRIDE + t * D + 32 * k + 4 * g);
+        x[k].x = fmaf(y.x, e, x[k].x); x[k].y = fmaf(y.y, e, x[k].y); x[k].z = fmaf(y.z, e, x[k].z); x[k].w = fmaf(y.w, e, x[k].w);
+      }
+    }
+  }
+  const int rr = r0 + t;
+  if (!live || rr >= count) return;
+  float *dst = a.parts == 1 ? a.out + (seq.first + rr / a.group) * (int64_t)a.heads * D + (int64_t)(head * a.group + rr % a.group) * D
+                            : a.part + ((tile_of * a.parts + part) * K2_ROWS + t) * (D + 2);
+  const float scale = a.parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    float *p = dst + 32 * k + 4 * g;
+    p[0] = x[k].x * scale; p[1] = x[k].y * scale; p[2] = x[k].z * scale; p[3] = x[k].w * scale;
+  }
+  if (a.parts > 1 && g == 0) { dst[D] = top; dst[D + 1] = sum; }
+}
+
 // ---- one row a sequence and key head ---------------------------------------------------------------
 // Whole numbers: codes - 8, sixteen times, are signed bytes (a mask and an exclusive or, where fp16 needs an addition besides), the other operand is
 // a fixed-point number of 31 bits in four signed bytes, each a column of its own: column 4 (block % 2) + j of the first product is digit j of q in that
@@ -602,12 +937,6 @@ __device__ __forceinline__ uint32_t digits_of(float x0, float x1, float x2, floa
   const uint32_t u2 = (uint32_t)__float2int_rn(x2) + 0x80808080u, u3 = (uint32_t)__float2int_rn(x3) + 0x80808080u;
   return __byte_perm(__byte_perm(u0, u1, pick), __byte_perm(u2, u3, pick), 0x5410) ^ 0x80808080u;
 }
-__device__ __forceinline__ float warp_max(float x) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 template <int NC, bool Q41, bool WIDE>   // WIDE: pages hold 64 tokens or more
 __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const Kv4AttnArgs a) {
   constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART;
@@ -1024,7 +1353,7 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
   if (batch < 0 || batch > (1 << 24) || rows < 0 || rows > 0x7fffffff || max_new <= 0 || max_length < 0 || max_length > 0x3fffffff) return fail(ctx, CATEN_B200_EINVAL, "%s: bad shape", who);
   const int64_t group = c->heads / c->kv_heads;
   if (max_new > (1 << 24) || max_new * group > 0x3fffffff) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: %lld new tokens of a sequence", who, (long long)max_new);
-  p->tile_rows = max_new * group == 1 ? 1 : K4_ROWS;
+  p->tile_rows = max_new * group == 1 ? 1 : max_new * group <= K2_ROWS ? K2_ROWS : K4_ROWS;
   p->row_tiles = (int)((max_new * group + p->tile_rows - 1) / p->tile_rows);
   if (batch && (int64_t)c->kv_heads * p->row_tiles > 0x7fffffff / batch) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
   p->units = batch * c->kv_heads * p->row_tiles;
@@ -1034,16 +1363,22 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
     // a warp each where that is enough (20 warps an SM), otherwise four
     p->warps = p->units >= 148 * 16 ? 1 : K1_WARPS;
     fill = 148 * 20 / p->warps; blocks = p->units; shares = p->warps;
+  } else if (p->tile_rows == K2_ROWS) {
+    p->warps = p->units >= 148 * 16 ? 1 : K2_WARPS;
+    fill = 148 * 48 / p->warps; blocks = p->units; shares = p->warps;
   } else {
     p->warps = p->row_tiles >= 4 ? 4 : p->row_tiles >= 2 ? 2 : 1;
     fill = 148 * 12; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = k4_warps(p->warps == 4) / p->warps;
   }
   // (blocks of several rows that fill the SMs as they are would only add the join: 5 prompts of up to 333 tokens 116 -> 136 us)
-  int64_t parts = !blocks || (p->tile_rows > 1 && blocks >= 148 * 4) ? 1 : (fill + blocks - 1) / blocks;
+  int64_t parts = !blocks || (p->tile_rows == K4_ROWS && blocks >= 148 * 4) ? 1 : (fill + blocks - 1) / blocks;
   // A part gives each warp two groups at least.  Single rows of up to four groups a warp are left whole: two groups less take no longer than the join
   // and its launch (25 heads x 700 tokens 7.2 us in parts, 5.3 whole; 1000 7.2 and 6.2; 1500 7.4 and 7.9).
   const bool whole = p->tile_rows == 1 && groups <= 4 * shares;
-  const int64_t most = whole ? 1 : (groups + 2 * shares - 1) / (2 * shares);
+  // Blocks of two to four rows that fill three quarters of their places on the SMs are cut into no less than eight groups a warp (64 sequences of 8
+  // key heads: 700 tokens 35 us in parts, 25 whole; 10000 229 and 248, with uneven lengths 164 and 220).
+  const bool coarse = p->tile_rows == K2_ROWS && blocks >= 148 * 3;
+  const int64_t most = whole ? 1 : coarse ? groups / (8 * shares) : (groups + 2 * shares - 1) / (2 * shares);
   if (parts > most) parts = most;
   if (parts > KJ_PARTS) parts = KJ_PARTS;
   if (parts < 1) parts = 1;
@@ -1063,6 +1398,12 @@ static int kv4_attention_launch(caten_b200_ctx *ctx, const Kv4AttnArgs &a, int64
     if (smem > 48 << 10) CB_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     CB_CUDA(ctx, launch_k(ctx, kernel, dim3((unsigned)((units * a.parts + per_block - 1) / per_block)), dim3(K1_WARPS * 32), smem, a));
     CB_LAUNCH_CHECK(ctx, "kv4_attention_row_kernel");
+  } else if (a.tile_rows == K2_ROWS) {
+    const int64_t per_block = K2_WARPS / a.warps;
+    const int smem = K2_WARPS * 2 * K4_TILES(NC) * kv4_tile_bytes(a.s);
+    if (smem > 48 << 10) CB_CUDA(ctx, cudaFuncSetAttribute(kv4_attention_few_kernel<NC, Q41>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    CB_CUDA(ctx, launch_k(ctx, kv4_attention_few_kernel<NC, Q41>, dim3((unsigned)((units * a.parts + per_block - 1) / per_block)), dim3(K2_WARPS * 32), smem, a));
+    CB_LAUNCH_CHECK(ctx, "kv4_attention_few_kernel");
   } else {
     const bool shared = a.warps == 4;
     // (no less than the sums of all warps where they are joined)

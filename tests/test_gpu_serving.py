@@ -259,7 +259,8 @@ LENGTHS = [1, 15, 16, 17, 0, 63, 64, 65, 130, 257]
 
 @pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
 @pytest.mark.parametrize("dim,page,heads,kv", [(64, 64, 25, 25), (64, 16, 4, 1), (128, 32, 6, 2), (128, 128, 16, 2), (192, 16, 3, 3), (256, 64, 10, 1),
-                                                (64, 32, 1, 1), (128, 32, 3, 3), (256, 16, 2, 2), (256, 128, 1, 1)])
+                                                (64, 32, 1, 1), (128, 32, 3, 3), (256, 16, 2, 2), (256, 128, 1, 1),
+                                                (64, 16, 6, 3), (128, 64, 8, 2), (192, 32, 4, 1), (256, 32, 3, 1), (128, 16, 12, 4)])
 def test_single_tokens(rt, kind, dim, page, heads, kv):
     rng = rng_of(dim, page, heads)
     c = Cache(rt, rng, kind, dim, page, heads, kv, LENGTHS)
@@ -281,13 +282,24 @@ def test_several_tokens_and_prompts(rt, kind, dim, page, heads, kv):
 
 
 @pytest.mark.parametrize("kind,dim,heads,kv,lengths,news", [("q4_0", 64, 2, 2, [5000], [1]), ("q4_1", 128, 8, 1, [4097, 1], [1, 1]), ("q4_0", 64, 2, 1, [3000, 2, 700], [9, 2, 1]),
-                                                            ("q4_1", 256, 1, 1, [2500], [1]), ("q4_0", 128, 4, 4, [1, 1, 2100], [1, 0, 3])])
+                                                            ("q4_1", 256, 1, 1, [2500], [1]), ("q4_0", 128, 4, 4, [1, 1, 2100], [1, 0, 3]), ("q4_1", 128, 8, 2, [5000, 3, 0, 700], [1, 1, 0, 1]),
+                                                            ("q4_0", 64, 6, 2, [4100], [1]), ("q4_1", 192, 4, 1, [2049], [1]), ("q4_1", 256, 3, 3, [1600, 90], [4, 2])])
 def test_long_histories_are_shared_out(rt, kind, dim, heads, kv, lengths, news):
     rng = rng_of(dim, heads, 3)
     c = Cache(rt, rng, kind, dim, 64, heads, kv, lengths, k_scale=0.5)
     q = rng.standard_normal((sum(news), heads, dim), dtype=np.float32) * 2
     check_attention(rt, c, q, news)
     check_attention(rt, c, q, news, max_length=max(lengths))
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("heads,kv,lengths", [(4, 4, [(i * 7) % 41 for i in range(601)]), (8, 4, [(i * 7) % 41 for i in range(601)]),
+                                              (8, 4, [5] * 57 + [4200] + [130, 1, 64, 0] * 14), (4, 4, [5] * 57 + [4200] + [130, 1, 64, 0] * 14)])
+def test_many_sequences(rt, kind, heads, kv, lengths):
+    rng = rng_of(len(lengths), heads, 4)
+    c = Cache(rt, rng, kind, 64, 16, heads, kv, lengths)
+    q = rng.standard_normal((len(lengths), heads, 64), dtype=np.float32)
+    check_attention(rt, c, q, [1] * len(lengths))
 
 
 def test_results_are_the_same_every_time(rt):
@@ -361,6 +373,42 @@ def test_what_later_tokens_hold_does_not_matter_to_earlier_ones(rt, kind, heads,
                 rt.kv4_store(c.desc, c.pool, *kept, slot)
                 if kind == "q4_0":   # (its own values are stored as they are)
                     np.testing.assert_array_equal(rt.kv4_load(c.desc, c.pool, slot)[0].numpy(), kept[0].numpy())
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("heads,news", [(1, 4), (1, 3), (2, 2)])
+def test_what_later_tokens_hold_does_not_matter_to_few_rows(rt, kind, heads, news):
+    """The same with two to four rows: a token of the last few that is not finite, or a row of q that is not."""
+    rng = rng_of(38, heads, news)
+    c = Cache(rt, rng, kind, 64, 16, heads, 1, [90])
+    q = rng.standard_normal((news, heads, 64), dtype=np.float32)
+    clean = check_attention(rt, c, q, [news])
+
+    def run(x):
+        return rt.kv4_attention(c.desc, put(rt, x.reshape(news, -1)), c.pool, put(rt, c.table, np.int32), put(rt, c.lengths, np.int32), put(rt, [0, news], np.int32),
+                                max_new=news).numpy().reshape(news, heads, 64)
+    for token in range(90 - news, 90):
+        for which in range(2):
+            for value in (np.nan, np.inf):
+                rows = [np.zeros((1, 64), np.float32) for _ in range(2)]
+                rows[which][0, 40] = value
+                slot = put(rt, [c.table[0, token // 16] * 16 + token % 16], np.int32)
+                kept = rt.kv4_load(c.desc, c.pool, slot)
+                rt.kv4_store(c.desc, c.pool, put(rt, rows[0]), put(rt, rows[1]), slot)
+                out, seen = run(q), token - (90 - news)
+                np.testing.assert_array_equal(out[:seen], clean[:seen])
+                assert not np.isfinite(out[seen:, :, 32:]).any()
+                rt.kv4_store(c.desc, c.pool, *kept, slot)
+    bad = q.copy()
+    bad[1, 0, 7], bad[0, heads - 1, 0] = np.nan, np.inf
+    hit = np.zeros((news, heads), bool)
+    hit[1, 0] = hit[0, heads - 1] = True
+    out = run(bad)
+    assert np.isnan(out[hit]).all()
+    if kind == "q4_0":   # (its own values were stored back as they are)
+        np.testing.assert_array_equal(out[~hit], clean[~hit])
+    else:
+        assert np.isfinite(out[~hit]).all()
 
 
 def test_what_the_device_says_is_checked(rt):
