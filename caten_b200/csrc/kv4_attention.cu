@@ -1360,11 +1360,13 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
   const int64_t groups = (max_length + K4_GROUP - 1) / K4_GROUP;
   int64_t fill, blocks, shares;   // units of work that fill the SMs; units without parts; warps over whom a unit's tokens are dealt
   if (p->tile_rows == 1) {
-    // a warp each where that is enough (20 warps an SM), otherwise four
-    p->warps = p->units >= 148 * 16 ? 1 : K1_WARPS;
+    // A warp each where that is enough (20 warps an SM), and for up to four groups already with four an SM: a second and third warp would have one group
+    // or none (592 of 128 dims: 200 tokens 8.4 us and 10.1, 400 15.4 and 13.5; 2000: 100 tokens 12.2 and 22).  Otherwise four.
+    p->warps = p->units >= 148 * 16 || (groups <= 4 && p->units >= 148 * 4) ? 1 : K1_WARPS;
     fill = 148 * 20 / p->warps; blocks = p->units; shares = p->warps;
   } else if (p->tile_rows == K2_ROWS) {
-    p->warps = p->units >= 148 * 16 ? 1 : K2_WARPS;
+    // (likewise, with a stage half as long: 1184, 200 tokens 19 us and 24; 592, 200 tokens 15.5 and 13)
+    p->warps = p->units >= 148 * 16 || (groups <= 4 && p->units >= 148 * 8) ? 1 : K2_WARPS;
     fill = 148 * 48 / p->warps; blocks = p->units; shares = p->warps;
   } else {
     p->warps = p->row_tiles >= 4 ? 4 : p->row_tiles >= 2 ? 2 : 1;
