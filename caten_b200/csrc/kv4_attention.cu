@@ -12,6 +12,8 @@
 // A warp has 8 rows (tokens x the heads that share a key head) and takes 64 tokens at a time: running maximum and sum of the softmax per row, the
 // group's p d scaled by a power of two for each block, so that the largest is near the top of fp16 whatever the cache's scales are, and joined
 // to the running sums in fp32.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kv4.cuh"
 #include "tcgen05.cuh"
@@ -33,7 +35,7 @@ struct Kv4AttnArgs {
   Kv4Shape s;
   int heads, group, max_pages, max_new, max_length, batch;
   int row_tiles, parts, part_tokens;
-  int tile_rows;   // 1, 4 or 8: which kernel
+  int tile_rows;   // 1, 4, 8 or 128: which kernel
   int warps;       // 1 and 4 rows: warps that share a unit; 8: row tiles of a block
   float scale;
 };
@@ -904,6 +906,508 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
   if (a.parts > 1 && g == 0) { dst[D] = top; dst[D + 1] = sum; }
 }
 
+// ---- prompts ----------------------------------------------------------------------------------------
+// 128 rows of a key head are the lanes of tensor memory, 64 tokens a step; a step's products are tcgen05.mma on fp16 halves, 22 bits of each operand:
+//   S = Q_hi (K_hi | K_lo)^T + Q_lo K_hi^T   (128 columns, whose halves the softmax adds)        O = P_hi V_hi + P_lo V_hi + P_hi V_lo
+// Scales are multiplied in before (d (code - 8) has 15 bits, so for Q4_0 two halves hold it exactly): a token's keys times a power of two that brings
+// its largest near the top of fp16, a step's values times one for all.  S, P and O lie in tensor memory; a row's two threads (warps w and w + 4) take
+// half of the tokens and half of the dims each, and keep the running output in registers, so that a moved maximum costs nothing more.  By warp:
+//   0 .. 7     rows of q; softmax of a step, its P, and the output of the step before
+//   8 .. 14    codes into operands, two steps ahead at most (two stages each); the last asks for the tiles of the step after
+//   15         issues the products: S a step ahead of the softmax
+constexpr int K3_ROWS = 128, K3_THREADS = 512, K3_SOFTMAX = 8, K3_CONVERT = 7;   // (warps)
+constexpr float K3_LIFT = 14.0f;   // p is taken times 2^14, its sum with it
+__host__ __device__ constexpr int k3_smem(int chunks, int tile_bytes) { return chunks * (32768 + 2 * 16384 + 2 * 16384) + 2 * 4 * tile_bytes + 1024; }
+// of an operand tile: rows of 64 halves, 128-byte swizzle
+__device__ __forceinline__ uint32_t k3_at(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+// (code - 8) d + n for two codes, as the upper and the lower half
+template <bool Q41>
+__device__ __forceinline__ void k3_split(uint32_t codes, uint32_t dd, float2 d, float2 n, uint32_t *hi, uint32_t *lo) {
+  if (Q41) {
+    const float2 c = half_pair(codes);
+    const float x = fmaf(c.x, d.x, n.x), y = fmaf(c.y, d.y, n.y);
+    *hi = pack_half(x, y);
+    *lo = pack_half_lo(x, y, *hi);
+  } else {   // exact
+    const __half2 c = *reinterpret_cast<const __half2 *>(&codes), x = *reinterpret_cast<const __half2 *>(&dd), h = __hmul2_rn(c, x), l = __hfma2(c, x, __hneg2(h));
+    *hi = *reinterpret_cast<const uint32_t *>(&h);
+    *lo = *reinterpret_cast<const uint32_t *>(&l);
+  }
+}
+
+template <int NC, bool Q41>
+__global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(const Kv4AttnArgs a) {
+  constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, HALF = D / 2;
+  constexpr uint32_t COL_P = 256, COL_O = 384, COLS = 512;   // (two blocks of scores, two of P)
+  constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(K3_ROWS >> 4) << 24);   // fp32 sums, fp16 by fp16, 128 rows
+  extern __shared__ unsigned char k3_raw[];
+  __shared__ float red[2][2][K3_ROWS];      // [step & 1][half][row]
+  __shared__ float qfactor[K3_ROWS];
+  // of four steps each, so that nobody need wait for their readers: a token's keys are to be multiplied with this
+  __shared__ __align__(16) float kdown[4][64];
+  __shared__ float ups[4];                    // what its values were taken times
+  __shared__ unsigned bad[4][64], any_bad[4][2];   // blocks of values that are not finite, by token; whether there are any, by half
+  // of two steps: scales (Q4_0: of keys, in both halves and times the token's power of two; of values, of an even and an odd block) and minima + 8 d
+  __shared__ uint32_t k_scale[2][64][NB], v_scale[2][64][NC];
+  __shared__ float k_off[2][64][Q41 ? NB : 1];
+  __shared__ uint32_t v_min[2][64][Q41 ? NC : 1];
+  __shared__ float largest[2][2];             // of the values, by half of the tokens
+  __shared__ unsigned theres[4];
+  __shared__ unsigned present[2];                    // tiles of each stage
+  __shared__ uint64_t bar_mem[17];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int gave_up[2];                // [1] is never set
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = warp_index(), g = lane >> 2, t = lane & 3, quad = warp & 3, hf = warp >> 2, row = quad * 32 + lane;
+  int64_t u = blockIdx.x;   // later rows see more: they start first
+  const int part = (int)(u % a.parts); u /= a.parts;
+  const int b = (int)(u % a.batch); u /= a.batch;
+  const int head = (int)(u % a.s.kv_heads); u /= a.s.kv_heads;
+  const int rt = a.row_tiles - 1 - (int)u;
+  const Kv4Seq seq = kv4_seq(a, b, tid == 0 && part == 0 && rt == 0 && head == 0);
+  const int count = seq.count * a.group, r0 = rt * K3_ROWS;
+  if (r0 >= count) return;
+  auto sees_of = [&](int r) { return r < count ? max(0, seq.length - seq.count + r / a.group + 1) : 0; };
+  const int least = r0 + K3_ROWS <= count ? sees_of(r0) : 0, reach = sees_of(min(count, r0 + K3_ROWS) - 1);
+  const int t0 = part * a.part_tokens, t1 = min(reach, t0 + a.part_tokens);
+  if (t0 >= t1 && part > 0) return;
+  const int sees = min(sees_of(r0 + row), t1), steps = t1 > t0 ? (t1 - t0 + 63) / 64 : 0;
+
+  unsigned char *const sq = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(k3_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char *const sk = sq + NC * 32768, *const sv = sk + 2 * NC * 16384, *const raw = sv + 2 * NC * 16384;
+  const uint32_t bars = smem_u32(bar_mem), q_full = bars + 112, p_full = bars + 120, o_full = bars + 128;
+  auto raw_full = [&](int k) { return bars + 8u * k; };
+  auto k_full = [&](int k) { return bars + 16u + 8u * k; };
+  auto k_empty = [&](int k) { return bars + 32u + 8u * k; };
+  auto v_full = [&](int k) { return bars + 48u + 8u * k; };
+  auto v_empty = [&](int k) { return bars + 64u + 8u * k; };
+  auto s_full = [&](int k) { return bars + 80u + 8u * k; };
+  auto s_empty = [&](int k) { return bars + 96u + 8u * k; };
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(raw_full(i), 1);
+      mbar_init(k_full(i), K3_CONVERT);
+      mbar_init(k_empty(i), 1);
+      mbar_init(v_full(i), K3_CONVERT);
+      mbar_init(v_empty(i), 1);
+      mbar_init(s_full(i), 2);   // the products, and the issuing warp for what the converters left beside K
+      mbar_init(s_empty(i), K3_SOFTMAX);
+    }
+    mbar_init(q_full, K3_SOFTMAX);
+    mbar_init(p_full, K3_SOFTMAX);
+    mbar_init(o_full, 2);
+    gave_up[0] = gave_up[1] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();   // not before this block has its tensor memory: the next kernel's blocks may ask for theirs and then wait for this grid
+  const uint32_t tmem = tmem_slot, tlane = tmem + ((uint32_t)(quad * 32) << 16);
+
+  const int *table = a.table + (int64_t)b * a.max_pages;
+  const int64_t page_bytes = kv4_page_bytes(a.s);
+  const int tile_shift = a.s.page == 16 ? 0 : a.s.page == 32 ? 1 : a.s.page == 64 ? 2 : 3;   // tiles of a page, log2
+  auto page_at = [&](int step) {
+    const int at = t0 + 64 * step + 16 * lane;
+    return lane < 4 && at < t1 ? table[(at >> 4) >> tile_shift] : -1;
+  };
+  auto issue = [&](int step, int id) {   // by one warp: what can be followed is copied, the rest counts for nothing
+    const int at = t0 + 64 * step + 16 * lane, stage = step & 1;
+    const bool wanted = lane < 4 && at < t1, good = wanted && kv4_page_ok(a.s, id);
+    if (wanted && !good) report_bad_index(a.status, 46, id);
+    const unsigned there = __ballot_sync(0xffffffffu, good);
+    if (lane == 0) {
+      present[stage] = there;
+      mbar_expect_tx(raw_full(stage), __popc(there) * TILE);   // (its arrival publishes `present`)
+    }
+    __syncwarp();
+    if (good) bulk_load(smem_u32(raw) + (stage * 4 + lane) * TILE, a.pool + id * page_bytes + ((int64_t)(head << tile_shift) + ((at >> 4) & ((1 << tile_shift) - 1))) * TILE,
+                        TILE, raw_full(stage));
+  };
+  int asked = 0, came = 0;   // stages asked for, stages seen (the warp that asks)
+  bool ok = true;   // of the warp; one whose wait ran out goes on through the barriers that it shares, and touches nothing else
+  auto wait = [&](uint32_t bar, uint32_t phase) {
+    if (ok && !mbar_wait(bar, phase, &gave_up[0])) {
+      ok = false;
+      if (lane == 0) {
+        gave_up[0] = 1;
+        atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
+        a.status[1] = 50;
+      }
+    }
+    return ok;
+  };
+
+  // rows of q, D / 8 lanes each: eight dims in the order (0, 4, 1, 5, 2, 6, 3, 7), as codes come out of a word
+  auto convert_q = [&]() {
+    constexpr int LANES = D / 8, ROWS = 32 / LANES;
+    const int chunk = lane % LANES;
+#pragma unroll 2
+    for (int i = 0; i < 16 / ROWS; ++i) {
+      const int q_row = warp * 16 + i * ROWS + lane / LANES, r = r0 + q_row;
+      float x[8], top = 0.0f;
+      const float *q = a.q + (seq.first + r / a.group) * a.ldq + (int64_t)(head * a.group + r % a.group) * D + 8 * chunk;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = r < count ? q[j] : 0.0f;
+        top = fmaxf(top, fabsf(x[j]));
+      }
+#pragma unroll
+      for (int j = 1; j < LANES; j <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, j));
+      const float up = to_top(top);
+      if (chunk == 0) qfactor[q_row] = a.scale * 1.4426950408889634f * (1.0f / up);
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float y = x[j] * up, z = x[j + 4] * up;
+        hi[j] = pack_half(y, z);
+        lo[j] = pack_half_lo(y, z, hi[j]);
+      }
+      unsigned char *dst = sq + chunk / 8 * 32768 + k3_at(q_row, chunk % 8);
+      *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4 *>(dst + 16384) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    fence_proxy_async();
+  };
+  // a step's scales, a token a thread: warps 0 and 1 those of keys, 2 and 3 of values (what stands behind the last token, or is not finite, is zero)
+  auto scales = [&](int step, int cw) {
+    const int st = step & 1, token = (cw & 1) * 32 + lane, tk = token & 15;
+    const bool in = present[st] >> (token >> 4) & 1 && t0 + 64 * step + token < t1;
+    const unsigned char *tile = raw + (st * 4 + (token >> 4)) * TILE + (cw < 2 ? 0 : PART) + 8 * D;
+    uint32_t d[NB], m[NB];
+#pragma unroll
+    for (int blk = 0; blk < NB; ++blk) {
+      const int at = 2 * kv4_scale_index(tk, blk, D);
+      d[blk] = *reinterpret_cast<const uint16_t *>(tile + at);
+      m[blk] = Q41 ? *reinterpret_cast<const uint16_t *>(tile + D + at) : 0;
+    }
+    float top = 0.0f;
+    if (cw < 2) {
+      float x[NB], y[NB];
+#pragma unroll
+      for (int blk = 0; blk < NB; ++blk) {
+        x[blk] = half_pair(d[blk]).x;
+        y[blk] = Q41 ? fmaf(8.0f, x[blk], half_pair(m[blk]).x) : 0.0f;
+        top = fmaxf(top, fmaf(8.0f, fabsf(x[blk]), fabsf(y[blk])));
+      }
+      const float up = to_top(top);
+      kdown[step & 3][token] = 1.0f / up;
+#pragma unroll
+      for (int blk = 0; blk < NB; ++blk) {
+        k_scale[st][token][blk] = Q41 ? __float_as_uint(x[blk] * up) : pack_half(x[blk] * up, x[blk] * up);
+        if (Q41) k_off[st][token][blk] = y[blk] * up;
+      }
+    } else {
+      unsigned lost = 0;
+#pragma unroll
+      for (int blk = 0; blk < NB; ++blk) {
+        const uint32_t x = in ? finite_halves(d[blk]) : 0u, y = in ? finite_halves(m[blk]) : 0u;
+        if (in && (x != d[blk] || y != m[blk])) lost |= 1u << blk;
+        d[blk] = x;
+        m[blk] = y;
+        top = fmaxf(top, fmaf(Q41 ? 16.0f : 8.0f, fabsf(half_pair(x).x), fabsf(half_pair(y).x)));
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        v_scale[st][token][c] = d[2 * c] | d[2 * c + 1] << 16;
+        if (Q41) v_min[st][token][c] = m[2 * c] | m[2 * c + 1] << 16;
+      }
+      bad[step & 3][token] = lost;
+      top = warp_max(top);
+      const unsigned any = __any_sync(0xffffffffu, lost);
+      if (lane == 0) {
+        largest[st][cw & 1] = top;
+        any_bad[step & 3][cw & 1] = any;
+      }
+    }
+  };
+  // keys of a tile and a block
+  auto convert_k = [&](int st, int unit) {
+    const int i = unit / (2 * NC), c = unit / 2 % NC, k = unit % 2;
+    const uint4 w = *reinterpret_cast<const uint4 *>(raw + (st * 4 + i) * TILE + c * 512 + lane * 16);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {   // tokens g, g + 8
+      const int token = 16 * i + g + 8 * h;
+      const uint32_t x = h ? (k ? w.w : w.z) : (k ? w.y : w.x), dd = k_scale[st][token][2 * c + k], codes[4] = {codes_lo(x), codes_hi(x), codes_lo(x >> 8), codes_hi(x >> 8)};
+      const float d = __uint_as_float(dd), n = Q41 ? k_off[st][token][2 * c + k] : 0.0f;
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) k3_split<Q41>(codes[e], dd, make_float2(d, d), make_float2(n, n), &hi[e], &lo[e]);
+      unsigned char *dst = sk + (st * NC + c) * 16384 + k3_at(token, 4 * k + t);
+      *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4 *>(dst + 8192) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+  };
+  // values of a tile, 64 dims and half of the tokens
+  auto convert_v = [&](int st, int unit, float up) {
+    const int i = unit / (2 * NC), c = unit / 2 % NC, h = unit % 2;   // tokens 2t + 8 h, 2t + 8 h + 1
+    const uint2 w = *reinterpret_cast<const uint2 *>(raw + (st * 4 + i) * TILE + PART + c * 512 + lane * 16 + 8 * h);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {   // (even, odd block) in the halves of each operation
+      const int token = 16 * i + 2 * t + 8 * h + j;
+      const uint32_t x = j ? w.y : w.x, codes[4] = {codes_lo(x), codes_hi(x), codes_lo(x >> 8), codes_hi(x >> 8)};
+      float2 d = half_pair(v_scale[st][token][c]), n = make_float2(0.f, 0.f);
+      if (Q41) {
+        n = half_pair(v_min[st][token][c]);
+        n.x = fmaf(8.0f, d.x, n.x) * up; n.y = fmaf(8.0f, d.y, n.y) * up;
+      }
+      d.x *= up; d.y *= up;
+      const uint32_t dd = pack_half(d.x, d.y);
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) k3_split<Q41>(codes[e], dd, d, n, &hi[e], &lo[e]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t how = k ? 0x7632 : 0x5410;
+        unsigned char *dst = sv + (st * NC + c) * 16384 + k3_at(token, 4 * k + (g >> 1)) + (g & 1) * 8;
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(__byte_perm(hi[0], hi[1], how), __byte_perm(hi[2], hi[3], how));
+        *reinterpret_cast<uint2 *>(dst + 8192) = make_uint2(__byte_perm(lo[0], lo[1], how), __byte_perm(lo[2], lo[3], how));
+      }
+    }
+  };
+
+  float o[HALF], run_max = -INFINITY, run_ref = -INFINITY, run_sum = 0.0f, run_down = 1.0f, lifted = 0.0f;   // (run_sum: this thread's tokens)
+#pragma unroll
+  for (int e = 0; e < HALF; ++e) o[e] = 0.0f;
+  auto take_outputs = [&](int step, float lift) {
+#pragma unroll
+    for (int e0 = 0; e0 < HALF; e0 += 16) {
+      uint32_t x[16];
+      tmem_ld16(tlane + COL_O + HALF * hf + e0, x);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e0 + e] = fmaf(o[e0 + e], lift, __uint_as_float(x[e]));
+    }
+    if (any_bad[step & 3][0] | any_bad[step & 3][1])
+      for (int k = 0; k < 64; ++k) {
+        const unsigned blocks = bad[step & 3][k];
+        if (blocks && t0 + 64 * step + k < sees)
+#pragma unroll
+          for (int kk = 0; kk < NC; ++kk)
+            if (blocks >> (hf * NC + kk) & 1)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[32 * kk + e] = __int_as_float(0x7fffffff);
+      }
+  };
+
+  if (warp >= K3_SOFTMAX && warp < K3_SOFTMAX + K3_CONVERT) {
+    // ---------------- operands ----------------
+    const int cw = warp - K3_SOFTMAX;
+    int id_next = -1;
+    if (cw == K3_CONVERT - 1) {
+      for (; asked < min(steps, 2); ++asked) issue(asked, page_at(asked));
+      id_next = page_at(2);
+    }
+    for (int step = 0; step < steps; ++step) {
+      const int st = step & 1;
+      const uint32_t phase = (uint32_t)(step >> 1) & 1u;
+      if (wait(raw_full(st), phase)) {
+        ++came;
+        if (cw < 4) scales(step, cw);
+      }
+      asm volatile("bar.sync 5, %0;" ::"n"(32 * K3_CONVERT) : "memory");   // also: the step before has been read
+      const float up = to_top(fmaxf(largest[st][0], largest[st][1]));
+      if (cw == K3_CONVERT - 1 && ok) {
+        if (step > 0 && asked < steps) {
+          issue(asked, id_next);
+          ++asked;
+          id_next = page_at(asked);
+        }
+        if (lane == 0) { ups[step & 3] = up; theres[step & 3] = present[st]; }
+      }
+      // units of K, then of V, dealt as one row (32 of heads of 128)
+      int unit = cw;
+      if (wait(k_empty(st), phase ^ 1u)) {
+#pragma unroll 1
+        for (; unit < 8 * NC; unit += K3_CONVERT) convert_k(st, unit);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(k_full(st));
+      }
+      if (wait(v_empty(st), phase ^ 1u)) {
+#pragma unroll 1
+        for (; unit < 16 * NC; unit += K3_CONVERT) convert_v(st, unit - 8 * NC, up);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_full(st));
+      }
+    }
+    if (!ok && cw == K3_CONVERT - 1)   // copies land before the block ends
+      for (int k = came; k < asked; ++k) mbar_wait_thread(raw_full(k & 1), (uint32_t)(k >> 1) & 1u, &gave_up[1]);
+  } else if (warp == K3_SOFTMAX + K3_CONVERT) {
+    // ---------------- products (uniform control flow, one elected lane issues) ----------------
+    const uint64_t dq = umma_desc(smem_u32(sq)), dk0 = umma_desc(smem_u32(sk));
+    // V has the dims contiguous: blocks of 64 dims 16 KB apart (the leading offset), 16 tokens 2 KB
+    const uint64_t dv0 = umma_desc(smem_u32(sv)) - (1ull << 16) + ((uint64_t)(16384 >> 4) << 16);
+    auto scores = [&](int step) {
+      const int st = step & 1;
+      const uint32_t phase = (uint32_t)(step >> 1) & 1u;
+      if (!wait(k_full(st), phase) || !wait(s_empty(st), phase ^ 1u)) return;
+      tc_fence_after();
+      const uint32_t el = elect_one(), acc = tmem + 128 * st;
+      const uint64_t dk = dk0 + (uint64_t)(st * NC * 1024);
+#pragma unroll
+      for (int k = 0; k < 4 * NC; ++k) {   // 16 halves are two descriptor units of 16 bytes
+        const uint64_t aq = dq + (uint64_t)((k >> 2) * 2048 + 2 * (k & 3)), ak = dk + (uint64_t)((k >> 2) * 1024 + 2 * (k & 3));
+        umma_bf16(acc, aq, ak, IDESC | (128u >> 3 << 17), k > 0 ? 1u : 0u, el);   // (fp16: the kind's types are IDESC's)
+        umma_bf16(acc, aq + 1024, ak, IDESC | (64u >> 3 << 17), 1u, el);
+      }
+      umma_commit(k_empty(st), el);
+      umma_commit(s_full(st), el);
+      if (el) mbar_arrive(s_full(st));
+      __syncwarp();
+    };
+    if (steps && wait(q_full, 0)) scores(0);
+    for (int step = 0; step < steps && ok; ++step) {
+      if (step + 1 < steps) scores(step + 1);
+      const int st = step & 1;
+      if (!wait(v_full(st), (uint32_t)(step >> 1) & 1u) || !wait(p_full, (uint32_t)step & 1u)) break;
+      tc_fence_after();
+      const int groups = (t1 - t0 - 64 * step + 15) / 16;
+      const uint32_t el = elect_one(), idesc = IDESC | (1u << 16) | ((uint32_t)(D >> 3) << 17);
+      const uint64_t dv = dv0 + (uint64_t)(st * NC * 1024);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (k >= groups) break;
+        const uint32_t p = tmem + COL_P + 64 * st + 8 * k;
+        umma_bf16_ts(tmem + COL_O, p, dv + 128 * k, idesc, k > 0 ? 1u : 0u, el);
+        umma_bf16_ts(tmem + COL_O, p + 32, dv + 128 * k, idesc, 1u, el);
+        umma_bf16_ts(tmem + COL_O, p, dv + 512 + 128 * k, idesc, 1u, el);
+      }
+      umma_commit(v_empty(st), el);
+      umma_commit(o_full, el);
+      if (el) mbar_arrive(o_full);
+      __syncwarp();
+    }
+  } else {
+    // ---------------- softmax ----------------
+    convert_q();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full);
+    asm volatile("bar.sync 6, 256;" ::: "memory");   // rows' factors
+    const float factor = qfactor[row];
+    for (int step = 0; step < steps; ++step) {
+      const int base = t0 + 64 * step, st = step & 1;
+      float x[32], top = run_max;
+      if (wait(s_full(st), (uint32_t)(step >> 1) & 1u)) {
+        tc_fence_after();
+        const unsigned there = theres[step & 3];
+#pragma unroll
+        for (int e0 = 0; e0 < 32; e0 += 8) {
+          uint32_t p[8], q[8];
+          tmem_ld8(tlane + 128 * st + 32 * hf + e0, p);
+          tmem_ld8(tlane + 128 * st + 64 + 32 * hf + e0, q);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            const float4 down = *reinterpret_cast<const float4 *>(kdown[step & 3] + 32 * hf + e0 + e);
+            x[e0 + e] = (__uint_as_float(p[e]) + __uint_as_float(q[e])) * factor * down.x;
+            x[e0 + e + 1] = (__uint_as_float(p[e + 1]) + __uint_as_float(q[e + 1])) * factor * down.y;
+            x[e0 + e + 2] = (__uint_as_float(p[e + 2]) + __uint_as_float(q[e + 2])) * factor * down.z;
+            x[e0 + e + 3] = (__uint_as_float(p[e + 3]) + __uint_as_float(q[e + 3])) * factor * down.w;
+          }
+        }
+        const bool hidden = base + 64 > least || base + 64 > t1 || there != 15u;   // some row does not see some token
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_empty(st));
+        if (hidden) {
+          keep_branch();
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (base + 32 * hf + e >= sees || !(there >> (2 * hf + e / 16) & 1)) x[e] = -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
+        red[st][hf][row] = top;
+      }
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");   // warps quad and quad + 4
+      if (!ok) continue;
+      top = fmaxf(red[st][0][row], red[st][1][row]);
+      const float ref = top == -INFINITY ? 0.0f : top - K3_LIFT;
+      const float corr = exp2_fast(run_ref - ref), up = ups[step & 3];
+      run_max = top;
+      run_ref = top == -INFINITY ? top : ref;
+      float sum = 0.0f;
+      // (this block of P was read two steps ago, whose outputs have been taken)
+#pragma unroll
+      for (int e0 = 0; e0 < 16; e0 += 8) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = exp2_fast(x[2 * (e0 + e)] - ref), z = exp2_fast(x[2 * (e0 + e) + 1] - ref);
+          sum += y + z;
+          hi[e] = pack_half(y, z);
+          lo[e] = pack_half_lo(y, z, hi[e]);
+        }
+        tmem_st8(tlane + COL_P + 64 * st + 16 * hf + e0, hi);   // token k in half k % 2 of column k / 2
+        tmem_st8(tlane + COL_P + 64 * st + 32 + 16 * hf + e0, lo);
+      }
+      run_sum = fmaf(run_sum, corr, sum);
+      if (step > 0) {
+        if (!wait(o_full, (uint32_t)(step - 1) & 1u)) continue;
+        tc_fence_after();
+        take_outputs(step - 1, lifted);
+      }
+      lifted = corr * (up * run_down);
+      run_down = 1.0f / up;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+    }
+    if (steps && wait(o_full, (uint32_t)(steps - 1) & 1u)) {
+      tc_fence_after();
+      take_outputs(steps - 1, lifted);
+    }
+  }
+  tc_fence_before();
+  const bool failed = __syncthreads_or(!ok);
+
+  // rows go out by way of shared memory (all products have been read): 32 dims of 128 rows are 16 KB
+  const bool rows_warp = warp < K3_SOFTMAX;
+  if (rows_warp) red[0][hf][row] = run_sum;
+  unsigned char *const so = sq;
+  if (!failed && rows_warp)
+#pragma unroll
+    for (int e = 0; e < HALF; e += 4)
+      *reinterpret_cast<float4 *>(so + (hf * NC + e / 32) * 16384 + k3_at(row, e % 32 / 4)) =
+          make_float4(o[e] * run_down, o[e + 1] * run_down, o[e + 2] * run_down, o[e + 3] * run_down);
+  __syncthreads();
+  if (warp < 4) {
+    const float sum = red[0][0][row] + red[0][1][row];
+    red[1][0][row] = a.parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (a.parts > 1 && !failed && r0 + row < count) {
+      float *dst = a.part + (((((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt) * a.parts + part) * K3_ROWS + row) * (D + 2) + D;
+      dst[0] = run_ref;   // (what outputs and sum are relative to)
+      dst[1] = sum;
+    }
+  }
+  __syncthreads();
+  if (!failed && rows_warp)
+    for (int i = 0; i < 16; ++i) {
+      const int out_row = warp * 16 + i, rr = r0 + out_row;
+      if (rr >= count) break;
+      const float scale = red[1][0][out_row];
+      float *dst = a.parts == 1 ? a.out + (seq.first + rr / a.group) * (int64_t)a.heads * D + (int64_t)(head * a.group + rr % a.group) * D
+                                : a.part + (((((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt) * a.parts + part) * K3_ROWS + out_row) * (D + 2);
+#pragma unroll
+      for (int k = 0; k < NB; ++k) dst[32 * k + lane] = *reinterpret_cast<const float *>(so + k * 16384 + k3_at(out_row, lane >> 2) + (lane & 3) * 4) * scale;
+    }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS) : "memory");
+  }
+}
+
 // ---- one row a sequence and key head ---------------------------------------------------------------
 // Whole numbers: codes - 8, sixteen times, are signed bytes (a mask and an exclusive or, where fp16 needs an addition besides), the other operand is
 // a fixed-point number of 31 bits in four signed bytes, each a column of its own: column 4 (block % 2) + j of the first product is digit j of q in that
@@ -1347,13 +1851,19 @@ struct Kv4Plan {
   int64_t units;   // row tiles of all sequences and key heads
   int tile_rows, row_tiles, parts, part_tokens, warps;
 };
+// Whether rows are enough for tiles of 128: half of one a sequence and key head on the average, and 1e8 products, below which the wider kernel's start
+// costs more than it saves (us in tiles of 8 rows and of 128: 64 tokens of 1 head of 64 dims 6.9 and 11.8; 64 over 500 of 25 such heads 17.8 and 19.6; 16
+// over 500 of 8 sequences, 16 heads of 128 over 4 29.8 and 25.4; 2000 of 25 heads of 64 201 and 117).
+static bool kv4_prompts(const caten_b200_kv4_desc *c, int64_t batch, int64_t rows, int64_t max_length) {
+  return c->dim <= 128 && rows * (c->heads / c->kv_heads) >= 64 * batch && (double)rows * c->heads * (double)max_length * c->dim >= 1e8;
+}
 static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_desc *c, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length, Kv4Plan *p) {
   Kv4Shape s;
   if (int rc = kv4_check(ctx, who, c, &s)) return rc;
   if (batch < 0 || batch > (1 << 24) || rows < 0 || rows > 0x7fffffff || max_new <= 0 || max_length < 0 || max_length > 0x3fffffff) return fail(ctx, CATEN_B200_EINVAL, "%s: bad shape", who);
   const int64_t group = c->heads / c->kv_heads;
   if (max_new > (1 << 24) || max_new * group > 0x3fffffff) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: %lld new tokens of a sequence", who, (long long)max_new);
-  p->tile_rows = max_new * group == 1 ? 1 : max_new * group <= K2_ROWS ? K2_ROWS : K4_ROWS;
+  p->tile_rows = max_new * group == 1 ? 1 : max_new * group <= K2_ROWS ? K2_ROWS : kv4_prompts(c, batch, rows, max_length) ? K3_ROWS : K4_ROWS;
   p->row_tiles = (int)((max_new * group + p->tile_rows - 1) / p->tile_rows);
   if (batch && (int64_t)c->kv_heads * p->row_tiles > 0x7fffffff / batch) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
   p->units = batch * c->kv_heads * p->row_tiles;
@@ -1368,6 +1878,9 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
     // (likewise, with a stage half as long: 1184, 200 tokens 19 us and 24; 592, 200 tokens 15.5 and 13)
     p->warps = p->units >= 148 * 16 || (groups <= 4 && p->units >= 148 * 8) ? 1 : K2_WARPS;
     fill = 148 * 48 / p->warps; blocks = p->units; shares = p->warps;
+  } else if (p->tile_rows == K3_ROWS) {
+    p->warps = 1;
+    fill = 148; blocks = p->units; shares = 1;
   } else {
     p->warps = p->row_tiles >= 4 ? 4 : p->row_tiles >= 2 ? 2 : 1;
     fill = 148 * 12; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = k4_warps(p->warps == 4) / p->warps;
@@ -1387,7 +1900,7 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
   const int64_t each = groups ? (groups + parts - 1) / parts : 1;
   p->part_tokens = (int)(each * K4_GROUP);
   p->parts = (int)(groups ? (groups + each - 1) / each : 1);
-  if (p->units * p->parts > 0x7fffffff / K4_ROWS) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
+  if (p->units * p->parts > 0x7fffffff / std::max(K4_ROWS, p->tile_rows)) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
   return 0;
 }
 
@@ -1406,6 +1919,13 @@ static int kv4_attention_launch(caten_b200_ctx *ctx, const Kv4AttnArgs &a, int64
     if (smem > 48 << 10) CB_CUDA(ctx, cudaFuncSetAttribute(kv4_attention_few_kernel<NC, Q41>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     CB_CUDA(ctx, launch_k(ctx, kv4_attention_few_kernel<NC, Q41>, dim3((unsigned)((units * a.parts + per_block - 1) / per_block)), dim3(K2_WARPS * 32), smem, a));
     CB_LAUNCH_CHECK(ctx, "kv4_attention_few_kernel");
+  } else if (a.tile_rows == K3_ROWS) {
+    if constexpr (NC <= 2) {
+      const int smem = k3_smem(NC, kv4_tile_bytes(a.s));
+      CB_CUDA(ctx, cudaFuncSetAttribute(kv4_attention_prompt_kernel<NC, Q41>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      CB_CUDA(ctx, launch_k(ctx, kv4_attention_prompt_kernel<NC, Q41>, dim3((unsigned)(units * a.parts)), dim3(K3_THREADS), smem, a));
+      CB_LAUNCH_CHECK(ctx, "kv4_attention_prompt_kernel");
+    }
   } else {
     const bool shared = a.warps == 4;
     // (no less than the sums of all warps where they are joined)

@@ -302,6 +302,62 @@ def test_many_sequences(rt, kind, heads, kv, lengths):
     check_attention(rt, c, q, [1] * len(lengths))
 
 
+def columns_for(rows, heads, dim, page):
+    """Spare columns of a table with which the call may be large enough (rows x heads x tokens x dims) for the kernel for prompts."""
+    return int(1.1e8 / (rows * heads * dim * page)) + 1
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("dim,page,heads,kv,lengths,news", [
+    (64, 16, 50, 50, [130, 257, 300], [130, 257, 40]), (128, 64, 80, 40, [150, 5, 260], [150, 5, 100]), (64, 16, 1, 1, [64], [64]), (128, 64, 2, 1, [65], [33]), (64, 64, 3, 3, [128, 129, 0, 200, 257], [128, 129, 0, 50, 257]), (128, 128, 8, 2, [300, 64, 1], [300, 64, 1]),
+    (128, 32, 4, 1, [1000, 20], [40, 60]), (64, 128, 2, 1, [2500], [70]), (128, 16, 2, 2, [2113], [129]), (64, 32, 9, 3, [191, 50, 63], [65, 50, 63])])
+def test_long_prompts(rt, kind, dim, page, heads, kv, lengths, news):
+    """Many rows a sequence: whole and ragged tiles of rows, histories shared out, sequences without tokens or with fewer tokens than rows; scales far apart."""
+    rng = rng_of(dim, page, heads, 5)
+    c = Cache(rt, rng, kind, dim, page, heads, kv, lengths, spare=columns_for(sum(news), heads, dim, page))
+    q = rng.standard_normal((sum(news) + 2, heads, dim), dtype=np.float32)
+    q[::3] *= 1e-3
+    one = check_attention(rt, c, q, news, rows_behind=2, extra_cols=3)
+    np.testing.assert_array_equal(check_attention(rt, c, q, news, rows_behind=2, extra_cols=3), one)
+    check_attention(rt, c, q, news, rows_behind=2, max_length=max(lengths))
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("k_scale,q_scale", [(1e-3, 1e3), (300.0, 1e-3), (30.0, 1.0), (1.0, 1e-30), (1.0, 0.0)])
+def test_prompts_with_scales_far_from_one(rt, kind, k_scale, q_scale):
+    rng = rng_of(39)
+    c = Cache(rt, rng, kind, 128, 64, 2, 1, [200], k_scale=k_scale, spare=columns_for(150, 2, 128, 64))
+    check_attention(rt, c, rng.standard_normal((150, 2, 128), dtype=np.float32) * np.float32(q_scale), [150])
+
+
+def test_a_prompt_whose_pages_or_lengths_are_wrong(rt):
+    """Reported by the next synchronising call; other sequences are answered as before."""
+    rng = rng_of(40)
+    c = Cache(rt, rng, "q4_0", 64, 16, 2, 1, [150, 150, 150], spare=columns_for(240, 2, 64, 16))
+    q = rng.standard_normal((240, 2, 64), dtype=np.float32)
+    clean = check_attention(rt, c, q, [80, 80, 80])
+
+    def run(table=c.table, lengths=c.lengths, starts=(0, 80, 160, 240)):
+        out = rt.kv4_attention(c.desc, put(rt, q.reshape(240, -1)), c.pool, put(rt, table, np.int32), put(rt, lengths, np.int32), put(rt, starts, np.int32), max_new=80)
+        with pytest.raises(B200Error) as e:
+            rt.sync()
+        assert e.value.code == L.EDEVICE
+        return out.numpy().reshape(240, 2, 64)
+    for wrong in (-1, c.desc.pages, 2**31 - 1, -2**31):
+        t = c.table.copy()
+        t[1, 4] = wrong
+        got = run(table=t)
+        np.testing.assert_array_equal(got[:80], clean[:80])
+        np.testing.assert_array_equal(got[160:], clean[160:])
+    for wrong in (-1, 2**31 - 1):
+        got = run(lengths=[150, wrong, 150])
+        np.testing.assert_array_equal(got[:80], clean[:80])
+        np.testing.assert_array_equal(got[160:], clean[160:])
+    got = run(starts=(0, 80, 1000, 240))
+    np.testing.assert_array_equal(got[:80], clean[:80])
+    rt.sync()
+
+
 def test_results_are_the_same_every_time(rt):
     rng = rng_of(21)
     c = Cache(rt, rng, "q4_0", 64, 64, 4, 2, [3000, 65, 900])
@@ -376,18 +432,18 @@ def test_what_later_tokens_hold_does_not_matter_to_earlier_ones(rt, kind, heads,
 
 
 @pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
-@pytest.mark.parametrize("heads,news", [(1, 4), (1, 3), (2, 2)])
+@pytest.mark.parametrize("heads,news", [(1, 4), (1, 3), (2, 2), (24, 4), (32, 2), (8, 40)])
 def test_what_later_tokens_hold_does_not_matter_to_few_rows(rt, kind, heads, news):
-    """The same with two to four rows: a token of the last few that is not finite, or a row of q that is not."""
+    """The same with two to four rows, and with many: a token of the last few that is not finite, or a row of q that is not."""
     rng = rng_of(38, heads, news)
-    c = Cache(rt, rng, kind, 64, 16, heads, 1, [90])
+    c = Cache(rt, rng, kind, 64, 16, heads, 1, [90], spare=columns_for(news, heads, 64, 16))
     q = rng.standard_normal((news, heads, 64), dtype=np.float32)
     clean = check_attention(rt, c, q, [news])
 
     def run(x):
         return rt.kv4_attention(c.desc, put(rt, x.reshape(news, -1)), c.pool, put(rt, c.table, np.int32), put(rt, c.lengths, np.int32), put(rt, [0, news], np.int32),
                                 max_new=news).numpy().reshape(news, heads, 64)
-    for token in range(90 - news, 90):
+    for token in {90 - news, 90 - news + 1, 90 - news // 2, 89}:
         for which in range(2):
             for value in (np.nan, np.inf):
                 rows = [np.zeros((1, 64), np.float32) for _ in range(2)]
