@@ -908,9 +908,9 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
 
 // ---- prompts ----------------------------------------------------------------------------------------
 // 128 rows of a key head are the lanes of tensor memory, 64 tokens a step; a step's products are tcgen05.mma on fp16 halves, 22 bits of each operand:
-//   S = Q_hi (K_hi | K_lo)^T + Q_lo K_hi^T   (128 columns, whose halves the softmax adds)        O = P_hi V_hi + P_lo V_hi + P_hi V_lo
-// Scales are multiplied in before (d (code - 8) has 15 bits, so for Q4_0 two halves hold it exactly): a token's keys times a power of two that brings
-// its largest near the top of fp16, a step's values times one for all.  S, P and O lie in tensor memory; a row's two threads (warps w and w + 4) take
+//   S = Q_hi K_hi^T + Q_hi K_lo^T + Q_lo K_hi^T        O = P_hi V_hi + P_lo V_hi + P_hi V_lo
+// Scales are multiplied in before (d (code - 8) has 15 bits, so for Q4_0 two halves hold it exactly): a step's keys and its
+// values times a power of two each that brings the largest near the top of fp16.  S, P and O lie in tensor memory; a row's two threads (warps w and w + 4) take
 // half of the tokens and half of the dims each, and keep the running output in registers, so that a moved maximum costs nothing more.  By warp:
 //   0 .. 7     rows of q; softmax of a step, its P, and the output of the step before
 //   8 .. 14    codes into operands, two steps ahead at most (two stages each); the last asks for the tiles of the step after
@@ -938,20 +938,19 @@ __device__ __forceinline__ void k3_split(uint32_t codes, uint32_t dd, float2 d, 
 template <int NC, bool Q41>
 __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(const Kv4AttnArgs a) {
   constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, HALF = D / 2;
-  constexpr uint32_t COL_P = 256, COL_O = 384, COLS = 512;   // (two blocks of scores, two of P)
+  constexpr uint32_t COL_P = 128, COL_O = 256, COLS = 512;   // (two blocks of scores, two of P)
   constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(K3_ROWS >> 4) << 24);   // fp32 sums, fp16 by fp16, 128 rows
   extern __shared__ unsigned char k3_raw[];
   __shared__ float red[2][2][K3_ROWS];      // [step & 1][half][row]
   __shared__ float qfactor[K3_ROWS];
-  // of four steps each, so that nobody need wait for their readers: a token's keys are to be multiplied with this
-  __shared__ __align__(16) float kdown[4][64];
-  __shared__ float ups[4];                    // what its values were taken times
+  __shared__ int64_t q_at[K3_ROWS], out_at[K3_ROWS];   // where rows begin (divided once)
+  // of four steps each, so that nobody need wait for their readers
+  __shared__ float downs[4], ups[4];          // what scores are to be multiplied with; what values were taken times
   __shared__ unsigned bad[4][64], any_bad[4][2];   // blocks of values that are not finite, by token; whether there are any, by half
-  // of two steps: scales (Q4_0: of keys, in both halves and times the token's power of two; of values, of an even and an odd block) and minima + 8 d
-  __shared__ uint32_t k_scale[2][64][NB], v_scale[2][64][NC];
-  __shared__ float k_off[2][64][Q41 ? NB : 1];
-  __shared__ uint32_t v_min[2][64][Q41 ? NC : 1];
-  __shared__ float largest[2][2];             // of the values, by half of the tokens
+  // of two steps: scales (of values, of an even and an odd block), minima (of keys, + 8 d)
+  __shared__ float k_scale[2][64][NB], k_off[2][64][Q41 ? NB : 1];
+  __shared__ uint32_t v_scale[2][64][NC], v_min[2][64][Q41 ? NC : 1];
+  __shared__ float largest[2][4];             // of keys and of values, by half of the tokens
   __shared__ unsigned theres[4];
   __shared__ unsigned present[2];                    // tiles of each stage
   __shared__ uint64_t bar_mem[17];
@@ -999,6 +998,13 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
     gave_up[0] = gave_up[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
+  }
+  if (tid >= 128 && tid < 128 + K3_ROWS) {
+    const int k = tid - 128, r = min(r0 + k, count - 1), token = r / a.group;
+    const int64_t column = (int64_t)(head * a.group + r % a.group) * D;
+    q_at[k] = (seq.first + token) * a.ldq + column;
+    out_at[k] = a.parts == 1 ? (seq.first + token) * (int64_t)a.heads * D + column
+                             : (((((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt) * a.parts + part) * K3_ROWS + k) * (D + 2);
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(COLS) : "memory");
@@ -1048,30 +1054,45 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
   auto convert_q = [&]() {
     constexpr int LANES = D / 8, ROWS = 32 / LANES;
     const int chunk = lane % LANES;
-#pragma unroll 2
-    for (int i = 0; i < 16 / ROWS; ++i) {
-      const int q_row = warp * 16 + i * ROWS + lane / LANES, r = r0 + q_row;
-      float x[8], top = 0.0f;
-      const float *q = a.q + (seq.first + r / a.group) * a.ldq + (int64_t)(head * a.group + r % a.group) * D + 8 * chunk;
+    const bool wide = (((uintptr_t)a.q | (uintptr_t)a.ldq * 4) & 15) == 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 16 / ROWS; i0 += 4) {
+      float4 in[4][2];   // four rows under way
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = r < count ? q[j] : 0.0f;
-        top = fmaxf(top, fabsf(x[j]));
+      for (int i = 0; i < 4; ++i) {
+        const int q_row = warp * 16 + (i0 + i) * ROWS + lane / LANES, r = r0 + q_row;
+        const float *q = a.q + q_at[q_row] + 8 * chunk;
+        in[i][0] = in[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < count && wide) {
+          in[i][0] = reinterpret_cast<const float4 *>(q)[0];
+          in[i][1] = reinterpret_cast<const float4 *>(q)[1];
+        } else if (r < count) {
+          in[i][0] = make_float4(q[0], q[1], q[2], q[3]);
+          in[i][1] = make_float4(q[4], q[5], q[6], q[7]);
+        }
       }
 #pragma unroll
-      for (int j = 1; j < LANES; j <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, j));
-      const float up = to_top(top);
-      if (chunk == 0) qfactor[q_row] = a.scale * 1.4426950408889634f * (1.0f / up);
-      uint32_t hi[4], lo[4];
+      for (int i = 0; i < 4; ++i) {
+        const int q_row = warp * 16 + (i0 + i) * ROWS + lane / LANES;
+        const float x[8] = {in[i][0].x, in[i][0].y, in[i][0].z, in[i][0].w, in[i][1].x, in[i][1].y, in[i][1].z, in[i][1].w};
+        float top = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float y = x[j] * up, z = x[j + 4] * up;
-        hi[j] = pack_half(y, z);
-        lo[j] = pack_half_lo(y, z, hi[j]);
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
+#pragma unroll
+        for (int j = 1; j < LANES; j <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, j));
+        const float up = to_top(top), sign_up = a.scale < 0.0f ? -up : up;
+        if (chunk == 0) qfactor[q_row] = fabsf(a.scale) * 1.4426950408889634f * (1.0f / up);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float y = x[j] * sign_up, z = x[j + 4] * sign_up;
+          hi[j] = pack_half(y, z);
+          lo[j] = pack_half_lo(y, z, hi[j]);
+        }
+        unsigned char *dst = sq + chunk / 8 * 32768 + k3_at(q_row, chunk % 8);
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4 *>(dst + 16384) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
-      unsigned char *dst = sq + chunk / 8 * 32768 + k3_at(q_row, chunk % 8);
-      *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4 *>(dst + 16384) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     fence_proxy_async();
   };
@@ -1094,14 +1115,10 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
       for (int blk = 0; blk < NB; ++blk) {
         x[blk] = half_pair(d[blk]).x;
         y[blk] = Q41 ? fmaf(8.0f, x[blk], half_pair(m[blk]).x) : 0.0f;
-        top = fmaxf(top, fmaf(8.0f, fabsf(x[blk]), fabsf(y[blk])));
-      }
-      const float up = to_top(top);
-      kdown[step & 3][token] = 1.0f / up;
-#pragma unroll
-      for (int blk = 0; blk < NB; ++blk) {
-        k_scale[st][token][blk] = Q41 ? __float_as_uint(x[blk] * up) : pack_half(x[blk] * up, x[blk] * up);
-        if (Q41) k_off[st][token][blk] = y[blk] * up;
+        const float most = fmaf(8.0f, fabsf(x[blk]), fabsf(y[blk]));
+        if (in && most < INFINITY) top = fmaxf(top, most);
+        k_scale[st][token][blk] = x[blk];
+        if (Q41) k_off[st][token][blk] = y[blk];
       }
     } else {
       unsigned lost = 0;
@@ -1119,23 +1136,22 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
         if (Q41) v_min[st][token][c] = m[2 * c] | m[2 * c + 1] << 16;
       }
       bad[step & 3][token] = lost;
-      top = warp_max(top);
       const unsigned any = __any_sync(0xffffffffu, lost);
-      if (lane == 0) {
-        largest[st][cw & 1] = top;
-        any_bad[step & 3][cw & 1] = any;
-      }
+      if (lane == 0) any_bad[step & 3][cw & 1] = any;
     }
+    top = warp_max(top);
+    if (lane == 0) largest[st][cw] = top;
   };
   // keys of a tile and a block
-  auto convert_k = [&](int st, int unit) {
+  auto convert_k = [&](int st, int unit, float up) {
     const int i = unit / (2 * NC), c = unit / 2 % NC, k = unit % 2;
     const uint4 w = *reinterpret_cast<const uint4 *>(raw + (st * 4 + i) * TILE + c * 512 + lane * 16);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {   // tokens g, g + 8
       const int token = 16 * i + g + 8 * h;
-      const uint32_t x = h ? (k ? w.w : w.z) : (k ? w.y : w.x), dd = k_scale[st][token][2 * c + k], codes[4] = {codes_lo(x), codes_hi(x), codes_lo(x >> 8), codes_hi(x >> 8)};
-      const float d = __uint_as_float(dd), n = Q41 ? k_off[st][token][2 * c + k] : 0.0f;
+      const uint32_t x = h ? (k ? w.w : w.z) : (k ? w.y : w.x), codes[4] = {codes_lo(x), codes_hi(x), codes_lo(x >> 8), codes_hi(x >> 8)};
+      const float d = k_scale[st][token][2 * c + k] * up, n = Q41 ? k_off[st][token][2 * c + k] * up : 0.0f;
+      const uint32_t dd = pack_half(d, d);
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) k3_split<Q41>(codes[e], dd, make_float2(d, d), make_float2(n, n), &hi[e], &lo[e]);
@@ -1212,20 +1228,20 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
         if (cw < 4) scales(step, cw);
       }
       asm volatile("bar.sync 5, %0;" ::"n"(32 * K3_CONVERT) : "memory");   // also: the step before has been read
-      const float up = to_top(fmaxf(largest[st][0], largest[st][1]));
+      const float up_k = to_top(fmaxf(largest[st][0], largest[st][1])), up = to_top(fmaxf(largest[st][2], largest[st][3]));
       if (cw == K3_CONVERT - 1 && ok) {
         if (step > 0 && asked < steps) {
           issue(asked, id_next);
           ++asked;
           id_next = page_at(asked);
         }
-        if (lane == 0) { ups[step & 3] = up; theres[step & 3] = present[st]; }
+        if (lane == 0) { ups[step & 3] = up; downs[step & 3] = 1.0f / up_k; theres[step & 3] = present[st]; }
       }
       // units of K, then of V, dealt as one row (32 of heads of 128)
       int unit = cw;
       if (wait(k_empty(st), phase ^ 1u)) {
 #pragma unroll 1
-        for (; unit < 8 * NC; unit += K3_CONVERT) convert_k(st, unit);
+        for (; unit < 8 * NC; unit += K3_CONVERT) convert_k(st, unit, up_k);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(k_full(st));
@@ -1250,13 +1266,14 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
       const uint32_t phase = (uint32_t)(step >> 1) & 1u;
       if (!wait(k_full(st), phase) || !wait(s_empty(st), phase ^ 1u)) return;
       tc_fence_after();
-      const uint32_t el = elect_one(), acc = tmem + 128 * st;
+      const uint32_t el = elect_one(), acc = tmem + 64 * st, idesc = IDESC | (64u >> 3 << 17);
       const uint64_t dk = dk0 + (uint64_t)(st * NC * 1024);
 #pragma unroll
       for (int k = 0; k < 4 * NC; ++k) {   // 16 halves are two descriptor units of 16 bytes
         const uint64_t aq = dq + (uint64_t)((k >> 2) * 2048 + 2 * (k & 3)), ak = dk + (uint64_t)((k >> 2) * 1024 + 2 * (k & 3));
-        umma_bf16(acc, aq, ak, IDESC | (128u >> 3 << 17), k > 0 ? 1u : 0u, el);   // (fp16: the kind's types are IDESC's)
-        umma_bf16(acc, aq + 1024, ak, IDESC | (64u >> 3 << 17), 1u, el);
+        umma_bf16(acc, aq, ak, idesc, k > 0 ? 1u : 0u, el);   // (fp16: the kind's types are the descriptor's)
+        umma_bf16(acc, aq + 1024, ak, idesc, 1u, el);
+        umma_bf16(acc, aq, ak + 512, idesc, 1u, el);
       }
       umma_commit(k_empty(st), el);
       umma_commit(s_full(st), el);
@@ -1294,25 +1311,15 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
     const float factor = qfactor[row];
     for (int step = 0; step < steps; ++step) {
       const int base = t0 + 64 * step, st = step & 1;
-      float x[32], top = run_max;
+      uint32_t x[32];
+      float top = -INFINITY, f = 0.0f;
       if (wait(s_full(st), (uint32_t)(step >> 1) & 1u)) {
         tc_fence_after();
         const unsigned there = theres[step & 3];
-#pragma unroll
-        for (int e0 = 0; e0 < 32; e0 += 8) {
-          uint32_t p[8], q[8];
-          tmem_ld8(tlane + 128 * st + 32 * hf + e0, p);
-          tmem_ld8(tlane + 128 * st + 64 + 32 * hf + e0, q);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 8; e += 4) {
-            const float4 down = *reinterpret_cast<const float4 *>(kdown[step & 3] + 32 * hf + e0 + e);
-            x[e0 + e] = (__uint_as_float(p[e]) + __uint_as_float(q[e])) * factor * down.x;
-            x[e0 + e + 1] = (__uint_as_float(p[e + 1]) + __uint_as_float(q[e + 1])) * factor * down.y;
-            x[e0 + e + 2] = (__uint_as_float(p[e + 2]) + __uint_as_float(q[e + 2])) * factor * down.z;
-            x[e0 + e + 3] = (__uint_as_float(p[e + 3]) + __uint_as_float(q[e + 3])) * factor * down.w;
-          }
-        }
+        f = fmaxf(factor * downs[step & 3], 1.17549435e-38f);   // (positive: it multiplies infinities)
+        tmem_ld16(tlane + 64 * st + 32 * hf, x);
+        tmem_ld16(tlane + 64 * st + 32 * hf + 16, x + 16);
+        tmem_ld_wait();
         const bool hidden = base + 64 > least || base + 64 > t1 || there != 15u;   // some row does not see some token
         tc_fence_before();
         __syncwarp();
@@ -1321,15 +1328,15 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
           keep_branch();
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (base + 32 * hf + e >= sees || !(there >> (2 * hf + e / 16) & 1)) x[e] = -INFINITY;
+            if (base + 32 * hf + e >= sees || !(there >> (2 * hf + e / 16) & 1)) x[e] = __float_as_uint(-INFINITY);
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
+        for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(x[e]));
         red[st][hf][row] = top;
       }
       asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");   // warps quad and quad + 4
       if (!ok) continue;
-      top = fmaxf(red[st][0][row], red[st][1][row]);
+      top = fmaxf(run_max, fmaxf(red[st][0][row], red[st][1][row]) * f);
       const float ref = top == -INFINITY ? 0.0f : top - K3_LIFT;
       const float corr = exp2_fast(run_ref - ref), up = ups[step & 3];
       run_max = top;
@@ -1341,7 +1348,7 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float y = exp2_fast(x[2 * (e0 + e)] - ref), z = exp2_fast(x[2 * (e0 + e) + 1] - ref);
+          const float y = exp2_fast(fmaf(__uint_as_float(x[2 * (e0 + e)]), f, -ref)), z = exp2_fast(fmaf(__uint_as_float(x[2 * (e0 + e) + 1]), f, -ref));
           sum += y + z;
           hi[e] = pack_half(y, z);
           lo[e] = pack_half_lo(y, z, hi[e]);
@@ -1384,22 +1391,28 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
     const float sum = red[0][0][row] + red[0][1][row];
     red[1][0][row] = a.parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
     if (a.parts > 1 && !failed && r0 + row < count) {
-      float *dst = a.part + (((((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt) * a.parts + part) * K3_ROWS + row) * (D + 2) + D;
+      float *dst = a.part + out_at[row] + D;
       dst[0] = run_ref;   // (what outputs and sum are relative to)
       dst[1] = sum;
     }
   }
   __syncthreads();
-  if (!failed && rows_warp)
-    for (int i = 0; i < 16; ++i) {
-      const int out_row = warp * 16 + i, rr = r0 + out_row;
-      if (rr >= count) break;
+  if (!failed && rows_warp) {
+    constexpr int LANES = D / 4, ROWS = 32 / LANES;
+    const int piece = lane % LANES;
+    const bool wide = a.parts == 1 && ((uintptr_t)a.out & 15) == 0;
+#pragma unroll 4
+    for (int i = 0; i < 16 / ROWS; ++i) {
+      const int out_row = warp * 16 + i * ROWS + lane / LANES;
+      if (r0 + out_row >= count) continue;
+      float4 x = *reinterpret_cast<const float4 *>(so + piece / 8 * 16384 + k3_at(out_row, piece % 8));
       const float scale = red[1][0][out_row];
-      float *dst = a.parts == 1 ? a.out + (seq.first + rr / a.group) * (int64_t)a.heads * D + (int64_t)(head * a.group + rr % a.group) * D
-                                : a.part + (((((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt) * a.parts + part) * K3_ROWS + out_row) * (D + 2);
-#pragma unroll
-      for (int k = 0; k < NB; ++k) dst[32 * k + lane] = *reinterpret_cast<const float *>(so + k * 16384 + k3_at(out_row, lane >> 2) + (lane & 3) * 4) * scale;
+      x.x *= scale; x.y *= scale; x.z *= scale; x.w *= scale;
+      float *dst = (a.parts == 1 ? a.out : a.part) + out_at[out_row] + 4 * piece;
+      if (wide) *reinterpret_cast<float4 *>(dst) = x;
+      else { dst[0] = x.x; dst[1] = x.y; dst[2] = x.z; dst[3] = x.w; }
     }
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
@@ -1880,7 +1893,7 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
     fill = 148 * 48 / p->warps; blocks = p->units; shares = p->warps;
   } else if (p->tile_rows == K3_ROWS) {
     p->warps = 1;
-    fill = 148; blocks = p->units; shares = 1;
+    fill = 148; blocks = p->units; shares = 1;   // (152 tiles over 2000 tokens, 600 rows of 32 heads over 8: 135 us whole, 156 in three parts)
   } else {
     p->warps = p->row_tiles >= 4 ? 4 : p->row_tiles >= 2 ? 2 : 1;
     fill = 148 * 12; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = k4_warps(p->warps == 4) / p->warps;
