@@ -112,7 +112,7 @@ __device__ __forceinline__ float to_top(float x, int k = 14) {
 // or 32 tokens, which bulk copies fill while the other is read (each stage is read by all its warps before it is filled again).
 // With four row tiles (SHARED) the warps first turn a stage's codes into operands and its scales into floats, a quarter each, in shared memory: of the
 // instructions of 16 tokens and a block of 32 dims, a hundred, that is nearly half, and each warp would do it for itself (5 prompts of 167 to 333
-// tokens, 16 heads over 4 of 128: 130 us).
+// tokens, 16 heads over 4 of 128: 130 us; they go in tiles of 128 rows now).
 template <int NC, bool Q41, bool SHARED>
 __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 : 1) : NC == 1 ? 4 : NC == 2 ? 3 : 2) kv4_attention_kernel(const Kv4AttnArgs a) {
   constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, TILES = K4_TILES(NC), GROUP = 16 * TILES, STAGE = TILES * TILE;
@@ -909,12 +909,18 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
 // ---- prompts ----------------------------------------------------------------------------------------
 // 128 rows of a key head are the lanes of tensor memory, 64 tokens a step; a step's products are tcgen05.mma on fp16 halves, 22 bits of each operand:
 //   S = Q_hi K_hi^T + Q_hi K_lo^T + Q_lo K_hi^T        O = P_hi V_hi + P_lo V_hi + P_hi V_lo
-// Scales are multiplied in before (d (code - 8) has 15 bits, so for Q4_0 two halves hold it exactly): a step's keys and its
-// values times a power of two each that brings the largest near the top of fp16.  S, P and O lie in tensor memory; a row's two threads (warps w and w + 4) take
-// half of the tokens and half of the dims each, and keep the running output in registers, so that a moved maximum costs nothing more.  By warp:
+// (lo lo, 2^-22 of a product, is left out).  Scales are multiplied in before (d (code - 8) has 15 bits, so for Q4_0 two halves hold it exactly), a step's
+// keys and its values times a power of two each that brings the largest near the top of fp16.  S, P and O lie in tensor memory; a row's two threads
+// (warps w and w + 4) take half of the tokens and half of the dims each, and keep the running output in registers, so that a moved maximum costs nothing
+// more.  A value that is not finite would reach rows that do not see it (0 times NaN): it is zero in the product, and NaN is put into the blocks of the rows
+// that see it.  By warp:
 //   0 .. 7     rows of q; softmax of a step, its P, and the output of the step before
 //   8 .. 14    codes into operands, two steps ahead at most (two stages each); the last asks for the tiles of the step after
 //   15         issues the products: S a step ahead of the softmax
+// A step takes 3.4 k cycles with heads of 64, 4.4 k of 128, of them 1.0 and 1.8 k of products; what bounds it is the instructions of warps 0 to 14 (0.5 a
+// cycle and scheduler), unpacking before the softmax.  All phases by eight warps one after the other: 6.4 and 6.7 k; four warps to unpack: 195 us in place
+// of 135 for 600 tokens over 2000, 32 heads of 128 over 8; two units at a time in registers: 130 in place of 127 (the code no longer fits the
+// instruction cache).  That case 127 us now (tiles of 8 rows 271), 2000 of 25 heads of 64 111 (201), 5 prompts of 333, 16 heads of 128 over 4, 30 (67).
 constexpr int K3_ROWS = 128, K3_THREADS = 512, K3_SOFTMAX = 8, K3_CONVERT = 7;   // (warps)
 constexpr float K3_LIFT = 14.0f;   // p is taken times 2^14, its sum with it
 __host__ __device__ constexpr int k3_smem(int chunks, int tile_bytes) { return chunks * (32768 + 2 * 16384 + 2 * 16384) + 2 * 4 * tile_bytes + 1024; }
@@ -1864,11 +1870,11 @@ struct Kv4Plan {
   int64_t units;   // row tiles of all sequences and key heads
   int tile_rows, row_tiles, parts, part_tokens, warps;
 };
-// Whether rows are enough for tiles of 128: half of one a sequence and key head on the average, and 1e8 products, below which the wider kernel's start
-// costs more than it saves (us in tiles of 8 rows and of 128: 64 tokens of 1 head of 64 dims 6.9 and 11.8; 64 over 500 of 25 such heads 17.8 and 19.6; 16
-// over 500 of 8 sequences, 16 heads of 128 over 4 29.8 and 25.4; 2000 of 25 heads of 64 201 and 117).
+// Whether rows are enough for tiles of 128: 48 a sequence and key head on the average, and 1e8 products of all, below which that kernel's start costs more
+// than it saves.  us in tiles of 8 rows and of 128: 32 rows over 2000 tokens (16 sequences, 8 key heads of 128) 94 and 120, 48 over 300 (64 sequences) 97
+// and 82; 8 prompts of 64, 8 heads of 128, 9.0 and 11.5, one of 256, 12 heads of 64, 10.1 and 17.0; 600 over 2000, 32 heads of 128 over 8, 271 and 127.
 static bool kv4_prompts(const caten_b200_kv4_desc *c, int64_t batch, int64_t rows, int64_t max_length) {
-  return c->dim <= 128 && rows * (c->heads / c->kv_heads) >= 64 * batch && (double)rows * c->heads * (double)max_length * c->dim >= 1e8;
+  return c->dim <= 128 && rows * (c->heads / c->kv_heads) >= 48 * batch && (double)rows * c->heads * (double)max_length * c->dim >= 1e8;
 }
 static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_desc *c, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length, Kv4Plan *p) {
   Kv4Shape s;
@@ -1898,7 +1904,7 @@ static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_d
     p->warps = p->row_tiles >= 4 ? 4 : p->row_tiles >= 2 ? 2 : 1;
     fill = 148 * 12; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = k4_warps(p->warps == 4) / p->warps;
   }
-  // (blocks of several rows that fill the SMs as they are would only add the join: 5 prompts of up to 333 tokens 116 -> 136 us)
+  // (blocks of several rows that fill the SMs as they are would only add the join: 5 prompts of up to 333 tokens in such tiles 116 -> 136 us)
   int64_t parts = !blocks || (p->tile_rows == K4_ROWS && blocks >= 148 * 4) ? 1 : (fill + blocks - 1) / blocks;
   // A part gives each warp two groups at least.  Single rows of up to four groups a warp are left whole: two groups less take no longer than the join
   // and its launch (25 heads x 700 tokens 7.2 us in parts, 5.3 whole; 1000 7.2 and 6.2; 1500 7.4 and 7.9).
