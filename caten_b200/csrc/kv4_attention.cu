@@ -9,7 +9,8 @@
 //   score(r, t) = sum over blocks of d_t,b (q_r . (codes - 8)) + n_t,b sum(q_r)          out(r, j) = sum_t (p_rt d_t,b) (code_tj - 8) + sum_t p_rt n_t,b
 // with n = 0 (Q4_0) or the minimum + 8 d (Q4_1).  From the middle of the codes, because a sum of thousands of p d code is many times what is left when
 // 8 p d is taken off it, and so is its error (100001 tokens: 3e-4).
-// A warp has 8 rows (tokens x the heads that share a key head) and takes 64 tokens at a time: running maximum and sum of the softmax per row, the
+// (So in the kernels for up to 48 rows; the one for prompts multiplies the scales in before.)
+// A warp has 8 rows (tokens x the heads that share a key head; kernels for one row and for two to four follow, and one for tiles of 128) and takes 64 tokens at a time: running maximum and sum of the softmax per row, the
 // group's p d scaled by a power of two for each block, so that the largest is near the top of fp16 whatever the cache's scales are, and joined
 // to the running sums in fp32.
 #include <algorithm>
