@@ -776,6 +776,51 @@ def test_captured_and_replayed_on_a_stream_of_the_caller(rt):
         r.close()
 
 
+def test_prompts_on_two_streams_at_once(rt):
+    """Graphs of attention over prompts, one cut into parts and one whole, and of few rows, each replayed on a stream of its own."""
+    import torch
+    from caten_b200.runtime import B200Runtime
+    r = B200Runtime(0)
+    try:
+        sets = []
+        for heads, kv, dim, lengths, news in ((4, 1, 128, [900], [200]), (50, 50, 64, [260, 131, 300], [260, 131, 300]), (8, 2, 64, [900, 40], [3, 3])):
+            rng = rng_of(64, heads)
+            c = Cache(r, rng, "q4_1", dim, 64, heads, kv, lengths, spare=columns_for(sum(news), heads, dim, 64) if heads == 4 else 2)
+            at = np.concatenate([[0], np.cumsum(news)])
+            q = rng.standard_normal((int(at[-1]), heads, dim), dtype=np.float32)
+            top = c.table.shape[1] * 64
+            s = dict(c=c, q=put(r, q.reshape(at[-1], -1)), table=put(r, c.table, np.int32), lengths=put(r, lengths, np.int32), starts=put(r, at, np.int32),
+                     out=r.open_buffer((int(at[-1]), heads * dim)), work=r.open_buffer(r.kv4_attention_work(c.desc, len(lengths), int(at[-1]), max(news), top), np.uint8),
+                     stream=torch.cuda.Stream(), graph=torch.cuda.CUDAGraph())
+
+            def step(s=s, c=c, news=news, top=top):
+                r.kv4_attention(c.desc, s["q"], c.pool, s["table"], s["lengths"], starts=s["starts"], max_new=max(news), max_length=top, out=s["out"], work=s["work"])
+            step()
+            r.sync()
+            s["want"] = s["out"].numpy().copy()
+            for b, m in enumerate(lengths):
+                part = slice(c.first[b], c.first[b + 1])
+                want = ref.attention(q[at[b]:at[b + 1]], c.k[part], c.v[part], m, c.desc.scale)
+                np.testing.assert_allclose(s["want"][at[b]:at[b + 1]].reshape(want.shape), want, rtol=0, atol=bound(c, q, m))
+            L.check(r.ctx, r.lib.caten_b200_set_stream(r.ctx, s["stream"].cuda_stream))
+            with torch.cuda.graph(s["graph"], stream=s["stream"], capture_error_mode="thread_local"):
+                step()
+            L.check(r.ctx, r.lib.caten_b200_set_stream(r.ctx, None))
+            L.check(r.ctx, r.lib.caten_b200_memset(r.ctx, s["out"].ptr, 0, s["out"].nbytes))
+            sets.append(s)
+        r.sync()
+        for _ in range(5):
+            for s in sets:
+                with torch.cuda.stream(s["stream"]):
+                    s["graph"].replay()
+        torch.cuda.synchronize()
+        for s in sets:
+            np.testing.assert_array_equal(s["out"].numpy(), s["want"])
+            del s["graph"]
+    finally:
+        r.close()
+
+
 def plain_beam_search(logits_of, prompt, beams, steps, eos):
     """[(tokens, score)] by beam search on the host, and the smallest gap between the last value taken and the first left."""
     hyps, gap = [(list(prompt), 0.0, False)], np.inf
