@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
 
   // q as the first product's operand: a block's two steps, {dims 8t + 0, 4 | 8t + 1, 5} and {2, 6 | 3, 7}; hi in rows g, lo in rows g + 8
   uint32_t qa[NB][2][4];
-  float qsum8[NB];   // 8 sum(q) of a block
+  float qsum[NB];   // Q4_1: sum(q) of a block
   float factor;
   {
     const float *q = a.q + (seq.first + tok) * a.ldq + (int64_t)(head * a.group + r % a.group) * D + 8 * t;
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
       if (Q41) {
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        qsum8[k] = 8.0f * sum;
+        qsum[k] = sum;
       }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
@@ -335,13 +335,13 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
                 const uint32_t lo = words[2 * n + k], hi = lo >> 8;
                 op = make_uint4(codes_lo(lo), codes_hi(lo), codes_lo(hi), codes_hi(hi));
               }
-              float p[4] = {Q41 ? qsum8[blk] : 0.0f, Q41 ? qsum8[blk] : 0.0f, 0.f, 0.f};   // (d code + m = d (code - 8 + 8) + m)
+              float p[4] = {0.f, 0.f, 0.f, 0.f};
               mma_16816(p, qa[blk][0], op.x, op.y);
               mma_16816(p, qa[blk][1], op.z, op.w);
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
                 const int e = 2 * n + j;
-                if (Q41) acc[e] = fmaf(m[e], 0.125f * qsum8[blk], acc[e]);
+                if (Q41) acc[e] = fmaf(fmaf(8.0f, d[e], m[e]), qsum[blk], acc[e]);   // (d code + m = d (code - 8) + (m + 8 d), which cancel before they are summed)
                 acc[e] = fmaf(d[e], p[j] + p[2 + j], acc[e]);
               }
             }
@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
 
     // q: this lane's column (row g / 2, half g % 2); dims {0, 4 | 1, 5} and {2, 6 | 3, 7} of the lane's eight in each block
     uint32_t qb[NB][4];
-    float qsum8[NB];   // Q4_1: 8 sum(q) of a block, row t
+    float qsum[NB];   // Q4_1: sum(q) of a block, row t
     float factor;
     {
       const int r = r0 + (g >> 1);
@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
         if (Q41) {
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          qsum8[k] = 8.0f * __shfl_sync(0xffffffffu, sum, 8 * t);
+          qsum[k] = __shfl_sync(0xffffffffu, sum, 8 * t);
         }
         qb[k][0] = pack_half(y[0], y[4]);
         qb[k][1] = pack_half(y[1], y[5]);
@@ -710,7 +710,7 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
             const uint32_t x = k ? w.y : w.x, y = k ? w.w : w.z;
             const uint32_t a0[4] = {codes_lo(x), codes_lo(y), codes_hi(x), codes_hi(y)};
             const uint32_t a1[4] = {codes_lo(x >> 8), codes_lo(y >> 8), codes_hi(x >> 8), codes_hi(y >> 8)};
-            float p[4] = {Q41 ? qsum8[blk] : 0.0f, 0.f, Q41 ? qsum8[blk] : 0.0f, 0.f};   // (d code + m = d (code - 8 + 8) + m)
+            float p[4] = {0.f, 0.f, 0.f, 0.f};
             mma_16816(p, a0, qb[blk][0], qb[blk][1]);
             mma_16816(p, a1, qb[blk][2], qb[blk][3]);
             const uint8_t *sc = tile + 8 * D + ((g >> 1) * NB + blk) * 8;
@@ -719,8 +719,8 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
             if (Q41) {
               const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
               const float2 m = half_pair(__byte_perm(m2.x, m2.y, g & 1 ? 0x7632 : 0x5410));
-              x0 = fmaf(m.x, 0.125f * qsum8[blk], x0);
-              x1 = fmaf(m.y, 0.125f * qsum8[blk], x1);
+              x0 = fmaf(fmaf(8.0f, d.x, m.x), qsum[blk], x0);   // (as above)
+              x1 = fmaf(fmaf(8.0f, d.y, m.y), qsum[blk], x1);
             }
             x0 = fmaf(d.x, p[0] + p[1], x0);
             x1 = fmaf(d.y, p[2] + p[3], x1);
