@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
 // columns, halves side by side (column 2 r + h), nothing is empty: half the products of the kernel above, a score in one lane (row t, tokens g and
 // g + 8), half the softmax; in the second product columns 2 r + h again, whose two sums a lane has both.  Each warp has a ring of its own.
 // Bound by instructions (unpacking, two roundings of p d).  4 heads to a key head of 128, Q4_0: 256 sequences of 768 tokens 84 us (the kernel above
-// 111), 64 of 768 25 (45), 3 of 100001 132 (167: 346 MB, 2.6 TB/s); Q4_1 the last in 152 (186); 32 heads over 16 key heads of 256, 8 sequences of
+// 111), 64 of 768 25 (45), 3 of 100001 132 (167: 346 MB, 2.6 TB/s); Q4_1 the last in 147 (186); 32 heads over 16 key heads of 256, 8 sequences of
 // 2900 63 (76).
 constexpr int K2_WARPS = 4;   // of a block; 1 or 4 of them share a unit
 constexpr int K2_ROWS = 4;
