@@ -17,6 +17,7 @@
 
 #include "common.cuh"
 #include "kv4.cuh"
+#include "kv4_ring.h"
 #include "tcgen05.cuh"
 
 namespace cb {
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
   constexpr int OPS = TILES * NC * 8 * 512, FLOATS = TILES * (Q41 ? 3 : 2) * PER_TILE * 4, SHARE = 2 * STAGE + (SHARED ? OPS + FLOATS : 0);   // bytes
   __shared__ float sm[WARPS][K4_ROWS], sl[WARPS][K4_ROWS];
   __shared__ uint64_t bars[WARPS][2];
-  __shared__ int gave_up[WARPS];
+  __shared__ int gave_up[WARPS], never;           // (never: not set by anyone)
   __shared__ unsigned present[WARPS][2];          // of a share: tiles of each stage
   __shared__ unsigned largest_scale[WARPS][2];       // SHARED: of a stage's values
   extern __shared__ __align__(128) uint8_t ring[];   // two stages a share (SHARED: then its operands); behind the last group, the warps' sums
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
     if (lane == 0) {
       mbar_init(bar, 1);
       mbar_init(bar + 8, 1);
-      gave_up[share] = 0;
+      gave_up[share] = never = 0;
       fence_proxy_async();
     }
     __syncwarp();
@@ -237,17 +238,19 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
   __syncthreads();   // the barriers are there
   int stage = 0;
   uint32_t phase = 0;
-  bool all_ok = true;
+  bool ok = true;
   for (int base = first; base < t1; base += step) {
-    // (a wait that runs out does not leave the loop: the share's warps meet below as often as each other, and further waits give up at once)
-    const bool ok = mbar_wait(bar + 8 * stage, phase, &gave_up[share]);
-    if (!ok && lane == 0) {
-      gave_up[share] = 1;
-      atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
-      a.status[1] = 48;
+    // (a wait that runs out does not leave the loop: the share's warps meet below as often as each other)
+    if (ok && !mbar_wait(bar + 8 * stage, phase, &gave_up[share])) {
+      ok = false;
+      if (lane == 0) {
+        gave_up[share] = 1;
+        atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
+        a.status[1] = 48;
+      }
+      if (sub == 0) ring_land(stage, phase, base + step < t1, [&](int s, uint32_t p) { mbar_wait_thread(bar + 8 * s, p, &never); });
     }
-    all_ok &= ok;
-    if (SHARED) {
+    if (SHARED && ok) {
       const uint8_t *tiles = stages + stage * STAGE;
       const unsigned there = present[share][stage];
 #pragma unroll
@@ -287,8 +290,8 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
       }
       largest = __reduce_max_sync(0xffffffffu, largest);
       if (lane == 0 && largest) atomicMax(&largest_scale[share][stage], largest);
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + share) : "memory");
     }
+    if (SHARED) asm volatile("bar.sync %0, 128;" ::"r"(1 + share) : "memory");
     if (ok && mine && base < most) {
       const uint8_t *tiles = stages + stage * STAGE;
       const unsigned there = present[share][stage];
@@ -494,15 +497,13 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
     if (row_warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + share), "r"(32 * row_warps) : "memory");
     else __syncwarp();
     if (SHARED && sub == 0 && lane == 0) largest_scale[share][stage] = 0;   // (two barriers before it is used again)
-    if (sub == 0 && base + 2 * step < t1) {
+    if (sub == 0 && ok && base + 2 * step < t1) {
       issue(base + 2 * step, id_next, stage);
       id_next = page_at(base + 3 * step);
     }
     phase ^= stage;
     stage ^= 1;
   }
-  if (!all_ok && sub == 0)
-    for (int i = 0; i < 2; ++i) mbar_wait_thread(bar + 8 * (stage ^ i), phase ^ (stage & i), &gave_up[share]);   // copies land before the block ends
 
   // the warp's sums: over the four lanes of a row, then the blocks' constant parts to the lanes that hold the outputs
   run_sum += __shfl_xor_sync(0xffffffffu, run_sum, 1);
@@ -522,7 +523,7 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
     for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] *= run_down;
   float *so = reinterpret_cast<float *>(ring) + warp * K4_ROWS * D;   // [row][D]
   if (shares > 1) {
-    __syncthreads();   // no stage is read or filled any more
+    if (__syncthreads_or(!ok)) return;   // no stage is read or filled any more; what did not come is nobody's output
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
       float *dst = so + 2 * t * D + 32 * k + 4 * g;
@@ -537,7 +538,7 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
     sl[warp][g] = run_sum;
   }
   __syncwarp();
-  if (!mine) return;
+  if (!mine || !ok) return;
   const int64_t tile_of = ((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {   // rows 2t and 2t + 1
@@ -622,6 +623,7 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
 
   const int first = t0 + (warp - first_warp) * GROUP, step = share * GROUP;
   uint8_t *const mine = ring + warp * 2 * STAGE;
+  bool ok = true;   // the copies came
   if (live && first < t1) {
     const uint32_t bar = smem_u32(&bars[warp][0]), dst = smem_u32(mine);
     if (lane == 0) {
@@ -686,10 +688,9 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
         qb[k][3] = pack_half(y[3], y[7]);
       }
     }
-    bool ok = true;
-    int stage = 0;
+    int stage = 0, base = first;
     uint32_t phase = 0;
-    for (int base = first; base < t1; base += step) {
+    for (; base < t1; base += step) {
       ok = mbar_wait(bar + 8 * stage, phase, &gave_up[warp]);
       if (!ok) break;
       const uint8_t *tiles = mine + stage * STAGE;
@@ -846,11 +847,10 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
     }
     if (!ok) {
       if (lane == 0) {
-        gave_up[warp] = 1;
         atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
         a.status[1] = 49;
       }
-      for (int i = 0; i < 2; ++i) mbar_wait_thread(bar + 8 * (stage ^ i), phase ^ (stage & i), &gave_up[warp]);   // copies land before the block ends
+      ring_land(stage, phase, base + step < t1, [&](int s, uint32_t p) { mbar_wait_thread(bar + 8 * s, p, &gave_up[warp]); });   // (a flag that nobody raises)
     }
   }
 
@@ -877,7 +877,7 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
 #pragma unroll
     for (int k = 0; k < NB; ++k) *reinterpret_cast<float4 *>(so + warp * STRIDE + t * D + 32 * k + 4 * g) = x[k];
     if (g == 0) { sm[warp][t] = run_max; sl[warp][t] = run_sum; }
-    __syncthreads();
+    if (__syncthreads_or(!ok)) return;   // (the block is one unit's; what did not come is nobody's output)
     if (warp != first_warp) return;
     for (int w = warp + 1; w < warp + share; ++w) top = fmaxf(top, sm[w][t]);
     const float ref = top == -INFINITY ? 0.0f : top;
@@ -895,7 +895,7 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
     }
   }
   const int rr = r0 + t;
-  if (!live || rr >= count) return;
+  if (!live || !ok || rr >= count) return;
   float *dst = a.parts == 1 ? a.out + (seq.first + rr / a.group) * (int64_t)a.heads * D + (int64_t)(head * a.group + rr % a.group) * D
                             : a.part + ((tile_of * a.parts + part) * K2_ROWS + t) * (D + 2);
   const float scale = a.parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -1506,6 +1506,7 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
 
   const int first = t0 + (warp - first_warp) * K4_GROUP, step = share * K4_GROUP;
   uint8_t *const mine = ring + warp * 2 * STAGE;
+  bool ok = true;   // the copies came
   if (live && first < t1) {
     // A stage is 64 tokens.  Lanes 0 to 3 have a tile each; of pages that hold them all, lane 0 copies what there is at once.  A tile that
     // cannot be followed is left out and counts for nothing.
@@ -1591,10 +1592,9 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
       }
     }
     const int k_scale = 8 * D + ((g >> 1) * NB + (t >> 1)) * 8, v_scale = PART + 8 * D + (t * NB + (g >> 2)) * 8;
-    bool ok = true;
-    int stage = 0;
+    int stage = 0, base = first;
     uint32_t phase = 0;
-    for (int base = first; base < t1; base += step) {
+    for (; base < t1; base += step) {
       ok = mbar_wait(bar + 8 * stage, phase, &gave_up[warp]);
       if (!ok) break;
       const uint8_t *tiles = mine + stage * STAGE;
@@ -1748,11 +1748,10 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
     }
     if (!ok) {
       if (lane == 0) {
-        gave_up[warp] = 1;
         atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
         a.status[1] = 47;
       }
-      for (int i = 0; i < 2; ++i) mbar_wait_thread(bar + 8 * (stage ^ i), phase ^ (stage & i), &gave_up[warp]);   // copies land before the block ends
+      ring_land(stage, phase, base + step < t1, [&](int s, uint32_t p) { mbar_wait_thread(bar + 8 * s, p, &gave_up[warp]); });   // (a flag that nobody raises)
     }
   }
 
@@ -1786,7 +1785,7 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
 #pragma unroll
     for (int c = 0; c < NC; ++c) *reinterpret_cast<float2 *>(&so[warp * STRIDE + 64 * c + at]) = r[c];
     if (lane == 0) { sm[warp] = run_max; sl[warp] = run_sum; }
-    __syncthreads();
+    if (__syncthreads_or(!ok)) return;   // (the block is one unit's; what did not come is nobody's output)
     if (warp != first_warp) return;
     for (int w = warp + 1; w < warp + share; ++w) top = fmaxf(top, sm[w]);
     const float ref = top == -INFINITY ? 0.0f : top;
@@ -1804,7 +1803,7 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
       }
     }
   }
-  if (!live) return;
+  if (!live || !ok) return;
   float *dst = a.parts == 1 ? a.out + seq.first * a.heads * D + (int64_t)head * D : a.part + unit * (D + 2);
   const float scale = a.parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll

@@ -180,6 +180,25 @@ def test_layout_is_the_stated_one(tmp_path):
     assert int(lines[at + 6][1]) == ((1 << 20) - 1) * 8 * 8 * 2560 + (7 * 8 + 7) * 2560   # beyond 32 bits
 
 
+def test_copies_of_a_ring_land_before_it_is_given_up(tmp_path):
+    """What the attention kernels wait for when a wait ran out (csrc/kv4_ring.h, as plain C++), at every step of rings of every length: the copies that
+    are under way then, each once with the parity of its own step, and no others (a wait for one that was never asked for would last to its limit)."""
+    src = tmp_path / "ring.cpp"
+    src.write_text('#include <cstdio>\n#include "kv4_ring.h"\nint main() {\n  for (int count = 1; count < 9; ++count) {\n    int stage = 0;\n    unsigned phase = 0;\n'
+                   '    for (int k = 0; k < count; ++k) {\n      printf("%d %d :", count, k);\n'
+                   '      cb::ring_land(stage, phase, k + 1 < count, [](int s, unsigned p) { printf(" %d %u", s, p); });\n      puts("");\n'
+                   '      phase ^= stage;\n      stage ^= 1;\n    }\n  }\n}\n')
+    exe = tmp_path / "ring"
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "caten_b200", "csrc"), str(src), "-o", str(exe)], check=True)
+    said = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()
+    want = []
+    for count in range(1, 9):
+        for k in range(count):   # steps before k were used, and for each of them the step two further on was asked for
+            under_way = [j for j in range(count) if j < 2 or j - 2 < k]
+            want.append(f"{count} {k} : " + " ".join(f"{j % 2} {j // 2 % 2}" for j in under_way if j >= k))
+    assert said == want
+
+
 def test_plain_blocks_are_those_of_the_file_format():
     """At values that are not next to a border: the codes of the GGUF package's quantisers, which work in fp32."""
     from gguf import quants
