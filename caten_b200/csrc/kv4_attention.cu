@@ -17,15 +17,13 @@
 
 #include "common.cuh"
 #include "kv4.cuh"
+#include "kv4_plan.h"
 #include "kv4_ring.h"
 #include "tcgen05.cuh"
 
 namespace cb {
 
-__host__ __device__ constexpr int k4_warps(bool shared) { return shared ? 8 : 4; }   // of a block
-constexpr int K4_GROUP = 64;       // tokens at a time with single rows
 __host__ __device__ constexpr int K4_TILES(int chunks) { return chunks == 1 ? 4 : 2; }   // 16 tokens at a time with several
-constexpr int K4_ROWS = 8;
 
 struct Kv4AttnArgs {
   const float *q;
@@ -586,8 +584,6 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
 // Bound by instructions (unpacking, two roundings of p d).  4 heads to a key head of 128, Q4_0: 256 sequences of 768 tokens 84 us (the kernel above
 // 111), 64 of 768 25 (45), 3 of 100001 132 (167: 346 MB, 2.6 TB/s); Q4_1 the last in 147 (186); 32 heads over 16 key heads of 256, 8 sequences of
 // 2900 63 (76).
-constexpr int K2_WARPS = 4;   // of a block; 1 or 4 of them share a unit
-constexpr int K2_ROWS = 4;
 
 template <int NC, bool Q41>
 __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_few_kernel(const Kv4AttnArgs a) {
@@ -922,7 +918,7 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
 // cycle and scheduler), unpacking before the softmax.  All phases by eight warps one after the other: 6.4 and 6.7 k; four warps to unpack: 195 us in place
 // of 135 for 600 tokens over 2000, 32 heads of 128 over 8; two units at a time in registers: 130 in place of 127 (the code no longer fits the
 // instruction cache).  That case 127 us now (tiles of 8 rows 271), 2000 of 25 heads of 64 111 (201), 5 prompts of 333, 16 heads of 128 over 4, 30 (67).
-constexpr int K3_ROWS = 128, K3_THREADS = 512, K3_SOFTMAX = 8, K3_CONVERT = 7;   // (warps)
+constexpr int K3_THREADS = 512, K3_SOFTMAX = 8, K3_CONVERT = 7;   // (warps)
 constexpr float K3_LIFT = 14.0f;   // p is taken times 2^14, its sum with it
 __host__ __device__ constexpr int k3_smem(int chunks, int tile_bytes) { return chunks * (32768 + 2 * 16384 + 2 * 16384) + 2 * 4 * tile_bytes + 1024; }
 // of an operand tile: rows of 64 halves, 128-byte swizzle
@@ -1445,7 +1441,6 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
 // (32 tokens) it is digit j of p d.  Sums are exact; they start at the integer that is 1.5 * 2^23 as a float, and so need no conversion.  A score
 // ends up in one lane (64 tokens: two registers a lane), so softmax and p d are not computed eight times over as by rows that are not there.
 // What it is bound by: instructions, then HBM.  (256 x 25 heads x 768 tokens: 139 us with fp16 operands, 261 instructions for 16 tokens of 64 dims.)
-constexpr int K1_WARPS = 4;      // of a block; 1, 2 or 4 of them share a sequence and key head's tokens
 constexpr int K1_MAGIC = 0x4b400000;
 constexpr float K1_MAGIC_F = 12582912.0f;
 
@@ -1817,7 +1812,6 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
 // The parts of a row into one, a block a row: the parts' weights first, by threads over parts, then threads over dims.  Parts behind what the row's
 // tile sees were not written.
 constexpr int KJ_THREADS = 128;
-constexpr int KJ_PARTS = 1024;   // at most, of a call
 
 __global__ void __launch_bounds__(KJ_THREADS) kv4_attention_join_kernel(const Kv4AttnArgs a) {
   __shared__ float weight[KJ_PARTS], red[2][KJ_THREADS / 32];
@@ -1875,61 +1869,12 @@ __global__ void __launch_bounds__(KJ_THREADS) kv4_attention_join_kernel(const Kv
   }
 }
 
-// How a call is cut: row tiles, and parts of the tokens where row tiles alone leave SMs idle.  By sizes that the host knows.
-struct Kv4Plan {
-  int64_t units;   // row tiles of all sequences and key heads
-  int tile_rows, row_tiles, parts, part_tokens, warps;
-};
-// Whether rows are enough for tiles of 128: 48 a sequence and key head on the average, and 1e8 products of all, below which that kernel's start costs more
-// than it saves.  us in tiles of 8 rows and of 128: 32 rows over 2000 tokens (16 sequences, 8 key heads of 128) 94 and 120, 48 over 300 (64 sequences) 97
-// and 82; 8 prompts of 64, 8 heads of 128, 9.0 and 11.5, one of 256, 12 heads of 64, 10.1 and 17.0; 600 over 2000, 32 heads of 128 over 8, 271 and 127.
-static bool kv4_prompts(const caten_b200_kv4_desc *c, int64_t batch, int64_t rows, int64_t max_length) {
-  return c->dim <= 128 && rows * (c->heads / c->kv_heads) >= 48 * batch && (double)rows * c->heads * (double)max_length * c->dim >= 1e8;
-}
 static int kv4_plan(caten_b200_ctx *ctx, const char *who, const caten_b200_kv4_desc *c, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length, Kv4Plan *p) {
   Kv4Shape s;
   if (int rc = kv4_check(ctx, who, c, &s)) return rc;
   if (batch < 0 || batch > (1 << 24) || rows < 0 || rows > 0x7fffffff || max_new <= 0 || max_length < 0 || max_length > 0x3fffffff) return fail(ctx, CATEN_B200_EINVAL, "%s: bad shape", who);
-  const int64_t group = c->heads / c->kv_heads;
-  if (max_new > (1 << 24) || max_new * group > 0x3fffffff) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: %lld new tokens of a sequence", who, (long long)max_new);
-  p->tile_rows = max_new * group == 1 ? 1 : max_new * group <= K2_ROWS ? K2_ROWS : kv4_prompts(c, batch, rows, max_length) ? K3_ROWS : K4_ROWS;
-  p->row_tiles = (int)((max_new * group + p->tile_rows - 1) / p->tile_rows);
-  if (batch && (int64_t)c->kv_heads * p->row_tiles > 0x7fffffff / batch) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
-  p->units = batch * c->kv_heads * p->row_tiles;
-  const int64_t groups = (max_length + K4_GROUP - 1) / K4_GROUP;
-  int64_t fill, blocks, shares;   // units of work that fill the SMs; units without parts; warps over whom a unit's tokens are dealt
-  if (p->tile_rows == 1) {
-    // A warp each where that is enough (20 warps an SM), and for up to four groups already with four an SM: a second and third warp would have one group
-    // or none (592 of 128 dims: 200 tokens 8.4 us and 10.1, 400 15.4 and 13.5; 2000: 100 tokens 12.2 and 22).  Otherwise four.
-    p->warps = p->units >= 148 * 16 || (groups <= 4 && p->units >= 148 * 4) ? 1 : K1_WARPS;
-    fill = 148 * 20 / p->warps; blocks = p->units; shares = p->warps;
-  } else if (p->tile_rows == K2_ROWS) {
-    // (likewise, with a stage half as long: 1184, 200 tokens 19 us and 24; 592, 200 tokens 15.5 and 13)
-    p->warps = p->units >= 148 * 16 || (groups <= 4 && p->units >= 148 * 8) ? 1 : K2_WARPS;
-    fill = 148 * 48 / p->warps; blocks = p->units; shares = p->warps;
-  } else if (p->tile_rows == K3_ROWS) {
-    p->warps = 1;
-    fill = 148; blocks = p->units; shares = 1;   // (152 tiles over 2000 tokens, 600 rows of 32 heads over 8: 135 us whole, 156 in three parts)
-  } else {
-    p->warps = p->row_tiles >= 4 ? 4 : p->row_tiles >= 2 ? 2 : 1;
-    fill = 148 * 12; blocks = p->units / p->row_tiles * ((p->row_tiles + p->warps - 1) / p->warps); shares = k4_warps(p->warps == 4) / p->warps;
-  }
-  // (blocks of several rows that fill the SMs as they are would only add the join: 5 prompts of up to 333 tokens in such tiles 116 -> 136 us)
-  int64_t parts = !blocks || (p->tile_rows == K4_ROWS && blocks >= 148 * 4) ? 1 : (fill + blocks - 1) / blocks;
-  // A part gives each warp two groups at least.  Single rows of up to four groups a warp are left whole: two groups less take no longer than the join
-  // and its launch (25 heads x 700 tokens 7.2 us in parts, 5.3 whole; 1000 7.2 and 6.2; 1500 7.4 and 7.9).
-  const bool whole = p->tile_rows == 1 && groups <= 4 * shares;
-  // Blocks of two to four rows that fill three quarters of their places on the SMs are cut into no less than eight groups a warp (64 sequences of 8
-  // key heads: 700 tokens 35 us in parts, 25 whole; 10000 229 and 248, with uneven lengths 164 and 220).
-  const bool coarse = p->tile_rows == K2_ROWS && blocks >= 148 * 3;
-  const int64_t most = whole ? 1 : coarse ? groups / (8 * shares) : (groups + 2 * shares - 1) / (2 * shares);
-  if (parts > most) parts = most;
-  if (parts > KJ_PARTS) parts = KJ_PARTS;
-  if (parts < 1) parts = 1;
-  const int64_t each = groups ? (groups + parts - 1) / parts : 1;
-  p->part_tokens = (int)(each * K4_GROUP);
-  p->parts = (int)(groups ? (groups + each - 1) / each : 1);
-  if (p->units * p->parts > 0x7fffffff / std::max(K4_ROWS, p->tile_rows)) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
+  if (max_new > (1 << 24) || max_new * (c->heads / c->kv_heads) > 0x3fffffff) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: %lld new tokens of a sequence", who, (long long)max_new);
+  if (!kv4_plan_of({c->dim, c->kv_heads, c->heads / c->kv_heads}, batch, rows, max_new, max_length, p)) return fail(ctx, CATEN_B200_EUNSUPPORTED, "%s: too many rows", who);
   return 0;
 }
 
@@ -1981,7 +1926,7 @@ extern "C" {
 int64_t caten_b200_kv4_attention_work(const caten_b200_kv4_desc *desc, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length) {
   Kv4Plan p;
   if (kv4_plan(nullptr, "kv4_attention_work", desc, batch, rows, max_new, max_length, &p)) return -1;
-  return p.parts > 1 ? p.units * p.parts * p.tile_rows * (desc->dim + 2) * (int64_t)sizeof(float) : 16;
+  return kv4_work_bound({desc->dim, desc->kv_heads, desc->heads / desc->kv_heads}, batch, max_new, max_length);
 }
 
 int caten_b200_kv4_attention(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, const float *d_q, int64_t ldq, const void *d_pool, const int32_t *d_table,

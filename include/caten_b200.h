@@ -308,8 +308,9 @@ int caten_b200_kv4_load(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, co
  * sequence are left as they were.  max_new: rows of a sequence at most; max_length: bound of the lengths, at most max_pages * page.  Arithmetic: codes are
  * exact operands of tensor-core products, q and the probabilities are split in two fp16 halves (2^-22), sums and softmax fp32.
  * Lengths, starts or page numbers outside what the call allows are cut or skipped and reported (CATEN_B200_EDEVICE) by the next synchronising call.
- * d_work: kv4_attention_work(..) bytes for the same arguments (a smaller call may be cut into more parts and need more), 16-byte aligned, nothing of
- * which is kept from call to call; calls that may overlap on the GPU need one each. */
+ * d_work: kv4_attention_work(..) bytes, 16-byte aligned, nothing of which is kept from call to call; calls that may overlap on the GPU need one each.
+ * What kv4_attention_work says for some sizes is enough for every call of the same heads with sizes up to those: a host that allocates for its
+ * largest batch, max_new and max_length need not ask again. */
 int64_t caten_b200_kv4_attention_work(const caten_b200_kv4_desc *desc, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length);
 int caten_b200_kv4_attention(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, const float *d_q, int64_t ldq, const void *d_pool,
                              const int32_t *d_table, int64_t max_pages, const int32_t *d_lengths, const int32_t *d_starts, int64_t batch, int64_t rows,

@@ -180,6 +180,53 @@ def test_layout_is_the_stated_one(tmp_path):
     assert int(lines[at + 6][1]) == ((1 << 20) - 1) * 8 * 8 * 2560 + (7 * 8 + 7) * 2560   # beyond 32 bits
 
 
+def test_attention_workspace_is_enough_for_every_smaller_call(lib, tmp_path):
+    """A host allocates once, for its largest turn.  The plan that a call is cut by (csrc/kv4_plan.h, as plain C++) needs no more than the stated bytes,
+    whatever smaller sizes it is made for, and the entry point says what that arithmetic says."""
+    src = tmp_path / "plan.cpp"
+    src.write_text('''#include <cmath>
+#include <cstdio>
+#include <random>
+#include "kv4_plan.h"
+using namespace cb;
+int main() {
+  std::mt19937_64 rng(7);
+  auto of = [&](double lo, double hi) { return (int64_t)std::exp(std::uniform_real_distribution<double>(std::log(lo), std::log(hi + 0.99))(rng)); };
+  auto some = [&](int64_t hi) { return hi < 2 || rng() % 4 == 0 ? hi : std::min(hi, of(1, (double)hi)); };
+  int64_t parts[4] = {0, 0, 0, 0}, smaller_needs_more = 0;
+  for (int i = 0; i < 300000; ++i) {
+    const Kv4Heads h = {(int)(64 * (1 + rng() % 4)), (int)of(1, 50), of(1, 16)};
+    const int64_t batch = of(1, 3000), max_new = rng() % 2 ? 1 : of(1, 2000), max_length = of(1, 300000), rows = some(batch * max_new);
+    Kv4Plan p, q;
+    if (!kv4_plan_of(h, batch, rows, max_new, max_length, &p)) continue;
+    const int64_t bound = kv4_work_bound(h, batch, max_new, max_length);
+    const int64_t b = some(batch), n = some(max_new), l = some(max_length), r = some(std::min(rows, b * n));
+    if (!kv4_plan_of(h, b, r, n, l, &q)) { printf("refused\\n"); return 1; }
+    for (const Kv4Plan *x : {&p, &q}) {
+      if (kv4_plan_bytes(*x, h.dim) > bound) {
+        printf("dim %d heads %d x %lld: %lld bytes for batch %lld rows %lld new %lld length %lld (tiles of %d), %lld stated for %lld %lld %lld\\n", h.dim, h.kv_heads, (long long)h.group,
+               (long long)kv4_plan_bytes(*x, h.dim), (long long)b, (long long)r, (long long)n, (long long)l, x->tile_rows, (long long)bound, (long long)batch, (long long)max_new, (long long)max_length);
+        return 1;
+      }
+      if (x->parts > 1) ++parts[x->tile_rows == 1 ? 0 : x->tile_rows == K2_ROWS ? 1 : x->tile_rows == K4_ROWS ? 2 : 3];
+    }
+    smaller_needs_more += kv4_plan_bytes(q, h.dim) > kv4_plan_bytes(p, h.dim);
+    if (kv4_work_bound(h, b, n, l) > bound) { printf("not monotonic\\n"); return 1; }
+  }
+  printf("%lld %lld %lld %lld %lld\\n", (long long)parts[0], (long long)parts[1], (long long)parts[2], (long long)parts[3], (long long)smaller_needs_more);
+  for (int64_t batch : {1, 7, 300}) for (int64_t n : {1, 2, 40}) for (int64_t l : {1, 700, 5000}) printf("%lld\\n", (long long)kv4_work_bound({128, 8, 2}, batch, n, l));
+}
+''')
+    exe = tmp_path / "plan"
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", os.path.join(ROOT, "caten_b200", "csrc"), str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout
+    seen, *said = r.stdout.splitlines()
+    assert min(map(int, seen.split())) > 100   # every kernel with parts; smaller calls that need more than the larger one itself
+    d = desc(dim=128, heads=16, kv_heads=8)
+    assert [lib.caten_b200_kv4_attention_work(C.byref(d), b, b * n, n, ln) for b in (1, 7, 300) for n in (1, 2, 40) for ln in (1, 700, 5000)] == [int(x) for x in said]
+
+
 def test_copies_of_a_ring_land_before_it_is_given_up(tmp_path):
     """What the attention kernels wait for when a wait ran out (csrc/kv4_ring.h, as plain C++), at every step of rings of every length: the copies that
     are under way then, each once with the parity of its own step, and no others (a wait for one that was never asked for would last to its limit)."""
