@@ -481,7 +481,10 @@ extern "C" {
 // Arguments are checked before the context is touched.
 int64_t caten_b200_beam_select_work(int64_t batch, int64_t beams, int64_t V, int64_t keep) {
   if (beam_check(nullptr, "beam_select_work", batch, beams, V, keep)) return -1;
-  return (batch * beams * beam_chunks(batch, beams, V) * beam_part_words((int)keep) + 1) * (int64_t)sizeof(u64);
+  // Enough for every call of sizes up to these: fewer rows, or a smaller V, may go in chunks of 2048, but only as long as the larger ones, of which
+  // each is four at most, would be fewer than 148.
+  const int64_t rows = batch * beams, parts = std::max(rows * ((V + 3 + 8191) / 8192), std::min<int64_t>(rows * ((V + 3 + 2047) / 2048), 4 * 147));
+  return (parts * beam_part_words((int)keep) + 1) * (int64_t)sizeof(u64);
 }
 
 int caten_b200_beam_select(caten_b200_ctx *ctx, const float *d_logits, const float *d_scores, const uint8_t *d_ended, int64_t batch, int64_t beams, int64_t V,

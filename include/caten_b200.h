@@ -249,7 +249,7 @@ int caten_b200_rope(caten_b200_ctx *ctx, const float *d_x, float *d_y, int64_t B
  * or +inf) are never taken; place i that none is left for has score -inf, parent min(i, beams - 1) and token eos (0 without one).
  * beams, keep <= 32; V <= 1040384; batch * beams <= 65535; eos < 0: none (d_ended NULL).  Outputs [batch, keep]; they do not overlap the inputs.
  * d_work: beam_select_work(..) bytes, 8-byte aligned, nothing of which is kept from call to call; calls that may overlap on the GPU need one
- * each.  beam_select_work is -1 for a call that would be refused. */
+ * each.  What beam_select_work says for some sizes is enough for every call with sizes up to those; it is -1 for a call that would be refused. */
 int64_t caten_b200_beam_select_work(int64_t batch, int64_t beams, int64_t V, int64_t keep);
 int caten_b200_beam_select(caten_b200_ctx *ctx, const float *d_logits, const float *d_scores, const uint8_t *d_ended, int64_t batch, int64_t beams,
                            int64_t V, int64_t eos, int64_t keep, float *d_out_scores, int32_t *d_out_parents, int64_t *d_out_tokens,

@@ -227,6 +227,23 @@ int main() {
     assert [lib.caten_b200_kv4_attention_work(C.byref(d), b, b * n, n, ln) for b in (1, 7, 300) for n in (1, 2, 40) for ln in (1, 700, 5000)] == [int(x) for x in said]
 
 
+def test_selection_workspace_is_enough_for_every_smaller_call(lib):
+    """A host allocates once, for its largest batch, and calls with what is left of it."""
+    work = lib.caten_b200_beam_select_work
+    for V in (50257, 1003, 130001):
+        for beams, keep in ((7, 16), (1, 1), (32, 32)):
+            said = [work(batch, beams, V, keep) for batch in range(1, 400)]
+            assert said == sorted(said)
+            for batch, n in zip(range(1, 400), said):   # in chunks of 2048 logits as long as those of 8192 are fewer than 148, and the request's lists at most 4096
+                few = batch * beams * -(-(V + 3) // 8192) < 148 and beams * -(-(V + 3) // 2048) <= 4096
+                assert n >= 8 * (keep + 1) * batch * beams * -(-(V + 3) // (2048 if few else 8192))
+    rng = np.random.Generator(np.random.PCG64(9))
+    for _ in range(3000):
+        large = [int(np.exp(rng.uniform(0, np.log(x)))) for x in (500, 32, 1040384, 32)]
+        small = [int(rng.integers(1, x + 1)) for x in large]
+        assert work(*small) <= work(*large)
+
+
 def test_copies_of_a_ring_land_before_it_is_given_up(tmp_path):
     """What the attention kernels wait for when a wait ran out (csrc/kv4_ring.h, as plain C++), at every step of rings of every length: the copies that
     are under way then, each once with the parity of its own step, and no others (a wait for one that was never asked for would last to its limit)."""
