@@ -217,12 +217,15 @@ constexpr int BJ_BEAMS = 32;
 constexpr int BJ_LISTS = 4096;   // of a request: beams x chunks
 constexpr int BJ_FOUND = BS_KEEP * BS_KEEP;
 
-// A candidate: the order-preserving image of its value, and b * V + token; larger: earlier in the result.
+// A candidate: the order-preserving images of its value and, for equal values, of its beam (lower), its logit and its token (lower): larger ones come
+// first.  (Beside a score of -1e30, or the lowest value as a mask, all of a beam's values are one number; what its logits say still counts.)
 struct __align__(16) Cand {
-  u64 value;
-  uint32_t id;
-  __device__ __forceinline__ bool operator>(const Cand &o) const { return value > o.value || (value == o.value && id < o.id); }
+  u64 value, tie;
+  __device__ __forceinline__ bool operator>(const Cand &o) const { return value > o.value || (value == o.value && tie > o.tie); }
+  __device__ __forceinline__ int beam() const { return BJ_BEAMS - 1 - (int)(tie >> 52); }
+  __device__ __forceinline__ int64_t token() const { return 0xfffff - (int64_t)(tie & 0xfffff); }
 };
+__device__ __forceinline__ u64 cand_tie(int beam, u64 key) { return (u64)(BJ_BEAMS - 1 - beam) << 52 | (key >> 32) << 20 | (u64)(0xfffff - beam_key_index(key)); }
 
 __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__restrict__ parts, int chunks, const float *__restrict__ scores, const uint8_t *__restrict__ ended,
                                                                int beams, int64_t V, int64_t eos, int keep, float *__restrict__ out_scores, int *__restrict__ out_parents,
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
   const int64_t words = beam_part_words(keep);
   const int lists = beams * chunks;
   const u64 *mine = parts + batch * lists * words;
-  if (tid == 0) { bound = {1, 0xffffffffu}; count = 0; queued = 0; }   // (that bound: every candidate)
+  if (tid == 0) { bound = {1, 0}; count = 0; queued = 0; }   // (that bound: every candidate)
   const u64 head = tid < min(lists, BJ_HEADS) ? mine[(int64_t)tid * words] : 0ull;     // (of an ended hypothesis: whatever is there, unused)
   for (int b = warp; b < beams; b += BJ_THREADS / 32) {
     const int64_t row = batch * beams + b;
@@ -273,8 +276,8 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
   auto cand_of = [&](int i, int j, u64 key) -> Cand {   // entry j of list i
     const int b = i / chunks;
     if (over[b])   // its one candidate stands first in its first list
-      return {i == b * chunks && j == 0 && eos >= 0 ? order_of(base[b]) : 0ull, (uint32_t)(b * V + eos)};
-    return {key ? order_of(base[b] + ((double)beam_key_value(key) - tops[b])) : 0ull, (uint32_t)(b * V + beam_key_index(key))};
+      return {i == b * chunks && j == 0 && eos >= 0 ? order_of(base[b]) : 0ull, cand_tie(b, (u64)~(uint32_t)eos)};
+    return {key ? order_of(base[b] + ((double)beam_key_value(key) - tops[b])) : 0ull, cand_tie(b, key)};
   };
   auto entry = [&](int i, int j) { return cand_of(i, j, mine[(int64_t)i * words + j]); };
   // for each i of the n found: then(candidate, how many are before it), by one of the threads that count them
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
   };
   // The keep-th of the lists' first entries: `keep` candidates are not behind it, and at most `keep` lists have any that are not.  Where a thread
   // has several lists, the threads' best give a first bound, and the few first entries that it leaves the second.
-  Cand best = tid < min(lists, BJ_HEADS) ? cand_of(tid, 0, head) : Cand{0ull, 0xffffffffu};
+  Cand best = tid < min(lists, BJ_HEADS) ? cand_of(tid, 0, head) : Cand{0ull, 0ull};
   if (tid < BJ_HEADS) {
     for (int i = tid + BJ_HEADS; i < lists; i += BJ_HEADS) {
       const Cand c = entry(i, 0);
@@ -338,8 +341,8 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
   __syncthreads();
   auto write = [&](int place, bool there, const Cand &c) {
     const int64_t at = batch * keep + place;
-    const int parent = there ? (int)(c.id / (uint32_t)V) : min(place, beams - 1);
-    const int64_t token = there ? (int64_t)(c.id % (uint32_t)V) : eos >= 0 ? eos : 0;
+    const int parent = there ? c.beam() : min(place, beams - 1);
+    const int64_t token = there ? c.token() : eos >= 0 ? eos : 0;
     out_scores[at] = there ? (float)value_of(c.value) : -INFINITY;
     out_parents[at] = parent;
     out_tokens[at] = token;
@@ -349,11 +352,12 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
   for_places(n, [&](const Cand &c, int place) {
     if (place < keep) write(place, true, c);
   });
-  if (tid >= n && tid < keep) write(tid, false, Cand{0ull, 0u});
+  if (tid >= n && tid < keep) write(tid, false, Cand{0ull, 0ull});
 }
 
 // Chunks of 8192 logits, or of 2048 where the larger ones would not give every SM a block.
 constexpr int64_t BS_VOCAB = (1 << 20) - 8192;
+static_assert(BS_VOCAB <= 0xfffff, "a candidate has 20 bits for its token");
 static_assert(BJ_BEAMS * ((BS_VOCAB + 3 + 8191) / 8192) <= BJ_LISTS && BS_KEEP * (BJ_LISTS / BJ_HEADS) <= BJ_FOUND, "lists of a request");
 static int beam_vecs(int64_t batch, int64_t beams, int64_t V) {
   return batch * beams * ((V + 3 + 8191) / 8192) >= 148 || beams * ((V + 3 + 2047) / 2048) > BJ_LISTS ? 8 : 2;

@@ -244,9 +244,10 @@ int caten_b200_rope(caten_b200_ctx *ctx, const float *d_x, float *d_y, int64_t B
  * One step of `batch` requests with `beams` hypotheses each: d_logits [batch * beams, V], d_scores [batch, beams] the hypotheses' sums of
  * log probabilities so far.  Candidate (beam b, token v) has the value score_b + x_v - log(sum exp(x)); a hypothesis whose d_ended byte is not 0
  * (NULL: none) has one candidate, (b, eos) with the value score_b, and its logits are not read.  Writes the `keep` candidates of largest value,
- * equal ones in the order of b * V + v: values rounded to fp32, the beam each goes on from, its token, and (d_out_ended not NULL) whether it has
- * ended.  The order is decided in 64 bits.  Candidates whose value is -inf or NaN (masked tokens, hypotheses with score -inf, rows with a NaN
- * or +inf) are never taken; place i that none is left for has score -inf, parent min(i, beams - 1) and token eos (0 without one).
+ * equal ones in the order of b * V + v (a beam's own are equal where their logits are, also where a score like -1e30 leaves no room for logits in a
+ * value): values rounded to fp32, the beam each goes on from, its token, and (d_out_ended not NULL) whether it has ended.  The order is decided in 64
+ * bits.  Candidates whose value is -inf or NaN (masked tokens, hypotheses with score -inf, rows with a NaN or +inf) are never taken; place i
+ * that none is left for has score -inf, parent min(i, beams - 1) and token eos (0 without one).
  * beams, keep <= 32; V <= 1040384; batch * beams <= 65535; eos < 0: none (d_ended NULL).  Outputs [batch, keep]; they do not overlap the inputs.
  * d_work: beam_select_work(..) bytes, 8-byte aligned, nothing of which is kept from call to call; calls that may overlap on the GPU need one
  * each.  What beam_select_work says for some sizes is enough for every call with sizes up to those; it is -1 for a call that would be refused. */

@@ -105,7 +105,10 @@ def select(logits, scores, ended, eos, keep):
             value[b] = -np.inf
             value[b, eos] = scores[b]
     value = np.where(np.isnan(value), -np.inf, value).reshape(-1)
-    order = np.argsort(-value, kind="stable")[:keep]
+    x, order = x.reshape(-1), np.argsort(-value, kind="stable")
+    last = value[order[min(keep, len(order)) - 1]]
+    order = np.flatnonzero(value >= last)   # where values of a beam coincide in 64 bits, its logits say which is larger
+    order = order[np.lexsort((order, -x[order], order // V, -value[order]))][:keep]
     order = [i for i in order if value[i] > -np.inf]
     parents = [i // V for i in order] + [min(i, beams - 1) for i in range(len(order), keep)]
     tokens = [i % V for i in order] + [max(eos, 0)] * (keep - len(order))

@@ -565,6 +565,17 @@ def test_selection_of_equal_values_takes_the_lowest_index(rt):
         check_select(rt, np.zeros((groups, beams, V)), np.zeros((groups, beams)), 32)
 
 
+@pytest.mark.parametrize("score", [-1e30, float(np.finfo(np.float32).min)])
+@pytest.mark.parametrize("groups,beams,V,keep", [(2, 3, 5000, 32), (20, 8, 9001, 16), (1, 4, 40, 20)])
+def test_selection_from_scores_that_leave_no_room_for_logits(rt, groups, beams, V, keep, score):
+    """Hypotheses kept out by a very low score, all of whose candidates have one value in 64 bits: in the order of their beams, and of a beam's
+    logits."""
+    rng = rng_of(groups, beams, V)
+    x = rng.integers(-40, 40, (groups, beams, V)).astype(np.float32) / 4
+    check_select(rt, x, np.full((groups, beams), score), keep)
+    check_select(rt, x, np.where(np.arange(beams) == 1, 0.0, score) + np.zeros((groups, 1)), keep, ended=np.arange(groups * beams).reshape(groups, beams) % 5 == 0, eos=3)
+
+
 @pytest.mark.parametrize("order", ["up", "down"])
 def test_selection_from_sorted_logits(rt, order):
     """The largest logits lie side by side, in one block's share."""
