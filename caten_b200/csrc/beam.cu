@@ -3,12 +3,15 @@
 //
 // Selection.  Candidate (beam b, token v) has the value score_b + x_bv - lse_b, lse_b = max + log(sum exp(x - max)); the first `keep` by value,
 // equal ones by b * V + v.  Within a beam that order is the order of the logits, so a pass over the logits needs no lse: each block reads a chunk
-// of a row once into registers and leaves its maximum, its sum of exponentials and its `keep` largest logits; a second kernel joins the
-// chunks' sums in 64 bits, turns the few logits left into values and picks among them.  Both pick by a bound first: `keep` values
+// of a row once into registers and leaves its maximum, its sum of exponentials (fp32) and its `keep` largest logits; a second kernel joins the
+// chunks' sums, turns the few logits left into values and picks among them; where the sums' errors could decide between beams it makes those rows' sums
+// in 64 bits, by a second pass over them, and picks again.  Both pick by a bound first: `keep` values
 // are not behind the `keep`-th of disjoint groups' largest, and with a few dozen candidates left each counts those before it, which is its place.
 // Bound by instructions and the barriers of the ranking: 64 x 8 beams over 50257 logits 34 us, 26 of them the chunks (79 MB at 3 TB/s; a quarter has
-// ended), 8 the join; one group of 4 beams 8.3 us, two dependent launches.
+// ended), 8 the join; one group of 4 beams 8.7 us, two dependent launches.  Rows summed again (of random logits, 16 kept of 8 beams: in one request of
+// some hundreds) take 13 us each, most of it exp in 64 bits on one SM.
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "kv4.cuh"
@@ -89,7 +92,8 @@ __host__ __device__ __forceinline__ int64_t beam_part_words(int keep) { return k
 template <int VECS>
 __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__restrict__ x, const uint8_t *__restrict__ ended, int64_t V, int keep, u64 *__restrict__ parts) {
   constexpr int CHUNK = BS_THREADS * VECS * 4;
-  __shared__ float group_top[32], sums[BS_THREADS / 32];
+  __shared__ float group_top[32];
+  __shared__ double sums[BS_THREADS / 32];
   __shared__ u64 lists[BS_THREADS / 32][32], answer;
   __shared__ u64 found[BS_FEW * VECS * 4];
   __shared__ float kth_top;
@@ -143,16 +147,20 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
   }
   // sum of exponentials; a maximum of -inf (nothing left) makes it 0, a NaN or +inf makes it NaN
   const float base = m == -INFINITY ? 0.0f : m;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  float q[VECS];
 #pragma unroll
-  for (int i = 0; i < VECS; ++i)
+  for (int i = 0; i < VECS; ++i) {
+    float e[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float e;
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((v[i][j] - base) * 1.4426950408889634f));
-      s[j] += e;
-    }
-  float sum = warp_sum((s[0] + s[1]) + (s[2] + s[3]));
+    for (int j = 0; j < 4; ++j) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[j]) : "f"((v[i][j] - base) * 1.4426950408889634f));
+    q[i] = (e[0] + e[1]) + (e[2] + e[3]);
+#pragma unroll
+    for (int k = 1; k < VECS; k <<= 1)   // (in pairs: five roundings for 32 logits)
+      if ((i & (2 * k - 1)) == 2 * k - 1) q[i] += q[i - k];
+  }
+  double sum = q[VECS - 1];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) sums[warp] = sum;
   __syncthreads();
   const float least = kth_top;
@@ -198,7 +206,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_chunk_kernel(const float *__r
     sum = sums[0];
 #pragma unroll
     for (int w = 1; w < BS_THREADS / 32; ++w) sum += sums[w];
-    part[keep] = (u64)__float_as_uint(base) << 32 | __float_as_uint(m < INFINITY ? sum : NAN);
+    part[keep] = (u64)__float_as_uint(base) << 32 | __float_as_uint(m < INFINITY ? (float)sum : NAN);
   }
 }
 
@@ -216,6 +224,7 @@ constexpr int BJ_LANES = 16;     // threads that find one candidate's place
 constexpr int BJ_BEAMS = 32;
 constexpr int BJ_LISTS = 4096;   // of a request: beams x chunks
 constexpr int BJ_FOUND = BS_KEEP * BS_KEEP;
+constexpr int BJ_QUEUE = 64;
 
 // A candidate: the order-preserving images of its value and, for equal values, of its beam (lower), its logit and its token (lower): larger ones come
 // first.  (Beside a score of -1e30, or the lowest value as a mask, all of a beam's values are one number; what its logits say still counts.)
@@ -227,26 +236,139 @@ struct __align__(16) Cand {
 };
 __device__ __forceinline__ u64 cand_tie(int beam, u64 key) { return (u64)(BJ_BEAMS - 1 - beam) << 52 | (key >> 32) << 20 | (u64)(0xfffff - beam_key_index(key)); }
 
-__global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__restrict__ parts, int chunks, const float *__restrict__ scores, const uint8_t *__restrict__ ended,
-                                                               int beams, int64_t V, int64_t eos, int keep, float *__restrict__ out_scores, int *__restrict__ out_parents,
-                                                               int64_t *__restrict__ out_tokens, uint8_t *__restrict__ out_ended) {
-  __shared__ double base[BJ_BEAMS], tops[BJ_BEAMS];   // a candidate's value: base + (x - top)
-  __shared__ uint8_t over[BJ_BEAMS];
-  __shared__ Cand found[BJ_FOUND], bound;
-  __shared__ int queue[BS_KEEP];
-  __shared__ int count, queued;
+struct JoinArgs {
+  const u64 *parts;
+  const float *x, *scores;
+  const uint8_t *ended;
+  float *out_scores;
+  int *out_parents;
+  int64_t *out_tokens;
+  uint8_t *out_ended;
+  int64_t V, eos;
+  int chunks, beams, keep;
+  float close;
+};
+struct JoinShared {
+  __align__(128) Cand found[BJ_FOUND];
+  Cand taken[BS_KEEP], bound;
+  double base[BJ_BEAMS], tops[BJ_BEAMS];   // a candidate's value: base + (x - top)
+  double sums[BJ_THREADS / 32];
+  uint8_t over[BJ_BEAMS];
+  int queue[BJ_QUEUE];
+  int count, queued;
+  unsigned close_beams;
+
+  // Candidates of different beams whose values, by the chunks' sums, are no farther apart than this may be in either order: by what the sums may be off,
+  // and what the additions of a value in 64 bits round off.
+  __device__ __forceinline__ double close_to(const JoinArgs &a, double value) const { return a.close + fabs(value) * 0x1p-50; }
+  __device__ __forceinline__ Cand cand_of(const JoinArgs &a, int i, int j, u64 key) const {   // entry j of list i
+    const int b = i / a.chunks;
+    if (over[b])   // its one candidate stands first in its first list
+      return {i == b * a.chunks && j == 0 && a.eos >= 0 ? order_of(base[b]) : 0ull, cand_tie(b, (u64)~(uint32_t)a.eos)};
+    return {key ? order_of(base[b] + ((double)beam_key_value(key) - tops[b])) : 0ull, cand_tie(b, key)};
+  }
+  // a found candidate's value by what base[] is now
+  __device__ __forceinline__ u64 value_at(const JoinArgs &a, const Cand &c) const {
+    const int b = c.beam();
+    return order_of(over[b] ? base[b] : base[b] + ((double)beam_key_value(c.tie >> 20 << 32) - tops[b]));
+  }
+  __device__ __forceinline__ void write(const JoinArgs &a, int place, bool there, const Cand &c) const {
+    const int64_t at = (int64_t)blockIdx.x * a.keep + place;
+    const int parent = there ? c.beam() : min(place, a.beams - 1);
+    const int64_t token = there ? c.token() : a.eos >= 0 ? a.eos : 0;
+    a.out_scores[at] = there ? (float)value_of(c.value) : -INFINITY;
+    a.out_parents[at] = parent;
+    a.out_tokens[at] = token;
+    if (a.out_ended) a.out_ended[at] = over[parent] || (a.eos >= 0 && token == a.eos);
+  }
+};
+
+// Sums of the given beams' rows in 64 bits, each in an order that depends on V alone (equal rows have equal sums), and the places of the n candidates
+// found anew; n < 0: too many were close to look at, so all lists give their best, one after another.  Rarely needed, and a function of its own:
+// inside the kernel it cost every call 0.4 us of registers and of instructions to fetch.
+__device__ __noinline__ void beam_join_exactly(const JoinArgs &a, JoinShared &sh) {
+  const int n = sh.queued > BJ_QUEUE || sh.count > BJ_FOUND ? -1 : sh.count;
+  const unsigned beams = n < 0 ? ~0u : sh.close_beams;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int b = 0; b < a.beams; ++b) {
+    if (!(beams >> b & 1) || sh.over[b]) continue;
+    const int64_t row = (int64_t)blockIdx.x * a.beams + b;
+    const float *x = a.x + row * a.V;
+    const double top = sh.tops[b];
+    double s = 0.0;
+#pragma unroll 8
+    for (int64_t i = tid; i < a.V; i += BJ_THREADS) s += exp((double)x[i] - top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) sh.sums[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+      s = sh.sums[lane];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0) sh.base[b] = (double)a.scores[row] - log(s);
+    }
+    __syncthreads();
+  }
+  if (n >= 0) {
+    for (int i = tid; i < n; i += BJ_THREADS) sh.found[i].value = sh.value_at(a, sh.found[i]);
+    __syncthreads();
+    for (int i = tid; i < n; i += BJ_THREADS) {
+      const Cand c = sh.found[i];
+      int place = 0;
+      for (int j = 0; j < n; ++j) place += sh.found[j] > c;
+      if (place < a.keep) sh.write(a, place, true, c);
+    }
+    return;
+  }
+  Cand *warps = sh.found;                                                  // their best
+  uint8_t *next = reinterpret_cast<uint8_t *>(sh.found + BJ_THREADS / 32);   // of each list, of which a thread has several
+  const int lists = a.beams * a.chunks;
+  const u64 *mine = a.parts + (int64_t)blockIdx.x * lists * beam_part_words(a.keep);
+  for (int i = tid; i < lists; i += BJ_THREADS) next[i] = 0;
+  for (int place = 0; place < a.keep; ++place) {
+    Cand best = {0ull, 0ull};
+    int of = 0;
+    for (int i = tid; i < lists; i += BJ_THREADS) {
+      if (next[i] == a.keep) continue;
+      const Cand c = sh.cand_of(a, i, next[i], mine[i * beam_part_words(a.keep) + next[i]]);
+      if (c.value && c > best) { best = c; of = i; }
+    }
+    Cand most = best;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Cand other = {__shfl_xor_sync(0xffffffffu, most.value, o), __shfl_xor_sync(0xffffffffu, most.tie, o)};
+      if (other > most) most = other;
+    }
+    if (lane == 0) warps[warp] = most;
+    __syncthreads();
+    for (int w = 0; w < BJ_THREADS / 32; ++w)
+      if (warps[w] > most) most = warps[w];
+    __syncthreads();
+    if (!most.value) {
+      if (tid == 0) sh.write(a, place, false, most);
+    } else if (best.value == most.value && best.tie == most.tie) {   // (one thread's)
+      sh.write(a, place, true, best);
+      ++next[of];
+    }
+  }
+}
+
+__global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_constant__ JoinArgs a) {
+  __shared__ JoinShared sh;
   pdl_enter();
   const int64_t batch = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int keep = a.keep, chunks = a.chunks;
   const int64_t words = beam_part_words(keep);
-  const int lists = beams * chunks;
-  const u64 *mine = parts + batch * lists * words;
-  if (tid == 0) { bound = {1, 0}; count = 0; queued = 0; }   // (that bound: every candidate)
+  const int lists = a.beams * chunks;
+  const u64 *mine = a.parts + batch * lists * words;
+  if (tid == 0) { sh.bound = {1, 0}; sh.count = 0; sh.queued = 0; sh.close_beams = 0; }   // (that bound: every candidate)
   const u64 head = tid < min(lists, BJ_HEADS) ? mine[(int64_t)tid * words] : 0ull;     // (of an ended hypothesis: whatever is there, unused)
-  for (int b = warp; b < beams; b += BJ_THREADS / 32) {
-    const int64_t row = batch * beams + b;
-    const float score = scores[row];
-    const bool end = ended && ended[row];
+  for (int b = warp; b < a.beams; b += BJ_THREADS / 32) {
+    const int64_t row = batch * a.beams + b;
+    const float score = a.scores[row];
+    const bool end = a.ended && a.ended[row];
     double log_sum = 0.0, top = 0.0;
     if (!end) {
       const u64 *part = mine + (int64_t)b * chunks * words + keep;
@@ -267,101 +389,114 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const u64 *__rest
       top = (double)m;
     }
     if (lane == 0) {
-      base[b] = (double)score - log_sum;
-      tops[b] = top;
-      over[b] = end;
+      sh.base[b] = (double)score - log_sum;
+      sh.tops[b] = top;
+      sh.over[b] = end;
     }
   }
   __syncthreads();
-  auto cand_of = [&](int i, int j, u64 key) -> Cand {   // entry j of list i
-    const int b = i / chunks;
-    if (over[b])   // its one candidate stands first in its first list
-      return {i == b * chunks && j == 0 && eos >= 0 ? order_of(base[b]) : 0ull, cand_tie(b, (u64)~(uint32_t)eos)};
-    return {key ? order_of(base[b] + ((double)beam_key_value(key) - tops[b])) : 0ull, cand_tie(b, key)};
-  };
-  auto entry = [&](int i, int j) { return cand_of(i, j, mine[(int64_t)i * words + j]); };
+  auto entry = [&](int i, int j) { return sh.cand_of(a, i, j, mine[(int64_t)i * words + j]); };
   // for each i of the n found: then(candidate, how many are before it), by one of the threads that count them
   auto for_places = [&](int n, auto then) {
     for (int i0 = 0; i0 < n; i0 += BJ_THREADS / BJ_LANES) {
       const int i = i0 + tid / BJ_LANES;
-      const Cand c = found[min(i, n - 1)];
+      const Cand c = sh.found[min(i, n - 1)];
       int place = 0;
 #pragma unroll 4
-      for (int j = tid % BJ_LANES; j < n; j += BJ_LANES) place += found[j] > c;
+      for (int j = tid % BJ_LANES; j < n; j += BJ_LANES) place += sh.found[j] > c;
 #pragma unroll
       for (int o = 1; o < BJ_LANES; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
       if (i < n && tid % BJ_LANES == 0) then(c, place);
     }
   };
   // The keep-th of the lists' first entries: `keep` candidates are not behind it, and at most `keep` lists have any that are not.  Where a thread
-  // has several lists, the threads' best give a first bound, and the few first entries that it leaves the second.
-  Cand best = tid < min(lists, BJ_HEADS) ? cand_of(tid, 0, head) : Cand{0ull, 0ull};
+  // has several lists, the threads' best give a first bound, and the few first entries that it leaves the second.  The last bound is lowered by
+  // what a value may be off, so that whatever could change places with one that is taken is found too.
+  Cand best = tid < min(lists, BJ_HEADS) ? sh.cand_of(a, tid, 0, head) : Cand{0ull, 0ull};
   if (tid < BJ_HEADS) {
     for (int i = tid + BJ_HEADS; i < lists; i += BJ_HEADS) {
       const Cand c = entry(i, 0);
       if (c > best) best = c;
     }
-    found[tid] = best;
+    sh.found[tid] = best;
   }
   __syncthreads();
+  auto lowered = [&](const Cand &c) { return Cand{max(1ull, order_of(value_of(c.value) - sh.close_to(a, value_of(c.value)))), 0ull}; };
   for_places(min(lists, BJ_HEADS), [&](const Cand &c, int place) {
-    if (c.value && place == keep - 1) bound = c;
+    if (c.value && place == keep - 1) sh.bound = lists > BJ_HEADS ? c : lowered(c);
   });
   __syncthreads();
   if (lists > BJ_HEADS) {
-    const Cand first = bound;
+    const Cand first = sh.bound;
     __syncthreads();
     for (int i = tid; i < lists; i += BJ_THREADS) {
       const Cand c = entry(i, 0);
-      if (c.value && !(first > c)) found[atomicAdd(&count, 1)] = c;   // (of at most `keep` threads, 16 lists each)
+      if (c.value && !(first > c)) sh.found[atomicAdd(&sh.count, 1)] = c;   // (of at most `keep` threads, 16 lists each)
     }
     __syncthreads();
-    const int n = count;
+    const int n = sh.count;
     for_places(n, [&](const Cand &c, int place) {
-      if (place == keep - 1) bound = c;
+      if (place == keep - 1) sh.bound = lowered(c);
     });
     __syncthreads();
-    if (tid == 0) count = 0;
+    if (tid == 0) sh.count = 0;
   }
-  const Cand least = bound;
+  const u64 least = sh.bound.value;
   __syncthreads();
+  auto enqueue = [&](int i) {
+    const int at = atomicAdd(&sh.queued, 1);
+    if (at < BJ_QUEUE) sh.queue[at] = i;
+  };
   if (lists <= BJ_HEADS) {
-    if (best.value && !(least > best)) queue[atomicAdd(&queued, 1)] = tid;
+    if (best.value >= least) enqueue(tid);
   } else {
-    for (int i = tid; i < lists; i += BJ_THREADS) {
-      const Cand c = entry(i, 0);
-      if (c.value && !(least > c)) queue[atomicAdd(&queued, 1)] = i;
+    for (int i = tid; i < lists; i += BJ_THREADS)
+      if (entry(i, 0).value >= least) enqueue(i);
+  }
+  __syncthreads();
+  for (int i = tid; i < min(sh.queued, BJ_QUEUE) * keep; i += BJ_THREADS) {
+    const Cand c = entry(sh.queue[i / keep], i % keep);
+    if (c.value >= least) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < BJ_FOUND) sh.found[at] = c;
     }
   }
   __syncthreads();
-  for (int i = tid; i < queued * keep; i += BJ_THREADS) {
-    const Cand c = entry(queue[i / keep], i % keep);
-    if (c.value && !(least > c)) found[atomicAdd(&count, 1)] = c;
+  const int n = min(sh.count, BJ_FOUND);
+  for_places(n, [&](const Cand &c, int place) {
+    if (place >= keep) return;
+    sh.write(a, place, true, c);
+    sh.taken[place] = c;
+  });
+  if (tid >= n && tid < keep) sh.write(a, tid, false, Cand{0ull, 0ull});
+  __syncthreads();
+  if (tid / BJ_LANES < min(n, keep)) {   // each that was taken, and whatever of other beams is close to it
+    const Cand c = sh.taken[tid / BJ_LANES];
+    const double value = value_of(c.value), apart = sh.close_to(a, value);
+    const u64 from = order_of(value - apart), to = order_of(value + apart);
+    unsigned close = 0;
+    for (int j = tid % BJ_LANES; j < n; j += BJ_LANES) {
+      const u64 v = sh.found[j].value;
+      if (v >= from && v <= to) close |= 1u << sh.found[j].beam();
+    }
+    if (close & ~(1u << c.beam())) atomicOr(&sh.close_beams, close | 1u << c.beam());
   }
   __syncthreads();
-  auto write = [&](int place, bool there, const Cand &c) {
-    const int64_t at = batch * keep + place;
-    const int parent = there ? c.beam() : min(place, beams - 1);
-    const int64_t token = there ? c.token() : eos >= 0 ? eos : 0;
-    out_scores[at] = there ? (float)value_of(c.value) : -INFINITY;
-    out_parents[at] = parent;
-    out_tokens[at] = token;
-    if (out_ended) out_ended[at] = over[parent] || (eos >= 0 && token == eos);
-  };
-  const int n = count;
-  for_places(n, [&](const Cand &c, int place) {
-    if (place < keep) write(place, true, c);
-  });
-  if (tid >= n && tid < keep) write(tid, false, Cand{0ull, 0ull});
+  if (sh.close_beams || sh.queued > BJ_QUEUE || sh.count > BJ_FOUND) beam_join_exactly(a, sh);
 }
 
 // Chunks of 8192 logits, or of 2048 where the larger ones would not give every SM a block.
 constexpr int64_t BS_VOCAB = (1 << 20) - 8192;
+static_assert(BS_KEEP * BJ_LANES <= BJ_THREADS, "a pass for those taken");
 static_assert(BS_VOCAB <= 0xfffff, "a candidate has 20 bits for its token");
 static_assert(BJ_BEAMS * ((BS_VOCAB + 3 + 8191) / 8192) <= BJ_LISTS && BS_KEEP * (BJ_LISTS / BJ_HEADS) <= BJ_FOUND, "lists of a request");
 static int beam_vecs(int64_t batch, int64_t beams, int64_t V) {
   return batch * beams * ((V + 3 + 8191) / 8192) >= 148 || beams * ((V + 3 + 2047) / 2048) > BJ_LISTS ? 8 : 2;
 }
+// How far apart two rows' log sums may be in fp32 and equal in truth: a sum's relative error is, in units of 2^-24, that of the exponents, 2.23 of each (two
+// roundings and the constant's), of which the sum of p (max - x) is the entropy less log(sum) and at most log(V); 4 of ex2.approx; 5 of the additions
+// in a thread (warps, blocks and chunks join in 64 bits); 1 of the chunk's sum.
+static float beam_close(int64_t V) { return (float)(2.0 * (11.0 + 2.25 * std::log((double)V)) * 0x1p-24); }
 static int64_t beam_chunks(int64_t batch, int64_t beams, int64_t V) {
   const int64_t chunk = beam_vecs(batch, beams, V) * BS_THREADS * 4;
   return (V + 3 + chunk - 1) / chunk;
@@ -508,8 +643,8 @@ int caten_b200_beam_select(caten_b200_ctx *ctx, const float *d_logits, const flo
   const dim3 grid((unsigned)chunks, (unsigned)(batch * beams));
   CB_CUDA(ctx, launch_k(ctx, beam_vecs(batch, beams, V) == 8 ? beam_chunk_kernel<8> : beam_chunk_kernel<2>, grid, dim3(BS_THREADS), 0, d_logits, d_ended, V, (int)keep, (u64 *)d_work));
   CB_LAUNCH_CHECK(ctx, "beam_chunk_kernel");
-  CB_CUDA(ctx, launch_k(ctx, beam_join_kernel, dim3((unsigned)batch), dim3(BJ_THREADS), 0, (const u64 *)d_work, (int)chunks, d_scores, d_ended, (int)beams, V, eos, (int)keep,
-                        d_out_scores, d_out_parents, d_out_tokens, d_out_ended));
+  const JoinArgs join = {(const u64 *)d_work, d_logits, d_scores, d_ended, d_out_scores, d_out_parents, d_out_tokens, d_out_ended, V, eos, (int)chunks, (int)beams, (int)keep, beam_close(V)};
+  CB_CUDA(ctx, launch_k(ctx, beam_join_kernel, dim3((unsigned)batch), dim3(BJ_THREADS), 0, join));
   CB_LAUNCH_CHECK(ctx, "beam_join_kernel");
   return 0;
 }

@@ -245,8 +245,8 @@ int caten_b200_rope(caten_b200_ctx *ctx, const float *d_x, float *d_y, int64_t B
  * log probabilities so far.  Candidate (beam b, token v) has the value score_b + x_v - log(sum exp(x)); a hypothesis whose d_ended byte is not 0
  * (NULL: none) has one candidate, (b, eos) with the value score_b, and its logits are not read.  Writes the `keep` candidates of largest value,
  * equal ones in the order of b * V + v (a beam's own are equal where their logits are, also where a score like -1e30 leaves no room for logits in a
- * value): values rounded to fp32, the beam each goes on from, its token, and (d_out_ended not NULL) whether it has ended.  The order is decided in 64
- * bits.  Candidates whose value is -inf or NaN (masked tokens, hypotheses with score -inf, rows with a NaN or +inf) are never taken; place i
+ * value): values rounded to fp32 (from sums of exponentials in fp32, 2^-18 at most), the beam each goes on from, its token, and (d_out_ended not
+ * NULL) whether it has ended.  The order is that of values in 64 bits: where the sums' errors could decide it, the rows are summed again.  Candidates whose value is -inf or NaN (masked tokens, hypotheses with score -inf, rows with a NaN or +inf) are never taken; place i
  * that none is left for has score -inf, parent min(i, beams - 1) and token eos (0 without one).
  * beams, keep <= 32; V <= 1040384; batch * beams <= 65535; eos < 0: none (d_ended NULL).  Outputs [batch, keep]; they do not overlap the inputs.
  * d_work: beam_select_work(..) bytes, 8-byte aligned, nothing of which is kept from call to call; calls that may overlap on the GPU need one

@@ -565,6 +565,36 @@ def test_selection_of_equal_values_takes_the_lowest_index(rt):
         check_select(rt, np.zeros((groups, beams, V)), np.zeros((groups, beams)), 32)
 
 
+@pytest.mark.parametrize("groups,beams,V,keep", [(1, 8, 50257, 32), (4, 8, 50257, 16), (3, 5, 1003, 32), (40, 4, 30011, 8), (1, 32, 20003, 32)])
+def test_selection_is_decided_in_64_bits_between_beams(rt, groups, beams, V, keep):
+    """Rows that are equal bit for bit, at every alignment that a vocabulary of odd size gives them, and rows whose sums differ by less than fp32 can
+    tell: which beam comes first is what 64 bits say, equal ones by their index."""
+    rng = rng_of(groups, beams, V)
+    row = rng.standard_normal((groups, 1, V), dtype=np.float32) * 3
+    same = np.repeat(row, beams, 1)
+    scores = np.full((groups, beams), -2.5)
+    for shift in range(4):
+        check_select(rt, same, scores, keep, shift=shift)
+    ended = np.zeros((groups, beams), bool)
+    ended[:, 1] = True
+    check_select(rt, same, scores, keep, ended=ended, eos=7)
+    # a logit of small probability raised in the beams before the last: their sums are larger by 1e-8 to 1e-10 of themselves, their candidates later
+    for down in (18.0, 20.0, 23.0):
+        x = same.copy()
+        low = x.argmin(-1)
+        for g in range(groups):
+            for b in range(beams):
+                x[g, b, low[g, b]] = x[g, b].max() - down - b / 64
+        check_select(rt, x, scores, keep, shift=1)
+        check_select(rt, x[:, ::-1], scores, keep, shift=2)
+    # the last that is taken and the first that is left: equal values of beams in turn, all but the first at a distance from those before
+    few = np.full((groups, beams, V), -30.0, np.float32)
+    few[:, :, V // 2:V // 2 + 5] = 0.0
+    check_select(rt, few, scores, min(keep, 7))
+    many = np.where(np.arange(V) < keep - 1, np.float32(1), np.float32(-20)) + np.zeros((groups, beams, 1), np.float32)
+    check_select(rt, many, scores - np.where(np.arange(beams) == 0, 0.0, 2.0), keep, shift=3)
+
+
 @pytest.mark.parametrize("score", [-1e30, float(np.finfo(np.float32).min)])
 @pytest.mark.parametrize("groups,beams,V,keep", [(2, 3, 5000, 32), (20, 8, 9001, 16), (1, 4, 40, 20)])
 def test_selection_from_scores_that_leave_no_room_for_logits(rt, groups, beams, V, keep, score):
