@@ -101,11 +101,11 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
 // keeps a rare branch a branch: as selects, its instructions would be everybody's
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// power of two 2^(k - floor(log2 x)), kept inside fp32's normal range; 1 for zero
+// power of two 2^(k - floor(log2 x)), for all of fp32's normal range (x of 2^127: 2^(k - 127)); at most 2^113, so that its reciprocal is normal too; 1 for zero
 __device__ __forceinline__ float to_top(float x, int k = 14) {
   const int e = (int)(__float_as_uint(x) >> 23 & 0xff);
   if (x == 0.0f) return 1.0f;
-  return __uint_as_float((uint32_t)min(max(127 + k - (e - 127), 30), 240) << 23);
+  return __uint_as_float((uint32_t)min(254 + k - e, 240) << 23);
 }
 
 // A block's warps (four, eight where they make operands) are `row_warps` row tiles times shares of the tokens.  The warps of a share work on one ring of two stages of 64

@@ -377,6 +377,31 @@ def test_scales_far_from_one(rt, k_scale, q_scale):
         check_attention(rt, c, q, [4])
 
 
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("heads,kv,dim,news", [(2, 2, 64, 1), (2, 1, 64, 1), (8, 1, 64, 1), (4, 1, 128, 12)])
+def test_queries_up_to_the_largest_float(rt, kind, heads, kv, dim, news):
+    """Rows of q whose largest value is anywhere up to fp32's end, beside keys that are small: one token has all of the probability, and which one is
+    plain from scores that differ in their second digit."""
+    rng = rng_of(32, heads, news)
+    c = Cache(rt, rng, kind, dim, 16, heads, kv, [70], k_scale=1e-6)
+    for top in (1e30, 1e34, 3e35, 1e37, 3e38):
+        q = rng.standard_normal((news, heads, dim), dtype=np.float32)
+        q *= np.float32(top) / np.abs(q).max(-1, keepdims=True)
+        out = rt.kv4_attention(c.desc, put(rt, q.reshape(news, -1)), c.pool, put(rt, c.table, np.int32), put(rt, c.lengths, np.int32), put(rt, [0, news], np.int32),
+                               max_new=news).numpy().reshape(news, heads, dim)
+        for i in range(news):
+            sees = 70 - news + i + 1
+            for h in range(heads):
+                k, v = c.k[:sees, h // (heads // kv)], c.v[:sees, h // (heads // kv)]
+                score = k.astype(np.float64) @ q[i, h].astype(np.float64)
+                order = np.argsort(-score)
+                # (scores are right to 2^-16 of sum |q k|, by far; the difference is many times that in units of the scale, so p is 1 and 0)
+                if score[order[0]] - score[order[1]] > 2.0 ** -16 * (np.abs(k).astype(np.float64) @ np.abs(q[i, h]).astype(np.float64)).max():
+                    np.testing.assert_allclose(out[i, h], v[order[0]], rtol=2.0 ** -20, atol=2.0 ** -20 * np.abs(v[order[0]]).max())
+                else:
+                    assert np.isfinite(out[i, h]).all()
+
+
 def test_values_of_very_different_sizes(rt):
     """Tokens of large values with small probabilities beside small values with large ones."""
     rng = rng_of(33)
