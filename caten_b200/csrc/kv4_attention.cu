@@ -1058,6 +1058,7 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
     constexpr int LANES = D / 8, ROWS = 32 / LANES;
     const int chunk = lane % LANES;
     const bool wide = (((uintptr_t)a.q | (uintptr_t)a.ldq * 4) & 15) == 0;
+    const float scale2 = a.scale * 1.4426950408889634f;
 #pragma unroll 1
     for (int i0 = 0; i0 < 16 / ROWS; i0 += 4) {
       float4 in[4][2];   // four rows under way
@@ -1083,8 +1084,10 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
         for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
 #pragma unroll
         for (int j = 1; j < LANES; j <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, j));
-        const float up = to_top(top), sign_up = a.scale < 0.0f ? -up : up;
-        if (chunk == 0) qfactor[q_row] = fabsf(a.scale) * 1.4426950408889634f * (1.0f / up);
+        // What scores are multiplied with stays a power of two: then that product is exact and a row's largest score less itself is zero however large it
+        // is (fused with the subtraction, from scores of 1e8 on, it was off by more than fp16 holds).  The rest of scale log2(e), in [1, 2), goes into q.
+        const float up = to_top(top, 13), power = fmaxf(__uint_as_float(__float_as_uint(scale2) & 0x7f800000u), 0x1p-126f), sign_up = scale2 * (1.0f / power) * up;
+        if (chunk == 0) qfactor[q_row] = power * (1.0f / up);
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1350,7 +1353,7 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
       asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");   // warps quad and quad + 4
       if (!ok) continue;
       top = fmaxf(run_max, fmaxf(red[st][0][row], red[st][1][row]) * f);
-      const float ref = top == -INFINITY ? 0.0f : top - K3_LIFT;
+      const float ref = top == -INFINITY ? 0.0f : __fsub_ru(top, K3_LIFT);   // (upwards: of a top of 1e9 only a part can be taken off)
       const float corr = exp2_fast(run_ref - ref), up = ups[step & 3];
       run_max = top;
       run_ref = top == -INFINITY ? top : ref;

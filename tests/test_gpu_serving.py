@@ -402,6 +402,30 @@ def test_queries_up_to_the_largest_float(rt, kind, heads, kv, dim, news):
                     assert np.isfinite(out[i, h]).all()
 
 
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("q_scale", [3e5, 1e8, 1e20, 1e38])
+@pytest.mark.parametrize("scale", [0.125, 0.0873, -3.1, 7e-20])
+def test_prompts_whose_scores_are_large(rt, kind, q_scale, scale):
+    """Scores beyond the whole numbers that fp32 holds: what has the largest one has all of the probability."""
+    rng = rng_of(34)
+    c = Cache(rt, rng, kind, 64, 16, 8, 1, [200], k_scale=1e-2, spare=columns_for(130, 8, 64, 16), scale=scale)
+    q = rng.uniform(-1, 1, (130, 8, 64)).astype(np.float32) * np.float32(q_scale)
+    out = rt.kv4_attention(c.desc, put(rt, q.reshape(130, -1)), c.pool, put(rt, c.table, np.int32), put(rt, c.lengths, np.int32), put(rt, [0, 130], np.int32),
+                           max_new=130).numpy().reshape(130, 8, 64)
+    assert np.isfinite(out).all()
+    sure = 0
+    for i in range(130):
+        k, v = c.k[:200 - 130 + i + 1, 0].astype(np.float64), c.v[:200 - 130 + i + 1, 0]
+        for h in range(8):
+            score = scale * (k @ q[i, h].astype(np.float64))
+            order = np.argsort(-score)
+            # (scores are right to 2^-18 of scale sum |q k|: 22 bits of either operand, and sums that are cut off at the last bit)
+            if score[order[0]] - score[order[1]] > 30 + 2.0 ** -17 * abs(scale) * (np.abs(k) @ np.abs(q[i, h]).astype(np.float64)).max():
+                np.testing.assert_allclose(out[i, h], v[order[0]], rtol=2.0 ** -20, atol=2.0 ** -20 * np.abs(v[order[0]]).max())
+                sure += 1
+    assert sure > (500 if abs(scale) * q_scale > 1e5 else -1)
+
+
 def test_values_of_very_different_sizes(rt):
     """Tokens of large values with small probabilities beside small values with large ones."""
     rng = rng_of(33)
