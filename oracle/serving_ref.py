@@ -115,3 +115,60 @@ def select(logits, scores, ended, eos, keep):
     with np.errstate(over="ignore"):
         found = np.array([value[i] for i in order] + [-np.inf] * (keep - len(order))).astype(np.float32)
     return found, np.array(parents), np.array(tokens), np.array([bool(ended[p]) or (eos >= 0 and t == eos) for p, t in zip(parents, tokens)])
+
+
+def parts(x, q4_1):
+    """|d (code - 8)| + |minimum + 8 d| (Q4_1) of the values that rows [.., n * 32] are stored as: what the kernels add up in the place of a value."""
+    code, d, m = blocks(x.reshape(*x.shape[:-1], x.shape[-1] // 32, 32), q4_1)
+    d = np.abs(d.astype(np.float64)) if not q4_1 else d.astype(np.float64)
+    y = d * np.abs(code.astype(np.float64) - 8)
+    return (y + np.abs(m.astype(np.float64) + 8 * d) if q4_1 else y).reshape(x.shape)
+
+
+def attention_bound(q, k, k_parts, v_parts, length, scale):
+    """How far the kernels' answers for these rows may be off, [rows, heads, dim], in roundings of u = 2^-23 (sums of tensor cores may be cut off instead of
+    rounded: a whole step).
+
+    A score's terms, of magnitude a = scale sum |q| parts(k): q in two halves 2 u, sums of 16 and their halves and blocks 8 + 10 / 2, factors 2: 20 u a
+    with room.  A probability is off by that and, relatively, by its power of two (2 u) and up to ten corrections when a larger score is met (2.5 u
+    each): 30 u.  It counts twice, in the outputs' sum and in the probabilities'.  Outputs add p times parts(v) in a block of 32 dims: halves of p d
+    2 u, sums of 16 and their halves 8 u, groups of 32 tokens at least u / 2 each, in both sums; what is left for joining parts: 20 u."""
+    rows, heads, dim = q.shape
+    group = heads // k.shape[1]
+    out = np.zeros(q.shape)
+    for i in range(rows):
+        sees = max(0, length - rows + i + 1)
+        for h in range(heads if sees else 0):
+            x = q[i, h].astype(np.float64)
+            s = k[:sees, h // group].astype(np.float64) @ x * scale
+            a = k_parts[:sees, h // group] @ np.abs(x) * abs(scale)
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            block = (p @ v_parts[:sees, h // group].reshape(sees, dim // 32, 32).max(2))
+            # (a token's own a counts as much as its probability; the normalising sum's is the mean)
+            mine = (p * (40 * a)) @ v_parts[:sees, h // group].reshape(sees, dim // 32, 32).max(2) / 2 + block * (p @ (40 * a)) / 2
+            out[i, h] = np.repeat((mine + (90 + sees / 32) * block) * 2.0 ** -23, 32)
+    return out
+
+
+def few_tokens(rng, length, kv, dim, heads, news, scale):
+    """(k, v, q) [tokens, kv, dim] and [news, heads, dim] of a sequence in which a dozen tokens have nearly all of every row's probability, each a share that
+    counts: the first, those on both sides of borders of 64 tokens and of halves, and the last ones, of which each row sees one more than the row before.
+    Values of q lie next to the middle between two of 16 bits, each block of 32 dims of v has one of the tokens stand out."""
+    marks = {0, 15, 16, 63, 64, length // 2 - 1, length // 2, length // 64 * 64 - 1, length // 64 * 64} | set(range(length - news, length))
+    marks = np.array(sorted(t for t in marks if 0 <= t < length))
+    way, even = rng.choice([-1.0, 1.0], (kv, dim)), np.arange(dim) % 2 == 0
+    # rounded to 16 bits, the even dims of q lose twice as much of themselves as the odd ones, and half of the tokens are turned to either
+    size = (np.where(even, 1.02, 1.92) * rng.uniform(1.0, 1.01, (news, heads, dim))).astype(np.float16)
+    size = size.astype(np.float64) + 0.49 * np.spacing(size).astype(np.float64)
+    to_even, to_odd = np.where(even, 1.0, 0.125), np.where(even, 0.125, 0.56)
+    turned = np.where((np.arange(len(marks)) % 2 == 0)[:, None, None], to_even, to_odd) * rng.uniform(0.97, 1.0, (len(marks), 1, 1))
+    k = rng.standard_normal((length, kv, dim)) * 0.1
+    k[marks] = way * turned
+    k *= (np.log(length) + 4) / (abs(scale) * dim * 0.63)
+    q = np.repeat(way[None], news, 0).repeat(heads // kv, 1) * size
+    v = rng.standard_normal((length, kv, dim // 32, 32)) * 0.05
+    for h in range(kv):
+        for b in range(dim // 32):
+            v[marks[-1 - (h * (dim // 32) + b) % len(marks)], h, b] *= 20
+    return k.astype(np.float32), v.reshape(length, kv, dim).astype(np.float32), q.astype(np.float32)

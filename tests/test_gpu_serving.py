@@ -439,6 +439,57 @@ def test_values_of_very_different_sizes(rt):
         check_attention(rt, c, rng.standard_normal((1, 1, 64), dtype=np.float32) * 2, [1])
 
 
+def refill(rt, c, kind, k, v):
+    """The cache's sequences hold these keys and values [tokens, kv_heads, dim]; what they are stored as, and the parts that they are added up from."""
+    page, q41 = c.desc.page, kind == "q4_1"
+    slots = [c.table[b, t // page] * page + t % page for b, n in enumerate(c.lengths) for t in range(n)]
+    rows = [np.ascontiguousarray(x.reshape(len(slots), -1), np.float32) for x in (k, v)]
+    rt.kv4_store(c.desc, c.pool, put(rt, rows[0]), put(rt, rows[1]), put(rt, slots, np.int32))
+    c.k, c.v = (ref.values(x, q41).reshape(k.shape) for x in rows)
+    c.k_parts, c.v_parts = (ref.parts(x, q41).reshape(k.shape) for x in rows)
+
+
+def check_closely(rt, c, q, news, max_length=0):
+    """Every value of every row against 64 bits, within the bound of its own row and block of 32 dims."""
+    heads, dim = c.desc.heads, c.desc.dim
+    at = np.concatenate([[0], np.cumsum(news)]).astype(int)
+    got = rt.kv4_attention(c.desc, put(rt, q.reshape(len(q), -1)), c.pool, put(rt, c.table, np.int32), put(rt, c.lengths, np.int32), put(rt, at, np.int32),
+                           max_new=max(news), max_length=max_length).numpy().reshape(-1, heads, dim)
+    for b, n in enumerate(c.lengths):
+        part, rows = slice(c.first[b], c.first[b + 1]), q[at[b]:at[b + 1]]
+        want = ref.attention(rows, c.k[part], c.v[part], n, c.desc.scale)
+        tol = ref.attention_bound(rows, c.k[part], c.k_parts[part], c.v_parts[part], n, c.desc.scale)
+        off = np.abs(got[at[b]:at[b + 1]] - want)
+        assert (off <= tol).all(), f"sequence {b} of {n}: {(off / np.maximum(tol, 1e-300)).max():.3g} times the bound"
+    return got
+
+
+# heads, key heads, dim, new tokens: the kernels for one row, for two to four, for tiles of eight, and for tiles of 128
+ONE_ROW = [(2, 2, 64, 1), (3, 3, 128, 1), (1, 1, 192, 1), (2, 2, 256, 1)]
+FEW_ROWS = [(2, 1, 64, 1), (8, 2, 128, 1), (3, 3, 64, 3), (4, 2, 192, 2), (3, 1, 256, 1), (4, 4, 128, 4)]
+EIGHT_ROWS = [(8, 1, 64, 1), (12, 2, 128, 1), (2, 2, 64, 13), (8, 1, 128, 5), (6, 1, 192, 3), (2, 1, 256, 9)]
+MANY_ROWS = [(8, 1, 64, 40), (4, 2, 128, 60), (3, 3, 64, 140)]
+
+
+def spare_for(rows, heads, dim, page):
+    return columns_for(rows, heads, dim, page) if rows >= 40 else 2
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("heads,kv,dim,news", ONE_ROW + FEW_ROWS + EIGHT_ROWS + MANY_ROWS)
+@pytest.mark.parametrize("length", [65, 257, 1200, 5000])
+def test_every_token_counts(rt, kind, heads, kv, dim, news, length):
+    """Rows whose probability is on a few tokens: the last that they see, the first, and both sides of every border of groups, pages and parts.  The bound is such
+    that none of them can be missing, nor one behind the last be seen, nor q or p be held in fewer bits (tests/test_serving.py)."""
+    rng = rng_of(71, heads, dim, length)
+    news = min(news, length)
+    c = Cache(rt, rng, kind, dim, 64, heads, kv, [length], spare=spare_for(news, heads, dim, 64))
+    k, v, q = ref.few_tokens(rng, length, kv, dim, heads, news, c.desc.scale)
+    refill(rt, c, kind, k, v)
+    check_closely(rt, c, q, [news])
+    check_closely(rt, c, q, [news], max_length=length)
+
+
 def test_nan_in_a_row_stays_in_it(rt):
     rng = rng_of(35)
     c = Cache(rt, rng, "q4_0", 64, 16, 2, 1, [40, 40])

@@ -244,6 +244,40 @@ def test_selection_workspace_is_enough_for_every_smaller_call(lib):
         assert work(*small) <= work(*large)
 
 
+def test_the_bound_on_attention_tells_mistakes():
+    """The bound that the GPU tests compare attention with, on their inputs: every row is beyond it if a token that it sees is left out, be it the last, the
+    first or one at a border, or if it sees one token more; some row of a call is if q, or p, is held in 16 bits."""
+    for length in (65, 257, 1200, 5000):
+        for heads, kv, dim, news in ((2, 1, 64, 1), (4, 4, 128, 4), (1, 1, 64, 1), (3, 1, 256, 1), (8, 1, 64, 12), (2, 2, 64, 60)):
+            rng = np.random.Generator(np.random.PCG64([length, heads, dim]))
+            scale, group = dim ** -0.5, heads // kv
+            k, v, q = ref.few_tokens(rng, length, kv, dim, heads, news, scale)
+            q = q[-4:]   # (the rest is the same)
+            for q41 in (False, True):
+                ks, vs = (ref.values(x.reshape(length, -1), q41).reshape(k.shape) for x in (k, v))
+                kp, vp = (ref.parts(x.reshape(length, -1), q41).reshape(k.shape) for x in (k, v))
+                want, tol = ref.attention(q, ks, vs, length, scale), ref.attention_bound(q, ks, kp, vp, length, scale)
+                off = lambda x: (np.abs(x - want) > tol).any(2)   # noqa: E731
+                assert (tol < 2e-4 * np.abs(vs).max()).all()
+                for left_out in (0, 16, 63, 64, length // 2, length // 64 * 64 - 1):
+                    there = np.arange(length) != left_out
+                    if left_out < length - len(q):
+                        assert off(ref.attention(q, ks[there], vs[there], length - 1, scale)).all(), left_out
+                shorter = np.concatenate([q, q[-1:]])   # a row fewer behind each: row i sees a token less
+                assert off(ref.attention(shorter, ks, vs, length, scale)[:-1]).all()
+                if len(q) > 1:                          # and one more
+                    assert off(np.concatenate([ref.attention(q[:-1], ks, vs, length, scale), want[-1:]]))[:-1].all()
+                assert off(ref.attention(q.astype(np.float16).astype(np.float32), ks, vs, length, scale)).any()
+                low = np.empty_like(want)
+                for i in range(len(q)):
+                    sees = length - len(q) + i + 1
+                    for h in range(heads):
+                        s = ks[:sees, h // group].astype(np.float64) @ q[i, h].astype(np.float64) * scale
+                        p = np.exp(s - s.max())
+                        low[i, h] = p.astype(np.float16).astype(np.float64) @ vs[:sees, h // group] / p.sum()
+                assert off(low).any() or news > 4   # (with more tokens to share a row's probability, their roundings are lost among them)
+
+
 def test_copies_of_a_ring_land_before_it_is_given_up(tmp_path):
     """What the attention kernels wait for when a wait ran out (csrc/kv4_ring.h, as plain C++), at every step of rings of every length: the copies that
     are under way then, each once with the parity of its own step, and no others (a wait for one that was never asked for would last to its limit)."""
