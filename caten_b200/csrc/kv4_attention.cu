@@ -108,6 +108,15 @@ __device__ __forceinline__ float to_top(float x, int k = 14) {
   return __uint_as_float((uint32_t)min(254 + k - e, 240) << 23);
 }
 
+// the same for x >= 0, with 2^113 for zero; the inverse of such a power; the largest magnitude (NaN is passed over)
+__device__ __forceinline__ float to_top_of(float x) { return __uint_as_float((uint32_t)min(254 + 14 - (int)(__float_as_uint(x) >> 23), 240) << 23); }
+__device__ __forceinline__ float inverse_power(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // A block's warps (four, eight where they make operands) are `row_warps` row tiles times shares of the tokens.  The warps of a share work on one ring of two stages of 64
 // or 32 tokens, which bulk copies fill while the other is read (each stage is read by all its warps before it is filled again).
 // With four row tiles (SHARED) the warps first turn a stage's codes into operands and its scales into floats, a quarter each, in shared memory: of the
@@ -581,9 +590,12 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
 // Key heads shared by two to four query heads, or as many tokens of one: with codes as the first operand (16 tokens) and the rows in the eight
 // columns, halves side by side (column 2 r + h), nothing is empty: half the products of the kernel above, a score in one lane (row t, tokens g and
 // g + 8), half the softmax; in the second product columns 2 r + h again, whose two sums a lane has both.  Each warp has a ring of its own.
-// Bound by instructions (unpacking, two roundings of p d).  4 heads to a key head of 128, Q4_0: 256 sequences of 768 tokens 84 us (the kernel above
-// 111), 64 of 768 25 (45), 3 of 100001 132 (167: 346 MB, 2.6 TB/s); Q4_1 the last in 147 (186); 32 heads over 16 key heads of 256, 8 sequences of
-// 2900 63 (76).
+// p d is scaled for each row, group and block of 32 dims by what the largest of them needs: a row's bits do not depend on tokens that it does not see, or
+// that have no probability, nor on other dims.  The lanes of a row's two columns have two of a lane's four tokens each, make both halves of theirs and
+// exchange one.
+// Bound by instructions (unpacking, two roundings of p d).  4 heads to a key head of 128, Q4_0: 256 sequences of 768 tokens 71 us, 3 of 20000 to 100001
+// 102 (in warps of 8 rows 167); Q4_1 79 and 111; 32 heads over 16 key heads of 256, 8 sequences of 580 to 2900 49 and 54.  (One power of two for a group, from
+// the scales alone: 70 and 99, 80 and 110, 47 and 52, and values of 1e-4 beside 1e5 off by 4e-3 of themselves.)
 
 template <int NC, bool Q41>
 __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_few_kernel(const Kv4AttnArgs a) {
@@ -609,13 +621,15 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
   const int t0 = part * a.part_tokens, t1 = r0 < count ? min(most, t0 + a.part_tokens) : 0;
   const bool live = r0 < count && (t0 < t1 || part == 0);
 
-  float run_max = -INFINITY, run_sum = 0.0f, run_down = 1.0f;   // of row t (run_sum: this lane's tokens); what outputs are to be multiplied with
-  float off[4] = {0.f, 0.f, 0.f, 0.f};                          // Q4_1: sums of p m_b (rows b of a product of their own) and p d_b (rows NB + b)
+  float run_max = -INFINITY, run_sum = 0.0f;   // of row t (run_sum: this lane's tokens)
+  float off[Q41 ? NB : 1];                     // Q4_1: sums of p (m + 8 d) of a block, the column's row, this lane's tokens
   float o[NB][2][4];                                            // columns 2t, 2t + 1; dims 4g + {0 | 1} and 4g + {2 | 3} of a block
 #pragma unroll
-  for (int k = 0; k < NB; ++k)
+  for (int k = 0; k < NB; ++k) {
+    if (Q41) off[k] = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] = 0.0f;
+  }
 
   const int first = t0 + (warp - first_warp) * GROUP, step = share * GROUP;
   uint8_t *const mine = ring + warp * 2 * STAGE;
@@ -693,7 +707,6 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
       const unsigned there = there_now;
       const bool clean = base + GROUP <= least && there == (1u << TILES) - 1u;   // every row sees every token
       float s[TILES][2];
-      __half2 big = __float2half2_rn(0.0f);   // the values' largest scale, lanes over blocks
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
         const uint8_t *tile = tiles + i * TILE;
@@ -725,30 +738,21 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
         }
         s[i][0] = x0 * factor;
         s[i][1] = x1 * factor;
-        const uint2 v2 = *reinterpret_cast<const uint2 *>(tile + PART + 8 * D + (t * NB + g % NB) * 8);
-        uint32_t vx = v2.x & 0x7fff7fffu, vy = v2.y & 0x7fff7fffu;
         if (!clean) {   // what stands behind the last token may be anything
           keep_branch();
-          const bool in = there >> i & 1;
-          const int at = base + 16 * i + 2 * t;
-          vx &= (in && at < t1 ? 0xffffu : 0u) | (in && at + 1 < t1 ? 0xffff0000u : 0u);
-          vy &= (in && at + 8 < t1 ? 0xffffu : 0u) | (in && at + 9 < t1 ? 0xffff0000u : 0u);
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (base + 16 * i + g + 8 * e >= min(sees, t1) || !in) s[i][e] = -INFINITY;
+            if (base + 16 * i + g + 8 * e >= min(sees, t1) || !(there >> i & 1)) s[i][e] = -INFINITY;
         }
-        big = __hmax2(big, __hmax2(*reinterpret_cast<const __half2 *>(&vx), *reinterpret_cast<const __half2 *>(&vy)));
       }
       float top = run_max;
 #pragma unroll
       for (int i = 0; i < TILES; ++i) top = fmaxf(top, fmaxf(s[i][0], s[i][1]));
 #pragma unroll
       for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-      const float up = to_top(warp_max(fmaxf(__low2float(big), __high2float(big))));
       const float ref = top == -INFINITY ? 0.0f : top;
-      const float corr = exp2_fast(run_max - ref), lifted = corr * (up * run_down);   // (-inf: 0); outputs so far are times the last group's power of two
+      const float corr = exp2_fast(run_max - ref);   // (-inf: 0)
       run_max = top;
-      run_down = 1.0f / up;
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < TILES; ++i)
@@ -756,48 +760,26 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
         for (int e = 0; e < 2; ++e) {
           s[i][e] = exp2_fast(s[i][e] - ref);
           sum += s[i][e];
-          s[i][e] *= up;
         }
       run_sum = fmaf(run_sum, corr, sum);
-      // p of the column's row and tokens 2t, 2t + 1, 2t + 8, 2t + 9
-      float p[TILES][4];
+      // p of the column's row: tokens 2t, 2t + 1 in an even column, 2t + 8, 2t + 9 in an odd one, which makes both halves of theirs
+      float p[TILES][2];
 #pragma unroll
       for (int i = 0; i < TILES; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[i][e] = __shfl_sync(0xffffffffu, s[i][e >> 1], 8 * t + 4 * (e & 1) + (g >> 1));
-      // the upper eleven bits of a number in an even column, what they leave in an odd one
-      auto half_of = [&](float x) {
-        float y = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
-        if (g & 1) y = x - y;
-        return y;
-      };
-      if (Q41) {   // minima and scales themselves as the first operand, as above
-        const float lift = run_down * 0x1p14f, unlift = up * 0x1p-14f;   // p at the top of fp16's range
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-          uint32_t av[4] = {0, 0, 0, 0};
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (8 * h < 2 * NB) {
-              const int row = 8 * h + g;
-              if (row < 2 * NB) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (row < NB ? D : 0) + (t * NB + (row < NB ? row : row - NB)) * 8);
-                av[h] = w.x;
-                av[2 + h] = w.y;
-              }
-              if (!clean) {
-                keep_branch();
-                const int at = base + 16 * i + 2 * t;
-                const bool in = there >> i & 1;
-                av[h] = finite_halves(av[h]) & ((in && at < t1 ? 0xffffu : 0u) | (in && at + 1 < t1 ? 0xffff0000u : 0u));
-                av[2 + h] = finite_halves(av[2 + h]) & ((in && at + 8 < t1 ? 0xffffu : 0u) | (in && at + 9 < t1 ? 0xffff0000u : 0u));
-              }
-            }
-          mma_16816(acc, av, pack_half(half_of(p[i][0] * lift), half_of(p[i][1] * lift)), pack_half(half_of(p[i][2] * lift), half_of(p[i][3] * lift)));
+        for (int e = 0; e < 2; ++e) {
+          const float even = __shfl_sync(0xffffffffu, s[i][0], 8 * t + 4 * e + (g >> 1)), odd = __shfl_sync(0xffffffffu, s[i][1], 8 * t + 4 * e + (g >> 1));
+          p[i][e] = g & 1 ? odd : even;
         }
+      if (__any_sync(0xffffffffu, corr != 1.0f)) {   // (in a long history nearly never)
+        keep_branch();
+        const float corr_col = __shfl_sync(0xffffffffu, corr, g >> 1);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) off[e] = fmaf(off[e], lifted, acc[e] * unlift);
+        for (int k = 0; k < NB; ++k) {
+          if (Q41) off[k] *= corr_col;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] *= corr;
+        }
       }
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -807,19 +789,39 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int blk = 2 * c + k;
-          float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          float pd[TILES][2], most = 0.0f, add = 0.0f;
 #pragma unroll
           for (int i = 0; i < TILES; ++i) {
-            const uint2 d2 = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8);
-            const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
-            float pd[4] = {p[i][0] * d01.x, p[i][1] * d01.y, p[i][2] * d23.x, p[i][3] * d23.y};
+            const uint8_t *sc = tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8 + 4 * (g & 1);
+            const float2 d = half_pair(*reinterpret_cast<const uint32_t *>(sc));
+            float2 n = make_float2(0.f, 0.f);
+            if (Q41) {
+              const float2 m = half_pair(*reinterpret_cast<const uint32_t *>(sc + D));
+              n = make_float2(fmaf(8.0f, d.x, m.x), fmaf(8.0f, d.y, m.y));
+            }
+            float pn[2] = {p[i][0] * n.x, p[i][1] * n.y};
+            pd[i][0] = p[i][0] * d.x;
+            pd[i][1] = p[i][1] * d.y;
             if (!clean) {   // (0 times what a scale behind the last token, or of a token that the row does not see, may be)
               keep_branch();
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1) >= min(sees_col, t1) || !(there >> i & 1)) pd[e] = 0.0f;
+              for (int e = 0; e < 2; ++e)
+                if (base + 16 * i + 2 * t + 8 * (g & 1) + e >= min(sees_col, t1) || !(there >> i & 1)) pd[i][e] = pn[e] = 0.0f;
             }
-            const uint32_t b0 = pack_half(half_of(pd[0]), half_of(pd[1])), b1 = pack_half(half_of(pd[2]), half_of(pd[3]));
+            if (Q41) add += pn[0] + pn[1];
+            most = max_abs(most, pd[i][0], pd[i][1]);
+          }
+          if (Q41) off[blk] += add;
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
+          const float up = to_top_of(most), down = __shfl_sync(0xffffffffu, inverse_power(up), 8 * t);
+          float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int i = 0; i < TILES; ++i) {
+            const float x0 = pd[i][0] * up, x1 = pd[i][1] * up;
+            const uint32_t hi = pack_half(x0, x1), lo = pack_half_lo(x0, x1, hi), other = __shfl_xor_sync(0xffffffffu, g & 1 ? hi : lo, 4);
+            const uint32_t b0 = g & 1 ? other : hi, b1 = g & 1 ? lo : other;   // upper halves in the even column, lower ones in the odd
             const uint32_t x = __byte_perm(w[i].x, w[i].y, k ? 0x7632 : 0x5410), y = __byte_perm(w[i].z, w[i].w, k ? 0x7632 : 0x5410);
             const uint32_t a0[4] = {codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y)};
             const uint32_t a1[4] = {codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8)};
@@ -829,7 +831,7 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[blk][n][e] = fmaf(o[blk][n][e], lifted, acc[n][e]);
+            for (int e = 0; e < 4; ++e) o[blk][n][e] = fmaf(acc[n][e], down, o[blk][n][e]);
         }
       }
       __syncwarp();   // the stage has been read
@@ -853,17 +855,17 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
   // row t: its sum over the lanes of its tokens; its outputs, halves together: four dims of a block a lane
 #pragma unroll
   for (int k = 4; k < 32; k <<= 1) run_sum += __shfl_xor_sync(0xffffffffu, run_sum, k);
-  const float off_lo = off[0] + off[1], off_hi = off[2] + off[3];
   float4 x[NB];
 #pragma unroll
   for (int k = 0; k < NB; ++k) {
     float add = 0.0f;
     if (Q41) {
-      const float pm = __shfl_sync(0xffffffffu, k < 8 ? off_lo : off_hi, k % 8 * 4 + t), pd = __shfl_sync(0xffffffffu, NB + k < 8 ? off_lo : off_hi, (NB + k) % 8 * 4 + t);
-      add = fmaf(8.0f, pd, pm);
+      off[k] += __shfl_xor_sync(0xffffffffu, off[k], 1);
+      off[k] += __shfl_xor_sync(0xffffffffu, off[k], 2);
+      off[k] += __shfl_xor_sync(0xffffffffu, off[k], 4);
+      add = __shfl_sync(0xffffffffu, off[k], 8 * t);
     }
-    x[k] = make_float4((o[k][0][0] + o[k][0][1] + add) * run_down, (o[k][0][2] + o[k][0][3] + add) * run_down, (o[k][1][0] + o[k][1][1] + add) * run_down,
-                       (o[k][1][2] + o[k][1][3] + add) * run_down);
+    x[k] = make_float4(o[k][0][0] + o[k][0][1] + add, o[k][0][2] + o[k][0][3] + add, o[k][1][0] + o[k][1][1] + add, o[k][1][2] + o[k][1][3] + add);
   }
   float top = run_max, sum = run_sum;
   if (share > 1) {

@@ -476,6 +476,37 @@ def spare_for(rows, heads, dim, page):
 
 
 @pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("heads,kv,dim,news", FEW_ROWS)
+def test_values_a_row_has_no_part_in_do_not_cost_it_bits(rt, kind, heads, kv, dim, news):
+    """Tokens and blocks of 32 dims whose values are 1e8 times others': each block of a row is as close as its own sum of p |v| allows, whether the large values
+    are behind the row's last token, have probabilities next to none, or are other dims'."""
+    rng = rng_of(70, heads, dim, news)
+    lengths = [90, 33, 200] if news < 40 else [news + 9, news, 200]
+    c = Cache(rt, rng, kind, dim, 16, heads, kv, lengths, spare=spare_for(news, heads, dim, 16))
+    total = sum(lengths)
+    q = rng.standard_normal((3 * news, heads, dim), dtype=np.float32)
+    shape = (total, kv, dim)
+    v = rng.standard_normal(shape, dtype=np.float32)
+    k = rng.standard_normal(shape, dtype=np.float32)
+    far = 10.0 ** rng.uniform(-4, 4, (total, kv, dim // 32, 1)).astype(np.float32)
+    refill(rt, c, kind, k, (v.reshape(*shape[:2], -1, 32) * far).reshape(shape))          # tokens and blocks in any order
+    check_closely(rt, c, q, [news] * 3)
+    of_block = 10.0 ** rng.uniform(-4, 4, (1, 1, dim // 32, 1)).astype(np.float32)
+    refill(rt, c, kind, k, (v.reshape(*shape[:2], -1, 32) * of_block).reshape(shape))     # dims that are always large
+    check_closely(rt, c, q, [news] * 3)
+    late = np.ones((total, 1, 1), np.float32)
+    for b in range(3):
+        late[c.first[b + 1] - max(1, news // 2):c.first[b + 1]] = 1e6                     # seen by the last rows only
+    refill(rt, c, kind, k, v * 1e-2 * late)
+    check_closely(rt, c, q, [news] * 3)
+    against = np.where(np.arange(total) % 3 == 0, np.float32(1e4), np.float32(1e-4))[:, None, None]
+    same = np.repeat(q[:1, :1], len(q), 0).repeat(heads, 1)                               # large values where the probability is e^-30
+    away = np.where(against > 1, -30.0, 0.0).astype(np.float32) / (c.desc.scale * (same[0, 0] ** 2).sum())
+    refill(rt, c, kind, (k * 0.05 + same[0, 0] * away).astype(np.float32), v * against)
+    check_closely(rt, c, same, [news] * 3)
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
 @pytest.mark.parametrize("heads,kv,dim,news", ONE_ROW + FEW_ROWS + EIGHT_ROWS + MANY_ROWS)
 @pytest.mark.parametrize("length", [65, 257, 1200, 5000])
 def test_every_token_counts(rt, kind, heads, kv, dim, news, length):
