@@ -10,9 +10,10 @@
 // with n = 0 (Q4_0) or the minimum + 8 d (Q4_1).  From the middle of the codes, because a sum of thousands of p d code is many times what is left when
 // 8 p d is taken off it, and so is its error (100001 tokens: 3e-4).
 // (So in the kernels for up to 48 rows; the one for prompts multiplies the scales in before.)
-// A warp has 8 rows (tokens x the heads that share a key head; kernels for one row and for two to four follow, and one for tiles of 128) and takes 64 tokens at a time: running maximum and sum of the softmax per row, the
-// group's p d scaled by a power of two for each block, so that the largest is near the top of fp16 whatever the cache's scales are, and joined
-// to the running sums in fp32.
+// A warp has 8 rows (tokens x the heads that share a key head; kernels for one row and for two to four follow, and one for tiles of 128) and takes 64 or
+// 32 tokens at a time: running maximum and sum of the softmax per row, the group's p d times a power of two for each row and block of 32 dims that
+// brings its largest near the top of fp16 (so what a row does not see, what has no probability and what other dims hold cost it no bits), and the sums
+// joined to the running ones in fp32.
 #include <algorithm>
 
 #include "common.cuh"
@@ -126,12 +127,12 @@ template <int NC, bool Q41, bool SHARED>
 __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 : 1) : NC == 1 ? 4 : NC == 2 ? 3 : 2) kv4_attention_kernel(const Kv4AttnArgs a) {
   constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, TILES = K4_TILES(NC), GROUP = 16 * TILES, STAGE = TILES * TILE;
   constexpr int WARPS = k4_warps(SHARED), PER_TILE = 16 * NB;   // (floats of a kind of a tile)
-  constexpr int OPS = TILES * NC * 8 * 512, FLOATS = TILES * (Q41 ? 3 : 2) * PER_TILE * 4, SHARE = 2 * STAGE + (SHARED ? OPS + FLOATS : 0);   // bytes
+  constexpr int KINDS = Q41 ? 4 : 2;   // SHARED: scales of K and V, and minima + 8 d
+  constexpr int OPS = TILES * NC * 8 * 512, FLOATS = TILES * KINDS * PER_TILE * 4, SHARE = 2 * STAGE + (SHARED ? OPS + FLOATS : 0);   // bytes
   __shared__ float sm[WARPS][K4_ROWS], sl[WARPS][K4_ROWS];
   __shared__ uint64_t bars[WARPS][2];
   __shared__ int gave_up[WARPS], never;           // (never: not set by anyone)
   __shared__ unsigned present[WARPS][2];          // of a share: tiles of each stage
-  __shared__ unsigned largest_scale[WARPS][2];       // SHARED: of a stage's values
   extern __shared__ __align__(128) uint8_t ring[];   // two stages a share (SHARED: then its operands); behind the last group, the warps' sums
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = warp_index(), g = lane >> 2, t = lane & 3;
@@ -230,19 +231,29 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
   }
 
   float run_max = -INFINITY, run_sum = 0.0f;   // of row g (run_sum: this lane's tokens)
-  float run_down = 1.0f;                       // what outputs (and Q4_1's sums) are to be multiplied with
-  float off[4] = {0.f, 0.f, 0.f, 0.f};         // Q4_1: sums of p m_b (rows b of a product of their own) and p d_b (rows NB + b) for rows 2t, 2t + 1
+  float off[Q41 ? NB : 1];                     // Q4_1: sums of p (m + 8 d) of a block, row g, this lane's tokens
   float o[NB][2][4];                           // rows 2t, 2t + 1; dims 4g + {0, 1} and 4g + {2, 3} of a block
 #pragma unroll
   for (int k = 0; k < NB; ++k) {
+    if (Q41) off[k] = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] = 0.0f;
   }
-  // SHARED: operands of a stage [tile][chunk][K: block, token half | V: block, dims][lane], then scales of K, of V and minima of K as floats
+  // SHARED: operands of a stage [tile][chunk][K: block, token half | V: block, dims][lane], then scales of K and of V as floats, and Q4_1's minima + 8 d
   uint4 *const ops = reinterpret_cast<uint4 *>(stages + 2 * STAGE);
   float *const floats = reinterpret_cast<float *>(stages + 2 * STAGE + OPS);
-  if (SHARED && sub == 0 && lane < 2) largest_scale[share][lane] = 0;
   __syncthreads();   // the barriers are there
+  // scales of tokens 2t, 2t + 1, 2t + 8, 2t + 9, and Q4_1's minima + 8 d
+  auto scales_of = [](const uint8_t *at, float (&d)[4], float (&n)[4]) {
+    const uint2 d2 = *reinterpret_cast<const uint2 *>(at);
+    const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
+    d[0] = d01.x; d[1] = d01.y; d[2] = d23.x; d[3] = d23.y;
+    if (Q41) {
+      const uint2 m2 = *reinterpret_cast<const uint2 *>(at + D);
+      const float2 m01 = half_pair(m2.x), m23 = half_pair(m2.y);
+      n[0] = fmaf(8.0f, d[0], m01.x); n[1] = fmaf(8.0f, d[1], m01.y); n[2] = fmaf(8.0f, d[2], m23.x); n[3] = fmaf(8.0f, d[3], m23.y);
+    }
+  };
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
@@ -279,24 +290,16 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
           }
         }
       }
-      unsigned largest = 0;
-      constexpr int KINDS = Q41 ? 3 : 2;
       for (int j = sub * 32 + lane; j < TILES * KINDS * PER_TILE / 2; j += 128) {
         const int i = j / (KINDS * PER_TILE / 2), rest = j % (KINDS * PER_TILE / 2), kind = rest / (PER_TILE / 2), pair = rest % (PER_TILE / 2);
-        uint32_t h = *reinterpret_cast<const uint32_t *>(tiles + i * TILE + (kind == 1 ? PART : 0) + (kind == 2 ? 9 : 8) * D + pair * 4);
-        if (kind == 1) {   // what stands behind the last token may be anything
-          const int at = base + 16 * i + pair / 2 / NB * 2 + 8 * (pair & 1);
-          h &= (there >> i & 1 && at < t1 ? 0xffffu : 0u) | (there >> i & 1 && at + 1 < t1 ? 0xffff0000u : 0u);
+        const uint8_t *at = tiles + i * TILE + (kind & 1) * PART + 8 * D + pair * 4;
+        float2 x = half_pair(*reinterpret_cast<const uint32_t *>(at));
+        if (kind >= 2) {
+          const float2 m = half_pair(*reinterpret_cast<const uint32_t *>(at + D));
+          x = make_float2(fmaf(8.0f, x.x, m.x), fmaf(8.0f, x.y, m.y));
         }
-        const float2 f = half_pair(h);
-        *reinterpret_cast<float2 *>(floats + (i * KINDS + kind) * PER_TILE + pair * 2) = f;
-        if (kind == 1) {
-          const unsigned u0 = __float_as_uint(fabsf(f.x)), u1 = __float_as_uint(fabsf(f.y));
-          largest = max(largest, max(u0 < 0x7f800000u ? u0 : 0u, u1 < 0x7f800000u ? u1 : 0u));
-        }
+        *reinterpret_cast<float2 *>(floats + (i * KINDS + kind) * PER_TILE + pair * 2) = x;
       }
-      largest = __reduce_max_sync(0xffffffffu, largest);
-      if (lane == 0 && largest) atomicMax(&largest_scale[share][stage], largest);
     }
     if (SHARED) asm volatile("bar.sync %0, 128;" ::"r"(1 + share) : "memory");
     if (ok && mine && base < most) {
@@ -304,7 +307,6 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
       const unsigned there = present[share][stage];
       const bool clean = base + GROUP <= least && there == (1u << TILES) - 1u;   // every row sees every token
       float s[TILES][4];
-      __half2 big = __float2half2_rn(0.0f);
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
         const uint8_t *tile = tiles + i * TILE;
@@ -318,23 +320,16 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
           for (int k = 0; k < 2; ++k) {
             const int blk = 2 * c + k;
             const uint8_t *sc = tile + 8 * D + (t * NB + blk) * 8;
-            float d[4], m[4];
+            float d[4], off_k[4];
             if (SHARED) {
-              const float4 f = *reinterpret_cast<const float4 *>(floats + i * (Q41 ? 3 : 2) * PER_TILE + (t * NB + blk) * 4);
-              d[0] = f.x; d[1] = f.y; d[2] = f.z; d[3] = f.w;
+              const float4 x = *reinterpret_cast<const float4 *>(floats + i * KINDS * PER_TILE + (t * NB + blk) * 4);
+              d[0] = x.x; d[1] = x.y; d[2] = x.z; d[3] = x.w;
               if (Q41) {
-                const float4 fm = *reinterpret_cast<const float4 *>(floats + (i * 3 + 2) * PER_TILE + (t * NB + blk) * 4);
-                m[0] = fm.x; m[1] = fm.y; m[2] = fm.z; m[3] = fm.w;
+                const float4 y = *reinterpret_cast<const float4 *>(floats + (i * KINDS + 2) * PER_TILE + (t * NB + blk) * 4);
+                off_k[0] = y.x; off_k[1] = y.y; off_k[2] = y.z; off_k[3] = y.w;
               }
             } else {
-              const uint2 d2 = *reinterpret_cast<const uint2 *>(sc);
-              const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
-              d[0] = d01.x; d[1] = d01.y; d[2] = d23.x; d[3] = d23.y;
-            }
-            if (Q41 && !SHARED) {
-              const uint2 m2 = *reinterpret_cast<const uint2 *>(sc + D);
-              const float2 m01 = half_pair(m2.x), m23 = half_pair(m2.y);
-              m[0] = m01.x; m[1] = m01.y; m[2] = m23.x; m[3] = m23.y;
+              scales_of(sc, d, off_k);
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n) {   // tokens 0..7, 8..15
@@ -351,22 +346,10 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
                 const int e = 2 * n + j;
-                if (Q41) acc[e] = fmaf(fmaf(8.0f, d[e], m[e]), qsum[blk], acc[e]);   // (d code + m = d (code - 8) + (m + 8 d), which cancel before they are summed)
+                if (Q41) acc[e] = fmaf(off_k[e], qsum[blk], acc[e]);   // (d code + m = d (code - 8) + (m + 8 d), which cancel before they are summed)
                 acc[e] = fmaf(d[e], p[j] + p[2 + j], acc[e]);
               }
             }
-            if (SHARED) continue;
-            // the values' largest scale
-            const uint2 v2 = *reinterpret_cast<const uint2 *>(sc + PART);
-            uint32_t vx = v2.x & 0x7fff7fffu, vy = v2.y & 0x7fff7fffu;
-            if (!clean) {   // what stands behind the last token may be anything
-              keep_branch();
-              const int at = base + 16 * i + 2 * t;
-              const bool in = there >> i & 1;
-              vx &= (in && at < t1 ? 0xffffu : 0u) | (in && at + 1 < t1 ? 0xffff0000u : 0u);
-              vy &= (in && at + 8 < t1 ? 0xffffu : 0u) | (in && at + 9 < t1 ? 0xffff0000u : 0u);
-            }
-            big = __hmax2(big, __hmax2(*reinterpret_cast<const __half2 *>(&vx), *reinterpret_cast<const __half2 *>(&vy)));
           }
         }
 #pragma unroll
@@ -382,7 +365,6 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
           }
         }
       }
-      // running maximum; p is taken times a power of two that brings the largest p d near the top of fp16
       float top = run_max;
 #pragma unroll
       for (int i = 0; i < TILES; ++i)
@@ -390,19 +372,9 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
         for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      float largest;
-      if (SHARED) {
-        largest = __uint_as_float(largest_scale[share][stage]);
-      } else {
-        largest = fmaxf(__low2float(big), __high2float(big));
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-      }
-      const float up = to_top(largest);
       const float ref = top == -INFINITY ? 0.0f : top;
-      const float corr = exp2_fast(run_max - ref), lifted = corr * (up * run_down);   // (-inf: 0); the outputs so far are times the last group's power of two
+      const float corr = exp2_fast(run_max - ref);   // (-inf: 0)
       run_max = top;
-      run_down = 1.0f / up;
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < TILES; ++i)
@@ -410,43 +382,17 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
         for (int e = 0; e < 4; ++e) {
           s[i][e] = exp2_fast(s[i][e] - ref);
           sum += s[i][e];
-          s[i][e] *= up;
         }
       run_sum = fmaf(run_sum, corr, sum);
-      const float lifted0 = __shfl_sync(0xffffffffu, lifted, 8 * t), lifted1 = __shfl_sync(0xffffffffu, lifted, 8 * t + 4);
-      if (Q41) {
-        // sum of p (m + 8 d), which the middle of the codes leaves: minima and scales lie in the cache as the product's first operand has them
-        const float lift = run_down * 0x1p14f, unlift = up * 0x1p-14f;   // p at the top of fp16's range
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      if (__any_sync(0xffffffffu, corr != 1.0f)) {   // (in a long history nearly never)
+        keep_branch();
+        const float corr0 = __shfl_sync(0xffffffffu, corr, 8 * t), corr1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-          const float x[4] = {s[i][0] * lift, s[i][1] * lift, s[i][2] * lift, s[i][3] * lift};
-          const uint32_t h0 = pack_half(x[0], x[1]), h1 = pack_half(x[2], x[3]);
-          const uint32_t l0 = pack_half_lo(x[0], x[1], h0), l1 = pack_half_lo(x[2], x[3], h1);
-          uint32_t av[4] = {0, 0, 0, 0};
+        for (int k = 0; k < NB; ++k) {
+          if (Q41) off[k] *= corr;
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (8 * h < 2 * NB) {
-              const int row = 8 * h + g;
-              if (row < 2 * NB) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (row < NB ? D : 0) + (t * NB + (row < NB ? row : row - NB)) * 8);
-                av[h] = w.x;
-                av[2 + h] = w.y;
-              }
-              if (!clean) {   // nothing of what is behind the last token, nor of what some rows may not see and is not finite (a block's minimum is finite or
-                              // its scale is NaN, and that is in p d)
-                keep_branch();
-                const int at = base + 16 * i + 2 * t;
-                const bool in = there >> i & 1;
-                av[h] = finite_halves(av[h]) & ((in && at < t1 ? 0xffffu : 0u) | (in && at + 1 < t1 ? 0xffff0000u : 0u));
-                av[2 + h] = finite_halves(av[2 + h]) & ((in && at + 8 < t1 ? 0xffffu : 0u) | (in && at + 9 < t1 ? 0xffff0000u : 0u));
-              }
-            }
-          mma_16816(acc, av, h0, h1);
-          mma_16816(acc, av, l0, l1);
+          for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] *= i & 1 ? corr1 : corr0;
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) off[e] = fmaf(off[e], e & 1 ? lifted1 : lifted0, acc[e] * unlift);
       }
       // values
 #pragma unroll
@@ -458,26 +404,46 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int blk = 2 * c + k;
-          float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          // p d, times a power of two that brings the row's largest of this block near the top of fp16
+          float pd[TILES][4], largest = 0.0f, add = 0.0f;
 #pragma unroll
           for (int i = 0; i < TILES; ++i) {
-            float4 d;
+            float d[4], n[4], pn[4];
             if (SHARED) {
-              d = *reinterpret_cast<const float4 *>(floats + (i * (Q41 ? 3 : 2) + 1) * PER_TILE + (t * NB + blk) * 4);
+              const float4 x = *reinterpret_cast<const float4 *>(floats + (i * KINDS + 1) * PER_TILE + (t * NB + blk) * 4);
+              d[0] = x.x; d[1] = x.y; d[2] = x.z; d[3] = x.w;
+              if (Q41) {
+                const float4 y = *reinterpret_cast<const float4 *>(floats + (i * KINDS + 3) * PER_TILE + (t * NB + blk) * 4);
+                n[0] = y.x; n[1] = y.y; n[2] = y.z; n[3] = y.w;
+              }
             } else {
-              const uint2 d2 = *reinterpret_cast<const uint2 *>(tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8);
-              const float2 d01 = half_pair(d2.x), d23 = half_pair(d2.y);
-              d = make_float4(d01.x, d01.y, d23.x, d23.y);
+              scales_of(tiles + i * TILE + PART + 8 * D + (t * NB + blk) * 8, d, n);
             }
-            float pd[4] = {s[i][0] * d.x, s[i][1] * d.y, s[i][2] * d.z, s[i][3] * d.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              pd[i][e] = s[i][e] * d[e];
+              if (Q41) pn[e] = s[i][e] * n[e];
+            }
             if (!clean) {   // (0 times what a scale behind the last token, or of a token that the row does not see, may be)
               keep_branch();
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1) >= min(sees, t1) || !(there >> i & 1)) pd[e] = 0.0f;
+                if (base + 16 * i + 2 * t + (e & 1) + 8 * (e >> 1) >= min(sees, t1) || !(there >> i & 1)) pd[i][e] = pn[e] = 0.0f;
             }
-            const uint32_t h0 = pack_half(pd[0], pd[1]), h1 = pack_half(pd[2], pd[3]);
-            const uint32_t l0 = pack_half_lo(pd[0], pd[1], h0), l1 = pack_half_lo(pd[2], pd[3], h1);
+            if (Q41) add += (pn[0] + pn[1]) + (pn[2] + pn[3]);
+            largest = max_abs(largest, pd[i][0], pd[i][1]);
+            largest = max_abs(largest, pd[i][2], pd[i][3]);
+          }
+          if (Q41) off[blk] += add;
+          largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+          largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+          const float up = to_top_of(largest), down = inverse_power(up);
+          const float down0 = __shfl_sync(0xffffffffu, down, 8 * t), down1 = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+          float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int i = 0; i < TILES; ++i) {
+            const float x0 = pd[i][0] * up, x1 = pd[i][1] * up, x2 = pd[i][2] * up, x3 = pd[i][3] * up;
+            const uint32_t h0 = pack_half(x0, x1), h1 = pack_half(x2, x3), l0 = pack_half_lo(x0, x1, h0), l1 = pack_half_lo(x2, x3, h1);
             uint4 va, vb;
             if (SHARED) {
               va = ops[((i * NC + c) * 8 + 4 + 2 * k) * 32 + lane];
@@ -496,14 +462,13 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[blk][n][e] = fmaf(o[blk][n][e], e & 1 ? lifted1 : lifted0, acc[n][e]);
+            for (int e = 0; e < 4; ++e) o[blk][n][e] = fmaf(acc[n][e], e & 1 ? down1 : down0, o[blk][n][e]);
         }
       }
     }
     // the stage has been read by all the share's warps
     if (row_warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + share), "r"(32 * row_warps) : "memory");
     else __syncwarp();
-    if (SHARED && sub == 0 && lane == 0) largest_scale[share][stage] = 0;   // (two barriers before it is used again)
     if (sub == 0 && ok && base + 2 * step < t1) {
       issue(base + 2 * step, id_next, stage);
       id_next = page_at(base + 3 * step);
@@ -517,17 +482,15 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
   run_sum += __shfl_xor_sync(0xffffffffu, run_sum, 2);
   if (Q41)
 #pragma unroll
-    for (int k = 0; k < NB; ++k)
+    for (int k = 0; k < NB; ++k) {
+      off[k] += __shfl_xor_sync(0xffffffffu, off[k], 1);
+      off[k] += __shfl_xor_sync(0xffffffffu, off[k], 2);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float pm = __shfl_sync(0xffffffffu, off[k / 8 * 2 + j], k % 8 * 4 + t), pd = __shfl_sync(0xffffffffu, off[(NB + k) / 8 * 2 + j], (NB + k) % 8 * 4 + t);
-        const float add = fmaf(8.0f, pd, pm);   // (still times 1 / run_down, as o is)
+        const float add = __shfl_sync(0xffffffffu, off[k], 8 * t + 4 * j);
         o[k][0][j] += add; o[k][0][2 + j] += add; o[k][1][j] += add; o[k][1][2 + j] += add;
       }
-#pragma unroll
-  for (int k = 0; k < NB; ++k)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[k][i >> 2][i & 3] *= run_down;
+    }
   float *so = reinterpret_cast<float *>(ring) + warp * K4_ROWS * D;   // [row][D]
   if (shares > 1) {
     if (__syncthreads_or(!ok)) return;   // no stage is read or filled any more; what did not come is nobody's output
@@ -1908,7 +1871,7 @@ static int kv4_attention_launch(caten_b200_ctx *ctx, const Kv4AttnArgs &a, int64
   } else {
     const bool shared = a.warps == 4;
     // (no less than the sums of all warps where they are joined)
-    const int smem = k4_warps(shared) / a.warps * K4_TILES(NC) * (2 * kv4_tile_bytes(a.s) + (shared ? NC * (8 * 512 + (Q41 ? 3 : 2) * 32 * 4) : 0));
+    const int smem = k4_warps(shared) / a.warps * K4_TILES(NC) * (2 * kv4_tile_bytes(a.s) + (shared ? NC * (8 * 512 + (Q41 ? 4 : 2) * 32 * 4) : 0));
     void (*kernel)(const Kv4AttnArgs) = shared ? kv4_attention_kernel<NC, Q41, true> : kv4_attention_kernel<NC, Q41, false>;
     const int64_t blocks = units / a.row_tiles * ((a.row_tiles + a.warps - 1) / a.warps) * a.parts;
     if (smem > 48 << 10) CB_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
