@@ -110,11 +110,17 @@ __device__ __forceinline__ float to_top(float x, int k = 14) {
 }
 
 // the same for x >= 0, with 2^113 for zero; the inverse of such a power; the largest magnitude (NaN is passed over)
-__device__ __forceinline__ float to_top_of(float x) { return __uint_as_float((uint32_t)min(254 + 14 - (int)(__float_as_uint(x) >> 23), 240) << 23); }
+__device__ __forceinline__ float to_top_of(float x, int k = 14) { return __uint_as_float((uint32_t)min(254 + k - (int)(__float_as_uint(x) >> 23 & 0xff), 240) << 23); }
 __device__ __forceinline__ float inverse_power(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 __device__ __forceinline__ float max_abs(float a, float b, float c) {
   float r;
   asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ float max_abs_nan(float a, float b, float c) {   // (NaN stays)
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -1406,7 +1412,7 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
 // Whole numbers: codes - 8, sixteen times, are signed bytes (a mask and an exclusive or, where fp16 needs an addition besides), the other operand is
 // a fixed-point number of 31 bits in four signed bytes, each a column of its own: column 4 (block % 2) + j of the first product is digit j of q in that
 // block, zero for the other block, so that one accumulator gathers two blocks for 16 tokens and each lane scales the sums of one; in the second product
-// (32 tokens) it is digit j of p d.  Sums are exact; they start at the integer that is 1.5 * 2^23 as a float, and so need no conversion.  A score
+// (32 tokens) it is digit j of p d, times a power of two that a group's largest p d of that block leaves room for.  Sums are exact; they start at the integer that is 1.5 * 2^23 as a float, and so need no conversion.  A score
 // ends up in one lane (64 tokens: two registers a lane), so softmax and p d are not computed eight times over as by rows that are not there.
 // What it is bound by: instructions, then HBM.  (256 x 25 heads x 768 tokens: 139 us with fp16 operands, 261 instructions for 16 tokens of 64 dims.)
 constexpr int K1_MAGIC = 0x4b400000;
@@ -1641,19 +1647,7 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
       }
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        __half2 big = __float2half2_rn(0.0f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          big = __hmax2_nan(big, __habs2(*reinterpret_cast<const __half2 *>(&vd[i][c].x)));
-          big = __hmax2_nan(big, __habs2(*reinterpret_cast<const __half2 *>(&vd[i][c].y)));
-        }
-        const uint32_t bw = *reinterpret_cast<const uint32_t *>(&big);   // (as whole numbers: a NaN is above infinity)
-        uint32_t most = max(bw & 0xffffu, bw >> 16);
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const float up = to_top(__half2float(__ushort_as_half((unsigned short)most)), 29);
-        float add = 0.0f;
-        uint32_t digits[4];   // of the four tiles
+        float pd[4][4], most = 0.0f, add = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float2 d01 = half_pair(vd[i][c].x), d23 = half_pair(vd[i][c].y);
@@ -1664,8 +1658,16 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
             add = fmaf(p[i][2], fmaf(8.0f, d23.x, m23.x), add);
             add = fmaf(p[i][3], fmaf(8.0f, d23.y, m23.y), add);
           }
-          digits[i] = digits_of(p[i][0] * (d01.x * up), p[i][1] * (d01.y * up), p[i][2] * (d23.x * up), p[i][3] * (d23.y * up), pick);
+          pd[i][0] = p[i][0] * d01.x; pd[i][1] = p[i][1] * d01.y; pd[i][2] = p[i][2] * d23.x; pd[i][3] = p[i][3] * d23.y;
+          most = max_abs_nan(most, pd[i][0], pd[i][1]);
+          most = max_abs_nan(most, pd[i][2], pd[i][3]);
         }
+        most = max_abs_nan(most, __shfl_xor_sync(0xffffffffu, most, 1), 0.0f);
+        most = max_abs_nan(most, __shfl_xor_sync(0xffffffffu, most, 2), 0.0f);
+        const float up = to_top_of(most, 29);
+        uint32_t digits[4];   // of the four tiles
+#pragma unroll
+        for (int i = 0; i < 4; ++i) digits[i] = digits_of(pd[i][0] * up, pd[i][1] * up, pd[i][2] * up, pd[i][3] * up, pick);
         if (Q41) off[c] = fmaf(off[c], corr, add);
         int acc[2][4];
 #pragma unroll
@@ -1693,7 +1695,7 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
           }
         }
         // (a scale that is not finite makes its block's values NaN, as it does in the formula)
-        const float down = __shfl_sync(0xffffffffu, most < 0x7c00u ? 0.0625f / up : NAN, 16 * (t >> 1));
+        const float down = __shfl_sync(0xffffffffu, most < INFINITY ? 0.0625f * inverse_power(up) : NAN, 16 * (t >> 1));
         const float f0 = down * w0, f1 = down * w1, n0 = -K1_MAGIC_F * f0, n1 = -K1_MAGIC_F * f1;
 #pragma unroll
         for (int n = 0; n < 2; ++n)

@@ -476,7 +476,7 @@ def spare_for(rows, heads, dim, page):
 
 
 @pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
-@pytest.mark.parametrize("heads,kv,dim,news", FEW_ROWS + EIGHT_ROWS)
+@pytest.mark.parametrize("heads,kv,dim,news", ONE_ROW + FEW_ROWS + EIGHT_ROWS)
 def test_values_a_row_has_no_part_in_do_not_cost_it_bits(rt, kind, heads, kv, dim, news):
     """Tokens and blocks of 32 dims whose values are 1e8 times others': each block of a row is as close as its own sum of p |v| allows, whether the large values
     are behind the row's last token, have probabilities next to none, or are other dims'."""
