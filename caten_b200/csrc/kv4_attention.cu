@@ -878,19 +878,29 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
 // 128 rows of a key head are the lanes of tensor memory, 64 tokens a step; a step's products are tcgen05.mma on fp16 halves, 22 bits of each operand:
 //   S = Q_hi K_hi^T + Q_hi K_lo^T + Q_lo K_hi^T        O = P_hi V_hi + P_lo V_hi + P_hi V_lo
 // (lo lo, 2^-22 of a product, is left out).  Scales are multiplied in before (d (code - 8) has 15 bits, so for Q4_0 two halves hold it exactly), a step's
-// keys and its values times a power of two each that brings the largest near the top of fp16.  S, P and O lie in tensor memory; a row's two threads
-// (warps w and w + 4) take half of the tokens and half of the dims each, and keep the running output in registers, so that a moved maximum costs nothing
-// more.  A value that is not finite would reach rows that do not see it (0 times NaN): it is zero in the product, and NaN is put into the blocks of the rows
-// that see it.  By warp:
+// keys and 64 dims of its values times a power of two each that brings the largest near the top of fp16; P takes the values' size in exchange, so that
+// steps of large values without probability do not cost others their bits.  Where the values of one step are far apart each row adds up what that may
+// have cost it, and a tile in which a row has lost too much is worked out again without tensor cores (kv4_prompt_plainly).  S, P and O lie in tensor memory; a
+// row's two threads (warps w and w + 4) take half of the tokens and half of the dims each, and keep the running output in registers, so that a moved maximum
+// costs nothing more.  A value that is not finite would reach rows that do not see it (0 times NaN): it is zero in the product, and NaN is put into the
+// blocks of the rows that see it.  By warp:
 //   0 .. 7     rows of q; softmax of a step, its P, and the output of the step before
 //   8 .. 14    codes into operands, two steps ahead at most (two stages each); the last asks for the tiles of the step after
 //   15         issues the products: S a step ahead of the softmax
 // A step takes 3.4 k cycles with heads of 64, 4.4 k of 128, of them 1.0 and 1.8 k of products; what bounds it is the instructions of warps 0 to 14 (0.5 a
 // cycle and scheduler), unpacking before the softmax.  All phases by eight warps one after the other: 6.4 and 6.7 k; four warps to unpack: 195 us in place
 // of 135 for 600 tokens over 2000, 32 heads of 128 over 8; two units at a time in registers: 130 in place of 127 (the code no longer fits the
-// instruction cache).  That case 127 us now (tiles of 8 rows 271), 2000 of 25 heads of 64 111 (201), 5 prompts of 333, 16 heads of 128 over 4, 30 (67).
+// instruction cache).  That case 133 us now (tiles of 8 rows 271), 2000 of 25 heads of 64 113 (201), 5 prompts of 167 to 333 over up to 1200, 16 heads
+// of 128 over 4, 62 (Q4_1 153, 123 and 69).
 constexpr int K3_THREADS = 512, K3_SOFTMAX = 8, K3_CONVERT = 7;   // (warps)
 constexpr float K3_LIFT = 14.0f;   // p is taken times 2^14, its sum with it
+// A step's keys share a power of two, and 64 dims of its values.  Which sizes they have is a bit for each four exponents, from 2^-27 (what is stored is
+// zero or 2^-24 at least) to 2^25: bit i is 2^(4i - 27) to 2^(4i - 23).  What is more than three bits below the largest would have less than 20 bits.
+constexpr int K3_SPREAD = 3;
+__device__ __forceinline__ unsigned k3_of_size(float x) { return x == 0.0f ? 0u : 1u << ((__float_as_uint(x) >> 25) - 25); }
+// what brings the largest size to [2^11, 2^15); its exponent, the upper one (none: below all that can be stored)
+__device__ __forceinline__ float k3_up(unsigned sizes) { return __uint_as_float((uint32_t)(127 + 38 - 4 * (31 - __clz(sizes | 1u))) << 23); }
+__device__ __forceinline__ int k3_exponent(unsigned sizes) { return sizes ? 4 * (31 - __clz(sizes)) - 24 : -26; }
 __host__ __device__ constexpr int k3_smem(int chunks, int tile_bytes) { return chunks * (32768 + 2 * 16384 + 2 * 16384) + 2 * 4 * tile_bytes + 1024; }
 // of an operand tile: rows of 64 halves, 128-byte swizzle
 __device__ __forceinline__ uint32_t k3_at(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
@@ -909,6 +919,64 @@ __device__ __forceinline__ void k3_split(uint32_t codes, uint32_t dd, float2 d, 
   }
 }
 
+// The rows of a tile in fp32 and without tensor cores, a row a warp at a time: where a step has keys or values too far apart for halves that share a power
+// of two, and a row's output is so small beside them that it counts.  Sixteen tokens make sums of their own.  (Some seventy times as long.)
+template <int NC, bool Q41>
+__device__ __forceinline__ void kv4_prompt_plainly(const Kv4AttnArgs &a, const Kv4Seq &seq, int b, int head, int rt, int part) {
+  constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D;
+  const int lane = threadIdx.x & 31, count = seq.count * a.group, t0 = part * a.part_tokens;
+  const int tile_shift = a.s.page == 16 ? 0 : a.s.page == 32 ? 1 : a.s.page == 64 ? 2 : 3;
+  for (int row = threadIdx.x >> 5; row < K3_ROWS; row += K3_THREADS / 32) {
+    const int r = rt * K3_ROWS + row;
+    if (r >= count) break;
+    const int64_t token = seq.first + r / a.group;
+    const int column = (head * a.group + r % a.group) * D, t1 = min(t0 + a.part_tokens, max(0, seq.length - seq.count + r / a.group + 1));
+    float q[NB], o[NB], run_max = -INFINITY, run_sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      q[k] = a.q[token * a.ldq + column + 32 * k + lane] * (a.scale * 1.4426950408889634f);
+      o[k] = 0.0f;
+    }
+    for (int base = t0; base < t1; base += 16) {
+      const int id = a.table[(int64_t)b * a.max_pages + (base >> 4 >> tile_shift)], n = min(16, t1 - base);
+      if (!kv4_page_ok(a.s, id)) continue;   // (reported by the copies)
+      const uint8_t *keys = a.pool + kv4_tile_at(a.s, id, head, base & (a.s.page - 1)), *values = keys + PART;
+      auto value = [&](const uint8_t *tile, int at, int k, int byte) {   // of token `at`, dim 32 k + lane
+        const __half *sc = reinterpret_cast<const __half *>(tile + 8 * D) + kv4_scale_index(at, k, D);
+        const float d = __half2float(sc[0]), code = (float)((tile[byte] >> (lane & 1) * 4 & 15) - 8);
+        return Q41 ? fmaf(d, code, fmaf(8.0f, d, __half2float(sc[D / 2]))) : d * code;
+      };
+      float s = -INFINITY;
+      for (int at = 0; at < n; ++at) {
+        float x = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NB; ++k) x = fmaf(q[k], value(keys, at, k, kv4_k_byte(at, 32 * k + lane)), x);
+        x = warp_sum(x);
+        if (lane == at) s = x;
+      }
+      const float top = fmaxf(run_max, warp_max(s)), ref = top == -INFINITY ? 0.0f : top, corr = exp2_fast(run_max - ref), p = exp2_fast(s - ref);
+      run_max = top;
+      run_sum = fmaf(run_sum, corr, warp_sum(p));
+      float sums[NB];
+#pragma unroll
+      for (int k = 0; k < NB; ++k) sums[k] = 0.0f;
+      for (int at = 0; at < n; ++at) {
+        const float w = __shfl_sync(0xffffffffu, p, at);
+#pragma unroll
+        for (int k = 0; k < NB; ++k) sums[k] = fmaf(w, value(values, at, k, kv4_v_byte(at, 32 * k + lane)), sums[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < NB; ++k) o[k] = fmaf(o[k], corr, sums[k]);
+    }
+    float *dst = a.parts == 1 ? a.out + token * a.heads * D + column
+                              : a.part + (((((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt) * a.parts + part) * K3_ROWS + row) * (D + 2);
+    const float scale = a.parts > 1 ? 1.0f : run_sum == 0.0f ? 0.0f : 1.0f / run_sum;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) dst[32 * k + lane] = o[k] * scale;
+    if (a.parts > 1 && lane == 0) { dst[D] = run_max; dst[D + 1] = run_sum; }
+  }
+}
+
 template <int NC, bool Q41>
 __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(const Kv4AttnArgs a) {
   constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, TILE = 2 * PART, HALF = D / 2;
@@ -919,12 +987,14 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
   __shared__ float qfactor[K3_ROWS];
   __shared__ int64_t q_at[K3_ROWS], out_at[K3_ROWS];   // where rows begin (divided once)
   // of four steps each, so that nobody need wait for their readers
-  __shared__ float downs[4], ups[4];          // what scores are to be multiplied with; what values were taken times
+  __shared__ float downs[4], ups[4][NC];      // what scores are to be multiplied with; what 64 dims of values were taken times
+  __shared__ int size[4];                     // exponent of the values' largest
   __shared__ unsigned bad[4][64], any_bad[4][2];   // blocks of values that are not finite, by token; whether there are any, by half
   // of two steps: scales (of values, of an even and an odd block), minima (of keys, + 8 d)
   __shared__ float k_scale[2][64][NB], k_off[2][64][Q41 ? NB : 1];
   __shared__ uint32_t v_scale[2][64][NC], v_min[2][64][Q41 ? NC : 1];
-  __shared__ float largest[2][4];             // of keys and of values, by half of the tokens
+  __shared__ __align__(8) unsigned k_sizes[4][2], v_sizes[4][NC][2];   // which sizes (k3_of_size) there are, by half of the tokens: of keys; of 64 dims of values
+  __shared__ int wide[4], uneven;             // whether sizes are far apart (bit c: of the values' dims 64 c on; bit NC: of keys); whether that costs a row
   __shared__ unsigned theres[4];
   __shared__ unsigned present[2];                    // tiles of each stage
   __shared__ uint64_t bar_mem[17];
@@ -969,7 +1039,7 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
     mbar_init(q_full, K3_SOFTMAX);
     mbar_init(p_full, K3_SOFTMAX);
     mbar_init(o_full, 2);
-    gave_up[0] = gave_up[1] = 0;
+    gave_up[0] = gave_up[1] = uneven = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
@@ -1058,7 +1128,7 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
         // What scores are multiplied with stays a power of two: then that product is exact and a row's largest score less itself is zero however large it
         // is (fused with the subtraction, from scores of 1e8 on, it was off by more than fp16 holds).  The rest of scale log2(e), in [1, 2), goes into q.
         const float up = to_top(top, 13), power = fmaxf(__uint_as_float(__float_as_uint(scale2) & 0x7f800000u), 0x1p-126f), sign_up = scale2 * (1.0f / power) * up;
-        if (chunk == 0) qfactor[q_row] = power * (1.0f / up);
+        if (chunk == 0) qfactor[q_row] = top > 0.0f ? power * (1.0f / up) : 0.0f;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1073,6 +1143,7 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
     }
     fence_proxy_async();
   };
+  auto both = [](const unsigned *x) { const uint2 y = *reinterpret_cast<const uint2 *>(x); return y.x | y.y; };
   // a step's scales, a token a thread: warps 0 and 1 those of keys, 2 and 3 of values (what stands behind the last token, or is not finite, is zero)
   auto scales = [&](int step, int cw) {
     const int st = step & 1, token = (cw & 1) * 32 + lane, tk = token & 15;
@@ -1085,27 +1156,32 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
       d[blk] = *reinterpret_cast<const uint16_t *>(tile + at);
       m[blk] = Q41 ? *reinterpret_cast<const uint16_t *>(tile + D + at) : 0;
     }
-    float top = 0.0f;
     if (cw < 2) {
-      float x[NB], y[NB];
+      unsigned sizes = 0;
 #pragma unroll
       for (int blk = 0; blk < NB; ++blk) {
-        x[blk] = half_pair(d[blk]).x;
-        y[blk] = Q41 ? fmaf(8.0f, x[blk], half_pair(m[blk]).x) : 0.0f;
-        const float most = fmaf(8.0f, fabsf(x[blk]), fabsf(y[blk]));
-        if (in && most < INFINITY) top = fmaxf(top, most);
-        k_scale[st][token][blk] = x[blk];
-        if (Q41) k_off[st][token][blk] = y[blk];
+        const float x = half_pair(d[blk]).x, y = Q41 ? fmaf(8.0f, x, half_pair(m[blk]).x) : 0.0f, most = fmaf(8.0f, fabsf(x), fabsf(y));
+        if (in && most < INFINITY) sizes |= k3_of_size(most);
+        k_scale[st][token][blk] = x;
+        if (Q41) k_off[st][token][blk] = y;
       }
+      sizes = __reduce_or_sync(0xffffffffu, sizes);
+      if (lane == 0) k_sizes[step & 3][cw] = sizes;
     } else {
-      unsigned lost = 0;
+      unsigned lost = 0, sizes[NC];
 #pragma unroll
       for (int blk = 0; blk < NB; ++blk) {
         const uint32_t x = in ? finite_halves(d[blk]) : 0u, y = in ? finite_halves(m[blk]) : 0u;
         if (in && (x != d[blk] || y != m[blk])) lost |= 1u << blk;
         d[blk] = x;
         m[blk] = y;
-        top = fmaxf(top, fmaf(Q41 ? 16.0f : 8.0f, fabsf(half_pair(x).x), fabsf(half_pair(y).x)));
+        const unsigned of = k3_of_size(fmaf(Q41 ? 16.0f : 8.0f, fabsf(half_pair(x).x), fabsf(half_pair(y).x)));
+        sizes[blk / 2] = blk % 2 ? sizes[blk / 2] | of : of;
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        sizes[c] = __reduce_or_sync(0xffffffffu, sizes[c]);
+        if (lane == 0) v_sizes[step & 3][c][cw & 1] = sizes[c];
       }
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -1116,8 +1192,6 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
       const unsigned any = __any_sync(0xffffffffu, lost);
       if (lane == 0) any_bad[step & 3][cw & 1] = any;
     }
-    top = warp_max(top);
-    if (lane == 0) largest[st][cw] = top;
   };
   // keys of a tile and a block
   auto convert_k = [&](int st, int unit, float up) {
@@ -1138,8 +1212,9 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
     }
   };
   // values of a tile, 64 dims and half of the tokens
-  auto convert_v = [&](int st, int unit, float up) {
+  auto convert_v = [&](int st, int unit, const float (&ups)[NC]) {
     const int i = unit / (2 * NC), c = unit / 2 % NC, h = unit % 2;   // tokens 2t + 8 h, 2t + 8 h + 1
+    const float up = NC == 1 || c == 0 ? ups[0] : ups[NC - 1];
     const uint2 w = *reinterpret_cast<const uint2 *>(raw + (st * 4 + i) * TILE + PART + c * 512 + lane * 16 + 8 * h);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {   // (even, odd block) in the halves of each operation
@@ -1166,17 +1241,20 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
   };
 
   float o[HALF], run_max = -INFINITY, run_ref = -INFINITY, run_sum = 0.0f, run_down = 1.0f, lifted = 0.0f;   // (run_sum: this thread's tokens)
+  float lost_bits = 0.0f;   // what o may be off because of steps in which values are far apart
 #pragma unroll
   for (int e = 0; e < HALF; ++e) o[e] = 0.0f;
-  auto take_outputs = [&](int step, float lift) {
+  auto take_outputs = [&](int step) {
 #pragma unroll
     for (int e0 = 0; e0 < HALF; e0 += 16) {
       uint32_t x[16];
       tmem_ld16(tlane + COL_O + HALF * hf + e0, x);
       tmem_ld_wait();
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[e0 + e] = fmaf(o[e0 + e], lift, __uint_as_float(x[e]));
+      for (int e = 0; e < 16; ++e) o[e0 + e] = fmaf(o[e0 + e], lifted, __uint_as_float(x[e]));
     }
+    // (64 tokens, each half a step of P's and of V's last bits, 2^-25, times the other's largest, 2^15 and 2^14)
+    lost_bits = fmaf(lost_bits, lifted, wide[step & 3] >> (NC == 1 ? 0 : hf) & 1 ? 0x1p-3f : 0.0f);
     if (any_bad[step & 3][0] | any_bad[step & 3][1])
       for (int k = 0; k < 64; ++k) {
         const unsigned blocks = bad[step & 3][k];
@@ -1205,20 +1283,36 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
         if (cw < 4) scales(step, cw);
       }
       asm volatile("bar.sync 5, %0;" ::"n"(32 * K3_CONVERT) : "memory");   // also: the step before has been read
-      const float up_k = to_top(fmaxf(largest[st][0], largest[st][1])), up = to_top(fmaxf(largest[st][2], largest[st][3]));
+      const float up_k = k3_up(both(k_sizes[step & 3]));
+      float up[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) up[c] = k3_up(both(v_sizes[step & 3][c]));
       if (cw == K3_CONVERT - 1 && ok) {
         if (step > 0 && asked < steps) {
           issue(asked, id_next);
           ++asked;
           id_next = page_at(asked);
         }
-        if (lane == 0) { ups[step & 3] = up; downs[step & 3] = 1.0f / up_k; theres[step & 3] = present[st]; }
+        if (lane == 0) theres[step & 3] = present[st];
       }
       // units of K, then of V, dealt as one row (32 of heads of 128)
       int unit = cw;
       if (wait(k_empty(st), phase ^ 1u)) {
 #pragma unroll 1
         for (; unit < 8 * NC; unit += K3_CONVERT) convert_k(st, unit, up_k);
+        if (cw == K3_CONVERT - 2) {   // what the softmax has to know of the step's scales, by a warp with fewer units
+          unsigned sizes = 0;
+          if (lane < NC) sizes = both(v_sizes[step & 3][lane]);
+          if (lane == NC) sizes = both(k_sizes[step & 3]);
+          const int exponent = k3_exponent(__reduce_or_sync(0xffffffffu, lane < NC ? sizes : 0u));
+          if (lane < NC) ups[step & 3][lane] = k3_up(sizes);
+          if (lane == NC) {
+            downs[step & 3] = inverse_power(up_k);
+            size[step & 3] = exponent;
+          }
+          const unsigned far = __ballot_sync(0xffffffffu, sizes && 31 - __clz(sizes) - (__ffs(sizes) - 1) > K3_SPREAD);
+          if (lane == 0) wide[step & 3] = (int)far;
+        }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(k_full(st));
@@ -1304,6 +1398,8 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
         tc_fence_after();
         const unsigned there = theres[step & 3];
         f = fmaxf(factor * downs[step & 3], 1.17549435e-38f);   // (positive: it multiplies infinities)
+        // a score is off by no more than 2^-3 f for the last bits of keys: as many of them as are too few matter only where scores may be millions
+        if (wide[step & 3] >> NC & 1 && f > 0x1p-17f && sees > 0) uneven = 1;
         tmem_ld16(tlane + 64 * st + 32 * hf, x);
         tmem_ld16(tlane + 64 * st + 32 * hf + 16, x + 16);
         tmem_ld_wait();
@@ -1323,9 +1419,13 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
       }
       asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");   // warps quad and quad + 4
       if (!ok) continue;
-      top = fmaxf(run_max, fmaxf(red[st][0][row], red[st][1][row]) * f);
-      const float ref = top == -INFINITY ? 0.0f : __fsub_ru(top, K3_LIFT);   // (upwards: of a top of 1e9 only a part can be taken off)
-      const float corr = exp2_fast(run_ref - ref), up = ups[step & 3];
+      // P is p times 2^size, so that beside the row's largest it has the bits that it counts for.  (From scores of some millions on, which leave no room for
+      // that and give one token all of p, without; and ref is rounded upwards, for then only a part of 14 can be taken off.)
+      const float most = fmaxf(red[st][0][row], red[st][1][row]) * f;
+      const int exponent = fabsf(most) < 0x1p22f ? size[step & 3] : 0;
+      top = fmaxf(run_max, most + (float)exponent);
+      const float ref = top == -INFINITY ? 0.0f : __fsub_ru(top, K3_LIFT), less = (float)exponent - ref;
+      const float corr = exp2_fast(run_ref - ref);
       run_max = top;
       run_ref = top == -INFINITY ? top : ref;
       float sum = 0.0f;
@@ -1335,7 +1435,7 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float y = exp2_fast(fmaf(__uint_as_float(x[2 * (e0 + e)]), f, -ref)), z = exp2_fast(fmaf(__uint_as_float(x[2 * (e0 + e) + 1]), f, -ref));
+          const float y = exp2_fast(fmaf(__uint_as_float(x[2 * (e0 + e)]), f, less)), z = exp2_fast(fmaf(__uint_as_float(x[2 * (e0 + e) + 1]), f, less));
           sum += y + z;
           hi[e] = pack_half(y, z);
           lo[e] = pack_half_lo(y, z, hi[e]);
@@ -1343,14 +1443,15 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
         tmem_st8(tlane + COL_P + 64 * st + 16 * hf + e0, hi);   // token k in half k % 2 of column k / 2
         tmem_st8(tlane + COL_P + 64 * st + 32 + 16 * hf + e0, lo);
       }
-      run_sum = fmaf(run_sum, corr, sum);
+      run_sum = fmaf(run_sum, corr, sum * __uint_as_float((uint32_t)(127 - exponent) << 23));
       if (step > 0) {
         if (!wait(o_full, (uint32_t)(step - 1) & 1u)) continue;
         tc_fence_after();
-        take_outputs(step - 1, lifted);
+        take_outputs(step - 1);
       }
+      const float up = ups[step & 3][NC == 1 ? 0 : hf] * __uint_as_float((uint32_t)(127 + exponent) << 23);
       lifted = corr * (up * run_down);
-      run_down = 1.0f / up;
+      run_down = inverse_power(up);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -1358,17 +1459,27 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
     }
     if (steps && wait(o_full, (uint32_t)(steps - 1) & 1u)) {
       tc_fence_after();
-      take_outputs(steps - 1, lifted);
+      take_outputs(steps - 1);
     }
   }
+  if (lost_bits > 0.0f)
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      float most = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) most = fmaxf(most, fabsf(o[32 * k + e]));
+      if (most > 0.0f && lost_bits > 0x1p-19f * most && sees > 0) uneven = 1;   // (zero: all of these dims' values are)
+    }
   tc_fence_before();
   const bool failed = __syncthreads_or(!ok);
+  if (uneven && !failed) kv4_prompt_plainly<NC, Q41>(a, seq, b, head, rt, part);
 
   // rows go out by way of shared memory (all products have been read): 32 dims of 128 rows are 16 KB
   const bool rows_warp = warp < K3_SOFTMAX;
   if (rows_warp) red[0][hf][row] = run_sum;
   unsigned char *const so = sq;
-  if (!failed && rows_warp)
+  const bool writes = !failed && !uneven;
+  if (writes && rows_warp)
 #pragma unroll
     for (int e = 0; e < HALF; e += 4)
       *reinterpret_cast<float4 *>(so + (hf * NC + e / 32) * 16384 + k3_at(row, e % 32 / 4)) =
@@ -1377,14 +1488,14 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
   if (warp < 4) {
     const float sum = red[0][0][row] + red[0][1][row];
     red[1][0][row] = a.parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (a.parts > 1 && !failed && r0 + row < count) {
+    if (a.parts > 1 && writes && r0 + row < count) {
       float *dst = a.part + out_at[row] + D;
       dst[0] = run_ref;   // (what outputs and sum are relative to)
       dst[1] = sum;
     }
   }
   __syncthreads();
-  if (!failed && rows_warp) {
+  if (writes && rows_warp) {
     constexpr int LANES = D / 4, ROWS = 32 / LANES;
     const int piece = lane % LANES;
     const bool wide = a.parts == 1 && ((uintptr_t)a.out & 15) == 0;

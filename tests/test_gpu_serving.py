@@ -476,7 +476,7 @@ def spare_for(rows, heads, dim, page):
 
 
 @pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
-@pytest.mark.parametrize("heads,kv,dim,news", ONE_ROW + FEW_ROWS + EIGHT_ROWS)
+@pytest.mark.parametrize("heads,kv,dim,news", ONE_ROW + FEW_ROWS + EIGHT_ROWS + MANY_ROWS)
 def test_values_a_row_has_no_part_in_do_not_cost_it_bits(rt, kind, heads, kv, dim, news):
     """Tokens and blocks of 32 dims whose values are 1e8 times others': each block of a row is as close as its own sum of p |v| allows, whether the large values
     are behind the row's last token, have probabilities next to none, or are other dims'."""
@@ -504,6 +504,70 @@ def test_values_a_row_has_no_part_in_do_not_cost_it_bits(rt, kind, heads, kv, di
     away = np.where(against > 1, -30.0, 0.0).astype(np.float32) / (c.desc.scale * (same[0, 0] ** 2).sum())
     refill(rt, c, kind, (k * 0.05 + same[0, 0] * away).astype(np.float32), v * against)
     check_closely(rt, c, same, [news] * 3)
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("heads,kv,dim,news", MANY_ROWS)
+def test_small_keys_beside_large_ones_that_are_never_chosen(rt, kind, heads, kv, dim, news):
+    """Every third key far against the queries, so that it has no probability, and 1e10 times as large as the others, whose scores decide."""
+    rng = rng_of(73, heads, dim)
+    c = Cache(rt, rng, kind, dim, 16, heads, kv, [160, 160], spare=spare_for(news, heads, dim, 16))
+    k, v = (rng.standard_normal((320, kv, dim), dtype=np.float32) for _ in range(2))
+    q = rng.standard_normal((2 * news, heads, dim), dtype=np.float32) * 5e4 + 1.5e5
+    large = 4e5 if kind == "q4_0" else 5e4   # (of what the format holds)
+    k = np.where(np.arange(320)[:, None, None] % 3 == 1, large * (-1 + 0.05 * k), k * 4e-6).astype(np.float32)
+    refill(rt, c, kind, k, v)
+    check_closely(rt, c, q, [news] * 2)
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("heads,kv,dim,spread", [(4, 1, 128, 0), (2, 2, 64, 0), (4, 1, 128, 400)])
+def test_prompts_over_values_far_apart(rt, kind, heads, kv, dim, spread):
+    """A few tokens whose keys or values halves of a common power of two cannot hold beside the others', with a token that is not finite behind them and a page that
+    is none: each row is as close as ever, later tokens do not matter, and the page is reported."""
+    rng = rng_of(72, heads, dim)
+    lengths, news = [300 + spread, 150], [150, 150]
+    c = Cache(rt, rng, kind, dim, 16, heads, kv, lengths, spare=0 if spread else columns_for(300, heads, dim, 16))
+    shape = (sum(lengths), kv, dim)
+    k, v = (rng.standard_normal(shape, dtype=np.float32) for _ in range(2))
+    k[20], v[21], v[130], k[295 + spread] = k[20] * 1e-4, v[21] * 1e-6, v[130] * 1e4, k[295 + spread] * 30   # (k of 30: a score of hundreds)
+    refill(rt, c, kind, k, v)
+    q = rng.standard_normal((300, heads, dim), dtype=np.float32) * 0.3
+    q[:, :, :32] = 0                                     # the large keys are elsewhere
+    top = max(lengths)
+    clean = check_closely(rt, c, q, news, max_length=top if spread else 0)
+    np.testing.assert_array_equal(check_closely(rt, c, q, news, max_length=top if spread else 0), clean)
+
+    def run(table=c.table):
+        return rt.kv4_attention(c.desc, put(rt, q.reshape(300, -1)), c.pool, put(rt, table, np.int32), put(rt, lengths, np.int32), put(rt, [0, 150, 300], np.int32), max_new=150,
+                                max_length=top if spread else 0).numpy().reshape(300, heads, dim)
+    token = 240 + spread                                 # row 90
+    for which in range(2):
+        rows = [np.zeros((1, kv * dim), np.float32) for _ in range(2)]
+        rows[which][0, 40::dim] = np.nan
+        slot = put(rt, [c.table[0, token // 16] * 16 + token % 16], np.int32)
+        kept = rt.kv4_load(c.desc, c.pool, slot)
+        rt.kv4_store(c.desc, c.pool, put(rt, rows[0]), put(rt, rows[1]), slot)
+        out = run()
+        np.testing.assert_array_equal(out[:90], clean[:90])
+        np.testing.assert_array_equal(out[150:], clean[150:])
+        assert np.isnan(out[90:150, :, 32:64]).all()
+        rt.kv4_store(c.desc, c.pool, *kept, slot)
+    table = c.table.copy()
+    table[0, 2] = -1                                     # tokens 32 to 47 count for nothing
+    out = rt.kv4_attention(c.desc, put(rt, q.reshape(300, -1)), c.pool, put(rt, table, np.int32), put(rt, lengths, np.int32), put(rt, [0, 150, 300], np.int32), max_new=150,
+                           max_length=top if spread else 0)
+    with pytest.raises(B200Error) as e:
+        rt.sync()
+    assert e.value.code == L.EDEVICE
+    out = out.numpy().reshape(300, heads, dim)
+    there = (np.arange(lengths[0]) < 32) | (np.arange(lengths[0]) >= 48)
+    part = slice(0, lengths[0])
+    if kind == "q4_0":                                   # (its own values were stored back as they are)
+        want = ref.attention(q[:150], c.k[part][there], c.v[part][there], lengths[0] - 16, c.desc.scale)
+        tol = ref.attention_bound(q[:150], c.k[part][there], c.k_parts[part][there], c.v_parts[part][there], lengths[0] - 16, c.desc.scale)
+        assert (np.abs(out[:150] - want) <= tol).all()
+        np.testing.assert_array_equal(out[150:], clean[150:])
 
 
 @pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
