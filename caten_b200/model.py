@@ -107,7 +107,11 @@ def beam_search(model: Model, prompt_ids, beams: int, max_length: int = 100, eos
     if beams <= 0 or model.batch % beams:
         raise ValueError(f"beam_search: {beams} beams over a batch of {model.batch}")
     rt, groups = model.rt, model.batch // beams
-    prompt = np.ascontiguousarray(prompt_ids, dtype=np.int64).reshape(groups, -1)
+    prompt = np.asarray(prompt_ids, dtype=np.int64)
+    if prompt.ndim == 1 and groups == 1:
+        prompt = prompt[None]
+    if prompt.ndim != 2 or prompt.shape[0] != groups:
+        raise ValueError(f"beam_search: prompts {prompt.shape} for {groups} of {beams} beams each")
     n = prompt.shape[1]
     if max_length <= 0:
         return np.repeat(prompt[:, None], beams, 1), np.zeros((groups, beams), np.float32)

@@ -347,3 +347,90 @@ def test_command_refuses_beams_it_cannot_have():
     for bad in (["--beams", "33"], ["--beams", "-1"], ["--beams", "4", "--temperature", "1"]):
         with pytest.raises(SystemExit):
             main(["--model", "none", "--ids", "1"] + bad)
+
+
+class HostRuntime:
+    """The runtime calls of ``beam_search`` on host arrays, which are counted."""
+
+    class Buffer:
+        def __init__(self, rt, a):
+            self.rt, self.a = rt, a
+            rt.open.append(self)
+
+        def view(self, at, shape):
+            v = object.__new__(type(self))
+            v.rt, v.a = self.rt, self.a.reshape(-1)[at:at + int(np.prod(shape))].reshape(shape)
+            return v
+
+        def numpy(self):
+            return self.a
+
+        def close(self):
+            self.rt.open.remove(self)
+
+    def __init__(self):
+        self.open, self.selects = [], 0
+
+    def open_buffer(self, shape, kind=np.float32):
+        return self.Buffer(self, np.zeros(shape, kind))
+
+    def transfer_from_array(self, a):
+        return self.Buffer(self, a.copy())
+
+    def beam_select_work(self, *sizes):
+        return 8
+
+    def beam_select(self, logits, scores, keep, ended=None, eos=-1, out=None, work=None):
+        self.selects += 1
+        for r, s in enumerate(scores.a):
+            x = logits.reshape(len(scores.a), -1, logits.shape[-1])[r]
+            for o, w in zip(out, ref.select(x, s, ended.a[r] if ended else np.zeros(len(s)), eos, keep)):
+                o.a[r] = w
+
+    def beam_reorder(self, states, parents, positions):
+        for x in states:
+            x[:] = x.reshape(len(parents.a), -1, x.shape[-1])[np.arange(len(parents.a))[:, None], parents.a].reshape(x.shape)
+
+
+def host_model(batch, vocab=20, length=16, fails_at=None):
+    """A model whose "cache" is the tokens that it has read, with logits that are a function of them."""
+    from caten_b200.model import Model
+
+    class Host(Model):
+        def __init__(self):
+            self.rt, self.batch, self.vocab_size, self.max_seq_len, self.read, self.steps = HostRuntime(), batch, vocab, length, np.zeros((batch, length), np.int64), 0
+
+        def _step(self, tokens, n):
+            self.steps += 1
+            if self.steps == fails_at:
+                raise RuntimeError("a step that fails")
+            self.read[:, n:n + tokens.shape[1]] = tokens
+            self.logits_now = np.stack([np.random.Generator(np.random.PCG64(list(r[:n + tokens.shape[1]]))).standard_normal(vocab).astype(np.float32) * 3 for r in self.read])
+            return self.logits_now.argmax(1)
+
+        def _step_device(self, ids, s, n, out):
+            out.a[:] = self._step(ids.a.reshape(batch, s), n)
+
+        def _logits_buffer(self):
+            return self.logits_now
+
+        def _caches(self):
+            return [self.read]
+    return Host()
+
+
+def test_beam_search_takes_a_prompt_a_group():
+    """On a model of host arrays: each prompt's hypotheses are its own, and prompts that are not one a group are refused, not cut anew."""
+    from caten_b200.model import beam_search
+    prompts = np.array([[1, 2, 3], [4, 5, 6]])
+    both = beam_search(host_model(6), prompts, 3, 5)
+    for g in range(2):
+        one = beam_search(host_model(3), prompts[g], 3, 5)
+        np.testing.assert_array_equal(both[0][g], one[0][0])
+        np.testing.assert_array_equal(both[1][g], one[1][0])
+    assert (both[0][:, :, :3] == prompts[:, None]).all()
+    for bad in (np.arange(8).reshape(4, 2), np.arange(6).reshape(1, 6), np.arange(6), np.arange(12).reshape(2, 3, 2)):
+        m = host_model(6)
+        with pytest.raises(ValueError):
+            beam_search(m, bad, 3, 5)
+        assert m.steps == 0
