@@ -115,27 +115,36 @@ def beam_search(model: Model, prompt_ids, beams: int, max_length: int = 100, eos
     n = prompt.shape[1]
     if max_length <= 0:
         return np.repeat(prompt[:, None], beams, 1), np.zeros((groups, beams), np.float32)
+    if eos >= model.vocab_size or n + max_length - 1 > model.max_seq_len:
+        raise ValueError(f"beam_search: eos {eos} of {model.vocab_size} ids, {n} + {max_length} tokens over {model.max_seq_len} positions")
+    need = rt.beam_select_work(groups, beams, model.vocab_size, beams)   # (refuses what cannot be selected from)
     caches = model._caches()
-    model.forward(np.repeat(prompt, beams, 0), n, 0)
-    first = np.full((groups, beams), -np.inf, np.float32)   # the hypotheses of a prompt are still one
-    first[:, 0] = 0.0
-    shape = (groups, beams)
-    scores = [rt.transfer_from_array(first), rt.open_buffer(shape, np.float32)]
-    ended = [rt.open_buffer(shape, np.uint8), rt.open_buffer(shape, np.uint8)]
-    parents, tokens = rt.open_buffer((max_length,) + shape, np.int32), rt.open_buffer((max_length,) + shape, np.int64)
-    unused = rt.open_buffer((model.batch,), np.int64)
-    work = rt.open_buffer(rt.beam_select_work(groups, beams, model.vocab_size, beams), np.uint8)
-    for i in range(max_length):
-        at = i * model.batch
-        out = scores[(i + 1) % 2], parents.view(at, shape), tokens.view(at, shape), ended[(i + 1) % 2]
-        rt.beam_select(model._logits_buffer(), scores[i % 2], beams, ended=ended[i % 2] if eos >= 0 else None, eos=eos, out=out, work=work)
-        if i + 1 < max_length:
-            rt.beam_reorder(caches, out[1], n)
-            model.forward_device(tokens.view(at, (model.batch, 1)), 1, n, unused)
-            n += 1
-    p, t, s = parents.numpy(), tokens.numpy(), scores[max_length % 2].numpy()
-    for b in (*scores, *ended, parents, tokens, unused, work):
-        b.close()
+    held = []
+
+    def hold(b):
+        held.append(b)
+        return b
+    try:
+        model.forward(np.repeat(prompt, beams, 0), n, 0)
+        first = np.full((groups, beams), -np.inf, np.float32)   # the hypotheses of a prompt are still one
+        first[:, 0] = 0.0
+        shape = (groups, beams)
+        scores = [hold(rt.transfer_from_array(first)), hold(rt.open_buffer(shape, np.float32))]
+        ended = [hold(rt.open_buffer(shape, np.uint8)), hold(rt.open_buffer(shape, np.uint8))]
+        parents, tokens = hold(rt.open_buffer((max_length,) + shape, np.int32)), hold(rt.open_buffer((max_length,) + shape, np.int64))
+        unused, work = hold(rt.open_buffer((model.batch,), np.int64)), hold(rt.open_buffer(need, np.uint8))
+        for i in range(max_length):
+            at = i * model.batch
+            out = scores[(i + 1) % 2], parents.view(at, shape), tokens.view(at, shape), ended[(i + 1) % 2]
+            rt.beam_select(model._logits_buffer(), scores[i % 2], beams, ended=ended[i % 2] if eos >= 0 else None, eos=eos, out=out, work=work)
+            if i + 1 < max_length:
+                rt.beam_reorder(caches, out[1], n)
+                model.forward_device(tokens.view(at, (model.batch, 1)), 1, n, unused)
+                n += 1
+        p, t, s = parents.numpy(), tokens.numpy(), scores[max_length % 2].numpy()
+    finally:
+        for b in held:
+            b.close()
     found = np.empty((groups, beams, max_length), np.int64)
     rows, beam = np.arange(groups)[:, None], np.repeat(np.arange(beams)[None], groups, 0)
     for i in range(max_length - 1, -1, -1):

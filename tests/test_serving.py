@@ -434,3 +434,35 @@ def test_beam_search_takes_a_prompt_a_group():
         with pytest.raises(ValueError):
             beam_search(m, bad, 3, 5)
         assert m.steps == 0
+
+
+def test_beam_search_closes_what_it_opened():
+    """Whether it ends, is refused (before the prompt is read), or a step or a selection fails on the way."""
+    from caten_b200 import _lib as L
+    from caten_b200.model import beam_search
+    prompts = np.array([[1, 2, 3], [4, 5, 6]])
+    m = host_model(6)
+    beam_search(m, prompts, 3, 5, eos=7)
+    assert not m.rt.open and m.steps == 5
+    for steps in (1, 2, 4):
+        m = host_model(6, fails_at=steps)
+        with pytest.raises(RuntimeError):
+            beam_search(m, prompts, 3, 5)
+        assert not m.rt.open and m.steps == steps
+    m = host_model(6)
+    m.rt.beam_select = lambda *a, **k: (_ for _ in ()).throw(L.B200Error(L.EUNSUPPORTED, "no"))
+    with pytest.raises(L.B200Error):
+        beam_search(m, prompts, 3, 5)
+    assert not m.rt.open
+    for bad in (dict(eos=20), dict(max_length=15)):          # 20 ids; 3 + 14 positions of 16
+        m = host_model(6)
+        with pytest.raises(ValueError):
+            beam_search(m, prompts, 3, **{"max_length": 5, **bad})
+        assert m.steps == 0 and not m.rt.open
+    m = host_model(6)
+    beam_search(m, prompts, 3, 14)                           # the last one's logits need no position
+    m = host_model(40)
+    m.rt.beam_select_work = lambda *a: (_ for _ in ()).throw(L.B200Error(L.EUNSUPPORTED, "40 beams"))
+    with pytest.raises(L.B200Error):
+        beam_search(m, prompts[:1], 40, 3)
+    assert m.steps == 0
