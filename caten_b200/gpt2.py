@@ -20,6 +20,8 @@ from .synthetic import GPT2_SIZES, GPT2Params, Packed
 
 
 class GPT2(Model):
+    _moved = None   # the caches, once they were asked for
+
     def __init__(self, runtime: B200Runtime, params: GPT2Params, state_dict: dict, max_seq_len: int = 1024,
                  batch: int = 1, precision: str = "fp32", max_rows: int = 0, device_blobs: Optional[dict] = None):
         """``state_dict``: reference keys -> fp32 arrays, or :class:`Packed` for Linear weights.
@@ -138,7 +140,9 @@ class GPT2(Model):
         return B200Buffer(self.rt, k.value, shp, np.float32, owned=False), B200Buffer(self.rt, v.value, shp, np.float32, owned=False)
 
     def _caches(self) -> list:
-        return [c for layer in range(self.params.n_layers) for c in self._kv(layer)]
+        if self._moved is None:   # (addresses that the model keeps)
+            self._moved = [c for layer in range(self.params.n_layers) for c in self._kv(layer)]
+        return self._moved
 
     @property
     def launch_count(self) -> int:
@@ -150,7 +154,7 @@ class GPT2(Model):
                 self._h = None
                 return
             self.rt.lib.caten_b200_gpt2_destroy(self._h)
-            self._h = None
+            self._h = self._moved = None
             for w in self._weights:
                 w.close()
             for b in self._bufs:

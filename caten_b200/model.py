@@ -118,7 +118,7 @@ def beam_search(model: Model, prompt_ids, beams: int, max_length: int = 100, eos
     if eos >= model.vocab_size or n + max_length - 1 > model.max_seq_len:
         raise ValueError(f"beam_search: eos {eos} of {model.vocab_size} ids, {n} + {max_length} tokens over {model.max_seq_len} positions")
     need = rt.beam_select_work(groups, beams, model.vocab_size, beams)   # (refuses what cannot be selected from)
-    caches = model._caches()
+    model._caches()                                                      # (so does a model whose states cannot be moved)
     held = []
 
     def hold(b):
@@ -138,7 +138,7 @@ def beam_search(model: Model, prompt_ids, beams: int, max_length: int = 100, eos
             out = scores[(i + 1) % 2], parents.view(at, shape), tokens.view(at, shape), ended[(i + 1) % 2]
             rt.beam_select(model._logits_buffer(), scores[i % 2], beams, ended=ended[i % 2] if eos >= 0 else None, eos=eos, out=out, work=work)
             if i + 1 < max_length:
-                rt.beam_reorder(caches, out[1], n)
+                model.reorder(out[1], n)
                 model.forward_device(tokens.view(at, (model.batch, 1)), 1, n, unused)
                 n += 1
         p, t, s = parents.numpy(), tokens.numpy(), scores[max_length % 2].numpy()

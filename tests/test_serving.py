@@ -466,3 +466,14 @@ def test_beam_search_closes_what_it_opened():
     with pytest.raises(L.B200Error):
         beam_search(m, prompts[:1], 40, 3)
     assert m.steps == 0
+
+
+def test_beam_search_moves_states_by_the_models_own_call():
+    """``Model.reorder`` is what a subclass with other states overrides."""
+    from caten_b200.model import beam_search
+    m, moved = host_model(3), []
+    own = m.reorder
+    m.reorder = lambda parents, positions: (moved.append(positions), own(parents, positions))
+    out = beam_search(m, [1, 2, 3], 3, 5)
+    assert moved == [3, 4, 5, 6]
+    np.testing.assert_array_equal(out[0], beam_search(host_model(3), [1, 2, 3], 3, 5)[0])
