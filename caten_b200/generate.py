@@ -8,7 +8,7 @@ from __future__ import annotations
 import argparse
 
 from .model import beam_search, generate
-from .registry import load_model
+from .registry import SEARCHABLE, architecture_of, load_model
 from .runtime import B200Runtime
 
 
@@ -29,6 +29,8 @@ def main(argv=None) -> int:
     args = ap.parse_args(argv)
     if args.beams < 0 or args.beams > 32 or (args.beams and args.temperature > 0):
         ap.error("--beams is between 1 and 32, without --temperature")
+    if args.beams and architecture_of(args.model) not in SEARCHABLE:
+        ap.error(f"--beams is for {', '.join(SEARCHABLE)}, whose caches can follow the hypotheses; {args.model} is of {architecture_of(args.model)}")
     tok = None
     if args.prompt is not None:
         from .bpe import gguf_to_bpe_tokenizer
@@ -39,6 +41,8 @@ def main(argv=None) -> int:
         ids = [int(x) for x in args.ids.split(",")]
     with B200Runtime(args.device) as rt:
         m = load_model(args.model, rt, max_seq_len=len(ids) + args.max_length, batch=max(1, args.beams), precision=args.precision)
+        if args.beams and args.eos >= m.vocab_size:
+            ap.error(f"--eos {args.eos} of {m.vocab_size} ids")
         if args.beams:
             out = beam_search(m, [ids], args.beams, args.max_length, args.eos)[0][0].tolist()
         else:

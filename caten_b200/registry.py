@@ -27,6 +27,7 @@ def _goselix(path: str, runtime: Optional[B200Runtime], **kw) -> Model:
 
 
 ARCHITECTURES = {"gpt2": _gpt2, "Binusun": _binusun, "Goselix": _goselix}
+SEARCHABLE = ("gpt2",)   # whose states beam search can move
 
 
 def architecture_of(path: str) -> str:

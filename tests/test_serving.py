@@ -477,3 +477,13 @@ def test_beam_search_moves_states_by_the_models_own_call():
     out = beam_search(m, [1, 2, 3], 3, 5)
     assert moved == [3, 4, 5, 6]
     np.testing.assert_array_equal(out[0], beam_search(host_model(3), [1, 2, 3], 3, 5)[0])
+
+
+def test_command_refuses_beams_over_models_whose_states_do_not_move(tmp_path, capsys):
+    """Said by the command before anything is loaded."""
+    from caten_b200.generate import main
+    for name in ("Binusun", "Goselix"):
+        (tmp_path / "config.json").write_text('{"architecture": "%s"}' % name)
+        with pytest.raises(SystemExit) as e:
+            main(["--model", str(tmp_path), "--ids", "1,2", "--beams", "2"])
+        assert e.value.code == 2 and name in capsys.readouterr().err
