@@ -272,7 +272,10 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
         atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
         a.status[1] = 48;
       }
-      if (sub == 0) ring_land(stage, phase, base + step < t1, [&](int s, uint32_t p) { mbar_wait_thread(bar + 8 * s, p, &never); });
+      if (sub == 0)
+        ring_land(stage, phase, base + step < t1, [&](int s, uint32_t p) {
+          mbar_wait_thread(bar + 8 * s, p, &never);
+        });
     }
     if (SHARED && ok) {
       const uint8_t *tiles = stages + stage * STAGE;
@@ -817,7 +820,9 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
         atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
         a.status[1] = 49;
       }
-      ring_land(stage, phase, base + step < t1, [&](int s, uint32_t p) { mbar_wait_thread(bar + 8 * s, p, &gave_up[warp]); });   // (a flag that nobody raises)
+      ring_land(stage, phase, base + step < t1, [&](int s, uint32_t p) {   // (with a flag that nobody raises)
+        mbar_wait_thread(bar + 8 * s, p, &gave_up[warp]);
+      });
     }
   }
 
@@ -1827,7 +1832,9 @@ __global__ void __launch_bounds__(K1_WARPS * 32) kv4_attention_row_kernel(const 
         atomicCAS(a.status, 0, DEV_WAIT_TIMEOUT);
         a.status[1] = 47;
       }
-      ring_land(stage, phase, base + step < t1, [&](int s, uint32_t p) { mbar_wait_thread(bar + 8 * s, p, &gave_up[warp]); });   // (a flag that nobody raises)
+      ring_land(stage, phase, base + step < t1, [&](int s, uint32_t p) {   // (with a flag that nobody raises)
+        mbar_wait_thread(bar + 8 * s, p, &gave_up[warp]);
+      });
     }
   }
 
