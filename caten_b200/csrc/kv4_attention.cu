@@ -124,8 +124,9 @@ __device__ __forceinline__ float max_abs_nan(float a, float b, float c) {   // (
   return r;
 }
 
-// A block's warps (four, eight where they make operands) are `row_warps` row tiles times shares of the tokens.  The warps of a share work on one ring of two stages of 64
-// or 32 tokens, which bulk copies fill while the other is read (each stage is read by all its warps before it is filled again).
+// A block's warps (four, eight where they make operands) are `row_warps` row tiles (one or two, then four) times two or four shares of the tokens.  The
+// warps of a share work on one ring of two stages of 64 or 32 tokens, which bulk copies fill while the other is read (each stage is read by all its
+// warps before it is filled again).
 // With four row tiles (SHARED) the warps first turn a stage's codes into operands and its scales into floats, a quarter each, in shared memory: of the
 // instructions of 16 tokens and a block of 32 dims, a hundred, that is nearly half, and each warp would do it for itself (5 prompts of 167 to 333
 // tokens, 16 heads over 4 of 128: 130 us; they go in tiles of 128 rows now).
@@ -501,23 +502,16 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
       }
     }
   float *so = reinterpret_cast<float *>(ring) + warp * K4_ROWS * D;   // [row][D]
-  if (shares > 1) {
-    if (__syncthreads_or(!ok)) return;   // no stage is read or filled any more; what did not come is nobody's output
+  if (__syncthreads_or(!ok)) return;   // no stage is read or filled any more; what did not come is nobody's output
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      float *dst = so + 2 * t * D + 32 * k + 4 * g;
-      *reinterpret_cast<float4 *>(dst) = make_float4(o[k][0][0], o[k][0][2], o[k][1][0], o[k][1][2]);
-      *reinterpret_cast<float4 *>(dst + D) = make_float4(o[k][0][1], o[k][0][3], o[k][1][1], o[k][1][3]);
-    }
-    if (t == 0) { sm[warp][g] = run_max; sl[warp][g] = run_sum; }
-    __syncthreads();
-    if (share > 0) return;
-  } else if (t == 0) {
-    sm[warp][g] = run_max;
-    sl[warp][g] = run_sum;
+  for (int k = 0; k < NB; ++k) {
+    float *dst = so + 2 * t * D + 32 * k + 4 * g;
+    *reinterpret_cast<float4 *>(dst) = make_float4(o[k][0][0], o[k][0][2], o[k][1][0], o[k][1][2]);
+    *reinterpret_cast<float4 *>(dst + D) = make_float4(o[k][0][1], o[k][0][3], o[k][1][1], o[k][1][3]);
   }
-  __syncwarp();
-  if (!mine || !ok) return;
+  if (t == 0) { sm[warp][g] = run_max; sl[warp][g] = run_sum; }
+  __syncthreads();
+  if (share > 0 || !mine) return;
   const int64_t tile_of = ((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {   // rows 2t and 2t + 1
@@ -527,22 +521,16 @@ __global__ void __launch_bounds__(k4_warps(SHARED) * 32, SHARED ? (NC <= 2 ? 2 :
     const float ref = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
     float4 x[NB];
-    if (shares == 1) {
-      sum = sl[warp][row];
 #pragma unroll
-      for (int k = 0; k < NB; ++k) x[k] = make_float4(o[k][0][j], o[k][0][2 + j], o[k][1][j], o[k][1][2 + j]);
-    } else {
+    for (int k = 0; k < NB; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < shares; ++w) {
+      const float e = exp2_fast(sm[warp + w * row_warps][row] - ref);
+      sum = fmaf(sl[warp + w * row_warps][row], e, sum);
+      const float *src = so + (w * row_warps * K4_ROWS + row) * D + 4 * g;
 #pragma unroll
-      for (int k = 0; k < NB; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int w = 0; w < shares; ++w) {
-        const float e = exp2_fast(sm[warp + w * row_warps][row] - ref);
-        sum = fmaf(sl[warp + w * row_warps][row], e, sum);
-        const float *src = so + (w * row_warps * K4_ROWS + row) * D + 4 * g;
-#pragma unroll
-        for (int k = 0; k < NB; ++k) {
-          const float4 y = *reinterpret_cast<const float4 *>(src + 32 * k);
-          x[k].x = fmaf(y.x, e, x[k].x); x[k].y = fmaf(y.y, e, x[k].y); x[k].z = fmaf(y.z, e, x[k].z); x[k].w = fmaf(y.w, e, x[k].w);
-        }
+      for (int k = 0; k < NB; ++k) {
+        const float4 y = *reinterpret_cast<const float4 *>(src + 32 * k);
+        x[k].x = fmaf(y.x, e, x[k].x); x[k].y = fmaf(y.y, e, x[k].y); x[k].z = fmaf(y.z, e, x[k].z); x[k].w = fmaf(y.w, e, x[k].w);
       }
     }
     if (rr >= count) continue;
