@@ -513,8 +513,9 @@ static int beam_check(caten_b200_ctx *ctx, const char *who, int64_t batch, int64
 // ---- reordering ------------------------------------------------------------------------------------
 // Row i of a group becomes what row parent(i) was, in place: a thread takes the same 16 (or 4) bytes of all the group's rows that change into
 // registers before it writes any of them, so nothing is read after it was overwritten, whatever the parents are.  Rows that stay
-// are neither read for themselves nor written.  Bound by HBM: 24 layers of 16 x 4 beams, 4.2 GB, 563 us (7.4 TB/s: a row that several children take
-// comes once); pages of 82 KB in no order, 16 x 8 beams, 251 MB, 53 us (4.7 TB/s).
+// are neither read for themselves nor written.  Bound by HBM: 24 layers of 16 x 4 beams, 4.2 GB, 543 to 576 us (7.3 to 7.7 TB/s: a row that several
+// children take comes once).  Pages, 16 x 8 beams of 24 of 82 KB, 251 MB: 54 us (4.7 TB/s, HBM 40 % busy): a block's four dependent loads (parents, lengths,
+// table, page), for a word of 16 bytes a thread.
 constexpr int RO_STATES = 128;   // of a launch
 constexpr int RO_MOST = 1024;    // of a call
 struct ReorderArgs {

@@ -306,8 +306,13 @@ int caten_b200_kv4_load(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, co
 /* Attention over the cache.  Sequence b holds d_lengths[b] tokens, its last ones (those of this step, stored already) are the rows [d_starts[b],
  * d_starts[b + 1]) of d_q [rows, ldq] (heads * dim columns used) and of d_out [rows, heads * dim]: a row sees its own token and all before it.
  * d_starts NULL: one row a sequence, row b (rows == batch).  A row that sees nothing (a sequence of length 0, or shorter than its rows) is 0; rows of no
- * sequence are left as they were.  max_new: rows of a sequence at most; max_length: bound of the lengths, at most max_pages * page.  Arithmetic: codes are
- * exact operands of tensor-core products, q and the probabilities are split in two fp16 halves (2^-22), sums and softmax fp32.
+ * sequence are left as they were.  max_new: rows of a sequence at most; max_length: bound of the lengths, at most max_pages * page.
+ * Arithmetic: sums, softmax statistics and outputs are fp32.  With one row (a token and a head that has its key head for itself) codes are exact int8 operands, q
+ * and p d fixed-point numbers of 31 bits; with more of them codes are exact fp16 operands, q and p d two halves each (22 bits); prompts of heads up to 128
+ * dims have keys and values as two halves too (exact in Q4_0), without the product of lower halves.  An output is within
+ * (40 a + 90 + length / 32) 2^-23 of its row's sum of p |v| in its block of 32 dims, with a = scale sum |q| |k| and |x| short for
+ * |d (code - 8)| + |minimum + 8 d|: tokens that the row does not see or that have no probability, and other dims, do not cost it bits.  A value that is not
+ * finite is NaN in its block of the rows that see it.
  * Lengths, starts or page numbers outside what the call allows are cut or skipped and reported (CATEN_B200_EDEVICE) by the next synchronising call.
  * d_work: kv4_attention_work(..) bytes, 16-byte aligned, nothing of which is kept from call to call; calls that may overlap on the GPU need one each.
  * What kv4_attention_work says for some sizes is enough for every call of the same heads with sizes up to those: a host that allocates for its
