@@ -156,6 +156,7 @@ SIGNATURES = {
     "caten_b200_kv4_store": (C.c_int, [_vp, C.POINTER(Kv4Desc), _vp, _vp, _vp, _i64, _vp, _i64]),
     "caten_b200_kv4_load": (C.c_int, [_vp, C.POINTER(Kv4Desc), _vp, _vp, _i64, _vp, _vp, _i64]),
     "caten_b200_kv4_attention_work": (_i64, [C.POINTER(Kv4Desc), _i64, _i64, _i64, _i64]),
+    "caten_b200_kv4_attention_call_work": (_i64, [C.POINTER(Kv4Desc), _i64, _i64, _i64, _i64]),
     "caten_b200_kv4_attention": (C.c_int, [_vp, C.POINTER(Kv4Desc), _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
     "caten_b200_gpt2_create": (C.c_int, [_vp, C.POINTER(GPT2Desc), _PFP]),
     "caten_b200_gpt2_destroy": (C.c_int, [_vp]),

@@ -2005,6 +2005,12 @@ int64_t caten_b200_kv4_attention_work(const caten_b200_kv4_desc *desc, int64_t b
   return kv4_work_bound({desc->dim, desc->kv_heads, desc->heads / desc->kv_heads}, batch, max_new, max_length);
 }
 
+int64_t caten_b200_kv4_attention_call_work(const caten_b200_kv4_desc *desc, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length) {
+  Kv4Plan p;
+  if (kv4_plan(nullptr, "kv4_attention_call_work", desc, batch, rows, max_new, max_length, &p)) return -1;
+  return std::max<int64_t>(16, kv4_plan_bytes(p, desc->dim));
+}
+
 int caten_b200_kv4_attention(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, const float *d_q, int64_t ldq, const void *d_pool, const int32_t *d_table,
                              int64_t max_pages, const int32_t *d_lengths, const int32_t *d_starts, int64_t batch, int64_t rows, int64_t max_new,
                              int64_t max_length, float *d_out, void *d_work) {

@@ -275,7 +275,7 @@ class B200Runtime:
 
     # ---- beam search ----
     def beam_select_work(self, batch: int, beams: int, V: int, keep: int) -> int:
-        """Bytes of workspace that a ``beam_select`` of these sizes needs."""
+        """Bytes of workspace that are enough for every ``beam_select`` of sizes up to these."""
         n = self.lib.caten_b200_beam_select_work(batch, beams, V, keep)
         if n < 0:
             L.check(None, L.EINVAL)
@@ -371,7 +371,7 @@ class B200Runtime:
         _room(who, pool, self.lib.caten_b200_kv4_nbytes(C.byref(desc)))
 
     def kv4_attention_work(self, desc: L.Kv4Desc, batch: int, rows: int, max_new: int, max_length: int) -> int:
-        """Bytes of workspace that a ``kv4_attention`` of these sizes needs."""
+        """Bytes of workspace that are enough for every ``kv4_attention`` of these heads with sizes up to these."""
         n = self.lib.caten_b200_kv4_attention_work(C.byref(desc), batch, rows, max_new, max_length)
         if n < 0:
             L.check(None, L.EINVAL)
@@ -386,7 +386,9 @@ class B200Runtime:
         max_length = max_length or table.shape[1] * desc.page
         if lengths.shape != (B,) or table.shape[0] != B or (starts is not None and starts.shape != (B + 1,)) or len(q.shape) != 2 or q.shape[1] < width:
             raise ValueError(f"kv4_attention: q {q.shape}, lengths {lengths.shape}, table {table.shape}, starts {starts and starts.shape}")
-        need = self.kv4_attention_work(desc, B, rows, max_new, max_length)
+        need = self.lib.caten_b200_kv4_attention_call_work(C.byref(desc), B, rows, max_new, max_length)
+        if need < 0:
+            L.check(None, L.EINVAL)
         out = out or self.open_buffer((rows, width))
         if out.shape != (rows, width):
             raise ValueError(f"kv4_attention: out {out.shape}, expected {(rows, width)}")

@@ -316,8 +316,9 @@ int caten_b200_kv4_load(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, co
  * Lengths, starts or page numbers outside what the call allows are cut or skipped and reported (CATEN_B200_EDEVICE) by the next synchronising call.
  * d_work: kv4_attention_work(..) bytes, 16-byte aligned, nothing of which is kept from call to call; calls that may overlap on the GPU need one each.
  * What kv4_attention_work says for some sizes is enough for every call of the same heads with sizes up to those: a host that allocates for its
- * largest batch, max_new and max_length need not ask again. */
+ * largest batch, max_new and max_length need not ask again.  kv4_attention_call_work is what a call of exactly these sizes uses, often far less. */
 int64_t caten_b200_kv4_attention_work(const caten_b200_kv4_desc *desc, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length);
+int64_t caten_b200_kv4_attention_call_work(const caten_b200_kv4_desc *desc, int64_t batch, int64_t rows, int64_t max_new, int64_t max_length);
 int caten_b200_kv4_attention(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, const float *d_q, int64_t ldq, const void *d_pool,
                              const int32_t *d_table, int64_t max_pages, const int32_t *d_lengths, const int32_t *d_starts, int64_t batch, int64_t rows,
                              int64_t max_new, int64_t max_length, float *d_out, void *d_work);

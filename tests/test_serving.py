@@ -214,7 +214,11 @@ int main() {
     if (kv4_work_bound(h, b, n, l) > bound) { printf("not monotonic\\n"); return 1; }
   }
   printf("%lld %lld %lld %lld %lld\\n", (long long)parts[0], (long long)parts[1], (long long)parts[2], (long long)parts[3], (long long)smaller_needs_more);
-  for (int64_t batch : {1, 7, 300}) for (int64_t n : {1, 2, 40}) for (int64_t l : {1, 700, 5000}) printf("%lld\\n", (long long)kv4_work_bound({128, 8, 2}, batch, n, l));
+  for (int64_t batch : {1, 7, 300}) for (int64_t n : {1, 2, 40}) for (int64_t l : {1, 700, 5000}) {
+    Kv4Plan p;
+    kv4_plan_of({128, 8, 2}, batch, batch * n, n, l, &p);
+    printf("%lld\\n%lld\\n", (long long)kv4_work_bound({128, 8, 2}, batch, n, l), (long long)std::max<int64_t>(16, kv4_plan_bytes(p, 128)));
+  }
 }
 ''')
     exe = tmp_path / "plan"
@@ -224,7 +228,9 @@ int main() {
     seen, *said = r.stdout.splitlines()
     assert min(map(int, seen.split())) > 100   # every kernel with parts; smaller calls that need more than the larger one itself
     d = desc(dim=128, heads=16, kv_heads=8)
-    assert [lib.caten_b200_kv4_attention_work(C.byref(d), b, b * n, n, ln) for b in (1, 7, 300) for n in (1, 2, 40) for ln in (1, 700, 5000)] == [int(x) for x in said]
+    for entry, want in ((lib.caten_b200_kv4_attention_work, said[::2]), (lib.caten_b200_kv4_attention_call_work, said[1::2])):
+        assert [entry(C.byref(d), b, b * n, n, ln) for b in (1, 7, 300) for n in (1, 2, 40) for ln in (1, 700, 5000)] == [int(x) for x in want]
+    refused(lib, lib.caten_b200_kv4_attention_call_work(C.byref(d), 2, 5, 0, 128), "bad shape")
 
 
 def test_selection_workspace_is_enough_for_every_smaller_call(lib):
