@@ -888,8 +888,9 @@ __global__ void __launch_bounds__(K2_WARPS * 32, NC <= 2 ? 4 : 2) kv4_attention_
 constexpr int K3_THREADS = 512, K3_SOFTMAX = 8, K3_CONVERT = 7;   // (warps)
 constexpr float K3_LIFT = 14.0f;   // p is taken times 2^14, its sum with it
 // A step's keys share a power of two, and 64 dims of its values.  Which sizes they have is a bit for each four exponents, from 2^-27 (what is stored is
-// zero or 2^-24 at least) to 2^25: bit i is 2^(4i - 27) to 2^(4i - 23).  What is more than three bits below the largest would have less than 20 bits.
-constexpr int K3_SPREAD = 3;
+// zero or 2^-24 at least) to 2^25: bit i is 2^(4i - 27) to 2^(4i - 23).  Where they are no more than two bits apart, 2^12, the last bits of 64 values and
+// probabilities, 2^-3, are 2^-20 of what the smallest alone makes.
+constexpr int K3_SPREAD = 2;
 __device__ __forceinline__ unsigned k3_of_size(float x) { return x == 0.0f ? 0u : 1u << ((__float_as_uint(x) >> 25) - 25); }
 // what brings the largest size to [2^11, 2^15); its exponent, the upper one (none: below all that can be stored)
 __device__ __forceinline__ float k3_up(unsigned sizes) { return __uint_as_float((uint32_t)(127 + 38 - 4 * (31 - __clz(sizes | 1u))) << 23); }
