@@ -358,6 +358,28 @@ def test_a_prompt_whose_pages_or_lengths_are_wrong(rt):
     rt.sync()
 
 
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+def test_one_workspace_for_every_call_up_to_the_largest(rt, kind):
+    """Sized by kv4_attention_work for the largest turn; no call writes beyond what kv4_attention_call_work says of it."""
+    rng = rng_of(22)
+    for heads, kv, dim in ((4, 4, 64), (8, 2, 128), (3, 1, 256)):
+        lengths = [2500, 700, 40, 1, 900, 64]
+        c = Cache(rt, rng, kind, dim, 64, heads, kv, lengths)
+        size = rt.kv4_attention_work(c.desc, 6, 6 * 60, 60, 2560)
+        work = rt.open_buffer((size,), np.uint8)
+        for batch, new, top in ((6, 60, 2560), (1, 60, 2560), (6, 1, 2560), (1, 1, 2560), (3, 3, 2560), (2, 12, 2500), (1, 2, 2500), (6, 60, 2500)):
+            rows = [min(new, n) for n in lengths[:batch]]
+            at = np.concatenate([[0], np.cumsum(rows)])
+            need = rt.lib.caten_b200_kv4_attention_call_work(C.byref(c.desc), batch, int(at[-1]), new, top)
+            assert 16 <= need <= size
+            L.check(rt.ctx, rt.lib.caten_b200_memset(rt.ctx, work.ptr, 0x5a, size))
+            q = rng.standard_normal((int(at[-1]), heads * dim), dtype=np.float32)
+            args = (c.desc, put(rt, q), c.pool, put(rt, c.table[:batch], np.int32), put(rt, lengths[:batch], np.int32), put(rt, at, np.int32))
+            out = rt.kv4_attention(*args, max_new=new, max_length=top, work=work).numpy()
+            assert (work.numpy()[need if need > 16 else 0:] == 0x5a).all()   # (16: none is used)
+            np.testing.assert_array_equal(out, rt.kv4_attention(*args, max_new=new, max_length=top).numpy())
+
+
 def test_results_are_the_same_every_time(rt):
     rng = rng_of(21)
     c = Cache(rt, rng, "q4_0", 64, 64, 4, 2, [3000, 65, 900])
@@ -788,6 +810,23 @@ def test_selection_is_decided_in_64_bits_between_beams(rt, groups, beams, V, kee
     check_select(rt, few, scores, min(keep, 7))
     many = np.where(np.arange(V) < keep - 1, np.float32(1), np.float32(-20)) + np.zeros((groups, beams, 1), np.float32)
     check_select(rt, many, scores - np.where(np.arange(beams) == 0, 0.0, 2.0), keep, shift=3)
+
+
+@pytest.mark.parametrize("groups,beams,V,keep", [(3, 4, 20000, 32), (30, 3, 9001, 20), (1, 32, 20000, 32)])
+def test_selection_among_more_equal_values_than_are_looked_at(rt, groups, beams, V, keep):
+    """Beams whose logits are a few values, so that hundreds of candidates are equal, with ended, masked and broken hypotheses between them."""
+    rng = rng_of(groups, beams, V, 1)
+    x = np.repeat(rng.integers(0, 2, (groups, 1, V)).astype(np.float32) * np.float32(0.7) - np.float32(0.3), beams, 1)
+    scores = np.full((groups, beams), -1.5, np.float32)
+    for eos, ended in ((-1, None), (5, rng.random((groups, beams)) < 0.4)):
+        check_select(rt, x, scores, keep, ended=ended, eos=eos, shift=1)
+    y = x.copy()
+    y[0, 0] = -np.inf
+    y[0, beams // 2, 7] = np.nan
+    y[:, beams - 1, :V - 3] = np.finfo(np.float32).min
+    scores[-1, 1] = -np.inf
+    for eos, ended in ((-1, None), (5, rng.random((groups, beams)) < 0.4)):
+        check_select(rt, y, scores, keep, ended=ended, eos=eos)
 
 
 @pytest.mark.parametrize("score", [-1e30, float(np.finfo(np.float32).min)])
