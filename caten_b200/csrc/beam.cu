@@ -250,7 +250,7 @@ struct JoinArgs {
 };
 struct JoinShared {
   __align__(128) Cand found[BJ_FOUND];
-  Cand taken[BS_KEEP], bound;
+  Cand sorted[BJ_FOUND], bound;
   double base[BJ_BEAMS], tops[BJ_BEAMS];   // a candidate's value: base + (x - top)
   double sums[BJ_THREADS / 32];
   uint8_t over[BJ_BEAMS];
@@ -428,7 +428,6 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
   __syncthreads();
   if (lists > BJ_HEADS) {
     const Cand first = sh.bound;
-    __syncthreads();
     for (int i = tid; i < lists; i += BJ_THREADS) {
       const Cand c = entry(i, 0);
       if (c.value && !(first > c)) sh.found[atomicAdd(&sh.count, 1)] = c;   // (of at most `keep` threads, 16 lists each)
@@ -442,7 +441,6 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
     if (tid == 0) sh.count = 0;
   }
   const u64 least = sh.bound.value;
-  __syncthreads();
   auto enqueue = [&](int i) {
     const int at = atomicAdd(&sh.queued, 1);
     if (at < BJ_QUEUE) sh.queue[at] = i;
@@ -464,25 +462,32 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_cons
   __syncthreads();
   const int n = min(sh.count, BJ_FOUND);
   for_places(n, [&](const Cand &c, int place) {
-    if (place >= keep) return;
-    sh.write(a, place, true, c);
-    sh.taken[place] = c;
+    if (place < keep) sh.write(a, place, true, c);
+    sh.sorted[place] = c;
   });
   if (tid >= n && tid < keep) sh.write(a, tid, false, Cand{0ull, 0ull});
   __syncthreads();
+  // Where two candidates of different beams are close, and one is taken, so are two neighbours, which are taken or close to the last that is.
+  bool close = false;
+  if (tid + 1 < n) {
+    const Cand c = sh.sorted[tid], next = sh.sorted[tid + 1];
+    const double value = value_of(next.value);
+    close = c.beam() != next.beam() && value_of(sh.sorted[min(tid, keep - 1)].value) - value <= sh.close_to(a, value);
+  }
+  if (!__syncthreads_or(close || sh.queued > BJ_QUEUE || sh.count > BJ_FOUND)) return;   // (or so many are equal that some were not looked at)
   if (tid / BJ_LANES < min(n, keep)) {   // each that was taken, and whatever of other beams is close to it
-    const Cand c = sh.taken[tid / BJ_LANES];
+    const Cand c = sh.sorted[tid / BJ_LANES];
     const double value = value_of(c.value), apart = sh.close_to(a, value);
     const u64 from = order_of(value - apart), to = order_of(value + apart);
-    unsigned close = 0;
+    unsigned beams = 0;
     for (int j = tid % BJ_LANES; j < n; j += BJ_LANES) {
       const u64 v = sh.found[j].value;
-      if (v >= from && v <= to) close |= 1u << sh.found[j].beam();
+      if (v >= from && v <= to) beams |= 1u << sh.found[j].beam();
     }
-    if (close & ~(1u << c.beam())) atomicOr(&sh.close_beams, close | 1u << c.beam());
+    if (beams & ~(1u << c.beam())) atomicOr(&sh.close_beams, beams | 1u << c.beam());
   }
   __syncthreads();
-  if (sh.close_beams || sh.queued > BJ_QUEUE || sh.count > BJ_FOUND) beam_join_exactly(a, sh);
+  beam_join_exactly(a, sh);
 }
 
 // Chunks of 8192 logits, or of 2048 where the larger ones would not give every SM a block.
