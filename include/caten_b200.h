@@ -311,8 +311,9 @@ int caten_b200_kv4_load(caten_b200_ctx *ctx, const caten_b200_kv4_desc *desc, co
  * and p d fixed-point numbers of 31 bits; with more of them codes are exact fp16 operands, q and p d two halves each (22 bits); prompts of heads up to 128
  * dims have keys and values as two halves too (exact in Q4_0), without the product of lower halves.  An output is within
  * (40 a + 90 + length / 32) 2^-23 of its row's sum of p |v| in its block of 32 dims, with a = scale sum |q| |k| and |x| short for
- * |d (code - 8)| + |minimum + 8 d|: tokens that the row does not see or that have no probability, and other dims, do not cost it bits.  A value that is not
- * finite is NaN in its block of the rows that see it.
+ * |d (code - 8)| + |minimum + 8 d|: tokens that the row does not see or that have no probability, and other dims, do not cost it bits.  (In prompts, where a
+ * token whose values are all zero has more than 0.9999 of p, 2^-33 of the largest |v| comes on top.)  A value that is not finite is NaN in its block of the
+ * rows that see it.
  * Lengths, starts or page numbers outside what the call allows are cut or skipped and reported (CATEN_B200_EDEVICE) by the next synchronising call.
  * d_work: kv4_attention_work(..) bytes, 16-byte aligned, nothing of which is kept from call to call; calls that may overlap on the GPU need one each.
  * What kv4_attention_work says for some sizes is enough for every call of the same heads with sizes up to those: a host that allocates for its
