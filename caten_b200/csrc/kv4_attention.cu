@@ -913,63 +913,131 @@ __device__ __forceinline__ void k3_split(uint32_t codes, uint32_t dd, float2 d, 
   }
 }
 
-// The rows of a tile in fp32 and without tensor cores, a row a warp at a time: where a step has keys or values too far apart for halves that share a power
-// of two, and a row's output is so small beside them that it counts.  Sixteen tokens make sums of their own.  (Some seventy times as long.)
+// The rows of a tile in fp32 and without tensor cores, eight rows a warp: where a step has keys or values too far apart for halves that share a power of
+// two, and a row's output is so small beside them that it counts.  64 tokens at a time become floats in shared memory (of which all else is done by now);
+// scores with a token a lane, outputs with a dim a lane and sums of their own for the 64.  (5 prompts of 333 tokens over
+// 1200: 1.85 ms, sixteen times as long; a row a warp, scores summed over lanes: 8.4 ms.)
 template <int NC, bool Q41>
-__device__ __forceinline__ void kv4_prompt_plainly(const Kv4AttnArgs &a, const Kv4Seq &seq, int b, int head, int rt, int part) {
-  constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D;
-  const int lane = threadIdx.x & 31, count = seq.count * a.group, t0 = part * a.part_tokens;
+__device__ __forceinline__ void kv4_prompt_plainly(const Kv4AttnArgs &a, const Kv4Seq &seq, int b, int head, int rt, int part, float *smem) {
+  constexpr int NB = 2 * NC, D = 64 * NC, PART = (Q41 ? 10 : 9) * D, ROWS = K3_ROWS * 32 / K3_THREADS, LD = D + 1;
+  float *const qs = smem, *const ks = qs + K3_ROWS * D, *const vs = ks + 64 * LD;   // q times the scale; keys, a bank further on each; values
+  const int tid = threadIdx.x, lane = tid & 31, count = seq.count * a.group, r0 = rt * K3_ROWS, first = tid >> 5 << 3, t0 = part * a.part_tokens;
   const int tile_shift = a.s.page == 16 ? 0 : a.s.page == 32 ? 1 : a.s.page == 64 ? 2 : 3;
-  for (int row = threadIdx.x >> 5; row < K3_ROWS; row += K3_THREADS / 32) {
-    const int r = rt * K3_ROWS + row;
-    if (r >= count) break;
-    const int64_t token = seq.first + r / a.group;
-    const int column = (head * a.group + r % a.group) * D, t1 = min(t0 + a.part_tokens, max(0, seq.length - seq.count + r / a.group + 1));
-    float q[NB], o[NB], run_max = -INFINITY, run_sum = 0.0f;
+  static_assert(ROWS == 8, "a warp's rows");
+  auto sees_of = [&](int r) { return r < count ? min(t0 + a.part_tokens, max(0, seq.length - seq.count + r / a.group + 1)) : 0; };
+  auto column_of = [&](int r) { return (int64_t)(head * a.group + r % a.group) * D; };
+  const int reach = sees_of(min(count, r0 + K3_ROWS) - 1);
+  for (int i = tid; i < K3_ROWS * D; i += K3_THREADS) {
+    const int r = r0 + i / D;
+    qs[i] = r < count ? a.q[(seq.first + r / a.group) * a.ldq + column_of(r) + i % D] * (a.scale * 1.4426950408889634f) : 0.0f;
+  }
+  float o[ROWS][NB], run_max[ROWS], run_sum[ROWS];
+  int sees[ROWS];
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      q[k] = a.q[token * a.ldq + column + 32 * k + lane] * (a.scale * 1.4426950408889634f);
-      o[k] = 0.0f;
-    }
-    for (int base = t0; base < t1; base += 16) {
-      const int id = a.table[(int64_t)b * a.max_pages + (base >> 4 >> tile_shift)], n = min(16, t1 - base);
+  for (int r = 0; r < ROWS; ++r) {
+    sees[r] = sees_of(r0 + first + r);
+    run_max[r] = -INFINITY;
+    run_sum[r] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) o[r][k] = 0.0f;
+  }
+  for (int base = t0; base < reach; base += 64) {
+    __syncthreads();   // the tokens before have been read
+    unsigned there = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = base + 16 * i, id = at < reach ? a.table[(int64_t)b * a.max_pages + (at >> 4 >> tile_shift)] : -1;
       if (!kv4_page_ok(a.s, id)) continue;   // (reported by the copies)
-      const uint8_t *keys = a.pool + kv4_tile_at(a.s, id, head, base & (a.s.page - 1)), *values = keys + PART;
-      auto value = [&](const uint8_t *tile, int at, int k, int byte) {   // of token `at`, dim 32 k + lane
-        const __half *sc = reinterpret_cast<const __half *>(tile + 8 * D) + kv4_scale_index(at, k, D);
-        const float d = __half2float(sc[0]), code = (float)((tile[byte] >> (lane & 1) * 4 & 15) - 8);
-        return Q41 ? fmaf(d, code, fmaf(8.0f, d, __half2float(sc[D / 2]))) : d * code;
-      };
-      float s = -INFINITY;
-      for (int at = 0; at < n; ++at) {
-        float x = 0.0f;
+      there |= 1u << i;
+      const uint8_t *tile = a.pool + kv4_tile_at(a.s, id, head, at & (a.s.page - 1));
+      for (int u = tid; u < 2 * 16 * D / 4; u += K3_THREADS) {   // four dims of a token's key or value
+        const int of_v = u / (16 * D / 4), token = u / (D / 4) % 16, dim = u % (D / 4) * 4;
+        const uint8_t *x = tile + of_v * PART;
+        const unsigned codes = *reinterpret_cast<const uint16_t *>(x + (of_v ? kv4_v_byte(token, dim) : kv4_k_byte(token, dim)));
+        const __half *sc = reinterpret_cast<const __half *>(x + 8 * D) + kv4_scale_index(token, dim / 32, D);
+        const float d = __half2float(sc[0]), n = Q41 ? fmaf(8.0f, d, __half2float(sc[D / 2])) : 0.0f;
+        float *dst = of_v ? vs + (16 * i + token) * D + dim : ks + (16 * i + token) * LD + dim;
 #pragma unroll
-        for (int k = 0; k < NB; ++k) x = fmaf(q[k], value(keys, at, k, kv4_k_byte(at, 32 * k + lane)), x);
-        x = warp_sum(x);
-        if (lane == at) s = x;
+        for (int e = 0; e < 4; ++e) {
+          const float code = (float)((int)(codes >> 4 * e & 15u) - 8);
+          dst[e] = Q41 ? fmaf(d, code, n) : d * code;
+        }
       }
-      const float top = fmaxf(run_max, warp_max(s)), ref = top == -INFINITY ? 0.0f : top, corr = exp2_fast(run_max - ref), p = exp2_fast(s - ref);
-      run_max = top;
-      run_sum = fmaf(run_sum, corr, warp_sum(p));
-      float sums[NB];
-#pragma unroll
-      for (int k = 0; k < NB; ++k) sums[k] = 0.0f;
-      for (int at = 0; at < n; ++at) {
-        const float w = __shfl_sync(0xffffffffu, p, at);
-#pragma unroll
-        for (int k = 0; k < NB; ++k) sums[k] = fmaf(w, value(values, at, k, kv4_v_byte(at, 32 * k + lane)), sums[k]);
-      }
-#pragma unroll
-      for (int k = 0; k < NB; ++k) o[k] = fmaf(o[k], corr, sums[k]);
     }
-    float *dst = a.parts == 1 ? a.out + token * a.heads * D + column
-                              : a.part + (((((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt) * a.parts + part) * K3_ROWS + row) * (D + 2);
-    const float scale = a.parts > 1 ? 1.0f : run_sum == 0.0f ? 0.0f : 1.0f / run_sum;
+    __syncthreads();
+    if (base >= sees[ROWS - 1] && base >= sees_of(min(count, r0 + first + ROWS) - 1)) continue;
+    float p[2][ROWS];
 #pragma unroll
-    for (int k = 0; k < NB; ++k) dst[32 * k + lane] = o[k] * scale;
-    if (a.parts > 1 && lane == 0) { dst[D] = run_max; dst[D + 1] = run_sum; }
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) p[h][r] = 0.0f;
+      const float *k = ks + (32 * h + lane) * LD, *q = qs + first * D;
+#pragma unroll 1
+      for (int j = 0; j < D; j += 4) {
+        const float k0 = k[j], k1 = k[j + 1], k2 = k[j + 2], k3 = k[j + 3];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          const float4 x = *reinterpret_cast<const float4 *>(q + r * D + j);
+          p[h][r] = fmaf(x.w, k3, fmaf(x.z, k2, fmaf(x.y, k1, fmaf(x.x, k0, p[h][r]))));
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+        if (base + 32 * h + lane >= sees[r] || !(there >> (2 * h + lane / 16) & 1)) p[h][r] = -INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const float top = fmaxf(run_max[r], warp_max(fmaxf(p[0][r], p[1][r]))), ref = top == -INFINITY ? 0.0f : top, corr = exp2_fast(run_max[r] - ref);
+      run_max[r] = top;
+      p[0][r] = exp2_fast(p[0][r] - ref);
+      p[1][r] = exp2_fast(p[1][r] - ref);
+      run_sum[r] = fmaf(run_sum[r], corr, warp_sum(p[0][r] + p[1][r]));
+#pragma unroll
+      for (int k = 0; k < NB; ++k) o[r][k] *= corr;
+    }
+#pragma unroll
+    for (int r1 = 0; r1 < ROWS; r1 += 4) {
+      float sums[4][NB];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int k = 0; k < NB; ++k) sums[r][k] = 0.0f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+        for (int at = 0; at < 32; ++at) {
+          if (!(there >> (2 * h + at / 16) & 1)) continue;
+          float v[NB];
+#pragma unroll
+          for (int k = 0; k < NB; ++k) v[k] = vs[(32 * h + at) * D + 32 * k + lane];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float w = __shfl_sync(0xffffffffu, p[h][r1 + r], at);
+            if (base + 32 * h + at < sees[r1 + r])   // (0 times what a row does not see may be NaN)
+#pragma unroll
+              for (int k = 0; k < NB; ++k) sums[r][k] = fmaf(w, v[k], sums[r][k]);
+          }
+        }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int k = 0; k < NB; ++k) o[r1 + r][k] += sums[r][k];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = r0 + first + i;
+    if (r >= count) continue;
+    float *dst = a.parts == 1 ? a.out + (seq.first + r / a.group) * a.heads * D + column_of(r)
+                              : a.part + (((((int64_t)b * a.s.kv_heads + head) * a.row_tiles + rt) * a.parts + part) * K3_ROWS + first + i) * (D + 2);
+    const float scale = a.parts > 1 ? 1.0f : run_sum[i] == 0.0f ? 0.0f : 1.0f / run_sum[i];
+#pragma unroll
+    for (int k = 0; k < NB; ++k) dst[32 * k + lane] = o[i][k] * scale;
+    if (a.parts > 1 && lane == 0) { dst[D] = run_max[i]; dst[D + 1] = run_sum[i]; }
   }
 }
+static_assert((K3_ROWS * 128 + 64 * 129 + 64 * 128) * 4 <= 2 * (32768 + 2 * 16384 + 2 * 16384) && (K3_ROWS * 64 + 64 * 65 + 64 * 64) * 4 <= 32768 + 2 * 16384 + 2 * 16384,
+              "that takes no more shared memory than the operands had");
 
 template <int NC, bool Q41>
 __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(const Kv4AttnArgs a) {
@@ -1466,7 +1534,7 @@ __global__ void __launch_bounds__(K3_THREADS, 1) kv4_attention_prompt_kernel(con
     }
   tc_fence_before();
   const bool failed = __syncthreads_or(!ok);
-  if (uneven && !failed) kv4_prompt_plainly<NC, Q41>(a, seq, b, head, rt, part);
+  if (uneven && !failed) kv4_prompt_plainly<NC, Q41>(a, seq, b, head, rt, part, reinterpret_cast<float *>(sq));
 
   // rows go out by way of shared memory (all products have been read): 32 dims of 128 rows are 16 KB
   const bool rows_warp = warp < K3_SOFTMAX;
